@@ -13,7 +13,7 @@ calls of the package. Four operators:
                prompts, or chunks of prompts behind a cached context.
 ``branch``     scheduler work on the page table: sequences are forked (full pages shared, tails copied), the copies grow
                by some tokens (pages are taken from the pool) and are dropped again (pages return to the pool).
-``compact``    all live pages move to the front of a new, smaller pool and the page table follows.
+``compact``    a new, independent cache with a smaller pool: all live pages move to its front and the page table follows.
 ``int8``       ``y = x @ W.T`` with int8 weights (one scale per output channel) and activations quantised per token.
 
 Layout of a cache: ``codes`` int8 [pages, layers, 2, kv_heads, 64 * head_dim] (keys [64][head_dim], values
@@ -163,7 +163,7 @@ def work(case):
     if op == "compact":
         sizes = _compact_sizes(case)
         pages = sum(n // BLOCK for n in sizes)
-        return {"bytes": 2 * case["layers"] * (pages * (BLOCK * token + 8 * kvh) + sum(n % BLOCK for n in sizes) * token * e), "flops": 0}
+        return {"bytes": 2 * case["layers"] * (pages * (BLOCK * token + 8 * kvh) + case["batch"] * BLOCK * token * e), "flops": 0}
     if op == "branch":
         parents, _, _ = _branch_sizes(case)
         tails = sum(n % BLOCK for n in parents) * token * e * case["layers"]
@@ -463,7 +463,7 @@ def _run_branch(state):
 def _run_compact(state):
     if own:
         small = state["cache"].compact(state["held"])
-        return {"codes": small.codes, "scales": small.scales, "table": small.table, "refs": small.refs}
+        return {n: getattr(small, n) for n in ("codes", "scales", "tail", "peak", "table", "lengths", "refs")}
     refs, table = state["refs"], state["table"]
     live = refs > 0
     place = live.cumsum(0) - 1                                                           # of every live page in the new pool
@@ -471,7 +471,8 @@ def _run_compact(state):
     source[torch.where(live, place, state["held"])] = torch.arange(refs.shape[0], device=refs.device)
     source = source[:-1]
     moved = torch.where(table >= 0, place[table.clamp_min(0).long()].int(), -1)
-    return {"codes": state["codes"][source], "scales": state["scales"][source], "table": moved, "refs": refs[source]}
+    return {"codes": state["codes"][source], "scales": state["scales"][source], "tail": state["tail"].clone(),
+            "peak": state["peak"].clone(), "table": moved, "lengths": state["lengths"].clone(), "refs": refs[source]}
 
 
 # ------------------------------------------------------------------------------------------------ 64 bits
