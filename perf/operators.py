@@ -272,7 +272,8 @@ def prepare(case, seed):
             state["held"] = held
         if own:
             from mylocal_llm_b200 import PagedKV8Cache
-            state["cache"] = PagedKV8Cache.from_tensors(**{n: state[n] for n in ("codes", "scales", "tail", "peak", "table", "lengths", "refs")})
+            state["cache"] = PagedKV8Cache.from_tensors(**{n: state[n] for n in ("codes", "scales", "tail", "peak", "table", "lengths", "refs")},
+                                                        max_length=_longest(case))
             if case["op"] == "branch":
                 state["batch"] = state["cache"].batch(list(range(b, 2 * b)), grow)
         return state
@@ -310,9 +311,16 @@ def prepare(case, seed):
                   "rows_part": torch.nonzero(pos >= (_ints([t for t, _ in sizes]) // BLOCK * BLOCK)[seq])[:, 0]}
     if own:
         from mylocal_llm_b200 import PagedKV8Cache
-        state["cache"] = PagedKV8Cache.from_tensors(**{n: state[n] for n in ("codes", "scales", "tail", "peak", "table", "lengths", "refs")})
+        state["cache"] = PagedKV8Cache.from_tensors(**{n: state[n] for n in ("codes", "scales", "tail", "peak", "table", "lengths", "refs")},
+                                                    max_length=_longest(case))
         state["batch"] = state["cache"].batch(list(range(b)), counts)
         state["batch"].starts.copy_(state["starts"])
+        if case["op"] == "append":
+            # the peaks that the new tokens of a tail meet are those of the tokens before the step
+            of, layer = state["block_seq"][state["part"]], state["layer"]
+            before = torch.arange(BLOCK, device="cuda") < (state["starts"][of] - state["block_no"][state["part"]] * BLOCK)[:, None]
+            magnitude = state["tail"][of, layer].float().abs()
+            state["peak"][of, layer] = (magnitude * before[:, None, None, :, None]).amax((-1, -2))
     return state
 
 
