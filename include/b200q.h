@@ -467,6 +467,88 @@ int b200q_expert_ffn_static(const void *gate, int gate_fmt, const void *up, int 
                             int down_fmt, int d_model, int d_ff, const void *x, int x_dtype, int m,
                             void *y, int y_dtype, void *stream);
 
+/* ---- Paged key/value cache in 8 bits -------------------------------------------------------------
+ * (No counterpart in the reference, whose caches are dense FP16 / FP32 per sequence,
+ * mini_llm/ops/attention_inference.py:255-277.) A block is 64 consecutive tokens of a sequence. Full blocks are int8 codes
+ * with one FP32 scale per block, layer, key/value head and part (0 = keys, 1 = values), in pages that hold one block of
+ * every layer; the up to 63 tokens behind the last full block of a sequence stay in a 16-bit tail:
+ *   codes  [pages][layers][2][kv_heads][64 * head_dim] int8, 16-byte aligned: keys as [64][head_dim], values as
+ *          [head_dim][64]; value = code * scale, scale = max |x| / 127 (at least 2^-126), codes rounded to nearest, ties to even
+ *   scales [pages][layers][2][kv_heads] FP32; a block with a NaN or an infinity has scale NaN
+ *   tail   [sequences][layers][2][kv_heads][64][head_dim] of type `dtype` (FP16 or BF16), 16-byte aligned
+ *   peak   [sequences][layers][2][kv_heads] FP32: largest magnitude in the tail (undefined for an empty tail)
+ *   table  [sequences][blocks] int32: page of every full block, -1 elsewhere
+ *   lengths[sequences] int32: tokens held;  refs [pages] int32: sequences that refer to a page
+ *   free_bits[(pages + 31) / 32]: bit p % 32 of word p / 32 is set while refs[p] == 0
+ * Keys and values are rounded to `dtype` before anything else, so the content of a cache does not depend on how many tokens
+ * arrived per call. head_dim 64 or 128; at most 65536 sequences and 2^20 pages. All of it lives on the device, every call
+ * but the sizes of b200q_kv8_compact's new pool is decided there, and calls on one cache have to be ordered by their stream.
+ * Device status words of refusals: 501 too few free pages, 502 a sequence would pass max_length (or a slot is out of range),
+ * 503 fork / free of slots out of range, of a target named twice, not empty or also a source, 504 compact into too few pages. */
+typedef struct b200q_kv8_cache {
+    int8_t *codes;
+    float *scales;
+    void *tail;
+    float *peak;
+    int32_t *table;
+    int32_t *lengths;
+    int32_t *refs;
+    uint32_t *free_bits;
+    int32_t layers, kv_heads, head_dim, pages, sequences, blocks, max_length, dtype;
+} b200q_kv8_cache;
+
+/* Sequence slots[b] (distinct slots) grows by offsets[b + 1] - offsets[b] >= 0 tokens: takes the lowest free pages for the
+ * blocks that become full, in the order of the batch; starts[b] = its length before. All or nothing: where that is
+ * impossible nothing changes, every start is -1 and the status word is 501 or 502. */
+int b200q_kv8_extend(const b200q_kv8_cache *cache, const int32_t *slots, const int32_t *offsets, int batch,
+                     int32_t *starts, void *stream);
+/* Keys and values of the new tokens of one layer, after b200q_kv8_extend: rows offsets[b] .. offsets[b + 1] - 1 of k and v
+ * (FP32, FP16 or BF16, kv_heads * head_dim wide, k_row / v_row elements from row to row) are positions starts[b] .. of
+ * slots[b]; at most max_new per sequence. Keys are rotated (rotate-half RoPE, tables [rope_rows][head_dim / 2] FP32 with at
+ * least max_length rows, 16-byte aligned) unless both tables are NULL. A sequence with starts[b] < 0 is skipped. */
+int b200q_kv8_append(const b200q_kv8_cache *cache, int layer, const void *k, const void *v, int in_dtype, int64_t k_row,
+                     int64_t v_row, const int32_t *slots, const int32_t *offsets, const int32_t *starts, int batch,
+                     int max_new, const float *cos_table, const float *sin_table, int rope_rows, void *stream);
+/* Causal attention of the new tokens of one layer over the cache they are in: row r of q (heads * head_dim wide, heads a
+ * multiple of kv_heads, q_row elements from row to row, not rotated yet where tables are given) is the query at position
+ * starts[b] + r - offsets[b] of slots[b] and sees the keys up to its own position. out [rows][heads * head_dim] has the
+ * cache's `dtype`. `rows` = offsets[batch]; max_new: most new tokens of a sequence; max_keys: most tokens a sequence holds
+ * after the step (a bound that the division of the work goes by; max_length is always right). The rows of a sequence with
+ * starts[b] < 0 are NaN. Scores and softmax statistics are FP32. workspace: b200q_kv8_attention_workspace(...) bytes,
+ * 16-byte aligned, used by one call at a time. */
+long long b200q_kv8_attention_workspace(const b200q_kv8_cache *cache, int heads, int batch, int rows, int max_new,
+                                        int max_keys);
+int b200q_kv8_attention(const b200q_kv8_cache *cache, int layer, const void *q, int q_dtype, int64_t q_row, int heads,
+                        const int32_t *slots, const int32_t *offsets, const int32_t *starts, int batch, int rows,
+                        int max_new, int max_keys, const float *cos_table, const float *sin_table, int rope_rows,
+                        float scale, void *out, void *workspace, long long workspace_bytes, void *stream);
+/* Sequence dst[i] (empty) becomes a copy of src[i]: its full pages are shared, the tokens of its tail copied. All or nothing
+ * (status 503). scratch: one int32, used by one call at a time. */
+int b200q_kv8_fork(const b200q_kv8_cache *cache, const int32_t *src, const int32_t *dst, int count, int32_t *scratch,
+                   void *stream);
+/* The sequences become empty; pages without a sequence return to the pool. A slot out of range is skipped (status 503). */
+int b200q_kv8_free(const b200q_kv8_cache *cache, const int32_t *slots, int count, void *stream);
+/* Everything in `from` into `to`, a cache of equal sizes but for its number of pages, with the live pages packed to the front
+ * in their order. All memory of `to` is written but the pages behind the live ones. Too few pages in `to`: status 504, and the
+ * table entries of the pages that have no place are -1. workspace: b200q_kv8_compact_workspace(from, to) bytes. */
+long long b200q_kv8_compact_workspace(const b200q_kv8_cache *from, const b200q_kv8_cache *to);
+int b200q_kv8_compact(const b200q_kv8_cache *from, const b200q_kv8_cache *to, void *workspace, long long workspace_bytes,
+                      void *stream);
+
+/* ---- Matrix product in 8-bit integers (opt-in; changes numerics) ----------------------------------
+ * y[m, n] = (sum over k of x_codes[m, k] * w_codes[n, k]) * x_scales[m] * w_scales[n]: int8 codes with one FP32 scale per
+ * token and per output channel, sums exact in 32-bit integers (k <= 131071), rounded to y_dtype once. Code rows are 16-byte
+ * aligned, their strides multiples of 16 bytes, and the bytes of a row behind k up to the next multiple of 16 are zero in at
+ * least one of the two operands (b200q_int8_quantize writes them as zeros). The whole-row counterpart of b200q_gemv_q8_1's
+ * block scales (mini_llm/ops/mixed_q8_gpu.py:203-251).
+ * b200q_int8_quantize: x[rows, k] (FP32, FP16, BF16; x_row elements from row to row) -> codes [rows][codes_row], scales
+ * [rows]: scale = max |x| / 127 of the row (at least 2^-126), codes = x / scale rounded to nearest, ties to even; a row with
+ * a NaN or an infinity has scale NaN. It serves activations (a row is a token) and weights (a row is an output channel). */
+int b200q_int8_quantize(const void *x, int x_dtype, int rows, int k, int64_t x_row, int8_t *codes, int64_t codes_row,
+                        float *scales, void *stream);
+int b200q_int8_gemm(const int8_t *w_codes, int64_t w_row, const float *w_scales, int n, int k, const int8_t *x_codes,
+                    int64_t x_row, const float *x_scales, int m, void *y, int y_dtype, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

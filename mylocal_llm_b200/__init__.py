@@ -23,6 +23,8 @@ from .grouped_quantized_experts import (grouped_quantized_experts_forward,
                                         supports_grouped_quantized_experts)
 from .moe_layer import PackedMoELayer, RMSNormInference
 from .gguf_index import GGUFPackedIndex, project_gguf_linear, project_gguf_swiglu, resolve_gguf_weight
+from .int8_linear import Int8Weight, int8_linear, int8_matmul, quantize_int8_rows
+from .kv8_cache import KV8Batch, PagedKV8Cache
 
 __all__ = [
     "RouterInference", "expert_topk_forward", "try_normalized_topk", "ExpertsInference", "PackedExpertBank",
@@ -31,5 +33,5 @@ __all__ = [
     "BLOCK_FORMATS", "PackedGGUFWeight", "SUPPORTED_GPU_PACKED_FORMATS", "DevicePackedGGUFWeight",
     "PackedExpertFFNInference", "packed_to_device", "quantized_linear", "quantized_swiglu",
     "supports_packed_gpu_type", "GGUFPackedIndex", "project_gguf_linear", "project_gguf_swiglu",
-    "resolve_gguf_weight",
+    "resolve_gguf_weight", "Int8Weight", "int8_linear", "int8_matmul", "quantize_int8_rows", "KV8Batch", "PagedKV8Cache",
 ]

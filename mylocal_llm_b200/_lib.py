@@ -109,6 +109,31 @@ SIGNATURES = {
                                _c_f32, _ptr, _ptr, _c_int, _ptr],
 }
 
+SIGNATURES.update({
+    "b200q_kv8_extend": [_ptr, _ptr, _ptr, _c_int, _ptr, _ptr],
+    "b200q_kv8_append": [_ptr, _c_int, _ptr, _ptr, _c_int, _c_i64, _c_i64, _ptr, _ptr, _ptr, _c_int, _c_int, _ptr, _ptr, _c_int,
+                         _ptr],
+    "b200q_kv8_attention_workspace": [_ptr, _c_int, _c_int, _c_int, _c_int, _c_int],
+    "b200q_kv8_attention": [_ptr, _c_int, _ptr, _c_int, _c_i64, _c_int, _ptr, _ptr, _ptr, _c_int, _c_int, _c_int, _c_int, _ptr,
+                            _ptr, _c_int, _c_f32, _ptr, _ptr, _c_i64, _ptr],
+    "b200q_kv8_fork": [_ptr, _ptr, _ptr, _c_int, _ptr, _ptr],
+    "b200q_kv8_free": [_ptr, _ptr, _c_int, _ptr],
+    "b200q_kv8_compact_workspace": [_ptr, _ptr],
+    "b200q_kv8_compact": [_ptr, _ptr, _ptr, _c_i64, _ptr],
+    "b200q_int8_quantize": [_ptr, _c_int, _c_int, _c_int, _c_i64, _ptr, _c_i64, _ptr, _ptr],
+    "b200q_int8_gemm": [_ptr, _c_i64, _ptr, _c_int, _c_int, _ptr, _c_i64, _ptr, _c_int, _ptr, _c_int, _ptr],
+})
+_RETURNS_BYTES = ("b200q_moe_decode_stack_workspace", "b200q_gemm_workspace_bytes", "b200q_kv8_attention_workspace",
+                  "b200q_kv8_compact_workspace")
+
+
+class KV8CacheStruct(ctypes.Structure):
+    """``b200q_kv8_cache`` of include/b200q.h."""
+    _fields_ = ([(name, _ptr) for name in ("codes", "scales", "tail", "peak", "table", "lengths", "refs", "free_bits")]
+                + [(name, ctypes.c_int32) for name in ("layers", "kv_heads", "head_dim", "pages", "sequences", "blocks",
+                                                       "max_length", "dtype")])
+
+
 _LOCK = threading.Lock()
 _LIB = None
 
@@ -130,7 +155,7 @@ def load():
         for name, argtypes in SIGNATURES.items():
             fn = getattr(lib, name)
             fn.argtypes = argtypes
-            fn.restype = _c_i64 if name in ("b200q_moe_decode_stack_workspace", "b200q_gemm_workspace_bytes") else _c_int
+            fn.restype = _c_i64 if name in _RETURNS_BYTES else _c_int
         lib.b200q_last_error.argtypes = []
         lib.b200q_last_error.restype = ctypes.c_char_p
         _LIB = lib

@@ -1,0 +1,630 @@
+// Paged 8-bit key/value cache (layout: kv8_cache.cuh): taking pages, appending tokens, sharing, dropping and packing pages.
+#include "kv8_cache.cuh"
+
+namespace b200q {
+
+constexpr int EXTEND_THREADS = 1024;
+
+// Exclusive prefix sum over the CTA (1024 threads); *total gets the sum.
+__device__ __forceinline__ int block_prefix(int v, int *total) {
+    __shared__ int warp_sums[32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int incl = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int up = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += up;
+    }
+    __syncthreads();                                     // (the sums of a previous call have been read)
+    if (lane == 31) warp_sums[warp] = incl;
+    __syncthreads();
+    if (warp == 0) {
+        const int s = lane < blockDim.x / 32 ? warp_sums[lane] : 0;
+        int t = s;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int up = __shfl_up_sync(0xffffffffu, t, o);
+            if (lane >= o) t += up;
+        }
+        warp_sums[lane] = t;
+    }
+    __syncthreads();
+    *total = warp_sums[31];
+    return incl - v + (warp ? warp_sums[warp - 1] : 0);
+}
+
+// Every sequence slots[b] grows by offsets[b + 1] - offsets[b] tokens: it gets a page for each block that becomes full
+// (the lowest free pages, in the order of the requests), starts[b] its length before. All or nothing: without enough pages,
+// or where a sequence would pass max_length, nothing changes, every start is -1 (which the other kernels skip) and the
+// status word tells. One CTA: the work is a prefix sum over the batch and, only when a block becomes full, a pass over the
+// free bits (32 pages per word), so a decode step costs little more than its launch.
+__global__ void __launch_bounds__(EXTEND_THREADS) kv8_extend_kernel(const b200q_kv8_cache c, const int32_t *slots,
+                                                                    const int32_t *offsets, int batch, int32_t *starts,
+                                                                    int *status) {
+    chain_trigger();
+    chain_wait();
+    const int tid = threadIdx.x;
+    int carry = 0, bad = 0;
+    for (int b0 = 0; b0 < batch; b0 += EXTEND_THREADS) {
+        const int b = b0 + tid;
+        int need = 0;
+        if (b < batch) {
+            const int slot = slots[b], add = offsets[b + 1] - offsets[b];
+            if (slot < 0 || slot >= c.sequences || add < 0) {
+                bad = 1;
+            } else {
+                const int have = c.lengths[slot];
+                if (add > c.max_length - have) bad = 1;
+                else need = (have + add) / KV8_BLOCK - have / KV8_BLOCK;
+            }
+        }
+        int sum;
+        const int before = block_prefix(need, &sum);
+        if (b < batch) starts[b] = carry + before;       // first page request of the entry, until the pages are assigned
+        carry += sum;
+    }
+    bad = __syncthreads_or(bad);
+    const int total = carry, words = (c.pages + 31) / 32;
+    if (total > 0 && !bad) {
+        int have = 0;
+        for (int w = tid; w < words; w += EXTEND_THREADS) have += __popc(c.free_bits[w]);
+        int all;
+        block_prefix(have, &all);
+        if (all < total) {
+            if (tid == 0) atomicExch(status, STATUS_KV8_POOL);
+            for (int b = tid; b < batch; b += EXTEND_THREADS) starts[b] = -1;
+            return;
+        }
+        int rank = 0;
+        for (int w0 = 0; w0 < words && rank < total; w0 += EXTEND_THREADS) {
+            const int w = w0 + tid;
+            uint32_t bits = w < words ? c.free_bits[w] : 0u;
+            int sum;
+            int r = rank + block_prefix(__popc(bits), &sum);
+            rank += sum;
+            if (bits == 0u || r >= total) continue;
+            uint32_t left = bits;
+            int e = 0;                                   // entry of request r: the last with starts[e] <= r that needs any
+            for (int lo = 0, hi = batch - 1; lo <= hi;) {
+                const int mid = (lo + hi) >> 1;
+                if (starts[mid] <= r) { e = mid; lo = mid + 1; } else { hi = mid - 1; }
+            }
+            while (left && r < total) {
+                const int bit = __ffs(left) - 1;
+                left &= left - 1;
+                while (e + 1 < batch && starts[e + 1] <= r) ++e;
+                const int page = w * 32 + bit, slot = slots[e];
+                c.table[static_cast<size_t>(slot) * c.blocks + c.lengths[slot] / KV8_BLOCK + (r - starts[e])] = page;
+                c.refs[page] = 1;
+                ++r;
+            }
+            c.free_bits[w] = left;
+        }
+        __syncthreads();
+    }
+    if (bad && tid == 0) atomicExch(status, STATUS_KV8_LENGTH);
+    for (int b = tid; b < batch; b += EXTEND_THREADS) {
+        if (bad) {
+            starts[b] = -1;
+        } else {
+            const int slot = slots[b], have = c.lengths[slot];
+            starts[b] = have;
+            c.lengths[slot] = have + (offsets[b + 1] - offsets[b]);
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------------- append
+struct Kv8Append {
+    const void *k, *v;
+    long long k_row, v_row;
+    int in_dtype, layer;
+    const int32_t *slots, *offsets, *starts;
+    const float *cos_t, *sin_t;           // [rope_rows][head_dim / 2], or NULL: keys are stored as they come
+    int rope_rows;
+};
+
+// Four consecutive values as floats. VEC: base and strides are such that one 8- or 16-byte load fetches them.
+template <bool VEC>
+__device__ __forceinline__ void load4(const void *p, int dtype, size_t i, float (&f)[4]) {
+    if (VEC && dtype == B200Q_F32) {
+        const float4 q = *reinterpret_cast<const float4 *>(static_cast<const float *>(p) + i);
+        f[0] = q.x; f[1] = q.y; f[2] = q.z; f[3] = q.w;
+    } else if (VEC) {
+        const uint2 q = *reinterpret_cast<const uint2 *>(static_cast<const uint16_t *>(p) + i);
+        const uint32_t w[2] = {q.x, q.y};
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            if (dtype == B200Q_BF16) {
+                f[2 * e] = __uint_as_float(w[e] << 16);
+                f[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
+            } else {
+                const float2 h = __half22float2(*reinterpret_cast<const __half2 *>(&w[e]));
+                f[2 * e] = h.x;
+                f[2 * e + 1] = h.y;
+            }
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) f[e] = load_as_float(p, dtype, i + e);
+    }
+}
+
+// A value as the cache's 16-bit type holds it.
+template <bool BF16>
+__device__ __forceinline__ float round16(float v) {
+    return BF16 ? __bfloat162float(__float2bfloat16_rn(v)) : __half2float(__float2half_rn(v));
+}
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack16(float lo, float hi) {
+    if (BF16) {
+        const __nv_bfloat162 p = __floats2bfloat162_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t *>(&p);
+    }
+    const __half2 p = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&p);
+}
+
+// x0 * c - x1 * s and x0 * s + x1 * c, correctly rounded to FP32 (both products are exact in 64 bits): the rounding to the
+// cache's type and the codes then follow from the inputs alone, whatever order another program computes in.
+__device__ __forceinline__ void rotate64(float x0, float x1, float c, float s, float &lo, float &hi) {
+    const double a = x0, b = x1, cc = c, ss = s;
+    lo = __double2float_rn(__fma_rn(a, cc, -__dmul_rn(b, ss)));
+    hi = __double2float_rn(__fma_rn(a, ss, __dmul_rn(b, cc)));
+}
+
+// One CTA of 256 threads = one block of 64 tokens of one sequence and key/value head. A thread holds quads of four
+// consecutive dimensions: of the keys the quad at i and its partner at i + head_dim / 2 (which the rotation needs), of the
+// values two quads, all in registers; 64 * head_dim / 8 / 256 such pairs per thread. A block that becomes full takes its
+// older tokens from the tail, finds the two largest magnitudes, and its codes pass through shared memory (the values
+// transposed) to 16-byte stores; one that does not goes to the tail. Bound by memory: every new token is read once (as
+// projection output) and written once.
+template <int DH, bool BF16, bool VEC>
+__global__ void __launch_bounds__(256) kv8_append_kernel(const b200q_kv8_cache c, const Kv8Append a) {
+    constexpr int HALF = DH / 2, QUADS = HALF / 4, TOKENS = 256 / QUADS, PASSES = KV8_BLOCK / TOKENS;
+    __shared__ __align__(16) uint8_t k_s[KV8_BLOCK * DH];
+    __shared__ __align__(16) uint8_t v_s[KV8_BLOCK * DH];
+    __shared__ uint32_t peaks[2][8];
+    chain_trigger();
+    chain_wait();
+    const int tid = threadIdx.x, b = blockIdx.z, head = blockIdx.y;
+    const int start = a.starts[b], row0 = a.offsets[b], n = a.offsets[b + 1] - row0;
+    if (start < 0 || n <= 0) return;
+    const int total = start + n, first = start / KV8_BLOCK, last = (total - 1) / KV8_BLOCK;
+    int block = first + blockIdx.x;
+    if (block > last) return;
+    const bool opened = start % KV8_BLOCK != 0;          // the first block holds older tokens
+    // The tail is read for the first block and written for the last: where these are two blocks, one CTA does both, in that
+    // order.
+    const bool both = opened && last > first && total % KV8_BLOCK != 0;
+    if (both && block == last) return;
+    const int slot = a.slots[b];
+    const size_t unit_k = kv8_unit(slot, c.layers, a.layer, 0, c.kv_heads, head), unit_v = unit_k + c.kv_heads;
+    uint16_t *tail_k = static_cast<uint16_t *>(c.tail) + unit_k * (KV8_BLOCK * DH);
+    uint16_t *tail_v = static_cast<uint16_t *>(c.tail) + unit_v * (KV8_BLOCK * DH);
+    const int i = (tid % QUADS) * 4, t0 = tid / QUADS;
+
+    for (;; block = last) {
+        const int base = block * KV8_BLOCK;
+        const bool full = base + KV8_BLOCK <= total;
+        float kq[PASSES][2][4], vq[PASSES][2][4];
+        uint32_t kp = 0u, vp = 0u;
+#pragma unroll
+        for (int p = 0; p < PASSES; ++p) {
+            const int t = p * TOKENS + t0, pos = base + t;
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) kq[p][h][e] = vq[p][h][e] = 0.f;
+            if (pos >= start && pos < total) {
+                const long long row = row0 + (pos - start);
+                const size_t at_k = row * a.k_row + static_cast<size_t>(head) * DH + i;
+                const size_t at_v = row * a.v_row + static_cast<size_t>(head) * DH + i;
+                float x[2][4];
+                load4<VEC>(a.k, a.in_dtype, at_k, x[0]);
+                load4<VEC>(a.k, a.in_dtype, at_k + HALF, x[1]);
+                load4<VEC>(a.v, a.in_dtype, at_v, vq[p][0]);
+                load4<VEC>(a.v, a.in_dtype, at_v + HALF, vq[p][1]);
+                if (a.cos_t) {
+                    const float4 cq = *reinterpret_cast<const float4 *>(a.cos_t + static_cast<size_t>(pos) * HALF + i);
+                    const float4 sq = *reinterpret_cast<const float4 *>(a.sin_t + static_cast<size_t>(pos) * HALF + i);
+                    const float cv[4] = {cq.x, cq.y, cq.z, cq.w}, sv[4] = {sq.x, sq.y, sq.z, sq.w};
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) rotate64(x[0][e], x[1][e], cv[e], sv[e], x[0][e], x[1][e]);
+                }
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        kq[p][h][e] = round16<BF16>(x[h][e]);
+                        vq[p][h][e] = round16<BF16>(vq[p][h][e]);
+                    }
+            } else if (full && pos < start) {            // (only the first block has older tokens)
+                const size_t at = static_cast<size_t>(t) * DH + i;
+                load4<true>(tail_k, BF16 ? B200Q_BF16 : B200Q_F16, at, kq[p][0]);
+                load4<true>(tail_k, BF16 ? B200Q_BF16 : B200Q_F16, at + HALF, kq[p][1]);
+                load4<true>(tail_v, BF16 ? B200Q_BF16 : B200Q_F16, at, vq[p][0]);
+                load4<true>(tail_v, BF16 ? B200Q_BF16 : B200Q_F16, at + HALF, vq[p][1]);
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    kp = max(kp, abs_bits(kq[p][h][e]));
+                    vp = max(vp, abs_bits(vq[p][h][e]));
+                }
+        }
+        kp = __reduce_max_sync(0xffffffffu, kp);
+        vp = __reduce_max_sync(0xffffffffu, vp);
+        if ((tid & 31) == 0) {
+            peaks[0][tid >> 5] = kp;
+            peaks[1][tid >> 5] = vp;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < 8; ++w) {
+            kp = max(kp, peaks[0][w]);
+            vp = max(vp, peaks[1][w]);
+        }
+        if (full) {
+            const float ks = int8_scale(kp), vs = int8_scale(vp);
+            const float ki = __fdiv_rn(1.f, ks), vi = __fdiv_rn(1.f, vs);
+#pragma unroll
+            for (int p = 0; p < PASSES; ++p) {
+                const int t = p * TOKENS + t0;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    uint32_t word = 0u;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        word |= (static_cast<uint32_t>(int8_code(kq[p][h][e], ks, ki)) & 0xffu) << (8 * e);
+                        v_s[(i + h * HALF + e) * KV8_BLOCK + t] = static_cast<uint8_t>(int8_code(vq[p][h][e], vs, vi));
+                    }
+                    *reinterpret_cast<uint32_t *>(k_s + t * DH + i + h * HALF) = word;
+                }
+            }
+            __syncthreads();
+            const int page = c.table[static_cast<size_t>(slot) * c.blocks + block];
+            if (page >= 0 && page < c.pages) {           // (a table that lacks the page loses the block, not memory)
+                const size_t u = kv8_unit(page, c.layers, a.layer, 0, c.kv_heads, head);
+                uint4 *kd = reinterpret_cast<uint4 *>(c.codes + u * (KV8_BLOCK * DH));
+                uint4 *vd = reinterpret_cast<uint4 *>(c.codes + (u + c.kv_heads) * (KV8_BLOCK * DH));
+                for (int j = tid; j < KV8_BLOCK * DH / 16; j += 256) {
+                    kd[j] = reinterpret_cast<const uint4 *>(k_s)[j];
+                    vd[j] = reinterpret_cast<const uint4 *>(v_s)[j];
+                }
+                if (tid == 0) {
+                    c.scales[u] = ks;
+                    c.scales[u + c.kv_heads] = vs;
+                }
+            }
+        } else {
+#pragma unroll
+            for (int p = 0; p < PASSES; ++p) {
+                const int t = p * TOKENS + t0, pos = base + t;
+                if (pos < start || pos >= total) continue;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const size_t at = static_cast<size_t>(t) * DH + i + h * HALF;
+                    *reinterpret_cast<uint2 *>(tail_k + at) = make_uint2(pack16<BF16>(kq[p][h][0], kq[p][h][1]),
+                                                                         pack16<BF16>(kq[p][h][2], kq[p][h][3]));
+                    *reinterpret_cast<uint2 *>(tail_v + at) = make_uint2(pack16<BF16>(vq[p][h][0], vq[p][h][1]),
+                                                                         pack16<BF16>(vq[p][h][2], vq[p][h][3]));
+                }
+            }
+            if (tid == 0) {
+                const bool older = block == first && opened;
+                const uint32_t ko = older ? abs_bits(c.peak[unit_k]) : 0u, vo = older ? abs_bits(c.peak[unit_v]) : 0u;
+                c.peak[unit_k] = __uint_as_float(max(kp, ko));
+                c.peak[unit_v] = __uint_as_float(max(vp, vo));
+            }
+        }
+        if (!both || block != first) break;
+        __syncthreads();                                 // every thread has read the tail and the shared peaks
+    }
+}
+
+// --------------------------------------------------------------------------------------------------------- fork, free
+// fork, first kernel (one CTA): the pairs are looked over as a whole. A slot out of range, a target named twice, one that is
+// not empty or that is a source too: nothing happens but status 503. *ok tells the copying kernel.
+__global__ void __launch_bounds__(1024) kv8_fork_check_kernel(const b200q_kv8_cache c, const int32_t *src, const int32_t *dst,
+                                                              int count, int32_t *ok, int *status) {
+    __shared__ uint32_t named[KV8_MAX_SEQUENCES / 32];
+    chain_trigger();
+    chain_wait();
+    const int tid = threadIdx.x;
+    for (int w = tid; w < KV8_MAX_SEQUENCES / 32; w += 1024) named[w] = 0u;
+    __syncthreads();
+    int bad = 0;
+    for (int i = tid; i < count; i += 1024) {
+        const int s = src[i], d = dst[i];
+        if (s < 0 || s >= c.sequences || d < 0 || d >= c.sequences) {
+            bad = 1;
+            continue;
+        }
+        if (atomicOr(&named[d >> 5], 1u << (d & 31)) & (1u << (d & 31))) bad = 1;
+        if (c.lengths[d] != 0) bad = 1;
+    }
+    __syncthreads();
+    if (!bad)
+        for (int i = tid; i < count; i += 1024)
+            if (src[i] >= 0 && src[i] < c.sequences && (named[src[i] >> 5] >> (src[i] & 31) & 1u)) bad = 1;
+    bad = __syncthreads_or(bad);
+    if (tid == 0) {
+        *ok = !bad;
+        if (bad) atomicExch(status, STATUS_KV8_SLOTS);
+    }
+    if (bad) return;
+    for (int i = tid; i < count; i += 1024) c.lengths[dst[i]] = c.lengths[src[i]];
+}
+
+// fork, second kernel: CTA (0, i) copies the table row of pair i and counts its pages, CTA (1 + layer, i) the tokens of the
+// tail of one layer - rows below length % 64 only, as 16-byte pieces.
+__global__ void __launch_bounds__(256) kv8_fork_copy_kernel(const b200q_kv8_cache c, const int32_t *src, const int32_t *dst,
+                                                            const int32_t *ok) {
+    chain_trigger();
+    chain_wait();
+    if (!*ok) return;
+    const int tid = threadIdx.x, s = src[blockIdx.y], d = dst[blockIdx.y], length = c.lengths[s];
+    if (blockIdx.x == 0) {
+        const int held = min(length / KV8_BLOCK, c.blocks);
+        for (int j = tid; j < held; j += 256) {
+            const int page = c.table[static_cast<size_t>(s) * c.blocks + j];
+            c.table[static_cast<size_t>(d) * c.blocks + j] = page;
+            if (page >= 0 && page < c.pages) atomicAdd(c.refs + page, 1);
+        }
+        return;
+    }
+    const int layer = blockIdx.x - 1, units = 2 * c.kv_heads;
+    const size_t from = kv8_unit(s, c.layers, layer, 0, c.kv_heads, 0), to = kv8_unit(d, c.layers, layer, 0, c.kv_heads, 0);
+    const int pieces = (length % KV8_BLOCK) * c.head_dim / 8, unit_pieces = KV8_BLOCK * c.head_dim / 8;
+    const uint4 *tail_from = static_cast<const uint4 *>(c.tail) + from * unit_pieces;
+    uint4 *tail_to = static_cast<uint4 *>(c.tail) + to * unit_pieces;
+    for (int u = tid >> 5; u < units; u += 8)
+        for (int j = tid & 31; j < pieces; j += 32) tail_to[u * unit_pieces + j] = tail_from[u * unit_pieces + j];
+    for (int u = tid; u < units; u += 256) c.peak[to + u] = c.peak[from + u];
+}
+
+// One CTA per slot: the sequence becomes empty, and a page that no sequence refers to any more becomes free. Counts and
+// free bits are the same whatever the order; a slot named twice is freed once.
+__global__ void __launch_bounds__(256) kv8_free_kernel(const b200q_kv8_cache c, const int32_t *slots, int *status) {
+    __shared__ int length;
+    chain_trigger();
+    chain_wait();
+    const int slot = slots[blockIdx.x];
+    if (slot < 0 || slot >= c.sequences) {
+        if (threadIdx.x == 0) atomicExch(status, STATUS_KV8_SLOTS);
+        return;
+    }
+    if (threadIdx.x == 0) length = atomicExch(c.lengths + slot, 0);
+    __syncthreads();
+    const int held = min(length / KV8_BLOCK, c.blocks);
+    for (int j = threadIdx.x; j < held; j += 256) {
+        int32_t *entry = c.table + static_cast<size_t>(slot) * c.blocks + j;
+        const int page = *entry;
+        *entry = -1;
+        if (page >= 0 && page < c.pages && atomicSub(c.refs + page, 1) == 1)
+            atomicOr(c.free_bits + (page >> 5), 1u << (page & 31));
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------------ compact
+// First kernel (one CTA): place[page] = the live page's number in the new pool (live pages keep their order), source[] the
+// reverse, and the new pool's counts and free bits.
+__global__ void __launch_bounds__(1024) kv8_compact_plan_kernel(const b200q_kv8_cache c, const b200q_kv8_cache to,
+                                                                int32_t *place, int32_t *source, int *status) {
+    chain_trigger();
+    chain_wait();
+    const int tid = threadIdx.x;
+    int live = 0;
+    for (int p0 = 0; p0 < c.pages; p0 += 1024) {
+        const int p = p0 + tid;
+        const int refs = p < c.pages ? c.refs[p] : 0;
+        int sum;
+        const int at = live + block_prefix(refs > 0, &sum);
+        if (p < c.pages) place[p] = refs > 0 && at < to.pages ? at : -1;
+        if (refs > 0 && at < to.pages) {
+            source[at] = p;
+            to.refs[at] = refs;
+        }
+        live += sum;
+    }
+    if (live > to.pages && tid == 0) atomicExch(status, STATUS_KV8_COMPACT);
+    for (int p = min(live, to.pages) + tid; p < to.pages; p += 1024) {
+        source[p] = -1;
+        to.refs[p] = 0;
+    }
+    for (int w = tid; w < (to.pages + 31) / 32; w += 1024) {
+        const int lo = max(live - 32 * w, 0), hi = min(to.pages - 32 * w, 32);        // bits lo .. hi - 1 are free
+        uint32_t bits = lo >= 32 ? 0u : 0xffffffffu << lo;
+        if (hi < 32) bits &= (1u << hi) - 1u;
+        to.free_bits[w] = bits;
+    }
+}
+
+// Second kernel: a grid over equal pieces of everything that moves - codes and scales of the live pages, the tails and
+// peaks of all sequences, table and lengths. Pure copying, bound by memory.
+constexpr int COPY_PIECES = 4;               // 16-byte pieces in flight per thread
+__global__ void __launch_bounds__(256) kv8_compact_copy_kernel(const b200q_kv8_cache c, const b200q_kv8_cache to,
+                                                               const int32_t *place, const int32_t *source,
+                                                               int chunks_per_page, int page_ctas, int tail_ctas) {
+    chain_trigger();
+    chain_wait();
+    const int tid = threadIdx.x;
+    const size_t page_pieces = static_cast<size_t>(c.layers) * 2 * c.kv_heads * KV8_BLOCK * c.head_dim / 16;
+    const int page_scales = c.layers * 2 * c.kv_heads;
+    if (static_cast<int>(blockIdx.x) < page_ctas) {
+        const int page = blockIdx.x / chunks_per_page, chunk = blockIdx.x - page * chunks_per_page, from = source[page];
+        if (from < 0) return;
+        const uint4 *in = reinterpret_cast<const uint4 *>(c.codes) + from * page_pieces;
+        uint4 *out = reinterpret_cast<uint4 *>(to.codes) + page * page_pieces;
+        const size_t at = static_cast<size_t>(chunk) * 256 * COPY_PIECES + tid;
+        uint4 v[COPY_PIECES];
+#pragma unroll
+        for (int j = 0; j < COPY_PIECES; ++j)
+            if (at + 256 * j < page_pieces) v[j] = in[at + 256 * j];
+#pragma unroll
+        for (int j = 0; j < COPY_PIECES; ++j)
+            if (at + 256 * j < page_pieces) out[at + 256 * j] = v[j];
+        if (chunk == 0)
+            for (int j = tid; j < page_scales; j += 256)
+                to.scales[static_cast<size_t>(page) * page_scales + j] = c.scales[static_cast<size_t>(from) * page_scales + j];
+        return;
+    }
+    int cta = blockIdx.x - page_ctas;
+    if (cta < tail_ctas) {
+        const size_t pieces = static_cast<size_t>(c.sequences) * page_scales * KV8_BLOCK * c.head_dim / 8;
+        const size_t at = static_cast<size_t>(cta) * 256 * COPY_PIECES + tid;
+        uint4 v[COPY_PIECES];
+#pragma unroll
+        for (int j = 0; j < COPY_PIECES; ++j)
+            if (at + 256 * j < pieces) v[j] = static_cast<const uint4 *>(c.tail)[at + 256 * j];
+#pragma unroll
+        for (int j = 0; j < COPY_PIECES; ++j)
+            if (at + 256 * j < pieces) static_cast<uint4 *>(to.tail)[at + 256 * j] = v[j];
+        return;
+    }
+    cta -= tail_ctas;                                    // the last CTAs: one per sequence
+    for (int j = tid; j < c.blocks; j += 256) {
+        const int page = c.table[static_cast<size_t>(cta) * c.blocks + j];
+        to.table[static_cast<size_t>(cta) * c.blocks + j] = page >= 0 && page < c.pages ? place[page] : -1;
+    }
+    for (int j = tid; j < page_scales; j += 256)
+        to.peak[static_cast<size_t>(cta) * page_scales + j] = c.peak[static_cast<size_t>(cta) * page_scales + j];
+    if (tid == 0) to.lengths[cta] = c.lengths[cta];
+}
+
+// ----------------------------------------------------------------------------------------------------------- host side
+int kv8_check(const char *what, const b200q_kv8_cache *c) {
+    if (!c || !c->codes || !c->scales || !c->tail || !c->peak || !c->table || !c->lengths || !c->refs || !c->free_bits)
+        return fail(B200Q_EINVAL, "%s: NULL pointer", what);
+    if (c->layers < 1 || c->kv_heads < 1 || c->pages < 1 || c->sequences < 1 || c->blocks < 1 || c->max_length < 1)
+        return fail(B200Q_EINVAL, "%s: layers, heads, pages, sequences, blocks and max_length must be positive", what);
+    if (c->head_dim != 64 && c->head_dim != 128) return fail(B200Q_EUNSUPPORTED, "%s: head_dim must be 64 or 128", what);
+    if (c->dtype != B200Q_F16 && c->dtype != B200Q_BF16)
+        return fail(B200Q_EUNSUPPORTED, "%s: the tail is FP16 or BF16", what);
+    if (c->sequences > KV8_MAX_SEQUENCES || c->pages > KV8_MAX_PAGES || c->kv_heads > 1024 || c->layers > 4096)
+        return fail(B200Q_EUNSUPPORTED, "%s: at most %d sequences, %d pages, 1024 heads and 4096 layers", what,
+                    KV8_MAX_SEQUENCES, KV8_MAX_PAGES);
+    if (c->max_length / KV8_BLOCK > c->blocks)
+        return fail(B200Q_EINVAL, "%s: max_length %d needs %d blocks, the table has %d", what, c->max_length,
+                    c->max_length / KV8_BLOCK, c->blocks);
+    if ((reinterpret_cast<uintptr_t>(c->codes) | reinterpret_cast<uintptr_t>(c->tail)) & 15)
+        return fail(B200Q_EINVAL, "%s: codes and tail must be 16-byte aligned", what);
+    return B200Q_OK;
+}
+
+}  // namespace b200q
+
+using namespace b200q;
+
+extern "C" int b200q_kv8_extend(const b200q_kv8_cache *cache, const int32_t *slots, const int32_t *offsets, int batch,
+                                int32_t *starts, void *stream) {
+    if (int rc = kv8_check("kv8_extend", cache)) return rc;
+    if (batch == 0) return B200Q_OK;
+    if (!slots || !offsets || !starts) return fail(B200Q_EINVAL, "kv8_extend: NULL pointer");
+    if (batch < 0 || batch > cache->sequences) return fail(B200Q_EINVAL, "kv8_extend: batch %d out of range", batch);
+    int *status = device_status_word();
+    if (!status) return fail(B200Q_ECUDA, "kv8_extend: no CUDA device");
+    launch_chained(kv8_extend_kernel, dim3(1), dim3(EXTEND_THREADS), 0, static_cast<cudaStream_t>(stream), *cache, slots,
+                   offsets, batch, starts, status);
+    return check_launch("kv8_extend");
+}
+
+extern "C" int b200q_kv8_append(const b200q_kv8_cache *cache, int layer, const void *k, const void *v, int in_dtype,
+                                int64_t k_row, int64_t v_row, const int32_t *slots, const int32_t *offsets,
+                                const int32_t *starts, int batch, int max_new, const float *cos_table,
+                                const float *sin_table, int rope_rows, void *stream) {
+    if (int rc = kv8_check("kv8_append", cache)) return rc;
+    if (batch == 0 || max_new == 0) return B200Q_OK;
+    if (!k || !v || !slots || !offsets || !starts) return fail(B200Q_EINVAL, "kv8_append: NULL pointer");
+    if (layer < 0 || layer >= cache->layers) return fail(B200Q_EINVAL, "kv8_append: layer %d out of range", layer);
+    if (!dtype_valid(in_dtype)) return fail(B200Q_EINVAL, "kv8_append: bad dtype");
+    if (batch < 0 || batch > cache->sequences || max_new < 0 || max_new > cache->max_length)
+        return fail(B200Q_EINVAL, "kv8_append: batch %d, new tokens %d out of range", batch, max_new);
+    const int64_t width = static_cast<int64_t>(cache->kv_heads) * cache->head_dim;
+    if (k_row < width || v_row < width) return fail(B200Q_EINVAL, "kv8_append: row stride below kv_heads * head_dim");
+    if (!cos_table != !sin_table) return fail(B200Q_EINVAL, "kv8_append: one of the two RoPE tables is NULL");
+    if (cos_table && rope_rows < cache->max_length)
+        return fail(B200Q_EINVAL, "kv8_append: RoPE tables of %d rows for sequences of up to %d tokens", rope_rows,
+                    cache->max_length);
+    if ((reinterpret_cast<uintptr_t>(cos_table) | reinterpret_cast<uintptr_t>(sin_table)) & 15)
+        return fail(B200Q_EINVAL, "kv8_append: RoPE tables must be 16-byte aligned");
+    if (batch > 65535) return fail(B200Q_EUNSUPPORTED, "kv8_append: at most 65535 sequences per call");
+    Kv8Append a{};
+    a.k = k; a.v = v; a.k_row = k_row; a.v_row = v_row; a.in_dtype = in_dtype; a.layer = layer;
+    a.slots = slots; a.offsets = offsets; a.starts = starts;
+    a.cos_t = cos_table; a.sin_t = sin_table; a.rope_rows = rope_rows;
+    const size_t quad = 4 * dtype_size(in_dtype);
+    const bool vec = (reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) % quad == 0 && k_row % 4 == 0 && v_row % 4 == 0;
+    const dim3 grid((max_new + 2 * KV8_BLOCK - 2) / KV8_BLOCK, cache->kv_heads, batch);
+    const bool bf16 = cache->dtype == B200Q_BF16;
+    auto kernel = cache->head_dim == 64
+        ? (bf16 ? (vec ? kv8_append_kernel<64, true, true> : kv8_append_kernel<64, true, false>)
+                : (vec ? kv8_append_kernel<64, false, true> : kv8_append_kernel<64, false, false>))
+        : (bf16 ? (vec ? kv8_append_kernel<128, true, true> : kv8_append_kernel<128, true, false>)
+                : (vec ? kv8_append_kernel<128, false, true> : kv8_append_kernel<128, false, false>));
+    launch_chained(kernel, grid, dim3(256), 0, static_cast<cudaStream_t>(stream), *cache, a);
+    return check_launch("kv8_append");
+}
+
+extern "C" int b200q_kv8_fork(const b200q_kv8_cache *cache, const int32_t *src, const int32_t *dst, int count,
+                              int32_t *scratch, void *stream) {
+    if (int rc = kv8_check("kv8_fork", cache)) return rc;
+    if (count == 0) return B200Q_OK;
+    if (!src || !dst || !scratch) return fail(B200Q_EINVAL, "kv8_fork: NULL pointer");
+    if (count < 0 || count > cache->sequences || count > 65535) return fail(B200Q_EINVAL, "kv8_fork: count %d out of range", count);
+    int *status = device_status_word();
+    if (!status) return fail(B200Q_ECUDA, "kv8_fork: no CUDA device");
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    launch_chained(kv8_fork_check_kernel, dim3(1), dim3(1024), 0, s, *cache, src, dst, count, scratch, status);
+    if (int rc = check_launch("kv8_fork")) return rc;
+    launch_chained(kv8_fork_copy_kernel, dim3(1 + cache->layers, count), dim3(256), 0, s, *cache, src, dst,
+                   static_cast<const int32_t *>(scratch));
+    return check_launch("kv8_fork");
+}
+
+extern "C" int b200q_kv8_free(const b200q_kv8_cache *cache, const int32_t *slots, int count, void *stream) {
+    if (int rc = kv8_check("kv8_free", cache)) return rc;
+    if (count == 0) return B200Q_OK;
+    if (!slots) return fail(B200Q_EINVAL, "kv8_free: NULL pointer");
+    if (count < 0 || count > cache->sequences) return fail(B200Q_EINVAL, "kv8_free: count %d out of range", count);
+    int *status = device_status_word();
+    if (!status) return fail(B200Q_ECUDA, "kv8_free: no CUDA device");
+    launch_chained(kv8_free_kernel, dim3(count), dim3(256), 0, static_cast<cudaStream_t>(stream), *cache, slots, status);
+    return check_launch("kv8_free");
+}
+
+extern "C" long long b200q_kv8_compact_workspace(const b200q_kv8_cache *from, const b200q_kv8_cache *to) {
+    if (!from || !to || from->pages < 1 || to->pages < 1) return 0;
+    return 4ll * (static_cast<long long>(from->pages) + to->pages);
+}
+
+extern "C" int b200q_kv8_compact(const b200q_kv8_cache *from, const b200q_kv8_cache *to, void *workspace,
+                                 long long workspace_bytes, void *stream) {
+    if (int rc = kv8_check("kv8_compact", from)) return rc;
+    if (int rc = kv8_check("kv8_compact", to)) return rc;
+    if (from->layers != to->layers || from->kv_heads != to->kv_heads || from->head_dim != to->head_dim ||
+        from->sequences != to->sequences || from->blocks != to->blocks || from->dtype != to->dtype)
+        return fail(B200Q_EINVAL, "kv8_compact: the caches differ in more than their pages");
+    if (from->codes == to->codes || from->tail == to->tail || from->table == to->table)
+        return fail(B200Q_EINVAL, "kv8_compact: the new cache must have memory of its own");
+    if (!workspace || workspace_bytes < b200q_kv8_compact_workspace(from, to))
+        return fail(B200Q_EINVAL, "kv8_compact: workspace too small");
+    int *status = device_status_word();
+    if (!status) return fail(B200Q_ECUDA, "kv8_compact: no CUDA device");
+    int32_t *place = static_cast<int32_t *>(workspace), *source = place + from->pages;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    const long long units = static_cast<long long>(from->layers) * 2 * from->kv_heads;
+    const long long chunk = 256 * COPY_PIECES, page_pieces = units * KV8_BLOCK * from->head_dim / 16;
+    const long long chunks = (page_pieces + chunk - 1) / chunk;
+    const long long tail_ctas = (from->sequences * units * KV8_BLOCK * from->head_dim / 8 + chunk - 1) / chunk;
+    const long long ctas = chunks * to->pages + tail_ctas + from->sequences;
+    if (ctas > 0x7fffffffll) return fail(B200Q_EUNSUPPORTED, "kv8_compact: pool too large");
+    launch_chained(kv8_compact_plan_kernel, dim3(1), dim3(1024), 0, s, *from, *to, place, source, status);
+    if (int rc = check_launch("kv8_compact")) return rc;
+    launch_chained(kv8_compact_copy_kernel, dim3(static_cast<unsigned>(ctas)), dim3(256), 0, s, *from, *to,
+                   static_cast<const int32_t *>(place), static_cast<const int32_t *>(source), static_cast<int>(chunks),
+                   static_cast<int>(chunks * to->pages), static_cast<int>(tail_ctas));
+    return check_launch("kv8_compact");
+}
