@@ -1,20 +1,18 @@
 // Causal attention over the paged 8-bit key/value cache (layout: kv8_cache.cuh).
-#include "kv8_cache.cuh"
+#include "kv8_attention.cuh"
 
 namespace b200q {
 
 int kv8_check(const char *what, const b200q_kv8_cache *c);       // kv8_cache.cu
 
-struct Kv8Attention {
-    const void *q;
-    long long q_row;
-    int q_dtype, layer, heads;
-    const int32_t *slots, *offsets, *starts;
-    int batch, rows;
-    const float *cos_t, *sin_t;
-    float scale;
-    void *out;
-};
+// kv8_decode.cu
+long long kv8_decode_workspace(const b200q_kv8_cache *c, int heads, int batch, int max_new, int max_keys);
+int kv8_decode(const b200q_kv8_cache *c, const Kv8Attention &a, int max_new, int max_keys, void *workspace,
+               long long workspace_bytes, cudaStream_t stream);
+
+// Whether a step goes to the kernel for few tokens per sequence: all rows of a key/value head are one tile of 16, or single
+// tokens.
+static bool few_rows(const b200q_kv8_cache *c, int heads, int max_new) { return max_new == 1 || max_new * (heads / c->kv_heads) <= 16; }
 
 // One CTA = one row of one head: a block of 64 keys at a time, a thread per key for the scores and a thread per dimension
 // for the values, with the running maximum and sum of the softmax.
@@ -103,7 +101,8 @@ using namespace b200q;
 
 extern "C" long long b200q_kv8_attention_workspace(const b200q_kv8_cache *cache, int heads, int batch, int rows, int max_new,
                                                    int max_keys) {
-    return 0;
+    if (!cache || heads < 1 || cache->kv_heads < 1 || heads % cache->kv_heads || max_new < 1) return 0;
+    return few_rows(cache, heads, max_new) ? kv8_decode_workspace(cache, heads, batch, max_new, max_keys) : 0;
 }
 
 extern "C" int b200q_kv8_attention(const b200q_kv8_cache *cache, int layer, const void *q, int q_dtype, int64_t q_row,
@@ -124,11 +123,16 @@ extern "C" int b200q_kv8_attention(const b200q_kv8_cache *cache, int layer, cons
     if (!cos_table != !sin_table) return fail(B200Q_EINVAL, "kv8_attention: one of the two RoPE tables is NULL");
     if (cos_table && rope_rows < cache->max_length)
         return fail(B200Q_EINVAL, "kv8_attention: RoPE tables of %d rows for sequences of up to %d tokens", rope_rows, cache->max_length);
+    if ((reinterpret_cast<uintptr_t>(cos_table) | reinterpret_cast<uintptr_t>(sin_table)) & 15)
+        return fail(B200Q_EINVAL, "kv8_attention: RoPE tables must be 16-byte aligned");
     if (heads > 65535) return fail(B200Q_EUNSUPPORTED, "kv8_attention: too many heads");
     Kv8Attention a{};
     a.q = q; a.q_row = q_row; a.q_dtype = q_dtype; a.layer = layer; a.heads = heads;
     a.slots = slots; a.offsets = offsets; a.starts = starts; a.batch = batch; a.rows = rows;
     a.cos_t = cos_table; a.sin_t = sin_table; a.scale = scale; a.out = out;
+    a.vec = (reinterpret_cast<uintptr_t>(q) & 15) == 0 && q_row * dtype_size(q_dtype) % 16 == 0;
+    if (few_rows(cache, heads, max_new))
+        return kv8_decode(cache, a, max_new, max_keys, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
     launch_chained(cache->head_dim == 64 ? kv8_attention_simple_kernel<64> : kv8_attention_simple_kernel<128>,
                    dim3(rows, heads), dim3(128), 0, static_cast<cudaStream_t>(stream), *cache, a);
     return check_launch("kv8_attention");

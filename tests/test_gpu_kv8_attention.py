@@ -230,6 +230,27 @@ def test_what_is_not_finite_shows_where_it_is_seen(cuda, counts):
     assert torch.equal(out[1:, :2], clean.reshape(sum(counts), 4, 64)[1:, :2])
 
 
+@pytest.mark.parametrize("part", [0, 1])
+@pytest.mark.parametrize("where", ["page", "tail"])
+@pytest.mark.parametrize("count", [4, 60])
+def test_a_block_that_is_not_finite_leaves_the_rows_before_it_alone(cuda, part, where, count):
+    """New tokens on both sides of a block's border: only those behind it see the block."""
+    torch = cuda
+    size = 130 if where == "tail" else 200
+    border = 128
+    cache = random_cache(torch, [size], 1, 1, 64, "bfloat16", 13)
+    counts = [size - border + count // 2]
+    q = query(torch, counts[0], 3 * 64, "float32", 13)
+    clean = cache.attention(0, q, step(cache, [size], counts)).clone()
+    if where == "tail":
+        cache.tail[0, 0, part, 0, 1, 7] = math.inf
+        cache.peak[0, 0, part, 0] = math.inf
+    else:
+        cache.scales[int(cache.table[0, 2]), 0, part, 0] = math.nan
+    out = cache.attention(0, q, step(cache, [size], counts))
+    assert torch.equal(out[:count // 2], clean[:count // 2]) and torch.isnan(out[count // 2:]).all()
+
+
 def test_offsets_beyond_32_bits(cuda):
     """A pool of more than 2^32 bytes whose last pages are the ones in use."""
     torch = cuda
