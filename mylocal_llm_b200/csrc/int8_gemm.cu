@@ -1,5 +1,8 @@
 // Matrix product in 8-bit integers with one scale per token and per output channel, and the quantiser of its operands.
+#include <algorithm>
+
 #include "kv8_cache.cuh"
+#include "umma.cuh"
 
 namespace b200q {
 
@@ -36,10 +39,10 @@ __device__ __forceinline__ void load8(const void *p, int dtype, size_t base, int
 
 template <bool VEC>
 __global__ void __launch_bounds__(256) int8_quantize_kernel(const void *x, int dtype, int k, long long x_row, int8_t *codes,
-                                                            long long codes_row, float *scales) {
+                                                            long long codes_row, float *scales, int early) {
     constexpr int KEEP = 4;
     __shared__ uint32_t peaks[8];
-    chain_trigger();
+    if (early) chain_trigger();
     chain_wait();
     const int tid = threadIdx.x;
     const size_t base = blockIdx.x * static_cast<size_t>(x_row);
@@ -88,44 +91,494 @@ __global__ void __launch_bounds__(256) int8_quantize_kernel(const void *x, int d
     }
 }
 
+// ---------------------------------------------------------------------------------------------
+// The product. Tokens are the M dimension of tcgen05.mma (kind::i8, signed by signed into 32-bit integers), output channels the
+// N dimension; both operands are K-major slabs of 128 codes a row, brought by TMA with the 128-byte swizzle (rows and codes past
+// the end arrive as zeros). One warp issues the loads, one the MMAs, four read the sums back from tensor memory, scale and
+// store them. There are two kernels:
+//   int8_tile_kernel  one tile of 128 tokens x NT channels per CTA. Few tiles (few tokens, few channels): the K range is
+//                     divided among the 2, 4 or 8 CTAs of a cluster, whose integer sums meet in shared memory - exact, so the
+//                     division does not show in the result. Weights that do not depend on the preceding kernel are requested
+//                     before it has ended.
+//   int8_pair_kernel  many tokens: CTAs 2p and 2p + 1 are one tensor-core unit (cta_group::2) and own 256 x 256 tiles, each
+//                     with half of both operands in its shared memory; the pairs walk the tiles in turn, and the sums of a tile
+//                     are stored while the next one is computed (two accumulators fill the tensor memory).
+// With few tokens the weights' bytes bound the product, with many the tensor cores.
+//
+// Every wait is bounded as in umma_gemm.cu: on expiry the status word tells, all roles leave their loops, copies in flight get
+// time to land, the tensor memory is freed and the CTAs return.
+// ---------------------------------------------------------------------------------------------
+constexpr int I8_BM = 128, I8_BK = 128;              // tokens per CTA; codes per slab (one 128-byte swizzle row)
+constexpr int I8_A_BYTES = I8_BM * I8_BK;
+constexpr int I8_THREADS = 6 * 32;                   // TMA, MMA, four epilogue warps
+constexpr int I8_MAX_STAGES = 8;
+constexpr int STATUS_INT8_WAIT_TMA = 121, STATUS_INT8_WAIT_MMA = 122, STATUS_INT8_WAIT_EPILOGUE = 123;
+
 struct Int8Gemm {
-    const int8_t *w, *x;
-    long long w_row, x_row;
     const float *w_scales, *x_scales;
     int n, k, m;
     void *y;
     int y_dtype;
+    int x_rows;               // rows of the activation box (a multiple of 8)
+    int stages, slabs;        // slabs of K
+    int tiles_m, tiles_n;     // int8_pair_kernel
+    int *status;
 };
 
-// A CTA computes 64 tokens x 64 channels with 4-way integer dots; a thread 4 x 4 of them.
-__global__ void __launch_bounds__(256) int8_gemm_simple_kernel(const Int8Gemm a) {
-    __shared__ int x_s[64][17], w_s[64][17];
-    chain_trigger();
-    chain_wait();
-    const int tid = threadIdx.x, m0 = blockIdx.y * 64, n0 = blockIdx.x * 64, tx = tid & 15, ty = tid >> 4;
-    const int padded = (a.k + 15) & ~15;
-    int acc[4][4] = {};
-    for (int k0 = 0; k0 < padded; k0 += 64) {
-        const int r = tid >> 2, c = k0 + 16 * (tid & 3);
-        int4 xv = make_int4(0, 0, 0, 0), wv = xv;
-        if (c < padded && m0 + r < a.m) xv = *reinterpret_cast<const int4 *>(a.x + (m0 + r) * a.x_row + c);
-        if (c < padded && n0 + r < a.n) wv = *reinterpret_cast<const int4 *>(a.w + (n0 + r) * a.w_row + c);
-        __syncthreads();
-        int *xs = &x_s[r][4 * (tid & 3)], *ws = &w_s[r][4 * (tid & 3)];
-        xs[0] = xv.x; xs[1] = xv.y; xs[2] = xv.z; xs[3] = xv.w;
-        ws[0] = wv.x; ws[1] = wv.y; ws[2] = wv.z; ws[3] = wv.w;
-        __syncthreads();
-        for (int i = 0; i < 16; ++i)
-            for (int u = 0; u < 4; ++u)
-                for (int v = 0; v < 4; ++v) acc[u][v] = __dp4a(x_s[ty + 16 * u][i], w_s[tx + 16 * v][i], acc[u][v]);
-    }
-    for (int u = 0; u < 4; ++u)
-        for (int v = 0; v < 4; ++v) {
-            const int m = m0 + ty + 16 * u, n = n0 + tx + 16 * v;
-            if (m < a.m && n < a.n)
-                store_from_float(a.y, a.y_dtype, static_cast<size_t>(m) * a.n + n,
-                                 static_cast<float>(acc[u][v]) * a.x_scales[m] * a.w_scales[n]);
+// Instruction descriptor of kind::i8: 32-bit integer accumulator (bits [4,6) = 2), A and B signed (bits [7,10) and [10,13) = 1),
+// both K-major, N >> 3 in [17,23), M >> 4 in [24,29).
+__host__ __device__ constexpr uint32_t umma_idesc_i8(int m, int n) {
+    return (2u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
+}
+
+template <bool PAIR>
+__device__ __forceinline__ void umma_i8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+    if (PAIR)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+            : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+            : "memory");
+}
+
+// Thirty-two scaled outputs of one token, channels col .. col + 31 of n.
+__device__ __forceinline__ void store_outputs(void *y, int y_dtype, size_t row_base, int col, int n, const float (&v)[32]) {
+    const size_t at = row_base + col;
+    const int esize = y_dtype == B200Q_F32 ? 4 : 2;
+    uint8_t *p = static_cast<uint8_t *>(y) + at * esize;
+    if (col + 32 <= n && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
+        if (y_dtype == B200Q_F32) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) reinterpret_cast<float4 *>(p)[e] = make_float4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
+        } else {
+            uint32_t w[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                if (y_dtype == B200Q_BF16) {
+                    const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * e], v[2 * e + 1]);
+                    w[e] = *reinterpret_cast<const uint32_t *>(&h);
+                } else {
+                    const __half2 h = __floats2half2_rn(v[2 * e], v[2 * e + 1]);
+                    w[e] = *reinterpret_cast<const uint32_t *>(&h);
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) reinterpret_cast<uint4 *>(p)[e] = make_uint4(w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3]);
         }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 32; ++e)
+            if (col + e < n) store_from_float(y, y_dtype, at + e, v[e]);
+    }
+}
+
+__device__ __forceinline__ uint32_t ld_cluster_u32(uint32_t addr) {
+    uint32_t v;
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+    return v;
+}
+
+// grid (channel tiles * SPLIT, token tiles), clusters of SPLIT along x: CTA r of a cluster owns slabs [slabs * r / SPLIT, ...).
+template <int NT, int SPLIT>
+__global__ void __launch_bounds__(I8_THREADS, 1) int8_tile_kernel(const __grid_constant__ CUtensorMap xmap,
+                                                                  const __grid_constant__ CUtensorMap wmap, const Int8Gemm a) {
+    constexpr int STAGE = I8_A_BYTES + NT * I8_BK;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ __align__(8) uint64_t full_bar[I8_MAX_STAGES], free_bar[I8_MAX_STAGES], acc_done;
+    __shared__ uint32_t tmem_base_slot;
+    __shared__ volatile int abort_flag;
+    __shared__ float w_scale[NT];
+    chain_trigger();
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int rank = SPLIT > 1 ? static_cast<int>(cluster_cta_rank()) : 0;
+    const int n0 = (blockIdx.x / SPLIT) * NT, m0 = blockIdx.y * I8_BM, S = a.stages;
+    const int slab0 = a.slabs * rank / SPLIT, nslab = a.slabs * (rank + 1) / SPLIT - slab0;
+    if (tid == 0) {
+        for (int s = 0; s < I8_MAX_STAGES; ++s) {
+            mbar_init(&full_bar[s], 1);
+            mbar_init(&free_bar[s], 1);
+        }
+        mbar_init(&acc_done, 1);
+        abort_flag = 0;
+        fence_barrier_init();
+    }
+    if (warp == 0) {
+        tmem_alloc<false>(&tmem_base_slot, NT);
+        tmem_relinquish<false>();
+    }
+    for (int i = tid; i < NT; i += I8_THREADS) w_scale[i] = n0 + i < a.n ? a.w_scales[n0 + i] : 0.f;
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_d = tmem_base_slot;
+
+    if (warp == 0) {
+        // ---- loads: the first stages' weights do not wait for the preceding kernel, whose result the activations are
+        const uint32_t bytes = static_cast<uint32_t>(a.x_rows * I8_BK + NT * I8_BK);
+        const int early = min(S, nslab);
+        if (elect_one())
+            for (int i = 0; i < early; ++i) {
+                mbar_arrive_expect_tx(&full_bar[i], bytes);
+                tma_load_2d(smem + i * STAGE + I8_A_BYTES, &wmap, (slab0 + i) * I8_BK, n0, &full_bar[i]);
+            }
+        __syncwarp();
+        chain_wait();
+        int issued = early, s = 0, wraps = 0;
+        if (elect_one())
+            for (int i = 0; i < early; ++i) tma_load_2d(smem + i * STAGE, &xmap, (slab0 + i) * I8_BK, m0, &full_bar[i]);
+        __syncwarp();
+        for (int i = early; i < nslab; ++i) {
+            if (__any_sync(0xffffffffu, abort_flag != 0)) break;
+            if (!__all_sync(0xffffffffu, mbar_wait_bounded(&free_bar[s], wraps & 1, a.status, STATUS_INT8_WAIT_MMA))) {
+                abort_flag = 1;
+                break;
+            }
+            if (elect_one()) {
+                mbar_arrive_expect_tx(&full_bar[s], bytes);
+                tma_load_2d(smem + s * STAGE + I8_A_BYTES, &wmap, (slab0 + i) * I8_BK, n0, &full_bar[s]);
+                tma_load_2d(smem + s * STAGE, &xmap, (slab0 + i) * I8_BK, m0, &full_bar[s]);
+            }
+            __syncwarp();
+            ++issued;
+            if (++s == S) {
+                s = 0;
+                ++wraps;
+            }
+        }
+        if (abort_flag) {
+            // copies already requested still write shared memory; they complete on their own within microseconds
+            const uint64_t t0 = global_timer_ns();
+            while (issued > 0 && global_timer_ns() - t0 < 100000) {
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        // ---- MMAs (the whole warp walks the loop, one elected lane issues)
+        constexpr uint32_t idesc = umma_idesc_i8(I8_BM, NT);
+        const uint64_t desc0 = smem_desc_sw128(smem);
+        int done = 0, s = 0, phase = 0;
+        for (int i = 0; i < nslab; ++i) {
+            if (__any_sync(0xffffffffu, abort_flag != 0)) break;
+            if (!__all_sync(0xffffffffu, mbar_wait_bounded(&full_bar[s], phase, a.status, STATUS_INT8_WAIT_TMA))) {
+                abort_flag = 1;
+                break;
+            }
+            tc_fence_after();
+            if (elect_one()) {
+                const uint64_t x_desc = desc0 + static_cast<uint32_t>(s * STAGE >> 4), w_desc = x_desc + (I8_A_BYTES >> 4);
+#pragma unroll
+                for (int q = 0; q < 4; ++q)            // 32 codes = 32 bytes per step: +2 in the address field
+                    umma_i8<false>(tmem_d, x_desc + 2 * q, w_desc + 2 * q, idesc, i + q > 0);
+                umma_commit<false>(smem_u32(&free_bar[s]));
+            }
+            __syncwarp();
+            done = i + 1;
+            if (++s == S) {
+                s = 0;
+                phase ^= 1;
+            }
+        }
+        if (done == nslab && elect_one()) umma_commit<false>(smem_u32(&acc_done));
+        __syncwarp();
+    }
+    // ---- the sums
+    bool ok = !abort_flag;
+    if (ok && !mbar_wait_bounded(&acc_done, 0, a.status, STATUS_INT8_WAIT_MMA)) {
+        abort_flag = 1;
+        ok = false;
+    }
+    ok = __syncthreads_and(ok) != 0;
+    const int quarter = warp & 3, row = 32 * quarter + lane, rows = min(I8_BM, a.m - m0);
+    if constexpr (SPLIT == 1) {
+        if (ok && warp >= 2 && 32 * quarter < rows) {
+            tc_fence_after();
+            chain_wait();                // y may still be read by what precedes this kernel; the scales are its result
+            const float xs = row < rows ? a.x_scales[m0 + row] : 0.f;
+#pragma unroll 1
+            for (int c = 0; c < NT / 32; ++c) {
+                uint32_t r[32];
+                tmem_ld32(tmem_d + (static_cast<uint32_t>(32 * quarter) << 16) + 32 * c, r);
+                tmem_ld_wait();
+                float v[32];
+#pragma unroll
+                for (int e = 0; e < 32; ++e) v[e] = static_cast<float>(static_cast<int>(r[e])) * xs * w_scale[32 * c + e];
+                if (row < rows) store_outputs(a.y, a.y_dtype, static_cast<size_t>(m0 + row) * a.n, n0 + 32 * c, a.n, v);
+            }
+        }
+        tc_fence_before();
+        __syncthreads();
+    } else {
+        // the cluster's partial sums, [row][NT + 1] integers where the stages were
+        constexpr int LD = NT + 1;
+        uint32_t *part = reinterpret_cast<uint32_t *>(smem);
+        if (ok && warp >= 2 && 32 * quarter < rows) {
+            tc_fence_after();
+#pragma unroll 1
+            for (int c = 0; c < NT / 32; ++c) {
+                uint32_t r[32];
+                tmem_ld32(tmem_d + (static_cast<uint32_t>(32 * quarter) << 16) + 32 * c, r);
+                tmem_ld_wait();
+                if (row < rows)
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) part[row * LD + 32 * c + e] = r[e];
+            }
+        }
+        tc_fence_before();
+        cluster_sync_all();
+        if (ok) {
+            chain_wait();
+            const int total = rows * NT, from = total * rank / SPLIT, to = total * (rank + 1) / SPLIT;
+            uint32_t base[SPLIT];
+#pragma unroll
+            for (int q = 0; q < SPLIT; ++q) base[q] = cluster_map(smem_u32(part), q);
+            for (int i = from + tid; i < to; i += I8_THREADS) {
+                const int rr = i / NT, col = i - rr * NT;
+                int sum = 0;
+#pragma unroll
+                for (int q = 0; q < SPLIT; ++q) sum += static_cast<int>(ld_cluster_u32(base[q] + 4u * (rr * LD + col)));
+                if (n0 + col < a.n)
+                    store_from_float(a.y, a.y_dtype, static_cast<size_t>(m0 + rr) * a.n + n0 + col,
+                                     static_cast<float>(sum) * a.x_scales[m0 + rr] * w_scale[col]);
+            }
+        }
+        cluster_sync_all();              // nobody leaves while its sums may still be read
+    }
+    if (warp == 0) tmem_dealloc<false>(tmem_d, NT);
+}
+
+// 256 tokens x 256 channels per pair of CTAs; tiles are numbered in bands of eight token tiles, so that the pairs at work share
+// the weights and activations that L2 holds.
+constexpr int I8_PAIR_STAGE = 2 * I8_A_BYTES;        // 128 rows of each operand
+__device__ __forceinline__ void pair_tile(const Int8Gemm &a, int tile, int &m0, int &n0) {
+    constexpr int BAND = 8;
+    const int per_band = BAND * a.tiles_n, band = tile / per_band, in = tile - band * per_band;
+    const int high = min(BAND, a.tiles_m - band * BAND);
+    const int tn = in / high;
+    m0 = (band * BAND + in - tn * high) * 256;
+    n0 = tn * 256;
+}
+
+__global__ void __launch_bounds__(I8_THREADS, 1) int8_pair_kernel(const __grid_constant__ CUtensorMap xmap,
+                                                                  const __grid_constant__ CUtensorMap wmap, const Int8Gemm a) {
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ __align__(8) uint64_t full_bar[I8_MAX_STAGES], free_bar[I8_MAX_STAGES], acc_full[2], acc_free[2];
+    __shared__ uint32_t tmem_base_slot;
+    __shared__ volatile int abort_flag;
+    __shared__ float w_scale[4][32];
+    chain_trigger();
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, S = a.stages;
+    const uint32_t rank = cluster_cta_rank();
+    const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1, tiles = a.tiles_m * a.tiles_n;
+    if (tid == 0) {
+        for (int s = 0; s < I8_MAX_STAGES; ++s) {
+            mbar_init(&full_bar[s], 1);
+            mbar_init(&free_bar[s], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&acc_full[i], 1);
+            mbar_init(&acc_free[i], 8);              // four epilogue warps of both CTAs
+        }
+        abort_flag = 0;
+        fence_barrier_init();
+    }
+    if (warp == 0) {
+        tmem_alloc<true>(&tmem_base_slot, 512);
+        tmem_relinquish<true>();
+    }
+    tc_fence_before();
+    cluster_sync_all();
+    tc_fence_after();
+    const uint32_t tmem_d = tmem_base_slot;
+
+    if (warp == 0) {
+        chain_wait();
+        const uint32_t full0 = cluster_map(smem_u32(&full_bar[0]), 0);
+        int issued = 0, s = 0, wraps = 0;
+        for (int tile = pair; tile < tiles; tile += pairs) {
+            int m0, n0;
+            pair_tile(a, tile, m0, n0);
+            m0 += 128 * static_cast<int>(rank);
+            n0 += 128 * static_cast<int>(rank);
+            for (int i = 0; i < a.slabs; ++i) {
+                if (__any_sync(0xffffffffu, abort_flag != 0)) break;
+                if (wraps > 0 && !__all_sync(0xffffffffu, mbar_wait_bounded(&free_bar[s], (wraps - 1) & 1, a.status, STATUS_INT8_WAIT_MMA))) {
+                    abort_flag = 1;
+                    break;
+                }
+                if (elect_one()) {
+                    // the first CTA announces the bytes of both; either half may land first
+                    if (rank == 0) mbar_arrive_expect_tx(&full_bar[s], 2 * I8_PAIR_STAGE);
+                    tma_load_2d_pair(smem + s * I8_PAIR_STAGE, &xmap, i * I8_BK, m0, full0 + 8u * s);
+                    tma_load_2d_pair(smem + s * I8_PAIR_STAGE + I8_A_BYTES, &wmap, i * I8_BK, n0, full0 + 8u * s);
+                }
+                __syncwarp();
+                issued = 1;
+                if (++s == S) {
+                    s = 0;
+                    ++wraps;
+                }
+            }
+            if (abort_flag) break;
+        }
+        if (abort_flag) {
+            const uint64_t t0 = global_timer_ns();
+            while (issued > 0 && global_timer_ns() - t0 < 100000) {
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1 && rank == 0) {
+        constexpr uint32_t idesc = umma_idesc_i8(256, 256);
+        const uint32_t free0 = smem_u32(&free_bar[0]), free0_peer = cluster_map(free0, 1);
+        const uint32_t done0 = smem_u32(&acc_full[0]), done0_peer = cluster_map(done0, 1);
+        const uint64_t desc0 = smem_desc_sw128(smem);
+        int s = 0, phase = 0, turn = 0;
+        for (int tile = pair; tile < tiles; tile += pairs, ++turn) {
+            const int acc = turn & 1;
+            bool fine = !__any_sync(0xffffffffu, abort_flag != 0);
+            if (fine && turn >= 2)
+                fine = __all_sync(0xffffffffu, mbar_wait_bounded_cluster(&acc_free[acc], ((turn >> 1) - 1) & 1, a.status, STATUS_INT8_WAIT_EPILOGUE));
+            tc_fence_after();
+            for (int i = 0; fine && i < a.slabs; ++i) {
+                if (__any_sync(0xffffffffu, abort_flag != 0) ||
+                    !__all_sync(0xffffffffu, mbar_wait_bounded_cluster(&full_bar[s], phase, a.status, STATUS_INT8_WAIT_TMA))) {
+                    fine = false;
+                    break;
+                }
+                tc_fence_after();
+                if (elect_one()) {
+                    const uint64_t x_desc = desc0 + static_cast<uint32_t>(s * I8_PAIR_STAGE >> 4), w_desc = x_desc + (I8_A_BYTES >> 4);
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) umma_i8<true>(tmem_d + 256 * acc, x_desc + 2 * q, w_desc + 2 * q, idesc, i + q > 0);
+                    umma_commit<true>(free0 + 8u * s);
+                    umma_commit<true>(free0_peer + 8u * s);
+                }
+                __syncwarp();
+                if (++s == S) {
+                    s = 0;
+                    phase ^= 1;
+                }
+            }
+            if (!fine) {
+                abort_flag = 1;
+                break;
+            }
+            if (elect_one()) {
+                umma_commit<true>(done0 + 8u * acc);
+                umma_commit<true>(done0_peer + 8u * acc);
+            }
+            __syncwarp();
+        }
+    } else if (warp >= 2) {
+        const int quarter = warp & 3;
+        const uint32_t acc_free0 = cluster_map(smem_u32(&acc_free[0]), 0);
+        chain_wait();
+        int turn = 0;
+        for (int tile = pair; tile < tiles; tile += pairs, ++turn) {
+            int m0, n0;
+            pair_tile(a, tile, m0, n0);
+            const int acc = turn & 1, row = m0 + 128 * static_cast<int>(rank) + 32 * quarter + lane;
+            const float xs = row < a.m ? a.x_scales[row] : 0.f;
+            bool fine = !__any_sync(0xffffffffu, abort_flag != 0);
+            if (fine) fine = __all_sync(0xffffffffu, mbar_wait_bounded(&acc_full[acc], (turn >> 1) & 1, a.status, STATUS_INT8_WAIT_MMA));
+            if (!fine) {
+                abort_flag = 1;
+                break;
+            }
+            tc_fence_after();
+#pragma unroll 1
+            for (int c = 0; c < 8; ++c) {
+                const int col = n0 + 32 * c;
+                __syncwarp();
+                w_scale[quarter][lane] = col + lane < a.n ? a.w_scales[col + lane] : 0.f;
+                __syncwarp();
+                uint32_t r[32];
+                tmem_ld32(tmem_d + (static_cast<uint32_t>(32 * quarter) << 16) + 256 * acc + 32 * c, r);
+                tmem_ld_wait();
+                if (c == 7) {                        // the accumulator is read: the next tile but one may have it
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive_cluster(acc_free0 + 8u * acc);
+                }
+                float v[32];
+#pragma unroll
+                for (int e = 0; e < 32; ++e) v[e] = static_cast<float>(static_cast<int>(r[e])) * xs * w_scale[quarter][e];
+                if (row < a.m && col < a.n) store_outputs(a.y, a.y_dtype, static_cast<size_t>(row) * a.n, col, a.n, v);
+            }
+        }
+    }
+    tc_fence_before();
+    cluster_sync_all();                  // both CTAs are done with the pair's barriers, operands and tensor memory
+    if (warp == 0) tmem_dealloc<true>(tmem_d, 512);
+}
+
+// ----------------------------------------------------------------------------------------------------------- host side
+int kv8_shared_memory(const void *kernel, int bytes);        // kv8_decode.cu
+
+// A [rows][row] int8 matrix, read in boxes of 128 codes x box_rows rows; codes from `columns` on read as zeros.
+static int int8_map(CUtensorMap *map, EncodeTiledFn encode, const int8_t *codes, int columns, long long row, int rows, int box_rows) {
+    const cuuint64_t dims[2] = {static_cast<cuuint64_t>(columns), static_cast<cuuint64_t>(rows)};
+    const cuuint64_t strides[1] = {static_cast<cuuint64_t>(row)};
+    const cuuint32_t box[2] = {I8_BK, static_cast<cuuint32_t>(box_rows)}, steps[2] = {1, 1};
+    const CUresult res = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<int8_t *>(codes), dims, strides, box, steps,
+                                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return res == CUDA_SUCCESS ? B200Q_OK : fail(B200Q_ECUDA, "int8_gemm: cuTensorMapEncodeTiled failed (%d)", static_cast<int>(res));
+}
+
+using Int8Fn = void (*)(const CUtensorMap, const CUtensorMap, const Int8Gemm);
+template <int NT>
+static Int8Fn tile_kernel(int split) {
+    return split == 1 ? int8_tile_kernel<NT, 1> : split == 2 ? int8_tile_kernel<NT, 2> : split == 4 ? int8_tile_kernel<NT, 4> : int8_tile_kernel<NT, 8>;
+}
+
+static int int8_gemm(const int8_t *w, long long w_row, const int8_t *x, long long x_row, Int8Gemm a, cudaStream_t stream) {
+    EncodeTiledFn encode = encode_tiled_fn();
+    if (!encode) return fail(B200Q_ECUDA, "int8_gemm: the driver does not provide cuTensorMapEncodeTiled");
+    a.status = device_status_word();
+    if (!a.status) return fail(B200Q_ECUDA, "int8_gemm: no CUDA device");
+    const int sms = sm_count(), columns = (a.k + 15) & ~15;
+    a.slabs = (a.k + I8_BK - 1) / I8_BK;
+    CUtensorMap xmap, wmap;
+    a.tiles_m = (a.m + 255) / 256;
+    a.tiles_n = (a.n + 255) / 256;
+    const long long big = static_cast<long long>(a.tiles_m) * a.tiles_n;
+    if (2 * big >= sms) {
+        if (big > 0x3fffffff) return fail(B200Q_EUNSUPPORTED, "int8_gemm: too many tiles");
+        if (int rc = int8_map(&xmap, encode, x, columns, x_row, a.m, 128)) return rc;
+        if (int rc = int8_map(&wmap, encode, w, columns, w_row, a.n, 128)) return rc;
+        a.stages = 6;
+        const int smem = a.stages * I8_PAIR_STAGE + 1024, pairs = static_cast<int>(std::min<long long>(big, sms / 2));
+        if (int rc = kv8_shared_memory(reinterpret_cast<const void *>(int8_pair_kernel), smem)) return rc;
+        launch_chained_cluster(int8_pair_kernel, dim3(2 * pairs), dim3(I8_THREADS), smem, stream, 2, xmap, wmap, a);
+        return check_launch("int8_gemm");
+    }
+    const int token_tiles = (a.m + I8_BM - 1) / I8_BM;
+    int nt = 128;
+    if (static_cast<long long>((a.n + 127) / 128) * token_tiles * 2 <= sms) nt = 64;
+    const int tiles_n = (a.n + nt - 1) / nt;
+    const long long tiles = static_cast<long long>(tiles_n) * token_tiles;
+    int split = 1;
+    while (split < 8 && tiles * split * 2 <= sms && a.slabs >= split * 4) split *= 2;
+    a.x_rows = a.m < I8_BM ? (a.m + 7) / 8 * 8 : I8_BM;
+    const int stage = I8_A_BYTES + nt * I8_BK;
+    a.stages = std::min(I8_MAX_STAGES, 200 * 1024 / stage);
+    if (int rc = int8_map(&xmap, encode, x, columns, x_row, a.m, a.x_rows)) return rc;
+    if (int rc = int8_map(&wmap, encode, w, columns, w_row, a.n, nt)) return rc;
+    const Int8Fn fn = nt == 64 ? tile_kernel<64>(split) : tile_kernel<128>(split);
+    const int smem = a.stages * stage + 1024;
+    if (int rc = kv8_shared_memory(reinterpret_cast<const void *>(fn), 200 * 1024 + 1024)) return rc;
+    const dim3 grid(tiles_n * split, token_tiles);
+    if (split > 1) launch_chained_cluster(fn, grid, dim3(I8_THREADS), smem, stream, split, xmap, wmap, a);
+    else launch_chained(fn, grid, dim3(I8_THREADS), smem, stream, xmap, wmap, a);
+    return check_launch("int8_gemm");
 }
 
 }  // namespace b200q
@@ -133,7 +586,7 @@ __global__ void __launch_bounds__(256) int8_gemm_simple_kernel(const Int8Gemm a)
 using namespace b200q;
 
 extern "C" int b200q_int8_quantize(const void *x, int x_dtype, int rows, int k, int64_t x_row, int8_t *codes,
-                                   int64_t codes_row, float *scales, void *stream) {
+                                   int64_t codes_row, float *scales, int early, void *stream) {
     if (rows == 0) return B200Q_OK;
     if (!x || !codes || !scales) return fail(B200Q_EINVAL, "int8_quantize: NULL pointer");
     if (!dtype_valid(x_dtype)) return fail(B200Q_EINVAL, "int8_quantize: bad dtype");
@@ -144,7 +597,7 @@ extern "C" int b200q_int8_quantize(const void *x, int x_dtype, int rows, int k, 
     const bool vec = (reinterpret_cast<uintptr_t>(x) & 15) == 0 && x_row * e % 16 == 0;
     launch_chained(vec ? int8_quantize_kernel<true> : int8_quantize_kernel<false>, dim3(rows), dim3(256), 0,
                    static_cast<cudaStream_t>(stream), x, x_dtype, k, static_cast<long long>(x_row), codes,
-                   static_cast<long long>(codes_row), scales);
+                   static_cast<long long>(codes_row), scales, early);
     return check_launch("int8_quantize");
 }
 
@@ -160,9 +613,6 @@ extern "C" int b200q_int8_gemm(const int8_t *w_codes, int64_t w_row, const float
         ((reinterpret_cast<uintptr_t>(w_codes) | reinterpret_cast<uintptr_t>(x_codes)) & 15))
         return fail(B200Q_EINVAL, "int8_gemm: code rows must be 16-byte aligned and at least k long");
     Int8Gemm a{};
-    a.w = w_codes; a.x = x_codes; a.w_row = w_row; a.x_row = x_row; a.w_scales = w_scales; a.x_scales = x_scales;
-    a.n = n; a.k = k; a.m = m; a.y = y; a.y_dtype = y_dtype;
-    launch_chained(int8_gemm_simple_kernel, dim3((n + 63) / 64, (m + 63) / 64), dim3(256), 0,
-                   static_cast<cudaStream_t>(stream), a);
-    return check_launch("int8_gemm");
+    a.w_scales = w_scales; a.x_scales = x_scales; a.n = n; a.k = k; a.m = m; a.y = y; a.y_dtype = y_dtype;
+    return int8_gemm(w_codes, w_row, x_codes, x_row, a, static_cast<cudaStream_t>(stream));
 }

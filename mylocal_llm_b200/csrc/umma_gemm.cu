@@ -40,15 +40,13 @@
 // Every mbarrier wait is bounded (2 s): on expiry the waiting thread records a status code and
 // raises the CTA's abort flag; every role then leaves its loop, the copies in flight are waited for
 // (bounded), the tensor memory is freed and the CTA returns.
-#include <cuda.h>
-
 #include <algorithm>
 #include <cstdlib>
 #include <mutex>
 #include <utility>
 #include <vector>
 
-#include "common.cuh"
+#include "umma.cuh"
 
 namespace b200q {
 
@@ -71,168 +69,6 @@ struct UmmaGemmArgs {
     int groups_per_split;     // 256-position groups of K per CTA along grid.z (split-K); k / 256 without a split
     float *partial;           // split-K: FP32 partial results [grid.z][m][n], summed by splitk_reduce_kernel
 };
-
-// ---------------------------------------------------------------------------------------------
-// tcgen05 / TMA wrappers (sm_100a)
-// ---------------------------------------------------------------------------------------------
-// PAIR: the two CTAs of a cluster work as one tensor-core unit (cta_group::2). Tensor memory is then allocated
-// and freed by the same warp of both CTAs, with the same shared-memory slot for the address.
-template <bool PAIR>
-__device__ __forceinline__ void tmem_alloc(uint32_t *dst_smem, uint32_t cols) {
-    if (PAIR)
-        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(dst_smem)),
-                     "r"(cols)
-                     : "memory");
-    else
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(dst_smem)),
-                     "r"(cols)
-                     : "memory");
-}
-template <bool PAIR>
-__device__ __forceinline__ void tmem_relinquish() {
-    if (PAIR) asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
-    else asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-}
-template <bool PAIR>
-__device__ __forceinline__ void tmem_dealloc(uint32_t taddr, uint32_t cols) {
-    if (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(cols) : "memory");
-    else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(cols) : "memory");
-}
-
-// True in exactly one lane of a converged warp. The warps that issue MMAs and TMA loads run their loops with all 32
-// lanes and elect the issuer per instruction group: a loop kept inside an `if (lane == 0)` branch is divergent code
-// to the compiler, which then feeds every tensor-core / TMA instruction (they take their operands from the warp-wide
-// uniform registers) through per-thread registers - the issuing lane spent ~0.55 us per slab that way, whatever
-// the tile size.
-__device__ __forceinline__ bool elect_one() {
-    uint32_t pred;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "elect.sync _|p, 0xffffffff;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(pred));
-    return pred != 0;
-}
-
-// Cluster helpers for the paired kernel.
-__device__ __forceinline__ uint32_t cluster_cta_rank() {
-    uint32_t r;
-    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-    return r;
-}
-// Every thread of both CTAs; orders shared-memory and barrier initialisation across the pair.
-__device__ __forceinline__ void cluster_sync_all() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-// The shared::cluster address of this CTA's shared-memory address `addr` as seen in CTA `rank` of the cluster.
-__device__ __forceinline__ uint32_t cluster_map(uint32_t addr, uint32_t rank) {
-    uint32_t r;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
-    return r;
-}
-__device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
-    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
-}
-// Waits of the MMA-issuing lane of a pair: the arrivals come from both CTAs.
-__device__ __forceinline__ bool mbar_try_wait_cluster(uint64_t *bar, uint32_t parity) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(smem_u32(bar)), "r"(parity)
-        : "memory");
-    return ok != 0;
-}
-__device__ __forceinline__ bool mbar_wait_bounded_cluster(uint64_t *bar, uint32_t parity, int *status, int code) {
-    if (mbar_try_wait_cluster(bar, parity)) return true;
-    const uint64_t t0 = global_timer_ns();
-    for (;;) {
-#pragma unroll 1
-        for (int i = 0; i < 64; ++i)
-            if (mbar_try_wait_cluster(bar, parity)) return true;
-        if (global_timer_ns() - t0 > WAIT_LIMIT_NS) {
-            atomicExch(status, code);
-            return false;
-        }
-    }
-}
-__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-
-// D[tmem] (+)= A[smem desc] * B[smem desc]; `accumulate` = 0 overwrites D.
-// In a pair (issued by the first CTA only) D is [256 x N]: each CTA's tensor memory holds the 128 rows of its own A
-// operand; the N rows of B come half from each CTA's shared memory, at the same offsets.
-template <bool PAIR>
-__device__ __forceinline__ void umma_bf16(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
-                                          uint32_t accumulate) {
-    if (PAIR)
-        asm volatile(
-            "{\n\t.reg .pred p;\n\t"
-            "setp.ne.b32 p, %4, 0;\n\t"
-            "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-            ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
-            : "memory");
-    else
-        asm volatile(
-            "{\n\t.reg .pred p;\n\t"
-            "setp.ne.b32 p, %4, 0;\n\t"
-            "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-            ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
-            : "memory");
-}
-// The mbarrier (a shared::cluster address: this CTA's or, in a pair, the partner's) receives one arrival when every
-// tcgen05.mma issued so far by this thread has completed.
-template <bool PAIR>
-__device__ __forceinline__ void umma_commit(uint32_t bar_addr) {
-    if (PAIR)
-        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar_addr)
-                     : "memory");
-    else
-        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar_addr)
-                     : "memory");
-}
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
-          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-        : "r"(taddr)
-        : "memory");
-}
-__device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-
-// 2-D tiled TMA load into this CTA's shared memory (no cluster, no multicast); coordinates in
-// elements: x = innermost (k), y = row. x * 2 bytes is a multiple of 128 here.
-__device__ __forceinline__ void tma_load_2d(void *dst_smem, const CUtensorMap *map, int x, int y, uint64_t *bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
-        ::"r"(smem_u32(dst_smem)), "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y)
-        : "memory");
-}
-
-// The same load issued by a CTA of a pair: the completion bytes go to the mbarrier at `bar_addr`, a shared::cluster
-// address that may lie in the partner CTA (the one that issues the MMAs); the data lands in this CTA.
-__device__ __forceinline__ void tma_load_2d_pair(void *dst_smem, const CUtensorMap *map, int x, int y, uint32_t bar_addr) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
-        ::"r"(smem_u32(dst_smem)), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar_addr), "r"(x), "r"(y)
-        : "memory");
-}
-
-// Shared-memory matrix descriptor of a K-major operand tile stored as rows of 128 bytes (64 BF16)
-// with the 128-byte swizzle, groups of eight rows 1024 bytes apart: start address >> 4 in bits
-// [0,14), leading byte offset (unused for swizzled K-major, 1) in [16,30), stride byte offset
-// 1024 >> 4 in [32,46), descriptor version 1 in [46,48), layout type 2 (128-byte swizzle) in [61,64).
-__device__ __forceinline__ uint64_t smem_desc_sw128(const void *tile) {
-    const uint64_t addr = (smem_u32(tile) & 0x3ffffu) >> 4;
-    return addr | (1ull << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
-}
 
 // Instruction descriptor of kind::f16: FP32 accumulator (bits [4,6) = 1), A and B BF16 (bits [7,10)
 // and [10,13) = 1), both K-major (bits 15, 16 = 0), N >> 3 in [17,23), M >> 4 in [24,29).
@@ -816,25 +652,6 @@ __global__ void __launch_bounds__(UG_THREADS, 1) umma_gemm_kernel(const __grid_c
 // ---------------------------------------------------------------------------------------------
 // Host side
 // ---------------------------------------------------------------------------------------------
-using EncodeTiledFn = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
-                                   const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
-                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-static EncodeTiledFn encode_tiled_fn() {
-    static std::once_flag once;
-    static EncodeTiledFn fn = nullptr;
-    std::call_once(once, [] {
-        void *p = nullptr;
-        cudaDriverEntryPointQueryResult res;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &res) == cudaSuccess &&
-            res == cudaDriverEntryPointSuccess)
-            fn = reinterpret_cast<EncodeTiledFn>(p);
-        else
-            cudaGetLastError();
-    });
-    return fn;
-}
-
 using GemmFn = void (*)(const CUtensorMap, const UmmaGemmArgs);
 
 template <bool SPLIT, bool PAIR>

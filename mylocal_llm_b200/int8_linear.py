@@ -25,6 +25,10 @@ def quantize_int8_rows(x):
     """``x`` ``[..., K]`` (FP32 / FP16 / BF16 CUDA tensor) -> (int8 codes ``[rows, K']``, FP32 scales ``[rows]``): scale = max |x| /
     127 of the row (at least 2^-126), codes = x / scale to the nearest integer, ties to even; K' is K rounded up to a multiple of
     16 and the codes behind K are zero. A row with a NaN or an infinity has the scale NaN."""
+    return _quantize(x, 0)
+
+
+def _quantize(x, early):
     torch = _torch()
     if not isinstance(x, torch.Tensor) or not x.is_cuda:
         raise TypeError("quantize_int8_rows expects a torch CUDA tensor")
@@ -42,7 +46,7 @@ def quantize_int8_rows(x):
     codes = torch.empty((rows, padded), dtype=torch.int8, device=x.device)
     scales = torch.empty(rows, dtype=torch.float32, device=x.device)
     if rows:
-        _launch(x.device, "b200q_int8_quantize", x.data_ptr(), ident, rows, k, x_row, codes.data_ptr(), padded, scales.data_ptr())
+        _launch(x.device, "b200q_int8_quantize", x.data_ptr(), ident, rows, k, x_row, codes.data_ptr(), padded, scales.data_ptr(), early)
     return codes, scales
 
 
@@ -124,6 +128,6 @@ def int8_linear(x, weight, *, out_dtype=None):
         raise TypeError("Expected an Int8Weight")
     if x.shape[-1] != weight.shape[1]:
         raise ValueError(f"Input K={x.shape[-1]} does not match weight K={weight.shape[1]}")
-    codes, scales = quantize_int8_rows(x)
+    codes, scales = _quantize(x, 1)
     y = int8_matmul(codes, scales, weight, out_dtype=out_dtype or x.dtype)
     return y.reshape(x.shape[:-1] + (weight.shape[0],))

@@ -85,7 +85,7 @@ def test_page_operations_refuse():
     (dict(x=None), 1), (dict(dtype=4), 1), (dict(k=0), 1), (dict(x_row=99), 1), (dict(codes_row=104), 1), (dict(codes_row=96), 1),
     (dict(codes=ONE + 4), 1), (dict(rows=-1), 1)])
 def test_int8_quantize_refuses(change, code):
-    a = dict(x=ONE, dtype=0, rows=3, k=100, x_row=100, codes=ONE, codes_row=112, scales=ONE)
+    a = dict(x=ONE, dtype=0, rows=3, k=100, x_row=100, codes=ONE, codes_row=112, scales=ONE, early=0)
     a.update(change)
     assert rc("b200q_int8_quantize", *a.values(), None) == code
 
