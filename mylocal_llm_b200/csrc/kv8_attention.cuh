@@ -89,6 +89,27 @@ __device__ __forceinline__ uint32_t tail_to_half(uint32_t w, float inv) {
     return pack_half(lo * inv, hi * inv);
 }
 
+// Four consecutive values as floats.
+__device__ __forceinline__ void load4f(const void *p, int dtype, size_t i, bool vec, float (&f)[4]) {
+    if (vec && dtype == B200Q_F32) {
+        const float4 q = *reinterpret_cast<const float4 *>(static_cast<const float *>(p) + i);
+        f[0] = q.x; f[1] = q.y; f[2] = q.z; f[3] = q.w;
+    } else if (vec) {
+        const uint2 q = *reinterpret_cast<const uint2 *>(static_cast<const uint16_t *>(p) + i);
+        const uint32_t w[2] = {q.x, q.y};
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const float2 v = dtype == B200Q_BF16 ? make_float2(__uint_as_float(w[e] << 16), __uint_as_float(w[e] & 0xffff0000u))
+                                                 : __half22float2(*reinterpret_cast<const __half2 *>(&w[e]));
+            f[2 * e] = v.x;
+            f[2 * e + 1] = v.y;
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) f[e] = load_as_float(p, dtype, i + e);
+    }
+}
+
 // Sixteen consecutive values as floats; `vec`: base and strides are such that 16-byte loads can fetch them.
 __device__ __forceinline__ void load16f(const void *p, int dtype, size_t i, bool vec, float (&f)[16]) {
     if (vec && dtype == B200Q_F32) {

@@ -2,20 +2,23 @@
 // tensor cores.
 //
 // One CTA owns 256 rows of one key/value head of one sequence (row = token * group + head of the group: the heads that share keys
-// are neighbours) as two tiles of 128, and walks the blocks of 64 keys that its last row sees, or a part of them. Warps have
-// roles that meet at mbarriers:
+// are neighbours) as two tiles of 128, and walks the units of 128 keys (two pages) that its last row sees, or a part of them.
+// Warps have roles that meet at mbarriers:
 //   loader      one bulk copy each for the keys and the values of a page (int8, contiguous) into a ring
-//   converters  (4 warps) codes -> FP16, exact, into the 128-byte-swizzled K-major operands: the keys as [64][head_dim], the
-//               values, which a page holds transposed, as [head_dim][64]; the 16-bit tail of a sequence goes the same way
+//   converters  (4 warps) codes -> FP16, exact, into the 128-byte-swizzled K-major operands: the keys as [128][head_dim], the
+//               values, which a page holds transposed, as [head_dim][64] twice; the 16-bit tail of a sequence goes the same way
 //   MMA         scores S = Q K^T (FP32, tensor memory) of one tile while the other tile's softmax runs, then O += P V with the
-//               softmax weights P read from tensor memory
+//               softmax weights P read from tensor memory, where they replace the second half of their scores
 //   softmax     (2 x 4 warps) a thread per row: maximum, weights, sum; the weights go back to tensor memory as FP16, times the
-//               block's value scale relative to a power of two U that follows the largest scale seen. A row's reference maximum
+//               block's value scale relative to a power of two U that follows the largest scale seen (as an addend of the
+//               exponent, which costs nothing; the sum is divided by it). A row's reference maximum
 //               moves only when it is passed by 2^8, so O is rescaled rarely (FP16 has the room for weights up to 2^8).
-// With a head dimension of 128 the tensor cores and the 16 exponentials per clock of an SM take about the same time, with 64
-// the exponentials take twice as long. Queries are rounded to FP16 (a power of two per row keeps them in range); where the
-// result is FP16 too the rounding would show next to the result's own, and a second product with the remainders (SPLIT) removes
-// it. Weights are rounded to FP16. Block scales below 2^-14 of the largest lose bits of their share accordingly.
+// 128 keys per step because an MMA of 128 rows x 64 keys reads 6 KB of operands for 32 clocks of work, more than shared memory
+// gives: with units of 64 keys the MMAs took 3200 of 3900 clocks per 64 keys (head dimension 128, SPLIT). With a head dimension
+// of 128 the tensor cores and the 16 exponentials per clock of an SM take about the same time, with 64 the exponentials take
+// twice as long. Queries are rounded to FP16 (a power of two per row keeps them in range); where the result is FP16 too the
+// rounding would show next to the result's own, and a second product with the remainders (SPLIT) removes it. Weights are rounded
+// to FP16. Block scales below 2^-14 of the largest lose bits of their share accordingly.
 //
 // Every wait is bounded: on expiry the status word tells, all roles leave, and the CTA ends.
 #include <algorithm>
@@ -28,12 +31,17 @@ namespace b200q {
 constexpr int STATUS_KV8_PROMPT = 512;       // gave up waiting at a barrier of the prompt kernel
 constexpr int KP_ROWS = 128, KP_CTA_ROWS = 256;
 constexpr int KP_SOFTMAX_WARPS = 8, KP_CONVERT_WARPS = 4;
-constexpr int KP_THREADS = (KP_SOFTMAX_WARPS + KP_CONVERT_WARPS + 2) * 32;
+constexpr int KP_THREADS = 512;              // and loader, MMA and two warps that only help with the queries
+// Registers per thread: a softmax thread holds its row's 128 scores. 256 x 176 + 256 x 80 = 512 x 128, what the launch has.
+constexpr int KP_SOFTMAX_REGS = 176, KP_OTHER_REGS = 80;
 
+constexpr int KP_KEYS = 2 * KV8_BLOCK;       // keys of a unit
+
+// Operand stages of keys and values (of a unit each) and half pages of codes in the ring, by what shared memory holds.
 template <int DH, bool SPLIT> struct PromptShape {
-    static constexpr int STAGES = DH == 64 ? 4 : SPLIT ? 2 : 3;          // operand stages, and as many pages of codes
-    static constexpr int Q = 2 * KP_ROWS * DH * 2, K = KV8_BLOCK * DH * 2, RAW = 2 * KV8_BLOCK * DH;
-    static constexpr int BYTES = (SPLIT ? 2 : 1) * Q + STAGES * (2 * K + RAW);
+    static constexpr int KS = DH == 128 && SPLIT ? 1 : 2, VS = DH == 128 ? 1 : 2, RING = DH == 128 && SPLIT ? 4 : 8;
+    static constexpr int Q = 2 * KP_ROWS * DH * 2, K = KP_KEYS * DH * 2, RAW = KV8_BLOCK * DH;
+    static constexpr int BYTES = (SPLIT ? 2 : 1) * Q + (KS + VS) * K + RING * RAW;
 };
 
 struct Kv8Prompt {
@@ -65,7 +73,52 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32
         "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr)
         : "memory");
 }
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};" ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]),
+        "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
+        "r"(taddr)
+        : "memory");
+}
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Pairs of FP32 numbers in one 64-bit register.
+__device__ __forceinline__ uint64_t pack2(float lo, float hi) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t x, float &lo, float &hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(x)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t x, uint64_t y, uint64_t z) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(x), "l"(y), "l"(z));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t x, uint64_t y) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
+    return r;
+}
+__device__ __forceinline__ float max3(float x, float y, float z) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
+    return r;
+}
+__device__ __forceinline__ float log2_approx(float x) {
+    float y;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 
 // Byte offset of 16-byte chunk c (eight FP16 values) of a row in a swizzled operand of 128-byte rows.
 __device__ __forceinline__ uint32_t swizzled(int row, int chunk) { return row * 128 + ((chunk ^ (row & 7)) << 4); }
@@ -84,12 +137,14 @@ __device__ __forceinline__ void convert16(const uint4 &w, uint8_t *operand, int 
 template <int DH, bool BF16, bool SPLIT>
 __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prompt_kernel(const b200q_kv8_cache c, const Kv8Prompt p) {
     using Shape = PromptShape<DH, SPLIT>;
-    constexpr int ST = Shape::STAGES, SLABS = DH / 64, HALF_PAGE = KV8_BLOCK * DH;
+    constexpr int KS = Shape::KS, VS = Shape::VS, RING = Shape::RING, SLABS = DH / 64, HALF_PAGE = KV8_BLOCK * DH;
+    constexpr int K_SLAB = KP_KEYS * 128, V_PAGE = DH * 128;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ __align__(8) uint64_t raw_full[ST], raw_free[ST], k_full[ST], k_free[ST], v_full[ST], v_free[ST], s_full[2], p_full[2],
-        o_done[2], q_full;
+    __shared__ __align__(8) uint64_t raw_full[RING], raw_free[RING], k_full[KS], k_free[KS], v_full[VS], v_free[VS], s_full[2],
+        p_full[2], o_done[2], q_full;
     __shared__ uint32_t tmem_base_slot;
     __shared__ volatile int abort_flag;
+    __shared__ float factor_s[KP_CTA_ROWS];
     const Kv8Attention &a = p.a;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     chain_trigger();
@@ -107,23 +162,27 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prompt_kernel(const b200q_k
             }
         return;
     }
-    // units (blocks of keys) of both tiles: all that the tile's last row sees; this CTA's part of the longer one
-    auto units_to = [&](int end_row) { return (start + (min(end_row, rows) - 1) / p.group) / KV8_BLOCK + 1; };
+    // units of both tiles: all that the tile's last row sees; this CTA's part of the longer one
+    auto units_to = [&](int end_row) { return (start + (min(end_row, rows) - 1) / p.group) / KP_KEYS + 1; };
     const int all = units_to(row0 + KP_CTA_ROWS), u0 = static_cast<int>(static_cast<long long>(all) * part / p.splits);
     const int u1 = static_cast<int>(static_cast<long long>(all) * (part + 1) / p.splits);
     if (u0 >= u1) return;                        // (the joining kernel knows)
     const int count1 = row0 + KP_ROWS < rows ? u1 - u0 : 0;
     const int count0 = max(0, min(units_to(row0 + KP_ROWS), u1) - u0), count = max(count0, count1);
-    const int full_units = total / KV8_BLOCK;    // units from here on are the tail
+    const int full_pages = total / KV8_BLOCK;    // the block after them is the tail, what follows does not exist
 
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint8_t *q_s = smem, *k_s = smem + (SPLIT ? 2 : 1) * Shape::Q, *v_s = k_s + ST * Shape::K, *raw_s = v_s + ST * Shape::K;
+    uint8_t *q_s = smem, *k_s = smem + (SPLIT ? 2 : 1) * Shape::Q, *v_s = k_s + KS * Shape::K, *raw_s = v_s + VS * Shape::K;
     if (tid == 0) {
-        for (int s = 0; s < ST; ++s) {
+        for (int s = 0; s < RING; ++s) {
             mbar_init(&raw_full[s], 1);
             mbar_init(&raw_free[s], KP_CONVERT_WARPS);
+        }
+        for (int s = 0; s < KS; ++s) {
             mbar_init(&k_full[s], KP_CONVERT_WARPS);
             mbar_init(&k_free[s], 1);
+        }
+        for (int s = 0; s < VS; ++s) {
             mbar_init(&v_full[s], KP_CONVERT_WARPS);
             mbar_init(&v_free[s], 1);
         }
@@ -132,7 +191,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prompt_kernel(const b200q_k
             mbar_init(&p_full[t], 4);
             mbar_init(&o_done[t], 1);
         }
-        mbar_init(&q_full, KP_SOFTMAX_WARPS);
+        mbar_init(&q_full, KP_THREADS / 32 - 1);
         abort_flag = 0;
         fence_barrier_init();
     }
@@ -144,7 +203,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prompt_kernel(const b200q_k
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = tmem_base_slot;
-    const uint32_t S_COL = 0, P_COL = 128, O_COL = 192;
+    const uint32_t S_COL = 0, P_COL = 64, O_COL = 256;       // per tile: S 128 columns, P the second 64 of them, O DH columns
     // the whole warp: false once anybody has given up
     auto wait = [&](uint64_t *bar, uint32_t parity) -> bool {
         bool ok = mbar_try_wait(bar, parity);
@@ -159,22 +218,82 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prompt_kernel(const b200q_k
         return true;
     };
 
-    if (warp == KP_SOFTMAX_WARPS + KP_CONVERT_WARPS) {
-        // ---- loader
+    constexpr int LOADER = KP_SOFTMAX_WARPS + KP_CONVERT_WARPS, MMA = LOADER + 1;
+    if (warp != LOADER) {
+        // ---- queries, by all warps but the loader: DH / 8 lanes hold four dimensions of a row and their partners; the largest
+        // magnitude, then FP16 (and remainders) relative to its power of two
+        constexpr int HALF = DH / 2, LANES = DH / 8, AT_ONCE = 32 / LANES, WARPS = KP_THREADS / 32 - 1, STEPS = (KP_CTA_ROWS / AT_ONCE + WARPS - 1) / WARPS;
+        const int wi = warp < LOADER ? warp : warp - 1, i = lane % LANES * 4;
+#pragma unroll 3
+        for (int step = 0; step < STEPS; ++step) {
+            const int local = (wi + WARPS * step) * AT_ONCE + lane / LANES, row = row0 + local, token = row / p.group;
+            float x[2][4];
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[h][e] = 0.f;
+            if (local < KP_CTA_ROWS && row < rows) {
+                const size_t base = (first + token) * static_cast<size_t>(a.q_row) + static_cast<size_t>(kvh * p.group + row - token * p.group) * DH + i;
+                load4f(a.q, a.q_dtype, base, a.vec, x[0]);
+                load4f(a.q, a.q_dtype, base + HALF, a.vec, x[1]);
+                if (a.cos_t) {
+                    const float4 c4 = *reinterpret_cast<const float4 *>(a.cos_t + static_cast<size_t>(start + token) * HALF + i);
+                    const float4 s4 = *reinterpret_cast<const float4 *>(a.sin_t + static_cast<size_t>(start + token) * HALF + i);
+                    const float cv[4] = {c4.x, c4.y, c4.z, c4.w}, sv[4] = {s4.x, s4.y, s4.z, s4.w};
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float lo = x[0][e] * cv[e] - x[1][e] * sv[e], hi = x[0][e] * sv[e] + x[1][e] * cv[e];
+                        x[0][e] = lo;
+                        x[1][e] = hi;
+                    }
+                }
+            }
+            uint32_t top = 0u;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) top = max(top, max(abs_bits(x[0][e]), abs_bits(x[1][e])));
+#pragma unroll
+            for (int o = 1; o < LANES; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+            const float power = power_of(top), inv = a.scale < 0.f ? -power_inverse(power) : power_inverse(power);
+            if (local < KP_CTA_ROWS) {
+                if (i == 0) factor_s[local] = power * (fabsf(a.scale) * 1.4426950408889634f);
+                uint8_t *q_to = q_s + (local / KP_ROWS) * (Shape::Q / 2);
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int d = i + h * HALF;
+                    uint32_t hi[2], lo[2];
+                    split_half(x[h][0] * inv, x[h][1] * inv, hi[0], lo[0]);
+                    split_half(x[h][2] * inv, x[h][3] * inv, hi[1], lo[1]);
+                    uint8_t *to = q_to + (d / 64) * (KP_ROWS * 128) + swizzled(local % KP_ROWS, d % 64 / 8) + d % 8 * 2;
+                    *reinterpret_cast<uint2 *>(to) = make_uint2(hi[0], hi[1]);
+                    if (SPLIT) *reinterpret_cast<uint2 *>(to + Shape::Q) = make_uint2(lo[0], lo[1]);
+                }
+            }
+        }
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&q_full);
+    }
+
+    if (warp >= LOADER) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(KP_OTHER_REGS));
+    if (warp == LOADER) {
+        // ---- loader: keys, keys, values, values of a unit's two pages
         int pages = 0;
         bool loading = false;
-        for (int i = 0; i < count; ++i) {
-            const int unit = u0 + i, s = i % ST;
-            if ((i & 31) == 0) pages = unit + lane < full_units ? c.table[static_cast<size_t>(slot) * c.blocks + unit + lane] : 0;
-            int page = __shfl_sync(0xffffffffu, pages, i & 31);
+        for (int e = 0; e < 4 * count; ++e) {
+            const int i = e >> 2, s = e % RING, block = 2 * (u0 + i) + (e & 1), part_kv = (e >> 1) & 1;
+            if ((e & 63) == 0) {                 // the next 32 pages
+                const int at = 2 * (u0 + i) + lane;
+                pages = at < full_pages ? c.table[static_cast<size_t>(slot) * c.blocks + at] : 0;
+            }
+            int page = __shfl_sync(0xffffffffu, pages, 2 * (i & 15) + (e & 1));
             page = page >= 0 && page < c.pages ? page : 0;       // (a table that lacks the page: not beyond the pool)
-            if (i >= ST && !wait(&raw_free[s], (i / ST - 1) & 1)) break;
+            if (e >= RING && !wait(&raw_free[s], (e / RING - 1) & 1)) break;
             if (lane == 0) {
-                if (unit < full_units) {
-                    const size_t u = kv8_unit(page, c.layers, a.layer, 0, c.kv_heads, kvh);
-                    mbar_arrive_expect_tx(&raw_full[s], 2 * HALF_PAGE);
+                if (block < full_pages) {
+                    const size_t u = kv8_unit(page, c.layers, a.layer, part_kv, c.kv_heads, kvh);
+                    mbar_arrive_expect_tx(&raw_full[s], HALF_PAGE);
                     bulk_copy_g2s(raw_s + s * Shape::RAW, c.codes + u * HALF_PAGE, HALF_PAGE, &raw_full[s]);
-                    bulk_copy_g2s(raw_s + s * Shape::RAW + HALF_PAGE, c.codes + (u + c.kv_heads) * HALF_PAGE, HALF_PAGE, &raw_full[s]);
                 } else {
                     mbar_arrive(&raw_full[s]);                   // the converters read the tail themselves
                 }
@@ -189,30 +308,31 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prompt_kernel(const b200q_k
             }
         }
         __syncwarp();
-    } else if (warp == KP_SOFTMAX_WARPS + KP_CONVERT_WARPS + 1) {
+    } else if (warp == MMA) {
         // ---- MMAs (the whole warp walks the loop, one elected lane issues)
-        constexpr uint32_t s_idesc = umma_idesc_f16(KP_ROWS, KV8_BLOCK), o_idesc = umma_idesc_f16(KP_ROWS, DH);
+        constexpr uint32_t s_idesc = umma_idesc_f16(KP_ROWS, KP_KEYS), o_idesc = umma_idesc_f16(KP_ROWS, DH);
         const uint64_t q_desc = smem_desc_sw128(q_s), k_desc = smem_desc_sw128(k_s), v_desc = smem_desc_sw128(v_s);
         auto scores = [&](int t, int i) {        // S of tile t for unit i
-            const uint64_t kd = k_desc + static_cast<uint32_t>((i % ST) * Shape::K >> 4);
+            const uint64_t kd = k_desc + static_cast<uint32_t>((i % KS) * Shape::K >> 4);
             const uint64_t qd = q_desc + static_cast<uint32_t>(t * (Shape::Q / 2) >> 4);
             if (elect_one()) {
 #pragma unroll
                 for (int part_q = 0; part_q < (SPLIT ? 2 : 1); ++part_q)
 #pragma unroll
                     for (int k = 0; k < DH / 16; ++k)
-                        umma_bf16<false>(tmem + S_COL + 64 * t, qd + static_cast<uint32_t>((part_q * Shape::Q + (k / 4) * (KP_ROWS * 128)) >> 4) + 2 * (k % 4),
-                                         kd + static_cast<uint32_t>(((k / 4) * (KV8_BLOCK * 128)) >> 4) + 2 * (k % 4), s_idesc, part_q + k > 0);
+                        umma_bf16<false>(tmem + S_COL + 128 * t, qd + static_cast<uint32_t>((part_q * Shape::Q + (k / 4) * (KP_ROWS * 128)) >> 4) + 2 * (k % 4),
+                                         kd + static_cast<uint32_t>(((k / 4) * K_SLAB) >> 4) + 2 * (k % 4), s_idesc, part_q + k > 0);
                 umma_commit<false>(smem_u32(&s_full[t]));
             }
             __syncwarp();
         };
         auto values = [&](int t, int i, bool last) {
-            const uint64_t vd = v_desc + static_cast<uint32_t>((i % ST) * Shape::K >> 4);
+            const uint64_t vd = v_desc + static_cast<uint32_t>((i % VS) * Shape::K >> 4);
             if (elect_one()) {
 #pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    umma_f16_ts(tmem + O_COL + DH * t, tmem + P_COL + 32 * t + 8 * k, vd + 2 * k, o_idesc, i + k > 0);
+                for (int k = 0; k < 8; ++k)
+                    umma_f16_ts(tmem + O_COL + DH * t, tmem + S_COL + 128 * t + P_COL + 8 * k, vd + static_cast<uint32_t>(((k / 4) * V_PAGE) >> 4) + 2 * (k % 4),
+                                o_idesc, i + k > 0);
                 if (last) umma_commit<false>(smem_u32(&o_done[t]));
             }
             __syncwarp();
@@ -221,7 +341,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prompt_kernel(const b200q_k
             if (elect_one()) umma_commit<false>(smem_u32(bar));
             __syncwarp();
         };
-        bool fine = wait(&q_full, 0) && wait(&k_full[0], 0);
+        const bool fine = wait(&q_full, 0) && wait(&k_full[0], 0);
         if (fine) {
             tc_fence_after();
             if (count0) scores(0, 0);
@@ -229,250 +349,227 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prompt_kernel(const b200q_k
             release(&k_free[0]);
         }
         for (int i = 0; fine && i < count; ++i) {
-            const int s = i % ST, s_next = (i + 1) % ST;
-            if (!wait(&v_full[s], (i / ST) & 1)) break;
+            const int next = i + 1;
+            if (!wait(&v_full[i % VS], (i / VS) & 1)) break;
             if (i < count0) {
                 if (!wait(&p_full[0], i & 1)) break;
                 tc_fence_after();
-                values(0, i, i + 1 == count0);
+                values(0, i, next == count0);
             }
-            if (i + 1 < count && !wait(&k_full[s_next], ((i + 1) / ST) & 1)) break;
+            if (next < count && !wait(&k_full[next % KS], (next / KS) & 1)) break;
             tc_fence_after();
-            if (i + 1 < count0) scores(0, i + 1);
+            if (next < count0) scores(0, next);
             if (i < count1) {
                 if (!wait(&p_full[1], i & 1)) break;
                 tc_fence_after();
-                values(1, i, i + 1 == count1);
+                values(1, i, next == count1);
             }
-            release(&v_free[s]);
-            if (i + 1 < count1) scores(1, i + 1);
-            if (i + 1 < count) release(&k_free[s_next]);
+            release(&v_free[i % VS]);
+            if (next < count1) scores(1, next);
+            if (next < count) release(&k_free[next % KS]);
         }
+    }
     } else if (warp >= KP_SOFTMAX_WARPS) {
         // ---- converters
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(KP_OTHER_REGS));
         const int ct = tid - KP_SOFTMAX_WARPS * 32;
-        for (int i = 0; i < count; ++i) {
-            const int s = i % ST, unit = u0 + i;
-            uint8_t *k_to = k_s + s * Shape::K, *v_to = v_s + s * Shape::K;
-            const uint8_t *raw = raw_s + s * Shape::RAW;
-            const size_t tail = kv8_unit(slot, c.layers, a.layer, 0, c.kv_heads, kvh);
-            const uint16_t *tail_k = static_cast<const uint16_t *>(c.tail) + tail * HALF_PAGE, *tail_v = tail_k + static_cast<size_t>(c.kv_heads) * HALF_PAGE;
-            const int rest = total - unit * KV8_BLOCK;
-            // Tail values pass relative to a power of two; where the largest is not finite the scale is NaN and they are zeros
-            // (a NaN here would reach rows that do not see the block).
-            auto tail_inverse = [&](int values_part) {
-                const uint32_t top = abs_bits(c.peak[tail + (values_part ? c.kv_heads : 0)]);
-                return top < 0x7f800000u ? power_inverse(power_of(top)) : 0.f;
-            };
-            auto half_of = [&](uint32_t w, float inv) { return inv == 0.f ? 0u : tail_to_half<BF16>(w, inv); };
-            if (!wait(&raw_full[s], (i / ST) & 1)) break;
-            if (i >= ST && !wait(&k_free[s], (i / ST - 1) & 1)) break;
-            if (unit < full_units) {
+        const size_t tail = kv8_unit(slot, c.layers, a.layer, 0, c.kv_heads, kvh);
+        const uint16_t *tail_k = static_cast<const uint16_t *>(c.tail) + tail * HALF_PAGE, *tail_v = tail_k + static_cast<size_t>(c.kv_heads) * HALF_PAGE;
+        const int rest = total - full_pages * KV8_BLOCK;
+        // Tail values pass relative to a power of two; where the largest is not finite the scale is NaN and they are zeros (a
+        // NaN here would reach rows that do not see the block).
+        auto tail_inverse = [&](int values_part) {
+            const uint32_t top = abs_bits(c.peak[tail + (values_part ? c.kv_heads : 0)]);
+            return top < 0x7f800000u ? power_inverse(power_of(top)) : 0.f;
+        };
+        auto half_of = [&](uint32_t w, float inv) { return inv == 0.f ? 0u : tail_to_half<BF16>(w, inv); };
+        bool fine = true;
+        for (int i = 0; fine && i < count; ++i) {
+#pragma unroll 1
+            for (int e = 4 * i; e < 4 * i + 4; ++e) {
+                const int s = e % RING, h = e & 1, block = 2 * (u0 + i) + h;
+                const bool keys = (e & 2) == 0;
+                const uint8_t *raw = raw_s + s * Shape::RAW;
+                fine = wait(&raw_full[s], (e / RING) & 1);
+                if (fine && h == 0) fine = keys ? i < KS || wait(&k_free[i % KS], (i / KS - 1) & 1) : i < VS || wait(&v_free[i % VS], (i / VS - 1) & 1);
+                if (!fine) break;
+                uint8_t *to = keys ? k_s + (i % KS) * Shape::K + h * (KV8_BLOCK * 128) : v_s + (i % VS) * Shape::K + h * V_PAGE;
+                if (block < full_pages) {
+                    // a thread's pieces of sixteen codes: (row, quarter) of 64-code rows
+                    uint4 w[SLABS * 2];
+                    if (keys) {
 #pragma unroll
-                for (int j = 0; j < SLABS * 2; ++j) {
-                    const int id = ct + 128 * j, key = (id >> 2) & 63, q = id & 3, slab = id >> 8;
-                    convert16(*reinterpret_cast<const uint4 *>(raw + key * DH + slab * 64 + q * 16), k_to + slab * (KV8_BLOCK * 128), key, q);
-                }
-            } else {
-                const float inv = tail_inverse(0);
-                for (int id = ct; id < KV8_BLOCK * DH / 8; id += 128) {
-                    const int key = id / (DH / 8), chunk = id % (DH / 8);
-                    uint4 w = make_uint4(0u, 0u, 0u, 0u);
-                    if (key < rest) w = *reinterpret_cast<const uint4 *>(tail_k + key * DH + 8 * chunk);
-                    *reinterpret_cast<uint4 *>(k_to + (chunk >> 3) * (KV8_BLOCK * 128) + swizzled(key, chunk & 7)) =
-                        make_uint4(half_of(w.x, inv), half_of(w.y, inv), half_of(w.z, inv), half_of(w.w, inv));
-                }
-            }
-            fence_proxy_async();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&k_full[s]);
-            if (i >= ST && !wait(&v_free[s], (i / ST - 1) & 1)) break;
-            if (unit < full_units) {
+                        for (int j = 0; j < SLABS * 2; ++j) w[j] = *reinterpret_cast<const uint4 *>(raw + ((ct >> 2) + 32 * (j & 1)) * DH + (j >> 1) * 64 + (ct & 3) * 16);
 #pragma unroll
-                for (int j = 0; j < SLABS * 2; ++j) {
-                    const int id = ct + 128 * j;
-                    convert16(*reinterpret_cast<const uint4 *>(raw + HALF_PAGE + id * 16), v_to, id >> 2, id & 3);
+                        for (int j = 0; j < SLABS * 2; ++j) convert16(w[j], to + (j >> 1) * K_SLAB, (ct >> 2) + 32 * (j & 1), ct & 3);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < SLABS * 2; ++j) w[j] = *reinterpret_cast<const uint4 *>(raw + (ct + 128 * j) * 16);
+#pragma unroll
+                        for (int j = 0; j < SLABS * 2; ++j) convert16(w[j], to, (ct >> 2) + 32 * j, ct & 3);
+                    }
+                } else {
+                    const int have = block == full_pages ? rest : 0;
+                    const float inv = have ? tail_inverse(!keys) : 0.f;
+                    if (keys) {
+                        for (int id = ct; id < KV8_BLOCK * DH / 8; id += 128) {
+                            const int key = id / (DH / 8), chunk = id % (DH / 8);
+                            uint4 w = make_uint4(0u, 0u, 0u, 0u);
+                            if (key < have) w = *reinterpret_cast<const uint4 *>(tail_k + key * DH + 8 * chunk);
+                            *reinterpret_cast<uint4 *>(to + (chunk >> 3) * K_SLAB + swizzled(key, chunk & 7)) =
+                                make_uint4(half_of(w.x, inv), half_of(w.y, inv), half_of(w.z, inv), half_of(w.w, inv));
+                        }
+                    } else {
+                        for (int id = ct; id < KV8_BLOCK * DH / 2; id += 128) {
+                            const int key = id / (DH / 2), d = id % (DH / 2) * 2;
+                            const uint32_t w = key < have ? half_of(*reinterpret_cast<const uint32_t *>(tail_v + key * DH + d), inv) : 0u;
+                            *reinterpret_cast<uint16_t *>(to + swizzled(d, key >> 3) + (key & 7) * 2) = static_cast<uint16_t>(w);
+                            *reinterpret_cast<uint16_t *>(to + swizzled(d + 1, key >> 3) + (key & 7) * 2) = static_cast<uint16_t>(w >> 16);
+                        }
+                    }
                 }
-            } else {
-                const float inv = tail_inverse(1);
-                for (int id = ct; id < KV8_BLOCK * DH / 2; id += 128) {
-                    const int key = id / (DH / 2), d = id % (DH / 2) * 2;
-                    const uint32_t w = key < rest ? half_of(*reinterpret_cast<const uint32_t *>(tail_v + key * DH + d), inv) : 0u;
-                    *reinterpret_cast<uint16_t *>(v_to + swizzled(d, key >> 3) + (key & 7) * 2) = static_cast<uint16_t>(w);
-                    *reinterpret_cast<uint16_t *>(v_to + swizzled(d + 1, key >> 3) + (key & 7) * 2) = static_cast<uint16_t>(w >> 16);
+                if (h == 1) fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(&raw_free[s]);
+                    if (h == 1) mbar_arrive(keys ? &k_full[i % KS] : &v_full[i % VS]);
                 }
-            }
-            fence_proxy_async();
-            __syncwarp();
-            if (lane == 0) {
-                mbar_arrive(&v_full[s]);
-                mbar_arrive(&raw_free[s]);
             }
         }
     } else {
         // ---- softmax: a thread per row
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(KP_SOFTMAX_REGS));
         const int t = warp >> 2, local = 32 * (warp & 3) + lane, row = row0 + t * KP_ROWS + local, mine = t ? count1 : count0;
         const bool valid = row < rows;
         const int token = valid ? row / p.group : 0, pos = start + token;
         const size_t out_row = static_cast<size_t>(first + token) * a.heads + kvh * p.group + (valid ? row - token * p.group : 0);
-        float factor = 0.f;
-        {
-            // the row's query: the largest magnitude, then FP16 (and remainders) into the operand; dimensions i and i + DH / 2 a
-            // sixteen at a time
-            constexpr int HALF = DH / 2;
-            const size_t base = (first + token) * static_cast<size_t>(a.q_row) + static_cast<size_t>(kvh * p.group + (valid ? row - token * p.group : 0)) * DH;
-            auto rotated = [&](int i, float (&x0)[16], float (&x1)[16]) {
-                load16f(a.q, a.q_dtype, base + i, a.vec, x0);
-                load16f(a.q, a.q_dtype, base + i + HALF, a.vec, x1);
-                if (a.cos_t) {
-                    float cv[16], sv[16];
-                    load16f(a.cos_t, B200Q_F32, static_cast<size_t>(pos) * HALF + i, true, cv);
-                    load16f(a.sin_t, B200Q_F32, static_cast<size_t>(pos) * HALF + i, true, sv);
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        const float lo = x0[e] * cv[e] - x1[e] * sv[e], hi = x0[e] * sv[e] + x1[e] * cv[e];
-                        x0[e] = lo;
-                        x1[e] = hi;
-                    }
-                }
-            };
-            uint32_t top = 0u;
-            if (valid && mine)
-#pragma unroll 1
-                for (int i = 0; i < HALF; i += 16) {
-                    float x0[16], x1[16];
-                    rotated(i, x0, x1);
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) top = max(top, max(abs_bits(x0[e]), abs_bits(x1[e])));
-                }
-            const float power = power_of(top), inv = a.scale < 0.f ? -power_inverse(power) : power_inverse(power);
-            factor = power * (fabsf(a.scale) * 1.4426950408889634f);
-            uint8_t *q_to = q_s + t * (Shape::Q / 2);
-            if (mine)
-#pragma unroll 1
-                for (int i = 0; i < HALF; i += 16) {
-                    float x[2][16];
-                    if (valid) {
-                        rotated(i, x[0], x[1]);
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) x[0][e] = x[1][e] = 0.f;
-                    }
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const int d = i + h * HALF;
-                        uint8_t *to = q_to + (d / 64) * (KP_ROWS * 128);
-#pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            uint32_t hi[4], lo[4];
-#pragma unroll
-                            for (int w = 0; w < 4; ++w) split_half(x[h][8 * e + 2 * w] * inv, x[h][8 * e + 2 * w + 1] * inv, hi[w], lo[w]);
-                            const uint32_t at = swizzled(local, (d % 64) / 8 + e);
-                            *reinterpret_cast<uint4 *>(to + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                            if (SPLIT) *reinterpret_cast<uint4 *>(to + Shape::Q + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-                        }
-                    }
-                }
-            fence_proxy_async();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&q_full);
-        }
         const uint32_t lanes = static_cast<uint32_t>(32 * (warp & 3)) << 16;
         float m = -INFINITY, l = 0.f, reference = 0.f;       // reference: U
-        bool fine = true;
-        // scales of the next unit, read a unit ahead (their page two units ahead)
-        auto page_at = [&](int unit) { return unit < full_units ? c.table[static_cast<size_t>(slot) * c.blocks + unit] : 0; };
-        auto scales_at = [&](int unit, int page, float &ks, float &vs) {
-            if (unit < full_units) {
+        bool fine = wait(&q_full, 0);
+        const float factor = factor_s[t * KP_ROWS + local];
+        // scales of a unit's two blocks, read a unit ahead (their pages two units ahead)
+        auto page_at = [&](int block) { return block < full_pages ? c.table[static_cast<size_t>(slot) * c.blocks + block] : 0; };
+        auto scales_at = [&](int block, int page, float &ks, float &vs) {
+            if (block < full_pages) {
                 const size_t u = kv8_unit(page >= 0 && page < c.pages ? page : 0, c.layers, a.layer, 0, c.kv_heads, kvh);
                 ks = c.scales[u];
                 vs = c.scales[u + c.kv_heads];
-            } else {
+            } else if (block * KV8_BLOCK < total) {
                 const size_t u = kv8_unit(slot, c.layers, a.layer, 0, c.kv_heads, kvh);
                 ks = power_of(abs_bits(c.peak[u]));
                 vs = power_of(abs_bits(c.peak[u + c.kv_heads]));
+            } else {
+                ks = vs = 0.f;
             }
         };
-        float ks_next = 0.f, vs_next = 0.f;
-        int page_next = 0;
-        if (mine) {
-            scales_at(u0, page_at(u0), ks_next, vs_next);
-            if (mine > 1) page_next = page_at(u0 + 1);
+        float ks_next[2] = {0.f, 0.f}, vs_next[2] = {0.f, 0.f};
+        int page_next[2] = {0, 0};
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            if (mine) scales_at(2 * u0 + h, page_at(2 * u0 + h), ks_next[h], vs_next[h]);
+            if (mine > 1) page_next[h] = page_at(2 * u0 + 2 + h);
         }
-        for (int i = 0; i < mine; ++i) {
-            const int unit = u0 + i;
-            const float ks = ks_next, vs = vs_next;
-            if (i + 1 < mine) scales_at(unit + 1, page_next, ks_next, vs_next);
-            if (i + 2 < mine) page_next = page_at(unit + 2);
-            const bool sees = pos >= unit * KV8_BLOCK;
-            // (not below the smallest normal number, where a hidden key's -inf would meet a zero)
-            float f = factor * ks;
-            if (f < KV8_MIN_SCALE || !sees) f = KV8_MIN_SCALE;
-            // U follows the largest scale: the same in every thread
-            float beta = 1.f;
-            const float power = power_of(abs_bits(vs));
-            if (power > 8.f * reference) {
-                beta = __fdiv_rn(reference, power);
-                reference = power;
-            }
-            const float relative = sees ? __fdiv_rn(vs, reference) : 0.f;
-            if (!wait(&s_full[t], i & 1)) {
-                fine = false;
-                break;
-            }
-            tc_fence_after();
-            uint32_t s0[32], s1[32];
-            tmem_ld32(tmem + lanes + S_COL + 64 * t, s0);
-            tmem_ld32(tmem + lanes + S_COL + 64 * t + 32, s1);
-            tmem_ld_wait();
-            if (__any_sync(0xffffffffu, pos < unit * KV8_BLOCK + KV8_BLOCK - 1)) {
-                const int limit = pos - unit * KV8_BLOCK;
+        for (int i = 0; fine && i < mine; ++i) {
+            const int block = 2 * (u0 + i), key0 = block * KV8_BLOCK;
+            float f[2], relative[2], alpha = 1.f;
 #pragma unroll
-                for (int e = 0; e < 32; ++e) {
-                    if (e > limit) s0[e] = 0xff800000u;
-                    if (e + 32 > limit) s1[e] = 0xff800000u;
+            for (int h = 0; h < 2; ++h) {
+                const float ks = ks_next[h], vs = vs_next[h];
+                if (i + 1 < mine) scales_at(block + 2 + h, page_next[h], ks_next[h], vs_next[h]);
+                if (i + 2 < mine) page_next[h] = page_at(block + 4 + h);
+                const bool sees = pos >= key0 + h * KV8_BLOCK;
+                // (not below the smallest normal number, where a hidden key's -inf would meet a zero)
+                f[h] = factor * ks;
+                if (f[h] < KV8_MIN_SCALE || !sees) f[h] = KV8_MIN_SCALE;
+                // U follows the largest scale: the same in every thread
+                const float power = power_of(abs_bits(vs));
+                if (power > 8.f * reference) {
+                    alpha *= reference * power_inverse(power);
+                    reference = power;
                 }
+                relative[h] = vs;
             }
-            float top = -INFINITY;
+            // a weight's factor `relative` as an addend of its exponent; one too small to matter next to U counts as zero, and
+            // its weights only enter the sum
+            const float per_reference = power_inverse(reference);
+            float addend[2], divide[2];
+            bool nothing[2];
 #pragma unroll
-            for (int e = 0; e < 32; ++e) top = fmaxf(top, fmaxf(__uint_as_float(s0[e]), __uint_as_float(s1[e])));
-            top *= f;
-            float alpha = beta;
+            for (int h = 0; h < 2; ++h) {
+                const float r = relative[h] * per_reference;
+                nothing[h] = r < 8.6736174e-19f;             // 2^-60
+                const bool plain = nothing[h] || pos < key0 + h * KV8_BLOCK;
+                addend[h] = plain ? 0.f : log2_approx(r);
+                divide[h] = plain ? 1.f : __fdividef(1.f, r);
+            }
+            fine = wait(&s_full[t], i & 1);
+            if (!fine) break;
+            tc_fence_after();
+            const uint32_t at = tmem + lanes + S_COL + 128 * t;
+            uint32_t s[4][32];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) tmem_ld32(at + 32 * q, s[q]);
+            tmem_ld_wait();
+            if (__any_sync(0xffffffffu, pos < key0 + KP_KEYS - 1)) {         // hidden keys
+                const int limit = pos - key0;
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+#pragma unroll
+                    for (int e = 0; e < 32; ++e)
+                        if (32 * q + e > limit) s[q][e] = 0xff800000u;
+            }
+            float tops[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                tops[q] = fmaxf(__uint_as_float(s[q][0]), __uint_as_float(s[q][1]));
+#pragma unroll
+                for (int e = 2; e < 32; e += 2) tops[q] = max3(tops[q], __uint_as_float(s[q][e]), __uint_as_float(s[q][e + 1]));
+            }
+            const float top = fmaxf(fmaxf(tops[0], tops[1]) * f[0], fmaxf(tops[2], tops[3]) * f[1]);
             if (top > m + 8.f) {
                 const float keep = exp2_approx(m - top);
                 alpha *= keep;
                 l *= keep;
                 m = top;
             }
-            if (i > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
+            if (i > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {            // (S of this unit follows the last value product)
 #pragma unroll 1
-                for (int d = 0; d < DH; d += 32) {
-                    uint32_t o[32];
-                    tmem_ld32(tmem + lanes + O_COL + DH * t + d, o);
+                for (int d = 0; d < DH; d += 16) {
+                    uint32_t o[16];
+                    tmem_ld16(tmem + lanes + O_COL + DH * t + d, o);
                     tmem_ld_wait();
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-                    tmem_st32(tmem + lanes + O_COL + DH * t + d, o);
+                    for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+                    tmem_st16(tmem + lanes + O_COL + DH * t + d, o);
                 }
             }
             const float shift = m == -INFINITY ? 0.f : m;
-            float sum0 = 0.f, sum1 = 0.f;
 #pragma unroll
-            for (int e = 0; e < 32; ++e) {
-                const float x = exp2_approx(fmaf(__uint_as_float(s0[e]), f, -shift)), y = exp2_approx(fmaf(__uint_as_float(s1[e]), f, -shift));
-                sum0 += x;
-                sum1 += y;
-                s0[e] = __float_as_uint(x * relative);
-                s1[e] = __float_as_uint(y * relative);
-            }
-            l += sum0 + sum1;
-            uint32_t w[32];
+            for (int h = 0; h < 2; ++h) {
+                const float move = addend[h] - shift;
+                const uint64_t f2 = pack2(f[h], f[h]), move2 = pack2(move, move);        // pairs: two per instruction
+                uint64_t sums[2] = {0ull, 0ull};
+                uint32_t w[32];
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                w[e] = pack_half(__uint_as_float(s0[2 * e]), __uint_as_float(s0[2 * e + 1]));
-                w[16 + e] = pack_half(__uint_as_float(s1[2 * e]), __uint_as_float(s1[2 * e + 1]));
+                for (int e = 0; e < 32; e += 2)
+#pragma unroll
+                    for (int q = 0; q < 2; ++q) {
+                        float lo, hi;
+                        unpack2(fma2(pack2(__uint_as_float(s[2 * h + q][e]), __uint_as_float(s[2 * h + q][e + 1])), f2, move2), lo, hi);
+                        lo = exp2_approx(lo);
+                        hi = exp2_approx(hi);
+                        sums[q] = add2(sums[q], pack2(lo, hi));
+                        w[16 * q + e / 2] = pack_half(lo, hi);
+                    }
+                if (nothing[h]) {
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) w[e] = 0u;
+                }
+                tmem_st32(at + P_COL + 32 * h, w);
+                float lo, hi;
+                unpack2(add2(sums[0], sums[1]), lo, hi);
+                l = fmaf(lo + hi, divide[h], l);
             }
-            tmem_st32(tmem + lanes + P_COL + 32 * t, w);
             tmem_st_wait();
             tc_fence_before();
             __syncwarp();
@@ -549,7 +646,7 @@ __global__ void __launch_bounds__(256) kv8_prompt_join_kernel(const b200q_kv8_ca
     if (start < 0) return;
     const int row = (token_row - a.offsets[b]) * p.group + head % p.group;
     const int end = min(row / KP_CTA_ROWS * KP_CTA_ROWS + KP_CTA_ROWS, rows);
-    const int all = (start + (end - 1) / p.group) / KV8_BLOCK + 1;       // units of the row's CTA
+    const int all = (start + (end - 1) / p.group) / KP_KEYS + 1;         // units of the row's CTA
     float top = -INFINITY, weight = 0.f, value[DH / 32];
 #pragma unroll
     for (int e = 0; e < DH / 32; ++e) value[e] = 0.f;
@@ -572,11 +669,11 @@ __global__ void __launch_bounds__(256) kv8_prompt_join_kernel(const b200q_kv8_ca
 // ----------------------------------------------------------------------------------------------------------- host side
 int kv8_shared_memory(const void *kernel, int bytes);        // kv8_decode.cu
 
-// Parts of the keys: as many as give every SM two CTAs, of eight blocks at least.
+// Parts of the keys: as many as give every SM two CTAs, of four units at least.
 static int prompt_splits(const b200q_kv8_cache *c, int heads, int batch, int max_new, int max_keys) {
-    const long long rows = static_cast<long long>(max_new) * (heads / c->kv_heads), units = (max_keys + KV8_BLOCK - 1) / KV8_BLOCK;
+    const long long rows = static_cast<long long>(max_new) * (heads / c->kv_heads), units = (max_keys + KP_KEYS - 1) / KP_KEYS;
     const long long ctas = (rows + KP_CTA_ROWS - 1) / KP_CTA_ROWS * c->kv_heads * batch;
-    return static_cast<int>(std::max(1ll, std::min({(2ll * sm_count() + ctas - 1) / ctas, units / 8, 16ll})));
+    return static_cast<int>(std::max(1ll, std::min({(2ll * sm_count() + ctas - 1) / ctas, units / 4, 16ll})));
 }
 
 long long kv8_prompt_workspace(const b200q_kv8_cache *c, int heads, int batch, int rows, int max_new, int max_keys) {
