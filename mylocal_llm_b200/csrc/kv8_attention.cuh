@@ -72,7 +72,10 @@ __device__ __forceinline__ float power_of(uint32_t bits) {
     return __uint_as_float(max(bits & 0x7f800000u, 0x00800000u));
 }
 // Its reciprocal, exact (2^-127 is a subnormal number); of NaN: NaN.
-__device__ __forceinline__ float power_inverse(float p) { return __fdiv_rn(1.0f, p); }
+__device__ __forceinline__ float power_inverse(float p) {
+    const uint32_t e = __float_as_uint(p) >> 23;
+    return __uint_as_float(e < 254 ? (254 - e) << 23 : e == 254 ? 0x00400000u : 0x7fc00000u);
+}
 
 // Two 16-bit values of the tail (as stored) times a power of two, as FP16.
 template <bool BF16>

@@ -4,11 +4,14 @@
 // One CTA owns 256 rows of one key/value head of one sequence (row = token * group + head of the group: the heads that share keys
 // are neighbours) as two tiles of 128, and walks the units of 128 keys (two pages) that its last row sees, or a part of them.
 // Warps have roles that meet at mbarriers:
-//   loader      one bulk copy each for the keys and the values of a page (int8, contiguous) into a ring
-//   converters  (4 warps) codes -> FP16, exact, into the 128-byte-swizzled K-major operands: the keys as [128][head_dim], the
-//               values, which a page holds transposed, as [head_dim][64] twice; the 16-bit tail of a sequence goes the same way
-//   MMA         scores S = Q K^T (FP32, tensor memory) of one tile while the other tile's softmax runs, then O += P V with the
-//               softmax weights P read from tensor memory, where they replace the second half of their scores
+//   converters  (4 warps) codes -> registers, a half page ahead (and asked into L2 four units ahead) -> FP16, exact, into the 128-byte-swizzled K-major operands: the
+//               keys as [128][head_dim], the values, which a page holds transposed, as [head_dim][64] twice; the 16-bit tail of a
+//               sequence goes the same way. (A ring of codes in shared memory took 64 KB of its traffic per unit, which the
+//               operands of the MMAs need: at head dimension 128 they read 256 to 320 KB per unit at 128 bytes a clock.)
+//   MMA         (a warp per tile) scores S = Q K^T (FP32, tensor memory), then, when the tile's softmax is done, O += P V with
+//               the softmax weights P read from tensor memory, where they replace the second half of their scores; one tile's
+//               products run while the other's softmax does. (One warp for both tiles needed more time to issue the
+//               instructions, among three other busy warps of its scheduler, than the tensor cores to execute them.)
 //   softmax     (2 x 4 warps) a thread per row: maximum, weights, sum; the weights go back to tensor memory as FP16, times the
 //               block's value scale relative to a power of two U that follows the largest scale seen (as an addend of the
 //               exponent, which costs nothing; the sum is divided by it). A row's reference maximum
@@ -31,18 +34,19 @@ namespace b200q {
 constexpr int STATUS_KV8_PROMPT = 512;       // gave up waiting at a barrier of the prompt kernel
 constexpr int KP_ROWS = 128, KP_CTA_ROWS = 256;
 constexpr int KP_SOFTMAX_WARPS = 8, KP_CONVERT_WARPS = 4;
-constexpr int KP_THREADS = 512;              // and loader, MMA and two warps that only help with the queries
+constexpr int KP_THREADS = 512;              // and two MMA warps and two that only help with the queries
 // Registers per thread: a softmax thread holds its row's 128 scores. 256 x 176 + 256 x 80 = 512 x 128, what the launch has.
 constexpr int KP_SOFTMAX_REGS = 176, KP_OTHER_REGS = 80;
 
 constexpr int KP_KEYS = 2 * KV8_BLOCK;       // keys of a unit
 
-// Operand stages of keys and values (of a unit each) and half pages of codes in the ring, by what shared memory holds.
+// Operand stages of keys and values (of a unit each), by what shared memory holds.
 template <int DH, bool SPLIT> struct PromptShape {
-    static constexpr int KS = DH == 128 && SPLIT ? 1 : 2, VS = DH == 128 ? 1 : 2, RING = DH == 128 && SPLIT ? 4 : 8;
-    static constexpr int Q = 2 * KP_ROWS * DH * 2, K = KP_KEYS * DH * 2, RAW = KV8_BLOCK * DH;
-    static constexpr int BYTES = (SPLIT ? 2 : 1) * Q + (KS + VS) * K + RING * RAW;
+    static constexpr int KS = 2, VS = DH == 128 && SPLIT ? 1 : 2;
+    static constexpr int Q = 2 * KP_ROWS * DH * 2, K = KP_KEYS * DH * 2;
+    static constexpr int BYTES = (SPLIT ? 2 : 1) * Q + (KS + VS) * K;
 };
+constexpr int KP_AHEAD = 4;                  // units between a page's request to L2 and its use
 
 struct Kv8Prompt {
     Kv8Attention a;
@@ -51,12 +55,22 @@ struct Kv8Prompt {
     int *status;
 };
 
-// D[tmem] (+)= A[tmem] * B[smem desc]
-__device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+// D[tmem] (+)= A * B, A described in shared memory or read from tensor memory. Descriptors as their low words (the address is in
+// them) and one high word, so that an operand costs one addition.
+__device__ __forceinline__ void umma_f16_ss(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t hi, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
+        "mov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\t"
+        "setp.ne.b32 p, %5, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, p;\n\t}" ::"r"(d_tmem), "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_lo, uint32_t hi, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\t"
+        "mov.b64 b, {%2, %3};\n\t"
+        "setp.ne.b32 p, %5, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t}" ::"r"(d_tmem), "r"(a_tmem), "r"(b_lo), "r"(hi), "r"(idesc), "r"(accumulate)
         : "memory");
 }
 // Instruction descriptor of kind::f16 with FP16 operands (bits [7,10), [10,13) = 0) and an FP32 accumulator.
@@ -137,11 +151,10 @@ __device__ __forceinline__ void convert16(const uint4 &w, uint8_t *operand, int 
 template <int DH, bool BF16, bool SPLIT>
 __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prompt_kernel(const b200q_kv8_cache c, const Kv8Prompt p) {
     using Shape = PromptShape<DH, SPLIT>;
-    constexpr int KS = Shape::KS, VS = Shape::VS, RING = Shape::RING, SLABS = DH / 64, HALF_PAGE = KV8_BLOCK * DH;
+    constexpr int KS = Shape::KS, VS = Shape::VS, SLABS = DH / 64, HALF_PAGE = KV8_BLOCK * DH;
     constexpr int K_SLAB = KP_KEYS * 128, V_PAGE = DH * 128;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ __align__(8) uint64_t raw_full[RING], raw_free[RING], k_full[KS], k_free[KS], v_full[VS], v_free[VS], s_full[2],
-        p_full[2], o_done[2], q_full;
+    __shared__ __align__(8) uint64_t k_full[KS], k_free[KS], v_full[VS], v_free[VS], s_full[2], p_full[2], o_done[2], q_full;
     __shared__ uint32_t tmem_base_slot;
     __shared__ volatile int abort_flag;
     __shared__ float factor_s[KP_CTA_ROWS];
@@ -172,26 +185,22 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prompt_kernel(const b200q_k
     const int full_pages = total / KV8_BLOCK;    // the block after them is the tail, what follows does not exist
 
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint8_t *q_s = smem, *k_s = smem + (SPLIT ? 2 : 1) * Shape::Q, *v_s = k_s + KS * Shape::K, *raw_s = v_s + VS * Shape::K;
+    uint8_t *q_s = smem, *k_s = smem + (SPLIT ? 2 : 1) * Shape::Q, *v_s = k_s + KS * Shape::K;
     if (tid == 0) {
-        for (int s = 0; s < RING; ++s) {
-            mbar_init(&raw_full[s], 1);
-            mbar_init(&raw_free[s], KP_CONVERT_WARPS);
-        }
         for (int s = 0; s < KS; ++s) {
             mbar_init(&k_full[s], KP_CONVERT_WARPS);
-            mbar_init(&k_free[s], 1);
+            mbar_init(&k_free[s], 2);            // both tiles
         }
         for (int s = 0; s < VS; ++s) {
             mbar_init(&v_full[s], KP_CONVERT_WARPS);
-            mbar_init(&v_free[s], 1);
+            mbar_init(&v_free[s], 2);
         }
         for (int t = 0; t < 2; ++t) {
             mbar_init(&s_full[t], 1);
             mbar_init(&p_full[t], 4);
             mbar_init(&o_done[t], 1);
         }
-        mbar_init(&q_full, KP_THREADS / 32 - 1);
+        mbar_init(&q_full, KP_THREADS / 32);
         abort_flag = 0;
         fence_barrier_init();
     }
@@ -202,7 +211,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prompt_kernel(const b200q_k
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = tmem_base_slot;
+    const uint32_t tmem = tmem_base_slot;                    // (all 512 columns: 0)
     const uint32_t S_COL = 0, P_COL = 64, O_COL = 256;       // per tile: S 128 columns, P the second 64 of them, O DH columns
     // the whole warp: false once anybody has given up
     auto wait = [&](uint64_t *bar, uint32_t parity) -> bool {
@@ -218,15 +227,15 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prompt_kernel(const b200q_k
         return true;
     };
 
-    constexpr int LOADER = KP_SOFTMAX_WARPS + KP_CONVERT_WARPS, MMA = LOADER + 1;
-    if (warp != LOADER) {
-        // ---- queries, by all warps but the loader: DH / 8 lanes hold four dimensions of a row and their partners; the largest
+    constexpr int MMA = KP_SOFTMAX_WARPS + KP_CONVERT_WARPS;
+    {
+        // ---- queries, by all warps: DH / 8 lanes hold four dimensions of a row and their partners; the largest
         // magnitude, then FP16 (and remainders) relative to its power of two
-        constexpr int HALF = DH / 2, LANES = DH / 8, AT_ONCE = 32 / LANES, WARPS = KP_THREADS / 32 - 1, STEPS = (KP_CTA_ROWS / AT_ONCE + WARPS - 1) / WARPS;
-        const int wi = warp < LOADER ? warp : warp - 1, i = lane % LANES * 4;
+        constexpr int HALF = DH / 2, LANES = DH / 8, AT_ONCE = 32 / LANES, WARPS = KP_THREADS / 32, STEPS = (KP_CTA_ROWS / AT_ONCE + WARPS - 1) / WARPS;
+        const int i = lane % LANES * 4;
 #pragma unroll 3
         for (int step = 0; step < STEPS; ++step) {
-            const int local = (wi + WARPS * step) * AT_ONCE + lane / LANES, row = row0 + local, token = row / p.group;
+            const int local = (warp + WARPS * step) * AT_ONCE + lane / LANES, row = row0 + local, token = row / p.group;
             float x[2][4];
 #pragma unroll
             for (int h = 0; h < 2; ++h)
@@ -274,101 +283,68 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prompt_kernel(const b200q_k
         if (lane == 0) mbar_arrive(&q_full);
     }
 
-    if (warp >= LOADER) {
+    if (warp >= MMA) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(KP_OTHER_REGS));
-    if (warp == LOADER) {
-        // ---- loader: keys, keys, values, values of a unit's two pages
-        int pages = 0;
-        bool loading = false;
-        for (int e = 0; e < 4 * count; ++e) {
-            const int i = e >> 2, s = e % RING, block = 2 * (u0 + i) + (e & 1), part_kv = (e >> 1) & 1;
-            if ((e & 63) == 0) {                 // the next 32 pages
-                const int at = 2 * (u0 + i) + lane;
-                pages = at < full_pages ? c.table[static_cast<size_t>(slot) * c.blocks + at] : 0;
-            }
-            int page = __shfl_sync(0xffffffffu, pages, 2 * (i & 15) + (e & 1));
-            page = page >= 0 && page < c.pages ? page : 0;       // (a table that lacks the page: not beyond the pool)
-            if (e >= RING && !wait(&raw_free[s], (e / RING - 1) & 1)) break;
-            if (lane == 0) {
-                if (block < full_pages) {
-                    const size_t u = kv8_unit(page, c.layers, a.layer, part_kv, c.kv_heads, kvh);
-                    mbar_arrive_expect_tx(&raw_full[s], HALF_PAGE);
-                    bulk_copy_g2s(raw_s + s * Shape::RAW, c.codes + u * HALF_PAGE, HALF_PAGE, &raw_full[s]);
+        if (warp < MMA + 2) {
+        // ---- MMAs of tile t (the whole warp walks the loop, one elected lane issues). Units that the tile does not need are
+        // released as they come.
+        constexpr uint32_t s_idesc = umma_idesc_f16(KP_ROWS, KP_KEYS), o_idesc = umma_idesc_f16(KP_ROWS, DH);
+        const int t = warp - MMA, mine = t ? count1 : count0;
+        const uint64_t any_desc = smem_desc_sw128(smem);
+        const uint32_t hi = static_cast<uint32_t>(any_desc >> 32), lo = static_cast<uint32_t>(any_desc);
+        const uint32_t q_lo = lo + t * (Shape::Q / 2 >> 4), k_lo = lo + ((SPLIT ? 2 : 1) * Shape::Q >> 4), v_lo = k_lo + (KS * Shape::K >> 4);
+        const uint32_t s_at = tmem + S_COL + 128 * t, o_at = tmem + O_COL + DH * t;
+        auto scores = [&](int i) {
+            const int s = i % KS;
+            const uint32_t kd = k_lo + s * (Shape::K >> 4);
+            if (elect_one()) {
+                if (i < mine) {
+#pragma unroll
+                    for (int part_q = 0; part_q < (SPLIT ? 2 : 1); ++part_q)
+#pragma unroll
+                        for (int k = 0; k < DH / 16; ++k)
+                            umma_f16_ss(s_at, q_lo + ((part_q * Shape::Q + (k / 4) * (KP_ROWS * 128)) >> 4) + 2 * (k % 4),
+                                        kd + (((k / 4) * K_SLAB) >> 4) + 2 * (k % 4), hi, s_idesc, part_q + k > 0);
+                    umma_commit<false>(smem_u32(&s_full[t]));
+                    umma_commit<false>(smem_u32(&k_free[s]));
                 } else {
-                    mbar_arrive(&raw_full[s]);                   // the converters read the tail themselves
+                    mbar_arrive(&k_free[s]);
                 }
             }
             __syncwarp();
-            loading = true;
-        }
-        if (abort_flag && loading) {
-            // copies already requested still write shared memory; they complete on their own within microseconds
-            const uint64_t t0 = global_timer_ns();
-            while (global_timer_ns() - t0 < 100000) {
-            }
-        }
-        __syncwarp();
-    } else if (warp == MMA) {
-        // ---- MMAs (the whole warp walks the loop, one elected lane issues)
-        constexpr uint32_t s_idesc = umma_idesc_f16(KP_ROWS, KP_KEYS), o_idesc = umma_idesc_f16(KP_ROWS, DH);
-        const uint64_t q_desc = smem_desc_sw128(q_s), k_desc = smem_desc_sw128(k_s), v_desc = smem_desc_sw128(v_s);
-        auto scores = [&](int t, int i) {        // S of tile t for unit i
-            const uint64_t kd = k_desc + static_cast<uint32_t>((i % KS) * Shape::K >> 4);
-            const uint64_t qd = q_desc + static_cast<uint32_t>(t * (Shape::Q / 2) >> 4);
+        };
+        auto values = [&](int i) {
+            const int s = i % VS;
+            const uint32_t vd = v_lo + s * (Shape::K >> 4);
             if (elect_one()) {
+                if (i < mine) {
 #pragma unroll
-                for (int part_q = 0; part_q < (SPLIT ? 2 : 1); ++part_q)
-#pragma unroll
-                    for (int k = 0; k < DH / 16; ++k)
-                        umma_bf16<false>(tmem + S_COL + 128 * t, qd + static_cast<uint32_t>((part_q * Shape::Q + (k / 4) * (KP_ROWS * 128)) >> 4) + 2 * (k % 4),
-                                         kd + static_cast<uint32_t>(((k / 4) * K_SLAB) >> 4) + 2 * (k % 4), s_idesc, part_q + k > 0);
-                umma_commit<false>(smem_u32(&s_full[t]));
+                    for (int k = 0; k < 8; ++k)
+                        umma_f16_ts(o_at, s_at + P_COL + 8 * k, vd + (((k / 4) * V_PAGE) >> 4) + 2 * (k % 4), hi, o_idesc, k > 0 ? 1u : i > 0);
+                    if (i + 1 == mine) umma_commit<false>(smem_u32(&o_done[t]));
+                    umma_commit<false>(smem_u32(&v_free[s]));
+                } else {
+                    mbar_arrive(&v_free[s]);
+                }
             }
             __syncwarp();
         };
-        auto values = [&](int t, int i, bool last) {
-            const uint64_t vd = v_desc + static_cast<uint32_t>((i % VS) * Shape::K >> 4);
-            if (elect_one()) {
-#pragma unroll
-                for (int k = 0; k < 8; ++k)
-                    umma_f16_ts(tmem + O_COL + DH * t, tmem + S_COL + 128 * t + P_COL + 8 * k, vd + static_cast<uint32_t>(((k / 4) * V_PAGE) >> 4) + 2 * (k % 4),
-                                o_idesc, i + k > 0);
-                if (last) umma_commit<false>(smem_u32(&o_done[t]));
-            }
-            __syncwarp();
-        };
-        auto release = [&](uint64_t *bar) {
-            if (elect_one()) umma_commit<false>(smem_u32(bar));
-            __syncwarp();
-        };
-        const bool fine = wait(&q_full, 0) && wait(&k_full[0], 0);
-        if (fine) {
-            tc_fence_after();
-            if (count0) scores(0, 0);
-            if (count1) scores(1, 0);
-            release(&k_free[0]);
-        }
+        bool fine = wait(&q_full, 0) && wait(&k_full[0], 0);
+        tc_fence_after();
+        if (fine) scores(0);
         for (int i = 0; fine && i < count; ++i) {
             const int next = i + 1;
-            if (!wait(&v_full[i % VS], (i / VS) & 1)) break;
-            if (i < count0) {
-                if (!wait(&p_full[0], i & 1)) break;
-                tc_fence_after();
-                values(0, i, next == count0);
-            }
-            if (next < count && !wait(&k_full[next % KS], (next / KS) & 1)) break;
+            fine = wait(&v_full[i % VS], (i / VS) & 1) && (i >= mine || wait(&p_full[t], i & 1));
+            if (!fine) break;
             tc_fence_after();
-            if (next < count0) scores(0, next);
-            if (i < count1) {
-                if (!wait(&p_full[1], i & 1)) break;
-                tc_fence_after();
-                values(1, i, next == count1);
-            }
-            release(&v_free[i % VS]);
-            if (next < count1) scores(1, next);
-            if (next < count) release(&k_free[next % KS]);
+            values(i);
+            if (next == count) break;
+            fine = wait(&k_full[next % KS], (next / KS) & 1);
+            if (!fine) break;
+            tc_fence_after();
+            scores(next);
         }
-    }
+        }
     } else if (warp >= KP_SOFTMAX_WARPS) {
         // ---- converters
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(KP_OTHER_REGS));
@@ -383,58 +359,92 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prompt_kernel(const b200q_k
             return top < 0x7f800000u ? power_inverse(power_of(top)) : 0.f;
         };
         auto half_of = [&](uint32_t w, float inv) { return inv == 0.f ? 0u : tail_to_half<BF16>(w, inv); };
-        bool fine = true;
-        for (int i = 0; fine && i < count; ++i) {
-#pragma unroll 1
-            for (int e = 4 * i; e < 4 * i + 4; ++e) {
-                const int s = e % RING, h = e & 1, block = 2 * (u0 + i) + h;
-                const bool keys = (e & 2) == 0;
-                const uint8_t *raw = raw_s + s * Shape::RAW;
-                fine = wait(&raw_full[s], (e / RING) & 1);
-                if (fine && h == 0) fine = keys ? i < KS || wait(&k_free[i % KS], (i / KS - 1) & 1) : i < VS || wait(&v_free[i % VS], (i / VS - 1) & 1);
-                if (!fine) break;
-                uint8_t *to = keys ? k_s + (i % KS) * Shape::K + h * (KV8_BLOCK * 128) : v_s + (i % VS) * Shape::K + h * V_PAGE;
-                if (block < full_pages) {
-                    // a thread's pieces of sixteen codes: (row, quarter) of 64-code rows
-                    uint4 w[SLABS * 2];
-                    if (keys) {
+        auto page_at = [&](int block) {
+            const int page = block < full_pages ? c.table[static_cast<size_t>(slot) * c.blocks + block] : 0;
+            return page;
+        };
+        // a thread's sixteen-code pieces of half a page: (row, quarter) of 64-code rows
+        using Half = uint4[SLABS * 2];
+        auto fetch = [&](Half &w, int block, int page, bool keys) {
+            if (block >= full_pages) return;
+            page = page >= 0 && page < c.pages ? page : 0;       // (a table that lacks the page: not beyond the pool)
+            const int8_t *from = c.codes + kv8_unit(page, c.layers, a.layer, keys ? 0 : 1, c.kv_heads, kvh) * HALF_PAGE;
 #pragma unroll
-                        for (int j = 0; j < SLABS * 2; ++j) w[j] = *reinterpret_cast<const uint4 *>(raw + ((ct >> 2) + 32 * (j & 1)) * DH + (j >> 1) * 64 + (ct & 3) * 16);
+            for (int j = 0; j < SLABS * 2; ++j)
+                w[j] = *reinterpret_cast<const uint4 *>(from + (keys ? ((ct >> 2) + 32 * (j & 1)) * DH + (j >> 1) * 64 + (ct & 3) * 16 : (ct + 128 * j) * 16));
+        };
+        auto store = [&](const Half &w, int block, bool keys, uint8_t *to) {
+            if (block < full_pages) {
 #pragma unroll
-                        for (int j = 0; j < SLABS * 2; ++j) convert16(w[j], to + (j >> 1) * K_SLAB, (ct >> 2) + 32 * (j & 1), ct & 3);
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < SLABS * 2; ++j) w[j] = *reinterpret_cast<const uint4 *>(raw + (ct + 128 * j) * 16);
-#pragma unroll
-                        for (int j = 0; j < SLABS * 2; ++j) convert16(w[j], to, (ct >> 2) + 32 * j, ct & 3);
-                    }
-                } else {
-                    const int have = block == full_pages ? rest : 0;
-                    const float inv = have ? tail_inverse(!keys) : 0.f;
-                    if (keys) {
-                        for (int id = ct; id < KV8_BLOCK * DH / 8; id += 128) {
-                            const int key = id / (DH / 8), chunk = id % (DH / 8);
-                            uint4 w = make_uint4(0u, 0u, 0u, 0u);
-                            if (key < have) w = *reinterpret_cast<const uint4 *>(tail_k + key * DH + 8 * chunk);
-                            *reinterpret_cast<uint4 *>(to + (chunk >> 3) * K_SLAB + swizzled(key, chunk & 7)) =
-                                make_uint4(half_of(w.x, inv), half_of(w.y, inv), half_of(w.z, inv), half_of(w.w, inv));
-                        }
-                    } else {
-                        for (int id = ct; id < KV8_BLOCK * DH / 2; id += 128) {
-                            const int key = id / (DH / 2), d = id % (DH / 2) * 2;
-                            const uint32_t w = key < have ? half_of(*reinterpret_cast<const uint32_t *>(tail_v + key * DH + d), inv) : 0u;
-                            *reinterpret_cast<uint16_t *>(to + swizzled(d, key >> 3) + (key & 7) * 2) = static_cast<uint16_t>(w);
-                            *reinterpret_cast<uint16_t *>(to + swizzled(d + 1, key >> 3) + (key & 7) * 2) = static_cast<uint16_t>(w >> 16);
-                        }
-                    }
+                for (int j = 0; j < SLABS * 2; ++j) {
+                    if (keys) convert16(w[j], to + (j >> 1) * K_SLAB, (ct >> 2) + 32 * (j & 1), ct & 3);
+                    else convert16(w[j], to, (ct >> 2) + 32 * j, ct & 3);
                 }
-                if (h == 1) fence_proxy_async();
-                __syncwarp();
-                if (lane == 0) {
-                    mbar_arrive(&raw_free[s]);
-                    if (h == 1) mbar_arrive(keys ? &k_full[i % KS] : &v_full[i % VS]);
+                return;
+            }
+            const int have = block == full_pages ? rest : 0;
+            const float inv = have ? tail_inverse(!keys) : 0.f;
+            if (keys) {
+                for (int id = ct; id < KV8_BLOCK * DH / 8; id += 128) {
+                    const int key = id / (DH / 8), chunk = id % (DH / 8);
+                    uint4 x = make_uint4(0u, 0u, 0u, 0u);
+                    if (key < have) x = *reinterpret_cast<const uint4 *>(tail_k + key * DH + 8 * chunk);
+                    *reinterpret_cast<uint4 *>(to + (chunk >> 3) * K_SLAB + swizzled(key, chunk & 7)) =
+                        make_uint4(half_of(x.x, inv), half_of(x.y, inv), half_of(x.z, inv), half_of(x.w, inv));
+                }
+            } else {
+                for (int id = ct; id < KV8_BLOCK * DH / 2; id += 128) {
+                    const int key = id / (DH / 2), d = id % (DH / 2) * 2;
+                    const uint32_t x = key < have ? half_of(*reinterpret_cast<const uint32_t *>(tail_v + key * DH + d), inv) : 0u;
+                    *reinterpret_cast<uint16_t *>(to + swizzled(d, key >> 3) + (key & 7) * 2) = static_cast<uint16_t>(x);
+                    *reinterpret_cast<uint16_t *>(to + swizzled(d + 1, key >> 3) + (key & 7) * 2) = static_cast<uint16_t>(x >> 16);
                 }
             }
+        };
+        auto publish = [&](uint64_t *bar) {
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar);
+        };
+        // asks L2 for a page: a thread for some of its 128-byte lines
+        auto ask = [&](int block, int page) {
+            if (block >= full_pages || page < 0 || page >= c.pages) return;
+            const int8_t *from = c.codes + kv8_unit(page, c.layers, a.layer, 0, c.kv_heads, kvh) * HALF_PAGE;
+            constexpr int LINES = HALF_PAGE / 128;           // of the keys; as many of the values
+            if (ct < 2 * LINES)
+                asm volatile("prefetch.global.L2 [%0];" ::"l"(from + (ct < LINES ? ct : ct - LINES) * 128 + (ct < LINES ? 0 : static_cast<size_t>(c.kv_heads) * HALF_PAGE)));
+        };
+        static_assert(2 * HALF_PAGE / 128 <= KP_CONVERT_WARPS * 32, "one line per thread");
+        Half even, odd;                          // the unit's first and second page: keys, then values
+        int far0 = page_at(2 * (u0 + KP_AHEAD)), far1 = page_at(2 * (u0 + KP_AHEAD) + 1);
+        int page0 = page_at(2 * u0), page1 = page_at(2 * u0 + 1);
+        fetch(even, 2 * u0, page0, true);
+        fetch(odd, 2 * u0 + 1, page1, true);
+        for (int i = 0; i < count; ++i) {
+            const int block = 2 * (u0 + i);
+            const bool more = i + 1 < count;
+            uint8_t *k_to = k_s + (i % KS) * Shape::K, *v_to = v_s + (i % VS) * Shape::K;
+            const int next0 = more ? page_at(block + 2) : 0, next1 = more ? page_at(block + 3) : 0;
+            if (i + KP_AHEAD < count) {
+                ask(block + 2 * KP_AHEAD, far0);
+                ask(block + 2 * KP_AHEAD + 1, far1);
+            }
+            far0 = page_at(block + 2 * KP_AHEAD + 2);
+            far1 = page_at(block + 2 * KP_AHEAD + 3);
+            if (i >= KS && !wait(&k_free[i % KS], (i / KS - 1) & 1)) break;
+            store(even, block, true, k_to);
+            fetch(even, block, page0, false);
+            store(odd, block + 1, true, k_to + KV8_BLOCK * 128);
+            fetch(odd, block + 1, page1, false);
+            publish(&k_full[i % KS]);
+            if (i >= VS && !wait(&v_free[i % VS], (i / VS - 1) & 1)) break;
+            store(even, block, false, v_to);
+            if (more) fetch(even, block + 2, next0, true);
+            store(odd, block + 1, false, v_to + V_PAGE);
+            if (more) fetch(odd, block + 3, next1, true);
+            publish(&v_full[i % VS]);
+            page0 = next0;
+            page1 = next1;
         }
     } else {
         // ---- softmax: a thread per row
@@ -444,16 +454,18 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prompt_kernel(const b200q_k
         const int token = valid ? row / p.group : 0, pos = start + token;
         const size_t out_row = static_cast<size_t>(first + token) * a.heads + kvh * p.group + (valid ? row - token * p.group : 0);
         const uint32_t lanes = static_cast<uint32_t>(32 * (warp & 3)) << 16;
-        float m = -INFINITY, l = 0.f, reference = 0.f;       // reference: U
+        float m = -INFINITY, l = 0.f, reference = 0.f, per_reference = power_inverse(0.f);      // U and its reciprocal
         bool fine = wait(&q_full, 0);
         const float factor = factor_s[t * KP_ROWS + local];
+        const float *layer_scales = c.scales + kv8_unit(0, c.layers, a.layer, 0, c.kv_heads, kvh);
+        const int page_scales = c.layers * 2 * c.kv_heads;
         // scales of a unit's two blocks, read a unit ahead (their pages two units ahead)
         auto page_at = [&](int block) { return block < full_pages ? c.table[static_cast<size_t>(slot) * c.blocks + block] : 0; };
         auto scales_at = [&](int block, int page, float &ks, float &vs) {
             if (block < full_pages) {
-                const size_t u = kv8_unit(page >= 0 && page < c.pages ? page : 0, c.layers, a.layer, 0, c.kv_heads, kvh);
-                ks = c.scales[u];
-                vs = c.scales[u + c.kv_heads];
+                const float *from = layer_scales + static_cast<size_t>(page >= 0 && page < c.pages ? page : 0) * page_scales;
+                ks = from[0];
+                vs = from[c.kv_heads];
             } else if (block * KV8_BLOCK < total) {
                 const size_t u = kv8_unit(slot, c.layers, a.layer, 0, c.kv_heads, kvh);
                 ks = power_of(abs_bits(c.peak[u]));
@@ -486,12 +498,12 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prompt_kernel(const b200q_k
                 if (power > 8.f * reference) {
                     alpha *= reference * power_inverse(power);
                     reference = power;
+                    per_reference = power_inverse(power);
                 }
                 relative[h] = vs;
             }
             // a weight's factor `relative` as an addend of its exponent; one too small to matter next to U counts as zero, and
             // its weights only enter the sum
-            const float per_reference = power_inverse(reference);
             float addend[2], divide[2];
             bool nothing[2];
 #pragma unroll
