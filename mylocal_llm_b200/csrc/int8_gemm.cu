@@ -74,9 +74,8 @@ __global__ void __launch_bounds__(256) int8_quantize_kernel(const void *x, int d
     const float s = int8_scale(peak), inv = __fdiv_rn(1.f, s);
     if (tid == 0) scales[blockIdx.x] = s;
     auto put = [&](int c, const float (&f)[8]) {
-        uint32_t w[2] = {0u, 0u};
-#pragma unroll
-        for (int e = 0; e < 8; ++e) w[e >> 2] |= (static_cast<uint32_t>(int8_code(f[e], s, inv)) & 0xffu) << (8 * (e & 3));
+        const float lo[4] = {f[0], f[1], f[2], f[3]}, hi[4] = {f[4], f[5], f[6], f[7]};
+        const uint32_t w[2] = {int8_codes(lo, s, inv), int8_codes(hi, s, inv)};
         *reinterpret_cast<uint2 *>(codes + blockIdx.x * static_cast<size_t>(codes_row) + c) = make_uint2(w[0], w[1]);
     };
 #pragma unroll

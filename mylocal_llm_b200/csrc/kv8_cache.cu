@@ -150,11 +150,6 @@ __device__ __forceinline__ void load4(const void *p, int dtype, size_t i, float 
     }
 }
 
-// A value as the cache's 16-bit type holds it.
-template <bool BF16>
-__device__ __forceinline__ float round16(float v) {
-    return BF16 ? __bfloat162float(__float2bfloat16_rn(v)) : __half2float(__float2half_rn(v));
-}
 template <bool BF16>
 __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
     if (BF16) {
@@ -164,30 +159,66 @@ __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
     const __half2 p = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t *>(&p);
 }
-
-// x0 * c - x1 * s and x0 * s + x1 * c, correctly rounded to FP32 (both products are exact in 64 bits): the rounding to the
-// cache's type and the codes then follow from the inputs alone, whatever order another program computes in.
-__device__ __forceinline__ void rotate64(float x0, float x1, float c, float s, float &lo, float &hi) {
-    const double a = x0, b = x1, cc = c, ss = s;
-    lo = __double2float_rn(__fma_rn(a, cc, -__dmul_rn(b, ss)));
-    hi = __double2float_rn(__fma_rn(a, ss, __dmul_rn(b, cc)));
+template <bool BF16>
+__device__ __forceinline__ float2 unpack16(uint32_t w) {
+    return BF16 ? make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)) : __half22float2(*reinterpret_cast<const __half2 *>(&w));
 }
 
-// One CTA of 256 threads = one block of 64 tokens of one sequence and key/value head. A thread holds quads of four
-// consecutive dimensions: of the keys the quad at i and its partner at i + head_dim / 2 (which the rotation needs), of the
-// values two quads, all in registers; 64 * head_dim / 8 / 256 such pairs per thread. A block that becomes full takes its
-// older tokens from the tail, finds the two largest magnitudes, and its codes pass through shared memory (the values
-// transposed) to 16-byte stores; one that does not goes to the tail. Bound by memory: every new token is read once (as
-// projection output) and written once.
+// Rotated pairs of four consecutive dimensions, rounded to FP32 and then to the cache's type as if both products and their sum
+// were exact up to 64 bits (both products are): what a cache holds then follows from the inputs alone, whatever order another
+// program computes in. FP32 first: with the error's bound added and taken off, both ends round to the same 16-bit number
+// unless a border lies between them, which about one in 2^11 (BF16) values meets; then the quad goes through 64 bits.
+template <bool BF16>
+static __device__ __noinline__ void rotate_exact(const float (&x0)[4], const float (&x1)[4], const float (&c)[4], const float (&s)[4], uint32_t (&out)[4]) {
+    float lo[4], hi[4];
+    for (int e = 0; e < 4; ++e) {
+        const double a = x0[e], b = x1[e], cc = c[e], ss = s[e];
+        lo[e] = __double2float_rn(__fma_rn(a, cc, -__dmul_rn(b, ss)));
+        hi[e] = __double2float_rn(__fma_rn(a, ss, __dmul_rn(b, cc)));
+    }
+    for (int e = 0; e < 2; ++e) {
+        out[e] = pack16<BF16>(lo[2 * e], lo[2 * e + 1]);
+        out[2 + e] = pack16<BF16>(hi[2 * e], hi[2 * e + 1]);
+    }
+}
+// out: the quad at i as two words, then its partner's.
+template <bool BF16>
+__device__ __forceinline__ void rotate_quad(const float (&x0)[4], const float (&x1)[4], const float (&c)[4], const float (&s)[4], uint32_t (&out)[4]) {
+    constexpr float BOUND = 2.3841858e-7f;               // 2^-22: twice the two roundings' 2^-24 of product and sum each
+    uint32_t differ = 0u;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+            float v[2], w[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int i = 2 * p + e;
+                const float product = h ? __fmul_rn(x1[i], c[i]) : -__fmul_rn(x1[i], s[i]);
+                v[e] = __fmaf_rn(x0[i], h ? s[i] : c[i], product);
+                w[e] = __fmul_rn(fabsf(product) + fabsf(v[e]), BOUND);
+            }
+            out[2 * h + p] = pack16<BF16>(v[0] + w[0], v[1] + w[1]);
+            differ |= out[2 * h + p] ^ pack16<BF16>(v[0] - w[0], v[1] - w[1]);
+        }
+    if (differ) rotate_exact<BF16>(x0, x1, c, s, out);
+}
+
+// One CTA of 4 DH threads = one block of 64 tokens of one sequence and key/value head, the first half of the threads its keys,
+// the second its values. A thread holds four consecutive tokens x (a quad of dimensions at i and its partner at i + DH / 2, which
+// the rotation needs), as 16-bit pairs. A block that becomes full takes its older tokens from the tail and finds the largest
+// magnitude (16-bit integers order 16-bit floats, NaN and infinities on top); keys go out as words of four codes, values as words
+// of four tokens of a dimension (a transposition of bytes in registers) that pass through shared memory. One that does not become
+// full goes to the tail. Bound by memory - every new token is read once, as projection output, and written once - and, next to
+// it, by the instructions per element: with 64-bit rotations, exact codes one by one and byte stores 3 x 8192 tokens took 83 us.
 template <int DH, bool BF16, bool VEC>
-__global__ void __launch_bounds__(256) kv8_append_kernel(const b200q_kv8_cache c, const Kv8Append a) {
-    constexpr int HALF = DH / 2, QUADS = HALF / 4, TOKENS = 256 / QUADS, PASSES = KV8_BLOCK / TOKENS;
-    __shared__ __align__(16) uint8_t k_s[KV8_BLOCK * DH];
-    __shared__ __align__(16) uint8_t v_s[KV8_BLOCK * DH];
-    __shared__ uint32_t peaks[2][8];
+__global__ void __launch_bounds__(4 * DH) kv8_append_kernel(const b200q_kv8_cache c, const Kv8Append a) {
+    constexpr int HALF = DH / 2, QUADS = HALF / 4, WARPS = DH / 16, LD = KV8_BLOCK / 4 + 1;      // warps per part; words of a row
+    __shared__ uint32_t v_s[DH * LD];
+    __shared__ uint32_t peaks[2 * WARPS];
     chain_trigger();
     chain_wait();
-    const int tid = threadIdx.x, b = blockIdx.z, head = blockIdx.y;
+    const int tid = threadIdx.x, part = tid / (2 * DH), at = tid % (2 * DH), b = blockIdx.z, head = blockIdx.y;
     const int start = a.starts[b], row0 = a.offsets[b], n = a.offsets[b + 1] - row0;
     if (start < 0 || n <= 0) return;
     const int total = start + n, first = start / KV8_BLOCK, last = (total - 1) / KV8_BLOCK;
@@ -199,124 +230,105 @@ __global__ void __launch_bounds__(256) kv8_append_kernel(const b200q_kv8_cache c
     const bool both = opened && last > first && total % KV8_BLOCK != 0;
     if (both && block == last) return;
     const int slot = a.slots[b];
-    const size_t unit_k = kv8_unit(slot, c.layers, a.layer, 0, c.kv_heads, head), unit_v = unit_k + c.kv_heads;
-    uint16_t *tail_k = static_cast<uint16_t *>(c.tail) + unit_k * (KV8_BLOCK * DH);
-    uint16_t *tail_v = static_cast<uint16_t *>(c.tail) + unit_v * (KV8_BLOCK * DH);
-    const int i = (tid % QUADS) * 4, t0 = tid / QUADS;
+    const size_t unit = kv8_unit(slot, c.layers, a.layer, part, c.kv_heads, head);
+    uint16_t *tail = static_cast<uint16_t *>(c.tail) + unit * (KV8_BLOCK * DH);
+    const int i = (at % QUADS) * 4, t0 = at / QUADS * 4;
+    const void *in = part ? a.v : a.k;
+    const long long in_row = part ? a.v_row : a.k_row;
 
     for (;; block = last) {
         const int base = block * KV8_BLOCK;
         const bool full = base + KV8_BLOCK <= total;
-        float kq[PASSES][2][4], vq[PASSES][2][4];
-        uint32_t kp = 0u, vp = 0u;
+        uint32_t x[4][4];                                // [token][quad as two words, partner]
+        uint32_t top = 0u;
 #pragma unroll
-        for (int p = 0; p < PASSES; ++p) {
-            const int t = p * TOKENS + t0, pos = base + t;
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) kq[p][h][e] = vq[p][h][e] = 0.f;
+        for (int j = 0; j < 4; ++j) {
+            const int pos = base + t0 + j;
+            float lo[4] = {0.f, 0.f, 0.f, 0.f}, hi[4] = {0.f, 0.f, 0.f, 0.f};
             if (pos >= start && pos < total) {
-                const long long row = row0 + (pos - start);
-                const size_t at_k = row * a.k_row + static_cast<size_t>(head) * DH + i;
-                const size_t at_v = row * a.v_row + static_cast<size_t>(head) * DH + i;
-                float x[2][4];
-                load4<VEC>(a.k, a.in_dtype, at_k, x[0]);
-                load4<VEC>(a.k, a.in_dtype, at_k + HALF, x[1]);
-                load4<VEC>(a.v, a.in_dtype, at_v, vq[p][0]);
-                load4<VEC>(a.v, a.in_dtype, at_v + HALF, vq[p][1]);
-                if (a.cos_t) {
-                    const float4 cq = *reinterpret_cast<const float4 *>(a.cos_t + static_cast<size_t>(pos) * HALF + i);
-                    const float4 sq = *reinterpret_cast<const float4 *>(a.sin_t + static_cast<size_t>(pos) * HALF + i);
-                    const float cv[4] = {cq.x, cq.y, cq.z, cq.w}, sv[4] = {sq.x, sq.y, sq.z, sq.w};
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) rotate64(x[0][e], x[1][e], cv[e], sv[e], x[0][e], x[1][e]);
+                const size_t from = (row0 + (pos - start)) * static_cast<size_t>(in_row) + static_cast<size_t>(head) * DH + i;
+                load4<VEC>(in, a.in_dtype, from, lo);
+                load4<VEC>(in, a.in_dtype, from + HALF, hi);
+            }
+            if (part == 0 && a.cos_t && pos >= start && pos < total) {
+                const float4 cq = *reinterpret_cast<const float4 *>(a.cos_t + static_cast<size_t>(pos) * HALF + i);
+                const float4 sq = *reinterpret_cast<const float4 *>(a.sin_t + static_cast<size_t>(pos) * HALF + i);
+                const float cv[4] = {cq.x, cq.y, cq.z, cq.w}, sv[4] = {sq.x, sq.y, sq.z, sq.w};
+                rotate_quad<BF16>(lo, hi, cv, sv, x[j]);
+            } else {
+                x[j][0] = pack16<BF16>(lo[0], lo[1]);
+                x[j][1] = pack16<BF16>(lo[2], lo[3]);
+                x[j][2] = pack16<BF16>(hi[0], hi[1]);
+                x[j][3] = pack16<BF16>(hi[2], hi[3]);
+                if (full && pos < start) {               // (only the first block has older tokens)
+                    const uint2 u = *reinterpret_cast<const uint2 *>(tail + (t0 + j) * DH + i), w = *reinterpret_cast<const uint2 *>(tail + (t0 + j) * DH + i + HALF);
+                    x[j][0] = u.x;
+                    x[j][1] = u.y;
+                    x[j][2] = w.x;
+                    x[j][3] = w.y;
                 }
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        kq[p][h][e] = round16<BF16>(x[h][e]);
-                        vq[p][h][e] = round16<BF16>(vq[p][h][e]);
-                    }
-            } else if (full && pos < start) {            // (only the first block has older tokens)
-                const size_t at = static_cast<size_t>(t) * DH + i;
-                load4<true>(tail_k, BF16 ? B200Q_BF16 : B200Q_F16, at, kq[p][0]);
-                load4<true>(tail_k, BF16 ? B200Q_BF16 : B200Q_F16, at + HALF, kq[p][1]);
-                load4<true>(tail_v, BF16 ? B200Q_BF16 : B200Q_F16, at, vq[p][0]);
-                load4<true>(tail_v, BF16 ? B200Q_BF16 : B200Q_F16, at + HALF, vq[p][1]);
             }
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    kp = max(kp, abs_bits(kq[p][h][e]));
-                    vp = max(vp, abs_bits(vq[p][h][e]));
-                }
+            for (int e = 0; e < 4; ++e) top = __vmaxu2(top, x[j][e] & 0x7fff7fffu);
         }
-        kp = __reduce_max_sync(0xffffffffu, kp);
-        vp = __reduce_max_sync(0xffffffffu, vp);
-        if ((tid & 31) == 0) {
-            peaks[0][tid >> 5] = kp;
-            peaks[1][tid >> 5] = vp;
-        }
+        top = __reduce_max_sync(0xffffffffu, max(top & 0xffffu, top >> 16));
+        if ((tid & 31) == 0) peaks[tid >> 5] = top;
         __syncthreads();
 #pragma unroll
-        for (int w = 0; w < 8; ++w) {
-            kp = max(kp, peaks[0][w]);
-            vp = max(vp, peaks[1][w]);
-        }
+        for (int w = 0; w < WARPS; ++w) top = max(top, peaks[part * WARPS + w]);
+        const uint32_t peak = abs_bits(unpack16<BF16>(top).x);
         if (full) {
-            const float ks = int8_scale(kp), vs = int8_scale(vp);
-            const float ki = __fdiv_rn(1.f, ks), vi = __fdiv_rn(1.f, vs);
+            const float s = int8_scale(peak), inv = __fdiv_rn(1.f, s);
+            const int page = c.table[static_cast<size_t>(slot) * c.blocks + block];
+            const bool held = page >= 0 && page < c.pages;       // (a table that lacks the page loses the block, not memory)
+            const size_t u = kv8_unit(held ? page : 0, c.layers, a.layer, part, c.kv_heads, head);
+            int8_t *to = c.codes + u * (KV8_BLOCK * DH);
+            uint32_t code[2][4];                         // [half][token]: four dimensions
 #pragma unroll
-            for (int p = 0; p < PASSES; ++p) {
-                const int t = p * TOKENS + t0;
+            for (int j = 0; j < 4; ++j)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    uint32_t word = 0u;
+                    const float2 p = unpack16<BF16>(x[j][2 * h]), q = unpack16<BF16>(x[j][2 * h + 1]);
+                    const float v[4] = {p.x, p.y, q.x, q.y};
+                    code[h][j] = int8_codes(v, s, inv);
+                }
+            if (part == 0) {
+                if (held)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        word |= (static_cast<uint32_t>(int8_code(kq[p][h][e], ks, ki)) & 0xffu) << (8 * e);
-                        v_s[(i + h * HALF + e) * KV8_BLOCK + t] = static_cast<uint8_t>(int8_code(vq[p][h][e], vs, vi));
+                    for (int j = 0; j < 4; ++j)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) *reinterpret_cast<uint32_t *>(to + (t0 + j) * DH + i + h * HALF) = code[h][j];
+            } else {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {            // four tokens x four dimensions of bytes, transposed
+                    const uint32_t a01 = __byte_perm(code[h][0], code[h][1], 0x5140), b01 = __byte_perm(code[h][0], code[h][1], 0x7362);
+                    const uint32_t a23 = __byte_perm(code[h][2], code[h][3], 0x5140), b23 = __byte_perm(code[h][2], code[h][3], 0x7362);
+                    uint32_t *row = v_s + (i + h * HALF) * LD + t0 / 4;
+                    row[0] = __byte_perm(a01, a23, 0x5410);
+                    row[LD] = __byte_perm(a01, a23, 0x7632);
+                    row[2 * LD] = __byte_perm(b01, b23, 0x5410);
+                    row[3 * LD] = __byte_perm(b01, b23, 0x7632);
+                }
+                named_barrier_sync(1, 2 * DH);
+                if (held)
+#pragma unroll
+                    for (int j = at; j < DH * 4; j += 2 * DH) {
+                        const uint32_t *row = v_s + (j >> 2) * LD + 4 * (j & 3);
+                        reinterpret_cast<uint4 *>(to)[j] = make_uint4(row[0], row[1], row[2], row[3]);
                     }
-                    *reinterpret_cast<uint32_t *>(k_s + t * DH + i + h * HALF) = word;
-                }
             }
-            __syncthreads();
-            const int page = c.table[static_cast<size_t>(slot) * c.blocks + block];
-            if (page >= 0 && page < c.pages) {           // (a table that lacks the page loses the block, not memory)
-                const size_t u = kv8_unit(page, c.layers, a.layer, 0, c.kv_heads, head);
-                uint4 *kd = reinterpret_cast<uint4 *>(c.codes + u * (KV8_BLOCK * DH));
-                uint4 *vd = reinterpret_cast<uint4 *>(c.codes + (u + c.kv_heads) * (KV8_BLOCK * DH));
-                for (int j = tid; j < KV8_BLOCK * DH / 16; j += 256) {
-                    kd[j] = reinterpret_cast<const uint4 *>(k_s)[j];
-                    vd[j] = reinterpret_cast<const uint4 *>(v_s)[j];
-                }
-                if (tid == 0) {
-                    c.scales[u] = ks;
-                    c.scales[u + c.kv_heads] = vs;
-                }
-            }
+            if (at == 0 && held) c.scales[u] = s;
         } else {
 #pragma unroll
-            for (int p = 0; p < PASSES; ++p) {
-                const int t = p * TOKENS + t0, pos = base + t;
+            for (int j = 0; j < 4; ++j) {
+                const int pos = base + t0 + j;
                 if (pos < start || pos >= total) continue;
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const size_t at = static_cast<size_t>(t) * DH + i + h * HALF;
-                    *reinterpret_cast<uint2 *>(tail_k + at) = make_uint2(pack16<BF16>(kq[p][h][0], kq[p][h][1]),
-                                                                         pack16<BF16>(kq[p][h][2], kq[p][h][3]));
-                    *reinterpret_cast<uint2 *>(tail_v + at) = make_uint2(pack16<BF16>(vq[p][h][0], vq[p][h][1]),
-                                                                         pack16<BF16>(vq[p][h][2], vq[p][h][3]));
-                }
+                *reinterpret_cast<uint2 *>(tail + (t0 + j) * DH + i) = make_uint2(x[j][0], x[j][1]);
+                *reinterpret_cast<uint2 *>(tail + (t0 + j) * DH + i + HALF) = make_uint2(x[j][2], x[j][3]);
             }
-            if (tid == 0) {
-                const bool older = block == first && opened;
-                const uint32_t ko = older ? abs_bits(c.peak[unit_k]) : 0u, vo = older ? abs_bits(c.peak[unit_v]) : 0u;
-                c.peak[unit_k] = __uint_as_float(max(kp, ko));
-                c.peak[unit_v] = __uint_as_float(max(vp, vo));
+            if (at == 0) {
+                const uint32_t older = block == first && opened ? abs_bits(c.peak[unit]) : 0u;
+                c.peak[unit] = __uint_as_float(max(peak, older));
             }
         }
         if (!both || block != first) break;
@@ -564,7 +576,7 @@ extern "C" int b200q_kv8_append(const b200q_kv8_cache *cache, int layer, const v
                 : (vec ? kv8_append_kernel<64, false, true> : kv8_append_kernel<64, false, false>))
         : (bf16 ? (vec ? kv8_append_kernel<128, true, true> : kv8_append_kernel<128, true, false>)
                 : (vec ? kv8_append_kernel<128, false, true> : kv8_append_kernel<128, false, false>));
-    launch_chained(kernel, grid, dim3(256), 0, static_cast<cudaStream_t>(stream), *cache, a);
+    launch_chained(kernel, grid, dim3(4 * cache->head_dim), 0, static_cast<cudaStream_t>(stream), *cache, a);
     return check_launch("kv8_append");
 }
 

@@ -39,7 +39,7 @@ __device__ __forceinline__ float int8_scale(uint32_t peak) {
 // 2^-15 (|x / s| < 128), so only the neighbours can be nearer, and the sign of x - (q +- 1/2) s as one FMA tells (an FMA
 // rounds once, so its sign is that of the exact difference). Scales near the smallest normal number, where that difference
 // can underflow, divide in 64 bits instead.
-__device__ __forceinline__ int int8_code(float x, float s, float inv) {
+static __device__ __noinline__ int int8_code_exact(float x, float s, float inv) {
     if (s < 7.8886e-31f) return __double2int_rn(static_cast<double>(x) / static_cast<double>(s));
     const float q = rintf(__fmul_rn(x, inv));
     const float up = __fmaf_rn(-(q + 0.5f), s, x), down = __fmaf_rn(-(q - 0.5f), s, x);
@@ -47,6 +47,26 @@ __device__ __forceinline__ int int8_code(float x, float s, float inv) {
     if (up > 0.f || (up == 0.f && (code & 1))) ++code;
     else if (down < 0.f || (down == 0.f && (code & 1))) --code;
     return code;
+}
+
+// The codes of four values as bytes of a word. x * inv + 1.5 * 2^23 has the nearest integer of x * inv in its low bits, and that
+// is the code unless x * inv lies within 2^-16 of a border (x / s does not differ from it by more than 2^-17 there): then, in
+// one of 2^13 groups or so, each of the four is looked at exactly.
+__device__ __forceinline__ uint32_t int8_codes(const float (&x)[4], float s, float inv) {
+    constexpr float MAGIC = 12582912.f;
+    uint32_t t[4];
+    float far = s < 7.8886e-31f ? 1.f : 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const float y = __fmaf_rn(x[e], inv, MAGIC);
+        far = fmaxf(far, fabsf(__fmaf_rn(x[e], inv, -__fadd_rn(y, -MAGIC))));
+        t[e] = __float_as_uint(y);
+    }
+    if (far > 0.49998f) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) t[e] = static_cast<uint32_t>(int8_code_exact(x[e], s, inv));
+    }
+    return __byte_perm(__byte_perm(t[0], t[1], 0x0040), __byte_perm(t[2], t[3], 0x0040), 0x5410);
 }
 
 __device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
