@@ -14,6 +14,7 @@
 #include <torch/csrc/utils/pybind.h>
 
 #include <ATen/ATen.h>
+#include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 
 #include <cmath>
@@ -34,7 +35,8 @@ struct Api {
     FN(residual_rmsnorm); FN(gemv_norm); FN(gemv_norm_supported); FN(router_logits_t); FN(router_topk_ex);
     FN(router_topk_plan_row); FN(shared_gate); FN(moe_plan_ex); FN(moe_token_image_bytes); FN(moe_token_images);
     FN(moe_gate_up); FN(moe_gate_up_images); FN(moe_down); FN(moe_hidden_image_bytes); FN(moe_gate_up_streams); FN(moe_down_streams); FN(moe_hidden_images); FN(moe_down_images); FN(moe_combine); FN(silu_mul); FN(rope_attention);
-    FN(prefill_attention); FN(embed_tokens);
+    FN(prefill_attention); FN(embed_tokens); FN(int8_quantize); FN(int8_gemm); FN(kv8_extend); FN(kv8_append); FN(kv8_attention);
+    FN(kv8_attention_workspace); FN(kv8_fork); FN(kv8_free);
 #undef FN
 } api;
 PyObject *b200q_error = nullptr;        // the package's exception for CUDA errors
@@ -45,7 +47,8 @@ void bind(const py::dict &addresses, py::object error_type) {
     FN(residual_rmsnorm); FN(gemv_norm); FN(gemv_norm_supported); FN(router_logits_t); FN(router_topk_ex);
     FN(router_topk_plan_row); FN(shared_gate); FN(moe_plan_ex); FN(moe_token_image_bytes); FN(moe_token_images);
     FN(moe_gate_up); FN(moe_gate_up_images); FN(moe_down); FN(moe_hidden_image_bytes); FN(moe_gate_up_streams); FN(moe_down_streams); FN(moe_hidden_images); FN(moe_down_images); FN(moe_combine); FN(silu_mul); FN(rope_attention);
-    FN(prefill_attention); FN(embed_tokens);
+    FN(prefill_attention); FN(embed_tokens); FN(int8_quantize); FN(int8_gemm); FN(kv8_extend); FN(kv8_append); FN(kv8_attention);
+    FN(kv8_attention_workspace); FN(kv8_fork); FN(kv8_free);
 #undef FN
     b200q_error = error_type.release().ptr();
 }
@@ -148,6 +151,204 @@ PyObject *linear_fast(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
     END_HANDLE_TH_ERRORS
 }
 PyMethodDef linear_def = {"linear", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(linear_fast)), METH_FASTCALL, nullptr};
+
+// ------------------------------------------------------------------------------------------------ int8 product, 8-bit cache
+// Like linear: positional arguments, None when the call needs the Python layer (other devices, what it has to refuse).
+#define FAST_METHOD(name) PyMethodDef name##_def = {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name##_fast)), METH_FASTCALL, nullptr}
+int as_int(PyObject *o) { return static_cast<int>(PyLong_AsLong(o)); }
+// Rows of consecutive elements that do not overlap: elements from row to row, or -1.
+int64_t row_stride(const at::Tensor &x) {
+    const int64_t rows = x.size(0), width = x.size(1);
+    if (x.stride(1) != 1 && width > 1) return -1;
+    if (rows <= 1) return width;
+    return x.stride(0) >= width ? x.stride(0) : -1;
+}
+
+// int8_linear(x, codes, scales, n, k, out_dtype | None)
+PyObject *int8_linear_fast(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+    if (nargs != 6 || !THPVariable_Check(args[0]) || !THPVariable_Check(args[1]) || !THPVariable_Check(args[2])) Py_RETURN_NONE;
+    HANDLE_TH_ERRORS
+        const at::Tensor &x = THPVariable_Unpack(args[0]), &w = THPVariable_Unpack(args[1]), &ws = THPVariable_Unpack(args[2]);
+        const int n = as_int(args[3]), k = as_int(args[4]);
+        if (PyErr_Occurred()) return nullptr;
+        const int64_t nd = x.dim();
+        const int dt = dtype_id(x.scalar_type());
+        if (!x.is_cuda() || (nd != 2 && nd != 3) || x.size(nd - 1) != k || dt < 0 || x.device() != w.device() ||
+            x.device().index() != c10::cuda::current_device())
+            Py_RETURN_NONE;
+        const int64_t x_row = nd == 2 ? row_stride(x) : x.is_contiguous() ? k : -1, m = x.numel() / k, padded = w.size(1);
+        at::ScalarType out_type = x.scalar_type();
+        if (args[5] != Py_None) {
+            if (!THPDtype_Check(args[5])) Py_RETURN_NONE;
+            out_type = reinterpret_cast<THPDtype *>(args[5])->scalar_type;
+        }
+        const int ydt = dtype_id(out_type);
+        if (ydt < 0 || x_row < 0 || m == 0 || m > 0x7fffffff) Py_RETURN_NONE;
+        at::Tensor y = nd == 2 ? empty({m, n}, out_type, x.device()) : empty({x.size(0), x.size(1), n}, out_type, x.device());
+        try {
+            py::gil_scoped_release unlocked;
+            const at::Tensor scratch = empty({m * padded + 4 * m}, at::kByte, x.device());       // (codes end on a multiple of 16)
+            int8_t *codes = static_cast<int8_t *>(scratch.data_ptr());
+            float *scales = reinterpret_cast<float *>(codes + m * padded);
+            CALL(int8_quantize, x.data_ptr(), dt, static_cast<int>(m), k, x_row, codes, padded, scales, 1, stream());
+            CALL(int8_gemm, static_cast<const int8_t *>(w.data_ptr()), padded, ws.data_ptr<float>(), n, k, codes, padded, scales,
+                 static_cast<int>(m), y.data_ptr(), ydt, stream());
+        } catch (const CallError &e) {
+            e.raise();
+            return nullptr;
+        }
+        return THPVariable_Wrap(std::move(y));
+    END_HANDLE_TH_ERRORS
+}
+FAST_METHOD(int8_linear);
+
+// What the calls on a cache begin with: (address of the b200q_kv8_cache, device index, ...).
+const b200q_kv8_cache *cache_at(PyObject *address) { return static_cast<const b200q_kv8_cache *>(PyLong_AsVoidPtr(address)); }
+template <typename T> T *pointer(PyObject *address) { return static_cast<T *>(PyLong_AsVoidPtr(address)); }
+// Tables of a rotation, or none (both None): false when the Python layer has to look at them.
+bool rope_tables(const b200q_kv8_cache *c, int device, PyObject *cos, PyObject *sin, const float *&cos_p, const float *&sin_p, int &rows) {
+    cos_p = sin_p = nullptr;
+    rows = 0;
+    if (cos == Py_None && sin == Py_None) return true;
+    if (!THPVariable_Check(cos) || !THPVariable_Check(sin)) return false;
+    const at::Tensor &a = THPVariable_Unpack(cos), &b = THPVariable_Unpack(sin);
+    for (const at::Tensor *t : {&a, &b})
+        if (!t->is_cuda() || t->device().index() != device || t->scalar_type() != at::kFloat || t->dim() != 2 || !t->is_contiguous() ||
+            t->size(1) * 2 != c->head_dim || t->size(0) < c->max_length)
+            return false;
+    if (a.size(0) != b.size(0)) return false;
+    cos_p = a.data_ptr<float>();
+    sin_p = b.data_ptr<float>();
+    rows = static_cast<int>(a.size(0));
+    return true;
+}
+// [rows, width] CUDA rows on `device`
+bool rows_fit(const at::Tensor &x, int device, int64_t rows, int64_t width) {
+    return x.is_cuda() && x.device().index() == device && x.dim() == 2 && x.size(0) == rows && x.size(1) == width && dtype_id(x.scalar_type()) >= 0 &&
+           row_stride(x) >= 0;
+}
+
+// kv8_append(cache, device, layer, k, v, slots, offsets, starts, batch, rows, max_new, cos | None, sin | None) -> True
+PyObject *kv8_append_fast(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+    if (nargs != 13 || !THPVariable_Check(args[3]) || !THPVariable_Check(args[4])) Py_RETURN_NONE;
+    HANDLE_TH_ERRORS
+        const b200q_kv8_cache *c = cache_at(args[0]);
+        const int device = as_int(args[1]), layer = as_int(args[2]), batch = as_int(args[8]), rows = as_int(args[9]), max_new = as_int(args[10]);
+        const int32_t *slots = pointer<int32_t>(args[5]), *offsets = pointer<int32_t>(args[6]), *starts = pointer<int32_t>(args[7]);
+        if (PyErr_Occurred()) return nullptr;
+        const at::Tensor &k = THPVariable_Unpack(args[3]), &v = THPVariable_Unpack(args[4]);
+        const int64_t width = static_cast<int64_t>(c->kv_heads) * c->head_dim;
+        const float *cos, *sin;
+        int positions;
+        if (device != c10::cuda::current_device() || rows < 1 || !rows_fit(k, device, rows, width) || !rows_fit(v, device, rows, width) ||
+            k.scalar_type() != v.scalar_type() || !rope_tables(c, device, args[11], args[12], cos, sin, positions))
+            Py_RETURN_NONE;
+        try {
+            py::gil_scoped_release unlocked;
+            CALL(kv8_append, c, layer, k.data_ptr(), v.data_ptr(), dtype_id(k.scalar_type()), row_stride(k), row_stride(v), slots, offsets,
+                 starts, batch, max_new, cos, sin, positions, stream());
+        } catch (const CallError &e) {
+            e.raise();
+            return nullptr;
+        }
+        Py_RETURN_TRUE;
+    END_HANDLE_TH_ERRORS
+}
+FAST_METHOD(kv8_append);
+
+// kv8_attention(cache, device, layer, q, slots, offsets, starts, batch, rows, max_new, max_keys, cos | None, sin | None, scale,
+// out | None) -> the context
+PyObject *kv8_attention_fast(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+    if (nargs != 15 || !THPVariable_Check(args[3])) Py_RETURN_NONE;
+    HANDLE_TH_ERRORS
+        const b200q_kv8_cache *c = cache_at(args[0]);
+        const int device = as_int(args[1]), layer = as_int(args[2]), batch = as_int(args[7]), rows = as_int(args[8]), max_new = as_int(args[9]),
+                  max_keys = as_int(args[10]);
+        const int32_t *slots = pointer<int32_t>(args[4]), *offsets = pointer<int32_t>(args[5]), *starts = pointer<int32_t>(args[6]);
+        const double scale = PyFloat_AsDouble(args[13]);
+        if (PyErr_Occurred()) return nullptr;
+        const at::Tensor &q = THPVariable_Unpack(args[3]);
+        const float *cos, *sin;
+        int positions;
+        if (device != c10::cuda::current_device() || rows < 1 || q.dim() != 2 || !rows_fit(q, device, rows, q.size(1)) ||
+            q.size(1) % (static_cast<int64_t>(c->head_dim) * c->kv_heads) || q.size(1) == 0 || !rope_tables(c, device, args[11], args[12], cos, sin, positions))
+            Py_RETURN_NONE;
+        const int heads = static_cast<int>(q.size(1) / c->head_dim);
+        const at::ScalarType type = c->dtype == B200Q_BF16 ? at::kBFloat16 : at::kHalf;
+        at::Tensor out;
+        if (args[14] == Py_None) {
+            out = empty({rows, q.size(1)}, type, q.device());
+        } else {
+            if (!THPVariable_Check(args[14])) Py_RETURN_NONE;
+            out = THPVariable_Unpack(args[14]);
+            if (!out.is_cuda() || out.device() != q.device() || out.sizes() != q.sizes() || out.scalar_type() != type || !out.is_contiguous()) Py_RETURN_NONE;
+        }
+        try {
+            py::gil_scoped_release unlocked;
+            const long long bytes = api.kv8_attention_workspace(c, heads, batch, rows, max_new, max_keys);
+            const at::Tensor space = bytes ? empty({bytes}, at::kByte, q.device()) : at::Tensor();
+            CALL(kv8_attention, c, layer, q.data_ptr(), dtype_id(q.scalar_type()), row_stride(q), heads, slots, offsets, starts, batch, rows,
+                 max_new, max_keys, cos, sin, positions, static_cast<float>(scale), out.data_ptr(), bytes ? space.data_ptr() : nullptr, bytes,
+                 stream());
+        } catch (const CallError &e) {
+            e.raise();
+            return nullptr;
+        }
+        return THPVariable_Wrap(std::move(out));
+    END_HANDLE_TH_ERRORS
+}
+FAST_METHOD(kv8_attention);
+
+// kv8_extend(cache, device, slots, offsets, batch, starts); kv8_fork(cache, device, src, dst, count); kv8_free(cache, device, slots,
+// count), arrays as addresses -> True
+template <typename F>
+PyObject *on_cache(PyObject *const *args, F launch) {
+    HANDLE_TH_ERRORS
+        const b200q_kv8_cache *c = cache_at(args[0]);
+        const int device = as_int(args[1]);
+        if (PyErr_Occurred()) return nullptr;
+        if (device != c10::cuda::current_device()) Py_RETURN_NONE;
+        try {
+            launch(c, device);
+        } catch (const CallError &e) {
+            e.raise();
+            return nullptr;
+        }
+        Py_RETURN_TRUE;
+    END_HANDLE_TH_ERRORS
+}
+PyObject *kv8_extend_fast(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+    if (nargs != 6) Py_RETURN_NONE;
+    return on_cache(args, [&](const b200q_kv8_cache *c, int) {
+        const int32_t *slots = pointer<int32_t>(args[2]), *offsets = pointer<int32_t>(args[3]);
+        int32_t *starts = pointer<int32_t>(args[5]);
+        const int batch = as_int(args[4]);
+        py::gil_scoped_release unlocked;
+        CALL(kv8_extend, c, slots, offsets, batch, starts, stream());
+    });
+}
+FAST_METHOD(kv8_extend);
+PyObject *kv8_fork_fast(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+    if (nargs != 5) Py_RETURN_NONE;
+    return on_cache(args, [&](const b200q_kv8_cache *c, int device) {
+        const int32_t *src = pointer<int32_t>(args[2]), *dst = pointer<int32_t>(args[3]);
+        const int count = as_int(args[4]);
+        py::gil_scoped_release unlocked;
+        const at::Tensor scratch = empty({1}, at::kInt, at::Device(at::kCUDA, static_cast<c10::DeviceIndex>(device)));
+        CALL(kv8_fork, c, src, dst, count, scratch.data_ptr<int32_t>(), stream());
+    });
+}
+FAST_METHOD(kv8_fork);
+PyObject *kv8_free_fast(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+    if (nargs != 4) Py_RETURN_NONE;
+    return on_cache(args, [&](const b200q_kv8_cache *c, int) {
+        const int32_t *slots = pointer<int32_t>(args[2]);
+        const int count = as_int(args[3]);
+        py::gil_scoped_release unlocked;
+        CALL(kv8_free, c, slots, count, stream());
+    });
+}
+FAST_METHOD(kv8_free);
 
 // ------------------------------------------------------------------------------------------------ MoE layer
 // 256-byte aligned pieces of one scratch allocation.
@@ -413,7 +614,8 @@ PYBIND11_MODULE(_b200q_host, m) {
         }
     });
     m.def("bind", &bind);
-    m.add_object("linear", py::reinterpret_steal<py::object>(PyCFunction_New(&linear_def, nullptr)));
+    for (PyMethodDef *def : {&linear_def, &int8_linear_def, &kv8_append_def, &kv8_attention_def, &kv8_extend_def, &kv8_fork_def, &kv8_free_def})
+        m.add_object(def->ml_name, py::reinterpret_steal<py::object>(PyCFunction_New(def, nullptr)));
     py::class_<MoeLayer>(m, "MoeLayer")
         .def(py::init([](at::Tensor router, py::object bias, py::object gate_vector, at::Tensor gate, at::Tensor up, at::Tensor down,
                          std::vector<int64_t> strides, std::vector<int> formats, py::object tables, bool aligned16, bool with_shared,

@@ -118,35 +118,38 @@ __global__ void __launch_bounds__(EXTEND_THREADS) kv8_extend_kernel(const b200q_
 struct Kv8Append {
     const void *k, *v;
     long long k_row, v_row;
-    int in_dtype, layer;
+    int layer;
     const int32_t *slots, *offsets, *starts;
     const float *cos_t, *sin_t;           // [rope_rows][head_dim / 2], or NULL: keys are stored as they come
     int rope_rows;
 };
 
-// Four consecutive values as floats. VEC: base and strides are such that one 8- or 16-byte load fetches them.
-template <bool VEC>
-__device__ __forceinline__ void load4(const void *p, int dtype, size_t i, float (&f)[4]) {
-    if (VEC && dtype == B200Q_F32) {
-        const float4 q = *reinterpret_cast<const float4 *>(static_cast<const float *>(p) + i);
-        f[0] = q.x; f[1] = q.y; f[2] = q.z; f[3] = q.w;
-    } else if (VEC) {
-        const uint2 q = *reinterpret_cast<const uint2 *>(static_cast<const uint16_t *>(p) + i);
-        const uint32_t w[2] = {q.x, q.y};
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            if (dtype == B200Q_BF16) {
-                f[2 * e] = __uint_as_float(w[e] << 16);
-                f[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
-            } else {
-                const float2 h = __half22float2(*reinterpret_cast<const __half2 *>(&w[e]));
-                f[2 * e] = h.x;
-                f[2 * e + 1] = h.y;
-            }
-        }
+// Four consecutive values of type IN as they are loaded (held in few registers until they are used). VEC: base and strides are
+// such that one 8- or 16-byte load fetches them.
+template <int IN> struct RawQuad { uint2 w; };
+template <> struct RawQuad<B200Q_F32> { float4 w; };
+template <int IN, bool VEC>
+__device__ __forceinline__ RawQuad<IN> load_quad(const void *p, size_t i) {
+    RawQuad<IN> r;
+    if constexpr (IN == B200Q_F32) {
+        const float *q = static_cast<const float *>(p) + i;
+        if (VEC) r.w = *reinterpret_cast<const float4 *>(q);
+        else r.w = make_float4(q[0], q[1], q[2], q[3]);
     } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) f[e] = load_as_float(p, dtype, i + e);
+        const uint16_t *q = static_cast<const uint16_t *>(p) + i;
+        if (VEC) r.w = *reinterpret_cast<const uint2 *>(q);
+        else r.w = make_uint2(q[0] | (static_cast<uint32_t>(q[1]) << 16), q[2] | (static_cast<uint32_t>(q[3]) << 16));
+    }
+    return r;
+}
+template <bool BF16> __device__ __forceinline__ float2 unpack16(uint32_t w);
+template <int IN>
+__device__ __forceinline__ void quad_values(const RawQuad<IN> &r, float (&f)[4]) {
+    if constexpr (IN == B200Q_F32) {
+        f[0] = r.w.x; f[1] = r.w.y; f[2] = r.w.z; f[3] = r.w.w;
+    } else {
+        const float2 a = unpack16<IN == B200Q_BF16>(r.w.x), b = unpack16<IN == B200Q_BF16>(r.w.y);
+        f[0] = a.x; f[1] = a.y; f[2] = b.x; f[3] = b.y;
     }
 }
 
@@ -184,7 +187,7 @@ static __device__ __noinline__ void rotate_exact(const float (&x0)[4], const flo
 // out: the quad at i as two words, then its partner's.
 template <bool BF16>
 __device__ __forceinline__ void rotate_quad(const float (&x0)[4], const float (&x1)[4], const float (&c)[4], const float (&s)[4], uint32_t (&out)[4]) {
-    constexpr float BOUND = 2.3841858e-7f;               // 2^-22: twice the two roundings' 2^-24 of product and sum each
+    constexpr float BOUND = 1.1920929e-7f;               // 2^-23: product, sum and the reference's own FP32 rounding, 2^-24 each
     uint32_t differ = 0u;
 #pragma unroll
     for (int h = 0; h < 2; ++h)
@@ -204,21 +207,22 @@ __device__ __forceinline__ void rotate_quad(const float (&x0)[4], const float (&
     if (differ) rotate_exact<BF16>(x0, x1, c, s, out);
 }
 
-// One CTA of 4 DH threads = one block of 64 tokens of one sequence and key/value head, the first half of the threads its keys,
-// the second its values. A thread holds four consecutive tokens x (a quad of dimensions at i and its partner at i + DH / 2, which
+// One CTA of 2 DH threads = the keys or the values of one block of 64 tokens of one sequence and head. A thread holds four consecutive tokens x (a quad of dimensions at i and its partner at i + DH / 2, which
 // the rotation needs), as 16-bit pairs. A block that becomes full takes its older tokens from the tail and finds the largest
 // magnitude (16-bit integers order 16-bit floats, NaN and infinities on top); keys go out as words of four codes, values as words
 // of four tokens of a dimension (a transposition of bytes in registers) that pass through shared memory. One that does not become
 // full goes to the tail. Bound by memory - every new token is read once, as projection output, and written once - and, next to
 // it, by the instructions per element: with 64-bit rotations, exact codes one by one and byte stores 3 x 8192 tokens took 83 us.
-template <int DH, bool BF16, bool VEC>
-__global__ void __launch_bounds__(4 * DH) kv8_append_kernel(const b200q_kv8_cache c, const Kv8Append a) {
+// All loads of inputs are issued before the first is used (rows past the ends repeat the first or last one); registers are held to
+// what lets half of an SM's threads be resident.
+template <int DH, bool BF16, int IN, bool VEC>
+__global__ void __launch_bounds__(2 * DH, 1024 / (2 * DH)) kv8_append_kernel(const b200q_kv8_cache c, const Kv8Append a) {
     constexpr int HALF = DH / 2, QUADS = HALF / 4, WARPS = DH / 16, LD = KV8_BLOCK / 4 + 1;      // warps per part; words of a row
     __shared__ uint32_t v_s[DH * LD];
-    __shared__ uint32_t peaks[2 * WARPS];
+    __shared__ uint32_t peaks[WARPS];
     chain_trigger();
     chain_wait();
-    const int tid = threadIdx.x, part = tid / (2 * DH), at = tid % (2 * DH), b = blockIdx.z, head = blockIdx.y;
+    const int at = threadIdx.x, part = blockIdx.y & 1, b = blockIdx.z, head = blockIdx.y >> 1;
     const int start = a.starts[b], row0 = a.offsets[b], n = a.offsets[b + 1] - row0;
     if (start < 0 || n <= 0) return;
     const int total = start + n, first = start / KV8_BLOCK, last = (total - 1) / KV8_BLOCK;
@@ -241,45 +245,73 @@ __global__ void __launch_bounds__(4 * DH) kv8_append_kernel(const b200q_kv8_cach
         const bool full = base + KV8_BLOCK <= total;
         uint32_t x[4][4];                                // [token][quad as two words, partner]
         uint32_t top = 0u;
+        const bool turn = part == 0 && a.cos_t;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int pos = base + t0 + j;
-            float lo[4] = {0.f, 0.f, 0.f, 0.f}, hi[4] = {0.f, 0.f, 0.f, 0.f};
-            if (pos >= start && pos < total) {
+        for (int j = 0; j < 4; ++j) x[j][0] = x[j][1] = x[j][2] = x[j][3] = 0u;
+        const int page = full ? c.table[static_cast<size_t>(slot) * c.blocks + block] : 0;
+        if (full || (base + t0 + 3 >= start && base + t0 < total)) {         // (few threads have a token of a decode step)
+            RawQuad<IN> lo[4], hi[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int pos = min(max(base + t0 + j, start), total - 1);
                 const size_t from = (row0 + (pos - start)) * static_cast<size_t>(in_row) + static_cast<size_t>(head) * DH + i;
-                load4<VEC>(in, a.in_dtype, from, lo);
-                load4<VEC>(in, a.in_dtype, from + HALF, hi);
+                lo[j] = load_quad<IN, VEC>(in, from);
+                hi[j] = load_quad<IN, VEC>(in, from + HALF);
             }
-            if (part == 0 && a.cos_t && pos >= start && pos < total) {
-                const float4 cq = *reinterpret_cast<const float4 *>(a.cos_t + static_cast<size_t>(pos) * HALF + i);
-                const float4 sq = *reinterpret_cast<const float4 *>(a.sin_t + static_cast<size_t>(pos) * HALF + i);
-                const float cv[4] = {cq.x, cq.y, cq.z, cq.w}, sv[4] = {sq.x, sq.y, sq.z, sq.w};
-                rotate_quad<BF16>(lo, hi, cv, sv, x[j]);
-            } else {
-                x[j][0] = pack16<BF16>(lo[0], lo[1]);
-                x[j][1] = pack16<BF16>(lo[2], lo[3]);
-                x[j][2] = pack16<BF16>(hi[0], hi[1]);
-                x[j][3] = pack16<BF16>(hi[2], hi[3]);
-                if (full && pos < start) {               // (only the first block has older tokens)
-                    const uint2 u = *reinterpret_cast<const uint2 *>(tail + (t0 + j) * DH + i), w = *reinterpret_cast<const uint2 *>(tail + (t0 + j) * DH + i + HALF);
+#pragma unroll
+            for (int jj = 0; jj < 4; jj += 2) {
+                float4 cq[2], sq[2];
+                if (turn)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const size_t from = static_cast<size_t>(min(max(base + t0 + jj + j, start), total - 1)) * HALF + i;
+                        cq[j] = *reinterpret_cast<const float4 *>(a.cos_t + from);
+                        sq[j] = *reinterpret_cast<const float4 *>(a.sin_t + from);
+                    }
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    float l4[4], h4[4];
+                    quad_values<IN>(lo[jj + j], l4);
+                    quad_values<IN>(hi[jj + j], h4);
+                    if (turn) {
+                        const float cv[4] = {cq[j].x, cq[j].y, cq[j].z, cq[j].w}, sv[4] = {sq[j].x, sq[j].y, sq[j].z, sq[j].w};
+                        rotate_quad<BF16>(l4, h4, cv, sv, x[jj + j]);
+                    } else {
+                        x[jj + j][0] = pack16<BF16>(l4[0], l4[1]);
+                        x[jj + j][1] = pack16<BF16>(l4[2], l4[3]);
+                        x[jj + j][2] = pack16<BF16>(h4[0], h4[1]);
+                        x[jj + j][3] = pack16<BF16>(h4[2], h4[3]);
+                    }
+                }
+            }
+            if (base < start || !full)                       // (only the first block has older tokens, only the last empty places)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int pos = base + t0 + j;
+                    if (pos >= start && pos < total) continue;
+                    uint2 u = make_uint2(0u, 0u), w = u;
+                    if (full) {
+                        u = *reinterpret_cast<const uint2 *>(tail + (t0 + j) * DH + i);
+                        w = *reinterpret_cast<const uint2 *>(tail + (t0 + j) * DH + i + HALF);
+                    }
                     x[j][0] = u.x;
                     x[j][1] = u.y;
                     x[j][2] = w.x;
                     x[j][3] = w.y;
                 }
-            }
 #pragma unroll
-            for (int e = 0; e < 4; ++e) top = __vmaxu2(top, x[j][e] & 0x7fff7fffu);
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) top = __vmaxu2(top, x[j][e] & 0x7fff7fffu);
         }
         top = __reduce_max_sync(0xffffffffu, max(top & 0xffffu, top >> 16));
-        if ((tid & 31) == 0) peaks[tid >> 5] = top;
+        if ((at & 31) == 0) peaks[at >> 5] = top;
         __syncthreads();
 #pragma unroll
-        for (int w = 0; w < WARPS; ++w) top = max(top, peaks[part * WARPS + w]);
+        for (int w = 0; w < WARPS; ++w) top = max(top, peaks[w]);
         const uint32_t peak = abs_bits(unpack16<BF16>(top).x);
         if (full) {
             const float s = int8_scale(peak), inv = __fdiv_rn(1.f, s);
-            const int page = c.table[static_cast<size_t>(slot) * c.blocks + block];
             const bool held = page >= 0 && page < c.pages;       // (a table that lacks the page loses the block, not memory)
             const size_t u = kv8_unit(held ? page : 0, c.layers, a.layer, part, c.kv_heads, head);
             int8_t *to = c.codes + u * (KV8_BLOCK * DH);
@@ -309,7 +341,7 @@ __global__ void __launch_bounds__(4 * DH) kv8_append_kernel(const b200q_kv8_cach
                     row[2 * LD] = __byte_perm(b01, b23, 0x5410);
                     row[3 * LD] = __byte_perm(b01, b23, 0x7632);
                 }
-                named_barrier_sync(1, 2 * DH);
+                __syncthreads();
                 if (held)
 #pragma unroll
                     for (int j = at; j < DH * 4; j += 2 * DH) {
@@ -507,6 +539,18 @@ __global__ void __launch_bounds__(256) kv8_compact_copy_kernel(const b200q_kv8_c
 }
 
 // ----------------------------------------------------------------------------------------------------------- host side
+using AppendFn = void (*)(const b200q_kv8_cache, const Kv8Append);
+template <int DH, bool BF16, int IN>
+static AppendFn append_kernel_of(bool vec) { return vec ? kv8_append_kernel<DH, BF16, IN, true> : kv8_append_kernel<DH, BF16, IN, false>; }
+template <int DH>
+static AppendFn append_kernel(int dtype, int in, bool vec) {
+    if (dtype == B200Q_BF16)
+        return in == B200Q_F32 ? append_kernel_of<DH, true, B200Q_F32>(vec) : in == B200Q_F16 ? append_kernel_of<DH, true, B200Q_F16>(vec)
+                                                                                           : append_kernel_of<DH, true, B200Q_BF16>(vec);
+    return in == B200Q_F32 ? append_kernel_of<DH, false, B200Q_F32>(vec) : in == B200Q_F16 ? append_kernel_of<DH, false, B200Q_F16>(vec)
+                                                                                        : append_kernel_of<DH, false, B200Q_BF16>(vec);
+}
+
 int kv8_check(const char *what, const b200q_kv8_cache *c) {
     if (!c || !c->codes || !c->scales || !c->tail || !c->peak || !c->table || !c->lengths || !c->refs || !c->free_bits)
         return fail(B200Q_EINVAL, "%s: NULL pointer", what);
@@ -564,19 +608,14 @@ extern "C" int b200q_kv8_append(const b200q_kv8_cache *cache, int layer, const v
         return fail(B200Q_EINVAL, "kv8_append: RoPE tables must be 16-byte aligned");
     if (batch > 65535) return fail(B200Q_EUNSUPPORTED, "kv8_append: at most 65535 sequences per call");
     Kv8Append a{};
-    a.k = k; a.v = v; a.k_row = k_row; a.v_row = v_row; a.in_dtype = in_dtype; a.layer = layer;
+    a.k = k; a.v = v; a.k_row = k_row; a.v_row = v_row; a.layer = layer;
     a.slots = slots; a.offsets = offsets; a.starts = starts;
     a.cos_t = cos_table; a.sin_t = sin_table; a.rope_rows = rope_rows;
     const size_t quad = 4 * dtype_size(in_dtype);
     const bool vec = (reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) % quad == 0 && k_row % 4 == 0 && v_row % 4 == 0;
-    const dim3 grid((max_new + 2 * KV8_BLOCK - 2) / KV8_BLOCK, cache->kv_heads, batch);
-    const bool bf16 = cache->dtype == B200Q_BF16;
-    auto kernel = cache->head_dim == 64
-        ? (bf16 ? (vec ? kv8_append_kernel<64, true, true> : kv8_append_kernel<64, true, false>)
-                : (vec ? kv8_append_kernel<64, false, true> : kv8_append_kernel<64, false, false>))
-        : (bf16 ? (vec ? kv8_append_kernel<128, true, true> : kv8_append_kernel<128, true, false>)
-                : (vec ? kv8_append_kernel<128, false, true> : kv8_append_kernel<128, false, false>));
-    launch_chained(kernel, grid, dim3(4 * cache->head_dim), 0, static_cast<cudaStream_t>(stream), *cache, a);
+    const dim3 grid((max_new + 2 * KV8_BLOCK - 2) / KV8_BLOCK, 2 * cache->kv_heads, batch);
+    auto kernel = cache->head_dim == 64 ? append_kernel<64>(cache->dtype, in_dtype, vec) : append_kernel<128>(cache->dtype, in_dtype, vec);
+    launch_chained(kernel, grid, dim3(2 * cache->head_dim), 0, static_cast<cudaStream_t>(stream), *cache, a);
     return check_launch("kv8_append");
 }
 

@@ -124,6 +124,12 @@ def int8_matmul(codes, scales, weight, *, out_dtype=None):
 def int8_linear(x, weight, *, out_dtype=None):
     """``quantized_linear`` in 8-bit integers: quantises ``x`` ``[..., K]`` per token, then ``int8_matmul``; the output has x's
     leading shape and, by default, x's type."""
+    if type(weight) is Int8Weight:
+        host = _lib.host()
+        if host is not None:
+            y = host.int8_linear(x, weight.codes, weight.scales, weight.shape[0], weight.shape[1], out_dtype)
+            if y is not None:
+                return y
     if not isinstance(weight, Int8Weight):
         raise TypeError("Expected an Int8Weight")
     if x.shape[-1] != weight.shape[1]:

@@ -132,7 +132,7 @@ class PagedKV8Cache:
         self._struct = _lib.KV8CacheStruct(*[_ptr(t) for t in (codes, scales, tail, peak, table, lengths, refs, free_bits)],
                                            layers, kv_heads, head_dim, pages, sequences, blocks, max_length,
                                            _lib.DTYPE_ID[str(tail.dtype)[6:]])
-        self._c = ctypes.addressof(self._struct)
+        self._c, self._index = ctypes.addressof(self._struct), codes.device.index
 
     # ------------------------------------------------------------------------------------------------ sequences and pages
     def batch(self, slots, counts, *, max_keys=None):
@@ -169,7 +169,9 @@ class PagedKV8Cache:
         blocks that become full. All sequences or none (status 501 / 502, ``starts`` -1)."""
         self._check_batch(batch)
         slots, offsets, starts = batch._pointers
-        _launch(self.device, "b200q_kv8_extend", self._c, slots, offsets, batch.size, starts)
+        host = _lib.host()
+        if host is None or not host.kv8_extend(self._c, self._index, slots, offsets, batch.size, starts):
+            _launch(self.device, "b200q_kv8_extend", self._c, slots, offsets, batch.size, starts)
         return batch
 
     def _slots(self, slots):
@@ -200,14 +202,18 @@ class PagedKV8Cache:
         if src.shape != dst.shape:
             raise ValueError("src and dst must be of the same length")
         if src.shape[0]:
-            scratch = torch.empty(1, dtype=torch.int32, device=self.device)
-            _launch(self.device, "b200q_kv8_fork", self._c, src.data_ptr(), dst.data_ptr(), src.shape[0], scratch.data_ptr())
+            host = _lib.host()
+            if host is None or not host.kv8_fork(self._c, self._index, src.data_ptr(), dst.data_ptr(), src.shape[0]):
+                scratch = torch.empty(1, dtype=torch.int32, device=self.device)
+                _launch(self.device, "b200q_kv8_fork", self._c, src.data_ptr(), dst.data_ptr(), src.shape[0], scratch.data_ptr())
 
     def free(self, slots):
         """The sequences become empty; pages that no sequence refers to any more return to the pool."""
         slots = self._slots(slots)
         if slots.shape[0]:
-            _launch(self.device, "b200q_kv8_free", self._c, slots.data_ptr(), slots.shape[0])
+            host = _lib.host()
+            if host is None or not host.kv8_free(self._c, self._index, slots.data_ptr(), slots.shape[0]):
+                _launch(self.device, "b200q_kv8_free", self._c, slots.data_ptr(), slots.shape[0])
 
     def compact(self, pages=None):
         """A new cache, independent of this one, with the same sequences and a pool of ``pages`` pages (default: the live ones)
@@ -260,6 +266,11 @@ class PagedKV8Cache:
         the new tokens of one layer, after ``extend(batch)``. ``rope`` = (cos, sin) tables ``[positions, head_dim / 2]``: the keys
         are rotated to their positions (rotate-half) first."""
         self._check_batch(batch)
+        host = _lib.host()
+        if host is not None and type(layer) is int:
+            cos, sin = rope or (None, None)
+            if host.kv8_append(self._c, self._index, layer, k, v, *batch._pointers, batch.size, batch.rows, batch.max_new, cos, sin):
+                return
         width = self.kv_heads * self.head_dim
         k_row, v_row = self._rows(k, batch, width, "k"), self._rows(v, batch, width, "v")
         if k.dtype != v.dtype:
@@ -273,8 +284,15 @@ class PagedKV8Cache:
         """Causal attention of the new tokens over the cache they are in (after ``append``): ``q`` ``[rows, heads * head_dim]``
         (FP32, FP16 or BF16; rotated here when ``rope`` is given) -> ``[rows, heads * head_dim]`` in the cache's type. ``heads`` is a
         multiple of ``kv_heads``; ``scale`` defaults to ``head_dim ** -0.5``."""
-        torch = _torch()
         self._check_batch(batch)
+        host = _lib.host()
+        if host is not None and type(layer) is int:
+            cos, sin = rope or (None, None)
+            result = host.kv8_attention(self._c, self._index, layer, q, *batch._pointers, batch.size, batch.rows, batch.max_new, batch.max_keys,
+                                        cos, sin, self.head_dim ** -0.5 if scale is None else scale, out)
+            if result is not None:
+                return result
+        torch = _torch()
         heads = q.shape[1] // self.head_dim if q.ndim == 2 else 0
         if heads < 1 or heads % self.kv_heads:
             raise ValueError(f"q must be [rows, heads * {self.head_dim}] with heads a multiple of {self.kv_heads}")
