@@ -484,7 +484,7 @@ int b200q_expert_ffn_static(const void *gate, int gate_fmt, const void *up, int 
  * arrived per call. head_dim 64 or 128; at most 65536 sequences and 2^20 pages. All of it lives on the device, every call
  * but the sizes of b200q_kv8_compact's new pool is decided there, and calls on one cache have to be ordered by their stream.
  * Device status words of refusals: 501 too few free pages, 502 a sequence would pass max_length (or a slot is out of range),
- * 503 fork / free of slots out of range, of a target named twice, not empty or also a source, 504 compact into too few pages. */
+ * 503 fork / free of slots out of range, of a target named twice, not empty or also a source; of waits that gave up: 511, 512. */
 typedef struct b200q_kv8_cache {
     int8_t *codes;
     float *scales;
@@ -529,11 +529,15 @@ int b200q_kv8_fork(const b200q_kv8_cache *cache, const int32_t *src, const int32
 /* The sequences become empty; pages without a sequence return to the pool. A slot out of range is skipped (status 503). */
 int b200q_kv8_free(const b200q_kv8_cache *cache, const int32_t *slots, int count, void *stream);
 /* Everything in `from` into `to`, a cache of equal sizes but for its number of pages, with the live pages packed to the front
- * in their order. All memory of `to` is written but the pages behind the live ones. Too few pages in `to`: status 504, and the
- * table entries of the pages that have no place are -1. workspace: b200q_kv8_compact_workspace(from, to) bytes. */
+ * in their order, in two calls: the plan (counts the live pages and decides where each goes) and the move. All memory of `to` is
+ * written but the pages behind the live ones. workspace: b200q_kv8_compact_workspace(from, to) bytes for both calls; after the
+ * plan its first int32 is the number of live pages. If that is more than `to` has, the pages that find no place are lost: the
+ * caller looks at the number and gives `to` up. */
 long long b200q_kv8_compact_workspace(const b200q_kv8_cache *from, const b200q_kv8_cache *to);
-int b200q_kv8_compact(const b200q_kv8_cache *from, const b200q_kv8_cache *to, void *workspace, long long workspace_bytes,
-                      void *stream);
+int b200q_kv8_compact_plan(const b200q_kv8_cache *from, const b200q_kv8_cache *to, void *workspace, long long workspace_bytes,
+                           void *stream);
+int b200q_kv8_compact_move(const b200q_kv8_cache *from, const b200q_kv8_cache *to, const void *workspace,
+                           long long workspace_bytes, void *stream);
 
 /* ---- Matrix product in 8-bit integers (opt-in; changes numerics) ----------------------------------
  * y[m, n] = (sum over k of x_codes[m, k] * w_codes[n, k]) * x_scales[m] * w_scales[n]: int8 codes with one FP32 scale per

@@ -119,7 +119,8 @@ SIGNATURES.update({
     "b200q_kv8_fork": [_ptr, _ptr, _ptr, _c_int, _ptr, _ptr],
     "b200q_kv8_free": [_ptr, _ptr, _c_int, _ptr],
     "b200q_kv8_compact_workspace": [_ptr, _ptr],
-    "b200q_kv8_compact": [_ptr, _ptr, _ptr, _c_i64, _ptr],
+    "b200q_kv8_compact_plan": [_ptr, _ptr, _ptr, _c_i64, _ptr],
+    "b200q_kv8_compact_move": [_ptr, _ptr, _ptr, _c_i64, _ptr],
     "b200q_int8_quantize": [_ptr, _c_int, _c_int, _c_int, _c_i64, _ptr, _c_i64, _ptr, _c_int, _ptr],
     "b200q_int8_gemm": [_ptr, _c_i64, _ptr, _c_int, _c_int, _ptr, _c_i64, _ptr, _c_int, _ptr, _c_int, _ptr],
 })

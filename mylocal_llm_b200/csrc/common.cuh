@@ -41,6 +41,11 @@ constexpr int STATUS_POSITION_RANGE = 301;  // a decode position lay outside the
 constexpr int NUM_SMS_FALLBACK = 148;
 int sm_count();
 
+// The opt-in to LARGE_SHARED_MEMORY bytes of dynamic shared memory (next to at most 2 KB of static), per kernel and device, done
+// once each; a return code as of the entry points.
+constexpr int LARGE_SHARED_MEMORY = 225 * 1024;
+int allow_large_shared_memory(const void *kernel);
+
 // ---------------------------------------------------------------------------------------------
 // Programmatic dependent launch. The decode step is a chain of short kernels on one stream; a
 // kernel launched through launch_chained() may become resident while its predecessor drains, and

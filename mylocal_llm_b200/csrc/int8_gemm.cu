@@ -6,87 +6,134 @@
 
 namespace b200q {
 
-// One CTA per row. The row's pieces of eight values stay in registers between the two passes (the largest magnitude, then
-// the codes) up to 256 * 8 * KEEP columns; longer rows are read again. VEC: 16-byte loads are possible.
-template <bool VEC>
-__device__ __forceinline__ void load8(const void *p, int dtype, size_t base, int c, int k, float (&f)[8]) {
-    if (VEC && c + 8 <= k) {
-        if (dtype == B200Q_F32) {
-            const float4 *q = reinterpret_cast<const float4 *>(static_cast<const float *>(p) + base + c);
-            const float4 lo = q[0], hi = q[1];
-            f[0] = lo.x; f[1] = lo.y; f[2] = lo.z; f[3] = lo.w;
-            f[4] = hi.x; f[5] = hi.y; f[6] = hi.z; f[7] = hi.w;
-        } else {
-            const uint4 q = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p) + base + c);
-            const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+// Eight consecutive values of type IN as they are loaded. VEC: 16-byte loads are possible.
+template <int IN> struct Raw8 {
+    uint4 w;
+    __device__ __forceinline__ void values(float (&f)[8]) const {
+        const uint32_t x[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                if (dtype == B200Q_BF16) {
-                    f[2 * e] = __uint_as_float(w[e] << 16);
-                    f[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
-                } else {
-                    const float2 h = __half22float2(*reinterpret_cast<const __half2 *>(&w[e]));
-                    f[2 * e] = h.x;
-                    f[2 * e + 1] = h.y;
-                }
-            }
+        for (int e = 0; e < 4; ++e) {
+            const float2 v = IN == B200Q_BF16 ? make_float2(__uint_as_float(x[e] << 16), __uint_as_float(x[e] & 0xffff0000u))
+                                              : __half22float2(*reinterpret_cast<const __half2 *>(&x[e]));
+            f[2 * e] = v.x;
+            f[2 * e + 1] = v.y;
         }
-        return;
     }
+};
+template <> struct Raw8<B200Q_F32> {
+    float4 w[2];
+    __device__ __forceinline__ void values(float (&f)[8]) const {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] = c + e < k ? load_as_float(p, dtype, base + c + e) : 0.f;
+        for (int h = 0; h < 2; ++h) {
+            f[4 * h] = w[h].x; f[4 * h + 1] = w[h].y; f[4 * h + 2] = w[h].z; f[4 * h + 3] = w[h].w;
+        }
+    }
+};
+template <int IN, bool VEC>
+__device__ __forceinline__ Raw8<IN> load8(const void *p, size_t base, int c, int k) {
+    Raw8<IN> r;
+    if constexpr (IN == B200Q_F32) {
+        const float *q = static_cast<const float *>(p) + base + c;
+        if (VEC && c + 8 <= k) {
+            r.w[0] = reinterpret_cast<const float4 *>(q)[0];
+            r.w[1] = reinterpret_cast<const float4 *>(q)[1];
+        } else {
+            float f[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f[e] = c + e < k ? q[e] : 0.f;
+            r.w[0] = make_float4(f[0], f[1], f[2], f[3]);
+            r.w[1] = make_float4(f[4], f[5], f[6], f[7]);
+        }
+    } else {
+        const uint16_t *q = static_cast<const uint16_t *>(p) + base + c;
+        if (VEC && c + 8 <= k) {
+            r.w = *reinterpret_cast<const uint4 *>(q);
+        } else {
+            uint32_t x[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                x[e] = (c + 2 * e < k ? q[2 * e] : 0u) | (c + 2 * e + 1 < k ? static_cast<uint32_t>(q[2 * e + 1]) << 16 : 0u);
+            r.w = make_uint4(x[0], x[1], x[2], x[3]);
+        }
+    }
+    return r;
+}
+// Largest magnitude of eight values, as the bits of a float (16-bit integers order 16-bit floats, NaN and infinities on top).
+template <int IN>
+__device__ __forceinline__ uint32_t peak8(const Raw8<IN> &r) {
+    if constexpr (IN == B200Q_F32) {
+        uint32_t top = 0u;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) top = max(max(top, max(abs_bits(r.w[h].x), abs_bits(r.w[h].y))), max(abs_bits(r.w[h].z), abs_bits(r.w[h].w)));
+        return top;
+    } else {
+        constexpr uint32_t SIGNS = 0x7fff7fffu;
+        const uint32_t top = __vmaxu2(__vmaxu2(r.w.x & SIGNS, r.w.y & SIGNS), __vmaxu2(r.w.z & SIGNS, r.w.w & SIGNS));
+        return max(top & 0xffffu, top >> 16);
+    }
+}
+template <int IN>
+__device__ __forceinline__ uint32_t peak_bits(uint32_t peak) {
+    if (IN == B200Q_F32) return peak;
+    if (IN == B200Q_BF16) return peak << 16;
+    return abs_bits(__half2float(__ushort_as_half(static_cast<unsigned short>(peak))));
 }
 
-template <bool VEC>
-__global__ void __launch_bounds__(256) int8_quantize_kernel(const void *x, int dtype, int k, long long x_row, int8_t *codes,
-                                                            long long codes_row, float *scales, int early) {
-    constexpr int KEEP = 4;
+// A CTA takes a row at a time: the largest magnitude, then the codes. The row's pieces of eight values stay in registers, as they
+// were loaded, between the two up to 256 * 8 * KEEP columns (longer rows are read again), and the next row's are on their way
+// meanwhile. Bound by memory (4096 x 8192 BF16: one row per CTA and held as floats 34 us; 15 us at the measured bandwidth).
+template <int IN, bool VEC>
+__global__ void __launch_bounds__(256, 4) int8_quantize_kernel(const void *x, int rows, int k, long long x_row, int8_t *codes,
+                                                               long long codes_row, float *scales, int early) {
+    constexpr int KEEP = IN == B200Q_F32 ? 2 : 4;
     __shared__ uint32_t peaks[8];
     if (early) chain_trigger();
     chain_wait();
-    const int tid = threadIdx.x;
-    const size_t base = blockIdx.x * static_cast<size_t>(x_row);
-    const int padded = (k + 15) & ~15;
-    float kept[KEEP][8];
-    uint32_t peak = 0u;
+    const int tid = threadIdx.x, padded = (k + 15) & ~15;
+    Raw8<IN> next[KEEP];
+    auto load_row = [&](int row) {
 #pragma unroll
-    for (int j = 0; j < KEEP; ++j) {
-        const int c = (tid + 256 * j) * 8;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) kept[j][e] = 0.f;
-        if (c < k) load8<VEC>(x, dtype, base, c, k, kept[j]);
-    }
-#pragma unroll
-    for (int j = 0; j < KEEP; ++j)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) peak = max(peak, abs_bits(kept[j][e]));
-    for (int c = (tid + 256 * KEEP) * 8; c < k; c += 256 * 8) {
-        float f[8];
-        load8<VEC>(x, dtype, base, c, k, f);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) peak = max(peak, abs_bits(f[e]));
-    }
-    peak = __reduce_max_sync(0xffffffffu, peak);
-    if ((tid & 31) == 0) peaks[tid >> 5] = peak;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < 8; ++w) peak = max(peak, peaks[w]);
-    const float s = int8_scale(peak), inv = __fdiv_rn(1.f, s);
-    if (tid == 0) scales[blockIdx.x] = s;
-    auto put = [&](int c, const float (&f)[8]) {
-        const float lo[4] = {f[0], f[1], f[2], f[3]}, hi[4] = {f[4], f[5], f[6], f[7]};
-        const uint32_t w[2] = {int8_codes(lo, s, inv), int8_codes(hi, s, inv)};
-        *reinterpret_cast<uint2 *>(codes + blockIdx.x * static_cast<size_t>(codes_row) + c) = make_uint2(w[0], w[1]);
+        for (int j = 0; j < KEEP; ++j) {
+            const int c = (tid + 256 * j) * 8;
+            next[j] = Raw8<IN>{};
+            if (row < rows && c < k) next[j] = load8<IN, VEC>(x, row * static_cast<size_t>(x_row), c, k);
+        }
     };
+    load_row(blockIdx.x);
+    for (int row = blockIdx.x; row < rows; row += gridDim.x) {
+        const size_t base = row * static_cast<size_t>(x_row);
+        Raw8<IN> kept[KEEP];
+        uint32_t peak = 0u;
 #pragma unroll
-    for (int j = 0; j < KEEP; ++j) {
-        const int c = (tid + 256 * j) * 8;
-        if (c < padded) put(c, kept[j]);
-    }
-    for (int c = (tid + 256 * KEEP) * 8; c < padded; c += 256 * 8) {
-        float f[8];
-        load8<VEC>(x, dtype, base, c, k, f);
-        put(c, f);
+        for (int j = 0; j < KEEP; ++j) {
+            kept[j] = next[j];
+            peak = max(peak, peak8<IN>(kept[j]));
+        }
+        load_row(row + gridDim.x);
+        for (int c = (tid + 256 * KEEP) * 8; c < k; c += 256 * 8) peak = max(peak, peak8<IN>(load8<IN, VEC>(x, base, c, k)));
+        peak = __reduce_max_sync(0xffffffffu, peak);
+        __syncthreads();                                 // (the previous row's peaks have been read)
+        if ((tid & 31) == 0) peaks[tid >> 5] = peak;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < 8; ++w) peak = max(peak, peaks[w]);
+        const float s = int8_scale(peak_bits<IN>(peak)), inv = __fdiv_rn(1.f, s);
+        if (tid == 0) scales[row] = s;
+        auto put = [&](int c, const Raw8<IN> &r) {
+            float f[8];
+            r.values(f);
+            const float lo[4] = {f[0], f[1], f[2], f[3]}, hi[4] = {f[4], f[5], f[6], f[7]};
+            *reinterpret_cast<uint2 *>(codes + row * static_cast<size_t>(codes_row) + c) = make_uint2(int8_codes(lo, s, inv), int8_codes(hi, s, inv));
+        };
+#pragma unroll
+        for (int j = 0; j < KEEP; ++j) {
+            const int c = (tid + 256 * j) * 8;
+            if (c < padded) put(c, kept[j]);
+        }
+        for (int c = (tid + 256 * KEEP) * 8; c < padded; c += 256 * 8) {
+            if (c < k) put(c, load8<IN, VEC>(x, base, c, k));
+            else put(c, Raw8<IN>{});
+        }
     }
 }
 
@@ -519,8 +566,6 @@ __global__ void __launch_bounds__(I8_THREADS, 1) int8_pair_kernel(const __grid_c
 }
 
 // ----------------------------------------------------------------------------------------------------------- host side
-int kv8_shared_memory(const void *kernel, int bytes);        // kv8_decode.cu
-
 // A [rows][row] int8 matrix, read in boxes of 128 codes x box_rows rows; codes from `columns` on read as zeros.
 static int int8_map(CUtensorMap *map, EncodeTiledFn encode, const int8_t *codes, int columns, long long row, int rows, int box_rows) {
     const cuuint64_t dims[2] = {static_cast<cuuint64_t>(columns), static_cast<cuuint64_t>(rows)};
@@ -555,7 +600,7 @@ static int int8_gemm(const int8_t *w, long long w_row, const int8_t *x, long lon
         if (int rc = int8_map(&wmap, encode, w, columns, w_row, a.n, 128)) return rc;
         a.stages = 6;
         const int smem = a.stages * I8_PAIR_STAGE + 1024, pairs = static_cast<int>(std::min<long long>(big, sms / 2));
-        if (int rc = kv8_shared_memory(reinterpret_cast<const void *>(int8_pair_kernel), smem)) return rc;
+        if (int rc = allow_large_shared_memory(reinterpret_cast<const void *>(int8_pair_kernel))) return rc;
         launch_chained_cluster(int8_pair_kernel, dim3(2 * pairs), dim3(I8_THREADS), smem, stream, 2, xmap, wmap, a);
         return check_launch("int8_gemm");
     }
@@ -573,7 +618,7 @@ static int int8_gemm(const int8_t *w, long long w_row, const int8_t *x, long lon
     if (int rc = int8_map(&wmap, encode, w, columns, w_row, a.n, nt)) return rc;
     const Int8Fn fn = nt == 64 ? tile_kernel<64>(split) : tile_kernel<128>(split);
     const int smem = a.stages * stage + 1024;
-    if (int rc = kv8_shared_memory(reinterpret_cast<const void *>(fn), 200 * 1024 + 1024)) return rc;
+    if (int rc = allow_large_shared_memory(reinterpret_cast<const void *>(fn))) return rc;
     const dim3 grid(tiles_n * split, token_tiles);
     if (split > 1) launch_chained_cluster(fn, grid, dim3(I8_THREADS), smem, stream, split, xmap, wmap, a);
     else launch_chained(fn, grid, dim3(I8_THREADS), smem, stream, xmap, wmap, a);
@@ -591,11 +636,14 @@ extern "C" int b200q_int8_quantize(const void *x, int x_dtype, int rows, int k, 
     if (!dtype_valid(x_dtype)) return fail(B200Q_EINVAL, "int8_quantize: bad dtype");
     if (rows < 0 || k < 1 || x_row < k || codes_row % 16 || codes_row < k)
         return fail(B200Q_EINVAL, "int8_quantize: bad shape rows=%d k=%d (code rows are multiples of 16 bytes)", rows, k);
+    if (rows > 0x7fff0000) return fail(B200Q_EUNSUPPORTED, "int8_quantize: too many rows");
     if (reinterpret_cast<uintptr_t>(codes) & 15) return fail(B200Q_EINVAL, "int8_quantize: codes must be 16-byte aligned");
     const size_t e = dtype_size(x_dtype);
     const bool vec = (reinterpret_cast<uintptr_t>(x) & 15) == 0 && x_row * e % 16 == 0;
-    launch_chained(vec ? int8_quantize_kernel<true> : int8_quantize_kernel<false>, dim3(rows), dim3(256), 0,
-                   static_cast<cudaStream_t>(stream), x, x_dtype, k, static_cast<long long>(x_row), codes,
+    auto kernel = x_dtype == B200Q_F32   ? (vec ? int8_quantize_kernel<B200Q_F32, true> : int8_quantize_kernel<B200Q_F32, false>)
+                  : x_dtype == B200Q_F16 ? (vec ? int8_quantize_kernel<B200Q_F16, true> : int8_quantize_kernel<B200Q_F16, false>)
+                                         : (vec ? int8_quantize_kernel<B200Q_BF16, true> : int8_quantize_kernel<B200Q_BF16, false>);
+    launch_chained(kernel, dim3(std::min(rows, 4 * sm_count())), dim3(256), 0, static_cast<cudaStream_t>(stream), x, rows, k, static_cast<long long>(x_row), codes,
                    static_cast<long long>(codes_row), scales, early);
     return check_launch("int8_quantize");
 }

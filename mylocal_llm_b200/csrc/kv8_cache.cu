@@ -43,7 +43,9 @@ __global__ void __launch_bounds__(EXTEND_THREADS) kv8_extend_kernel(const b200q_
                                                                     int *status) {
     chain_trigger();
     chain_wait();
+    __shared__ int first_s[EXTEND_THREADS];              // of a batch that fits: searched for every page taken
     const int tid = threadIdx.x;
+    const bool small = batch <= EXTEND_THREADS;
     int carry = 0, bad = 0;
     for (int b0 = 0; b0 < batch; b0 += EXTEND_THREADS) {
         const int b = b0 + tid;
@@ -60,10 +62,14 @@ __global__ void __launch_bounds__(EXTEND_THREADS) kv8_extend_kernel(const b200q_
         }
         int sum;
         const int before = block_prefix(need, &sum);
-        if (b < batch) starts[b] = carry + before;       // first page request of the entry, until the pages are assigned
+        if (b < batch) {                                 // first page request of the entry, until the pages are assigned
+            if (small) first_s[b] = before;
+            else starts[b] = carry + before;
+        }
         carry += sum;
     }
     bad = __syncthreads_or(bad);
+    const int *request = small ? first_s : starts;
     const int total = carry, words = (c.pages + 31) / 32;
     if (total > 0 && !bad) {
         int have = 0;
@@ -87,14 +93,14 @@ __global__ void __launch_bounds__(EXTEND_THREADS) kv8_extend_kernel(const b200q_
             int e = 0;                                   // entry of request r: the last with starts[e] <= r that needs any
             for (int lo = 0, hi = batch - 1; lo <= hi;) {
                 const int mid = (lo + hi) >> 1;
-                if (starts[mid] <= r) { e = mid; lo = mid + 1; } else { hi = mid - 1; }
+                if (request[mid] <= r) { e = mid; lo = mid + 1; } else { hi = mid - 1; }
             }
             while (left && r < total) {
                 const int bit = __ffs(left) - 1;
                 left &= left - 1;
-                while (e + 1 < batch && starts[e + 1] <= r) ++e;
+                while (e + 1 < batch && request[e + 1] <= r) ++e;
                 const int page = w * 32 + bit, slot = slots[e];
-                c.table[static_cast<size_t>(slot) * c.blocks + c.lengths[slot] / KV8_BLOCK + (r - starts[e])] = page;
+                c.table[static_cast<size_t>(slot) * c.blocks + c.lengths[slot] / KV8_BLOCK + (r - request[e])] = page;
                 c.refs[page] = 1;
                 ++r;
             }
@@ -402,6 +408,8 @@ __global__ void __launch_bounds__(1024) kv8_fork_check_kernel(const b200q_kv8_ca
     for (int i = tid; i < count; i += 1024) c.lengths[dst[i]] = c.lengths[src[i]];
 }
 
+constexpr int COPY_PIECES = 8;               // 16-byte pieces in flight per thread of the copying kernels
+
 // fork, second kernel: CTA (0, i) copies the table row of pair i and counts its pages, CTA (1 + layer, i) the tokens of the
 // tail of one layer - rows below length % 64 only, as 16-byte pieces.
 __global__ void __launch_bounds__(256) kv8_fork_copy_kernel(const b200q_kv8_cache c, const int32_t *src, const int32_t *dst,
@@ -421,11 +429,21 @@ __global__ void __launch_bounds__(256) kv8_fork_copy_kernel(const b200q_kv8_cach
     }
     const int layer = blockIdx.x - 1, units = 2 * c.kv_heads;
     const size_t from = kv8_unit(s, c.layers, layer, 0, c.kv_heads, 0), to = kv8_unit(d, c.layers, layer, 0, c.kv_heads, 0);
-    const int pieces = (length % KV8_BLOCK) * c.head_dim / 8, unit_pieces = KV8_BLOCK * c.head_dim / 8;
+    const int pieces = (length % KV8_BLOCK) * c.head_dim / 8, unit_pieces = KV8_BLOCK * c.head_dim / 8, all = units * pieces;
     const uint4 *tail_from = static_cast<const uint4 *>(c.tail) + from * unit_pieces;
     uint4 *tail_to = static_cast<uint4 *>(c.tail) + to * unit_pieces;
-    for (int u = tid >> 5; u < units; u += 8)
-        for (int j = tid & 31; j < pieces; j += 32) tail_to[u * unit_pieces + j] = tail_from[u * unit_pieces + j];
+    for (int j0 = tid; j0 < all; j0 += 256 * COPY_PIECES) {
+        uint4 v[COPY_PIECES];
+        size_t at[COPY_PIECES];
+#pragma unroll
+        for (int q = 0; q < COPY_PIECES; ++q) {
+            const int j = min(j0 + 256 * q, all - 1), u = j / pieces;        // (the last piece again, past the end)
+            at[q] = static_cast<size_t>(u) * unit_pieces + (j - u * pieces);
+            v[q] = __ldcs(tail_from + at[q]);
+        }
+#pragma unroll
+        for (int q = 0; q < COPY_PIECES; ++q) __stcs(tail_to + at[q], v[q]);
+    }
     for (int u = tid; u < units; u += 256) c.peak[to + u] = c.peak[from + u];
 }
 
@@ -456,7 +474,7 @@ __global__ void __launch_bounds__(256) kv8_free_kernel(const b200q_kv8_cache c, 
 // First kernel (one CTA): place[page] = the live page's number in the new pool (live pages keep their order), source[] the
 // reverse, and the new pool's counts and free bits.
 __global__ void __launch_bounds__(1024) kv8_compact_plan_kernel(const b200q_kv8_cache c, const b200q_kv8_cache to,
-                                                                int32_t *place, int32_t *source, int *status) {
+                                                                int32_t *count, int32_t *place, int32_t *source) {
     chain_trigger();
     chain_wait();
     const int tid = threadIdx.x;
@@ -473,7 +491,7 @@ __global__ void __launch_bounds__(1024) kv8_compact_plan_kernel(const b200q_kv8_
         }
         live += sum;
     }
-    if (live > to.pages && tid == 0) atomicExch(status, STATUS_KV8_COMPACT);
+    if (tid == 0) *count = live;
     for (int p = min(live, to.pages) + tid; p < to.pages; p += 1024) {
         source[p] = -1;
         to.refs[p] = 0;
@@ -488,7 +506,6 @@ __global__ void __launch_bounds__(1024) kv8_compact_plan_kernel(const b200q_kv8_
 
 // Second kernel: a grid over equal pieces of everything that moves - codes and scales of the live pages, the tails and
 // peaks of all sequences, table and lengths. Pure copying, bound by memory.
-constexpr int COPY_PIECES = 4;               // 16-byte pieces in flight per thread
 __global__ void __launch_bounds__(256) kv8_compact_copy_kernel(const b200q_kv8_cache c, const b200q_kv8_cache to,
                                                                const int32_t *place, const int32_t *source,
                                                                int chunks_per_page, int page_ctas, int tail_ctas) {
@@ -506,10 +523,10 @@ __global__ void __launch_bounds__(256) kv8_compact_copy_kernel(const b200q_kv8_c
         uint4 v[COPY_PIECES];
 #pragma unroll
         for (int j = 0; j < COPY_PIECES; ++j)
-            if (at + 256 * j < page_pieces) v[j] = in[at + 256 * j];
+            if (at + 256 * j < page_pieces) v[j] = __ldcs(in + at + 256 * j);
 #pragma unroll
         for (int j = 0; j < COPY_PIECES; ++j)
-            if (at + 256 * j < page_pieces) out[at + 256 * j] = v[j];
+            if (at + 256 * j < page_pieces) __stcs(out + at + 256 * j, v[j]);
         if (chunk == 0)
             for (int j = tid; j < page_scales; j += 256)
                 to.scales[static_cast<size_t>(page) * page_scales + j] = c.scales[static_cast<size_t>(from) * page_scales + j];
@@ -648,34 +665,43 @@ extern "C" int b200q_kv8_free(const b200q_kv8_cache *cache, const int32_t *slots
 
 extern "C" long long b200q_kv8_compact_workspace(const b200q_kv8_cache *from, const b200q_kv8_cache *to) {
     if (!from || !to || from->pages < 1 || to->pages < 1) return 0;
-    return 4ll * (static_cast<long long>(from->pages) + to->pages);
+    return 4ll * (1 + static_cast<long long>(from->pages) + to->pages);
 }
 
-extern "C" int b200q_kv8_compact(const b200q_kv8_cache *from, const b200q_kv8_cache *to, void *workspace,
-                                 long long workspace_bytes, void *stream) {
-    if (int rc = kv8_check("kv8_compact", from)) return rc;
-    if (int rc = kv8_check("kv8_compact", to)) return rc;
+static int compact_check(const char *what, const b200q_kv8_cache *from, const b200q_kv8_cache *to, const void *workspace,
+                         long long workspace_bytes) {
+    if (int rc = kv8_check(what, from)) return rc;
+    if (int rc = kv8_check(what, to)) return rc;
     if (from->layers != to->layers || from->kv_heads != to->kv_heads || from->head_dim != to->head_dim ||
         from->sequences != to->sequences || from->blocks != to->blocks || from->dtype != to->dtype)
-        return fail(B200Q_EINVAL, "kv8_compact: the caches differ in more than their pages");
+        return fail(B200Q_EINVAL, "%s: the caches differ in more than their pages", what);
     if (from->codes == to->codes || from->tail == to->tail || from->table == to->table)
-        return fail(B200Q_EINVAL, "kv8_compact: the new cache must have memory of its own");
+        return fail(B200Q_EINVAL, "%s: the new cache must have memory of its own", what);
     if (!workspace || workspace_bytes < b200q_kv8_compact_workspace(from, to))
-        return fail(B200Q_EINVAL, "kv8_compact: workspace too small");
-    int *status = device_status_word();
-    if (!status) return fail(B200Q_ECUDA, "kv8_compact: no CUDA device");
-    int32_t *place = static_cast<int32_t *>(workspace), *source = place + from->pages;
-    cudaStream_t s = static_cast<cudaStream_t>(stream);
+        return fail(B200Q_EINVAL, "%s: workspace too small", what);
+    return B200Q_OK;
+}
+
+extern "C" int b200q_kv8_compact_plan(const b200q_kv8_cache *from, const b200q_kv8_cache *to, void *workspace,
+                                      long long workspace_bytes, void *stream) {
+    if (int rc = compact_check("kv8_compact_plan", from, to, workspace, workspace_bytes)) return rc;
+    int32_t *count = static_cast<int32_t *>(workspace), *place = count + 1;
+    launch_chained(kv8_compact_plan_kernel, dim3(1), dim3(1024), 0, static_cast<cudaStream_t>(stream), *from, *to, count, place,
+                   place + from->pages);
+    return check_launch("kv8_compact_plan");
+}
+
+extern "C" int b200q_kv8_compact_move(const b200q_kv8_cache *from, const b200q_kv8_cache *to, const void *workspace,
+                                      long long workspace_bytes, void *stream) {
+    if (int rc = compact_check("kv8_compact_move", from, to, workspace, workspace_bytes)) return rc;
+    const int32_t *place = static_cast<const int32_t *>(workspace) + 1, *source = place + from->pages;
     const long long units = static_cast<long long>(from->layers) * 2 * from->kv_heads;
     const long long chunk = 256 * COPY_PIECES, page_pieces = units * KV8_BLOCK * from->head_dim / 16;
     const long long chunks = (page_pieces + chunk - 1) / chunk;
     const long long tail_ctas = (from->sequences * units * KV8_BLOCK * from->head_dim / 8 + chunk - 1) / chunk;
     const long long ctas = chunks * to->pages + tail_ctas + from->sequences;
-    if (ctas > 0x7fffffffll) return fail(B200Q_EUNSUPPORTED, "kv8_compact: pool too large");
-    launch_chained(kv8_compact_plan_kernel, dim3(1), dim3(1024), 0, s, *from, *to, place, source, status);
-    if (int rc = check_launch("kv8_compact")) return rc;
-    launch_chained(kv8_compact_copy_kernel, dim3(static_cast<unsigned>(ctas)), dim3(256), 0, s, *from, *to,
-                   static_cast<const int32_t *>(place), static_cast<const int32_t *>(source), static_cast<int>(chunks),
-                   static_cast<int>(chunks * to->pages), static_cast<int>(tail_ctas));
-    return check_launch("kv8_compact");
+    if (ctas > 0x7fffffffll) return fail(B200Q_EUNSUPPORTED, "kv8_compact_move: pool too large");
+    launch_chained(kv8_compact_copy_kernel, dim3(static_cast<unsigned>(ctas)), dim3(256), 0, static_cast<cudaStream_t>(stream), *from,
+                   *to, place, source, static_cast<int>(chunks), static_cast<int>(chunks * to->pages), static_cast<int>(tail_ctas));
+    return check_launch("kv8_compact_move");
 }

@@ -2,15 +2,12 @@
 //
 // Bound by memory: every byte of a context is read once per key/value head, for the `group` query heads that share it (one or
 // two tiles of eight rows, kv8_attention.cuh). The work of a call is a list of
-// units - blocks of 64 keys of (key/value head, tile of rows, sequence) - cut into equal parts, one per CTA and a CTA per SM,
+// units - blocks of 64 keys of (key/value head, tile of rows, sequence) - cut into equal parts, one per CTA and two CTAs per SM,
 // wherever the borders of the sequences lie; a sequence cut in two leaves FP32 partial results (maximum, sum, values) that a
-// second kernel joins. Inside a CTA the units of a part go to the warps in turn. A warp keeps its next pages on their way with
+// second kernel joins. Short sequences are not cut, and very short ones (SOLO) belong to one warp each, which needs no other. Inside a CTA the units of a part go to the warps in turn. A warp keeps its next pages on their way with
 // one bulk copy each for keys and values (contiguous in a page) into its own stages in shared memory, so 100 to 200 KB per SM
 // are in flight without a register, and its warps meet only at the end of a sequence.
 #include <algorithm>
-#include <mutex>
-#include <utility>
-#include <vector>
 
 #include "kv8_attention.cuh"
 
@@ -18,19 +15,24 @@ namespace b200q {
 
 constexpr int STATUS_KV8_WAIT = 511;        // gave up waiting for a page
 constexpr int KV8_MAX_BATCH = 1024;         // sequences of one launch
+constexpr int KV8_MAX_PARTS = 1024;         // parts that a joining kernel looks through
 
 // Warps of a CTA and pages that a warp has in shared memory. The work of a page is a long chain of dependent instructions
 // (1400 for a head dimension of 128): warps hide it, so there are as many as their registers allow.
-template <int DH, int RT> struct DecodeShape {
-    static constexpr int WARPS = RT == 1 ? 12 : 8, STAGES = DH == 64 ? 2 : 1;
+// What parts consist of: any units, with two CTAs per SM so that one's work goes on while the other's warps meet; whole
+// sequences; whole sequences for each warp by itself.
+enum DecodeMode { CUT = 0, WHOLE = 1, SOLO = 2 };
+template <int DH, int RT, int MODE> struct DecodeShape {
+    static constexpr int CTAS = MODE == CUT ? 2 : 1, WARPS = (RT == 1 ? 12 : 8) / CTAS, STAGES = DH == 64 ? 2 : 1;
 };
 
 struct Kv8Decode {
     Kv8Attention a;
     int group, tiles;             // query heads per key/value head; lists of 8 RT rows (tokens x heads of the group) per head
-    int whole;                    // parts consist of whole sequences (nothing to join)
     float *partial;               // [CTA][2][8 RT][DH + 2]
-    int32_t *prefix;              // units of the sequences before each, [batch + 1]: for the joining kernel
+    int4 *cuts;                   // [CTA], for the joining kernel: slot of the sequence that begins in the part and goes on behind
+                                  // it (-1: none), its list, its number; list * batch + number of the one that goes on from
+                                  // the part before (-1: none)
     int *status;
 };
 
@@ -40,9 +42,9 @@ __device__ __forceinline__ int units_of(const Kv8Attention &a, int b) {
     return start < 0 || n <= 0 ? 0 : (start + n + KV8_BLOCK - 1) / KV8_BLOCK;
 }
 
-template <int DH, bool BF16, int RT>
-__global__ void __launch_bounds__(DecodeShape<DH, RT>::WARPS * 32, 1) kv8_decode_kernel(const b200q_kv8_cache c, const Kv8Decode p) {
-    constexpr int W = DecodeShape<DH, RT>::WARPS, ST = DecodeShape<DH, RT>::STAGES, HALF_PAGE = KV8_BLOCK * DH, DT = DH / 8, LD = DH + 4;
+template <int DH, bool BF16, int RT, int MODE>
+__global__ void __launch_bounds__(DecodeShape<DH, RT, MODE>::WARPS * 32, DecodeShape<DH, RT, MODE>::CTAS) kv8_decode_kernel(const b200q_kv8_cache c, const Kv8Decode p) {
+    constexpr int W = DecodeShape<DH, RT, MODE>::WARPS, ST = DecodeShape<DH, RT, MODE>::STAGES, HALF_PAGE = KV8_BLOCK * DH, DT = DH / 8, LD = DH + 4;
     extern __shared__ __align__(128) uint8_t smem[];
     uint8_t *ring = smem;                                                            // [W][ST][2][HALF_PAGE]
     float *merged = reinterpret_cast<float *>(smem + W * ST * 2 * HALF_PAGE);        // [W][4][LD]: values of 4 rows, maximum, sum
@@ -79,8 +81,6 @@ __global__ void __launch_bounds__(DecodeShape<DH, RT>::WARPS * 32, 1) kv8_decode
         if (b < a.batch) prefix[b + 1] = before + incl;
     }
     __syncthreads();
-    if (blockIdx.x == 0 && p.prefix)
-        for (int b = tid; b <= a.batch; b += W * 32) p.prefix[b] = prefix[b];
     // rows of refused sequences
     for (int b = blockIdx.x; b < a.batch; b += gridDim.x)
         if (a.starts[b] < 0)
@@ -91,18 +91,24 @@ __global__ void __launch_bounds__(DecodeShape<DH, RT>::WARPS * 32, 1) kv8_decode
     const int lists = c.kv_heads * p.tiles;                  // a list of all sequences per head and tile
     const long long all = static_cast<long long>(lists) * total_units;
     long long lo, hi;
-    if (p.whole) {
+    if constexpr (MODE != CUT) {
         const long long segments = static_cast<long long>(lists) * a.batch;
-        const long long s0 = segments * blockIdx.x / gridDim.x, s1 = segments * (blockIdx.x + 1) / gridDim.x;
+        const int parts = MODE == SOLO ? gridDim.x * W : gridDim.x, part = MODE == SOLO ? blockIdx.x * W + warp : blockIdx.x;
+        const long long s0 = segments * part / parts, s1 = segments * (part + 1) / parts;
         lo = s0 / a.batch * total_units + prefix[s0 % a.batch];
         hi = s1 / a.batch * total_units + prefix[s1 % a.batch];
     } else {
         lo = all * blockIdx.x / gridDim.x;
         hi = all * (blockIdx.x + 1) / gridDim.x;
     }
-    if (lo >= hi) return;
+    if (lo >= hi) {                                          // (SOLO: the warp; nothing below is for the whole CTA then)
+        if (MODE == CUT && tid == 0) p.cuts[blockIdx.x] = make_int4(-1, 0, 0, -1);
+        return;
+    }
 
-    // ---- this warp's units warp, warp + W, ... of the part, numbered from its beginning
+    // ---- this warp's units of the part, numbered from its beginning: every W-th, or all of them
+    constexpr int STEP = MODE == SOLO ? 1 : W;
+    const int first = MODE == SOLO ? 0 : warp;
     const int count = static_cast<int>(hi - lo);
     uint8_t *my_ring = ring + warp * ST * 2 * HALF_PAGE;
     uint64_t *my_bars = bars + warp * 2 * ST;
@@ -120,7 +126,7 @@ __global__ void __launch_bounds__(DecodeShape<DH, RT>::WARPS * 32, 1) kv8_decode
 
     // The next unit to be looked up: its page is read from the table one unit before its copies are requested.
     constexpr int PAGE = 0, TAIL = 1, NONE = 2;
-    int pu = warp, plist = list, pseq = s, pbegin = begin, pend = begin, pfull = 0;
+    int pu = first, plist = list, pseq = s, pbegin = begin, pend = begin, pfull = 0;
     const int32_t *prow = nullptr;
     struct Unit { int kind, page, list, seq; };
     auto open = [&] {                                        // sequence pseq of plist
@@ -142,7 +148,7 @@ __global__ void __launch_bounds__(DecodeShape<DH, RT>::WARPS * 32, 1) kv8_decode
             open();
         }
         const int unit = pu - pbegin;
-        pu += W;
+        pu += STEP;
         return unit < pfull ? Unit{PAGE, prow[unit], plist, pseq} : Unit{TAIL, 0, plist, pseq};
     };
     // (a table that lacks the page reads another one, not beyond the pool)
@@ -213,7 +219,7 @@ __global__ void __launch_bounds__(DecodeShape<DH, RT>::WARPS * 32, 1) kv8_decode
         if (++st == ST) st = 0;
     };
 
-    int u = warp;
+    int u = first, from_before = -1;
     for (;;) {
         // ---- one segment: the units [at, end) of sequence s
         const int seq_end = begin + prefix[s + 1] - prefix[s], end = min(seq_end, count);
@@ -241,7 +247,7 @@ __global__ void __launch_bounds__(DecodeShape<DH, RT>::WARPS * 32, 1) kv8_decode
                     a, valid ? (row_of + token) * a.q_row + static_cast<long long>(head * p.group + row - token * p.group) * DH : -1,
                     pos[r], t, qf[r]);
             }
-            for (; u < end; u += W) {
+            for (; u < end; u += STEP) {
                 const int unit = u - begin;
                 const bool tail = kind_at[0] == TAIL;
                 const uint8_t *stage = my_ring + st * 2 * HALF_PAGE;
@@ -370,7 +376,7 @@ __global__ void __launch_bounds__(DecodeShape<DH, RT>::WARPS * 32, 1) kv8_decode
                 advance();
             }
         } else {
-            for (; u < end; u += W) {                        // rows that do not exist: the units pass by
+            for (; u < end; u += STEP) {                     // rows that do not exist: the units pass by
                 if (kind_at[0] == PAGE) arrived(0, st, k_phases);
                 arrived(1, st, v_phases);
                 request(0, next, st);
@@ -378,6 +384,23 @@ __global__ void __launch_bounds__(DecodeShape<DH, RT>::WARPS * 32, 1) kv8_decode
                 advance();
             }
         }
+        // ---- a warp by itself has its rows' results
+        if constexpr (MODE == SOLO) {
+#pragma unroll
+            for (int r = 0; r < RT; ++r) {
+                float sum = l[r];
+                sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+                if (g + 8 * r >= rows) continue;
+                const int row = row0 + g + 8 * r, token = row / p.group;
+                const size_t to = (static_cast<size_t>(row_of + token) * a.heads + head * p.group + row - token * p.group) * DH + 2 * t;
+#pragma unroll
+                for (int i = 0; i < DT; ++i) {
+                    store_from_float(a.out, c.dtype, to + 8 * i, o[r][i][0] / sum);
+                    store_from_float(a.out, c.dtype, to + 8 * i + 1, o[r][i][1] / sum);
+                }
+            }
+        } else {
         // ---- join the warps, four rows at a time
         const bool complete = at == begin && end == seq_end;
 #pragma unroll
@@ -424,7 +447,13 @@ __global__ void __launch_bounds__(DecodeShape<DH, RT>::WARPS * 32, 1) kv8_decode
             }
             __syncthreads();
         }
-        if (end == count) break;
+        }
+        if (MODE == CUT && begin < 0) from_before = list * a.batch + s;
+        if (end == count) {
+            if (MODE == CUT && tid == 0)
+                p.cuts[blockIdx.x] = make_int4(begin >= 0 && seq_end > count ? (at == 0 ? 0 : 1) : -1, list, s, from_before);
+            break;
+        }
         at = end;
         begin = seq_end;
         do {
@@ -442,39 +471,40 @@ __global__ void __launch_bounds__(DecodeShape<DH, RT>::WARPS * 32, 1) kv8_decode
     }
 }
 
-// Joins the partial results of the sequences that were cut: one CTA per (list, sequence).
+// Joins the partial results of the sequences that were cut: CTA i joins the one that begins in part i and goes on behind it.
 template <int DH>
-__global__ void __launch_bounds__(128) kv8_decode_join_kernel(const b200q_kv8_cache c, const Kv8Decode p, int ctas, int tile) {
+__global__ void __launch_bounds__(256) kv8_decode_join_kernel(const b200q_kv8_cache c, const Kv8Decode p, int ctas, int tile) {
+    __shared__ uint8_t holds[KV8_MAX_PARTS];                 // parts that hold some of the sequence (some parts are empty)
+    __shared__ int last_s;
     chain_trigger();
     chain_wait();
     const Kv8Attention &a = p.a;
-    const int s = blockIdx.x, list = blockIdx.y;
-    const int total_units = p.prefix[a.batch], first = p.prefix[s], last = p.prefix[s + 1];
-    if (first == last) return;
-    const long long all = static_cast<long long>(c.kv_heads) * p.tiles * total_units;
-    const long long lo = static_cast<long long>(list) * total_units + first, hi = static_cast<long long>(list) * total_units + last;
-    // the part that holds unit x: the largest i with all * i / ctas <= x
-    auto part_of = [&](long long x) {
-        int i = static_cast<int>(x * ctas / all);
-        while (i + 1 < ctas && all * (i + 1) / ctas <= x) ++i;
-        while (i > 0 && all * i / ctas > x) --i;
-        return i;
-    };
-    const int p0 = part_of(lo), p1 = part_of(hi - 1);
-    if (p0 == p1) return;
+    const int i = blockIdx.x;
+    const int4 cut = p.cuts[i];
+    if (cut.x < 0) return;
+    const int list = cut.y, s = cut.z, slot0 = cut.x;
+    if (threadIdx.x == 0) last_s = i;
+    __syncthreads();
+    for (int q = i + threadIdx.x; q < ctas; q += 256) {
+        const bool mine = q == i || p.cuts[q].w == list * a.batch + s;
+        holds[q] = mine;
+        if (mine && q > i) atomicMax(&last_s, q);
+    }
+    __syncthreads();
+    const int last = last_s;
     const int head = list / p.tiles, row0 = (list - head * p.tiles) * tile;
     const int rows = min((a.offsets[s + 1] - a.offsets[s]) * p.group - row0, tile);
-    const int slot0 = all * p0 / ctas == lo ? 0 : 1;         // the first part may begin with an earlier sequence
-    for (int i = threadIdx.x; i < rows * DH; i += 128) {
-        const int row = i / DH, d = i - row * DH;
+    for (int j = threadIdx.x; j < rows * DH; j += 256) {
+        const int row = j / DH, d = j - row * DH;
+        auto part = [&](int q) { return p.partial + ((static_cast<size_t>(q) * 2 + (q == i ? slot0 : 0)) * tile + row) * (DH + 2); };
         float top = -INFINITY;
-        for (int q = p0; q <= p1; ++q)
-            top = fmaxf(top, p.partial[((static_cast<size_t>(q) * 2 + (q == p0 ? slot0 : 0)) * tile + row) * (DH + 2) + DH]);
+        for (int q = i; q <= last; ++q)
+            if (holds[q]) top = fmaxf(top, part(q)[DH]);
         const float shift = top == -INFINITY ? 0.f : top;
         float value = 0.f, weight = 0.f;
-        for (int q = p0; q <= p1; ++q) {
-            const float *from = p.partial + ((static_cast<size_t>(q) * 2 + (q == p0 ? slot0 : 0)) * tile + row) * (DH + 2);
-            const float f = exp2_approx(from[DH] - shift);
+        for (int q = i; q <= last; ++q) {
+            if (!holds[q]) continue;
+            const float *from = part(q), f = exp2_approx(from[DH] - shift);
             value += f * from[d];
             weight += f * from[DH + 1];
         }
@@ -487,22 +517,26 @@ __global__ void __launch_bounds__(128) kv8_decode_join_kernel(const b200q_kv8_ca
 // ----------------------------------------------------------------------------------------------------------- host side
 // How a call is divided: CTAs, and whether parts are cut at the borders of sequences.
 struct DecodePlan {
-    int tile, tiles, ctas, whole;       // rows per list (8 or 16), lists per head
+    int tile, tiles, ctas, mode;        // rows per list (8 or 16), lists per head
     long long bytes;
 };
 
 static DecodePlan decode_plan(const b200q_kv8_cache *c, int heads, int batch, int max_new, int max_keys) {
     DecodePlan d{};
-    const int group = heads / c->kv_heads, warps = max_new * group <= 8 ? DecodeShape<64, 1>::WARPS : DecodeShape<64, 2>::WARPS;
+    const int group = heads / c->kv_heads;
     const int b = std::min(batch, KV8_MAX_BATCH);
     d.tile = max_new * group <= 8 ? 8 : 16;
     d.tiles = (max_new * group + d.tile - 1) / d.tile;
+    const int warps = d.tile == 8 ? DecodeShape<64, 1, WHOLE>::WARPS : DecodeShape<64, 2, WHOLE>::WARPS;
     const long long units = (max_keys + KV8_BLOCK - 1) / KV8_BLOCK, segments = static_cast<long long>(c->kv_heads) * d.tiles * b;
     const int sms = sm_count();
-    // Up to four rounds of a CTA's warps per sequence are not worth a second kernel.
-    d.whole = units <= 4 * warps;
-    d.ctas = static_cast<int>(std::min<long long>(sms, d.whole ? segments : std::max<long long>(1, segments * units / warps)));
-    d.bytes = d.whole ? 0 : static_cast<long long>(d.ctas) * 2 * d.tile * (c->head_dim + 2) * 4 + (KV8_MAX_BATCH + 1) * 4;
+    // Up to four rounds of a CTA's warps per sequence are not worth a second kernel. A CTA takes about 5 us per sequence whatever
+    // its length (queries, the warps' meeting), a warp by itself one unit in 2 us: 112 sequences of one token and 32 heads took
+    // 117 us by CTAs and take 26 us by warps.
+    d.mode = units > 4 * warps ? CUT : units <= 4 || segments >= 4ll * sms * warps ? SOLO : WHOLE;
+    const long long work = d.mode == SOLO ? (segments + warps - 1) / warps : d.mode == WHOLE ? segments : std::max<long long>(1, segments * units / (warps / 2));
+    d.ctas = static_cast<int>(std::min<long long>({d.mode == CUT ? 2 * sms : sms, work, KV8_MAX_PARTS}));
+    d.bytes = d.mode != CUT ? 0 : static_cast<long long>(d.ctas) * (16 + 2 * d.tile * (c->head_dim + 2) * 4);
     return d;
 }
 
@@ -510,43 +544,37 @@ long long kv8_decode_workspace(const b200q_kv8_cache *c, int heads, int batch, i
     return decode_plan(c, heads, batch, max_new, max_keys).bytes;
 }
 
-// The opt-in to large dynamic shared memory is per function and device: done once each.
-int kv8_shared_memory(const void *kernel, int bytes) {
-    static std::mutex mu;
-    static std::vector<std::pair<const void *, int>> opted;
-    int dev = 0;
-    cudaGetDevice(&dev);
-    std::lock_guard<std::mutex> lock(mu);
-    const std::pair<const void *, int> key(kernel, dev);
-    if (std::find(opted.begin(), opted.end(), key) != opted.end()) return B200Q_OK;
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) {
-        cudaGetLastError();
-        return fail(B200Q_ECUDA, "shared memory opt-in failed");
-    }
-    opted.push_back(key);
-    return B200Q_OK;
-}
-
-template <int DH, bool BF16, int RT>
+template <int DH, bool BF16, int RT, int MODE>
 static int launch_decode(const b200q_kv8_cache &c, Kv8Decode p, const DecodePlan &d, cudaStream_t stream) {
-    constexpr int W = DecodeShape<DH, RT>::WARPS, ST = DecodeShape<DH, RT>::STAGES;
+    constexpr int W = DecodeShape<DH, RT, MODE>::WARPS, ST = DecodeShape<DH, RT, MODE>::STAGES;
     constexpr size_t fixed = static_cast<size_t>(W) * ST * 2 * KV8_BLOCK * DH + W * 4 * (DH + 4) * 4 + W * ST * 16;
     const size_t smem = fixed + (KV8_MAX_BATCH + 1) * 4;
-    static_assert(fixed + (KV8_MAX_BATCH + 1) * 4 + 64 <= 227 * 1024, "shared memory of the decode kernel");
-    if (int rc = kv8_shared_memory(reinterpret_cast<const void *>(kv8_decode_kernel<DH, BF16, RT>), static_cast<int>(smem))) return rc;
+    static_assert((fixed + (KV8_MAX_BATCH + 1) * 4 + 128 + 1024) * DecodeShape<DH, RT, MODE>::CTAS <= 228 * 1024, "shared memory of the decode kernel");
+    if (int rc = allow_large_shared_memory(reinterpret_cast<const void *>(kv8_decode_kernel<DH, BF16, RT, MODE>))) return rc;
     const Kv8Attention whole = p.a;
     for (int b0 = 0; b0 < whole.batch; b0 += KV8_MAX_BATCH) {
         p.a.batch = std::min(KV8_MAX_BATCH, whole.batch - b0);
         p.a.slots = whole.slots + b0;
         p.a.offsets = whole.offsets + b0;
         p.a.starts = whole.starts + b0;
-        launch_chained(kv8_decode_kernel<DH, BF16, RT>, dim3(d.ctas), dim3(W * 32), smem, stream, c, p);
+        launch_chained(kv8_decode_kernel<DH, BF16, RT, MODE>, dim3(d.ctas), dim3(W * 32), smem, stream, c, p);
         if (int rc = check_launch("kv8_attention")) return rc;
-        if (d.whole) continue;
-        launch_chained(kv8_decode_join_kernel<DH>, dim3(p.a.batch, c.kv_heads * d.tiles), dim3(128), 0, stream, c, p, d.ctas, d.tile);
+        if (MODE != CUT) continue;
+        if (d.ctas > 1) launch_chained(kv8_decode_join_kernel<DH>, dim3(d.ctas - 1), dim3(256), 0, stream, c, p, d.ctas, d.tile);
         if (int rc = check_launch("kv8_attention (join)")) return rc;
     }
     return B200Q_OK;
+}
+
+using DecodeLaunch = int (*)(const b200q_kv8_cache &, Kv8Decode, const DecodePlan &, cudaStream_t);
+template <int DH, bool BF16, int RT>
+static DecodeLaunch decode_launch_of(int mode) {
+    return mode == CUT ? launch_decode<DH, BF16, RT, CUT> : mode == WHOLE ? launch_decode<DH, BF16, RT, WHOLE> : launch_decode<DH, BF16, RT, SOLO>;
+}
+template <int DH>
+static DecodeLaunch decode_launch(bool bf16, bool wide, int mode) {
+    return bf16 ? (wide ? decode_launch_of<DH, true, 2>(mode) : decode_launch_of<DH, true, 1>(mode))
+                : (wide ? decode_launch_of<DH, false, 2>(mode) : decode_launch_of<DH, false, 1>(mode));
 }
 
 int kv8_decode(const b200q_kv8_cache *c, const Kv8Attention &a, int max_new, int max_keys, void *workspace,
@@ -561,16 +589,12 @@ int kv8_decode(const b200q_kv8_cache *c, const Kv8Attention &a, int max_new, int
     p.a = a;
     p.group = a.heads / c->kv_heads;
     p.tiles = d.tiles;
-    p.whole = d.whole;
-    p.partial = static_cast<float *>(workspace);
-    p.prefix = d.whole ? nullptr : reinterpret_cast<int32_t *>(p.partial + static_cast<size_t>(d.ctas) * 2 * d.tile * (c->head_dim + 2));
+    p.cuts = static_cast<int4 *>(workspace);
+    p.partial = reinterpret_cast<float *>(p.cuts + (d.mode == CUT ? d.ctas : 0));
     p.status = device_status_word();
     if (!p.status) return fail(B200Q_ECUDA, "kv8_attention: no CUDA device");
     const bool bf16 = c->dtype == B200Q_BF16;
-    auto launch = c->head_dim == 64 ? (d.tile == 8 ? (bf16 ? launch_decode<64, true, 1> : launch_decode<64, false, 1>)
-                                                   : (bf16 ? launch_decode<64, true, 2> : launch_decode<64, false, 2>))
-                                    : (d.tile == 8 ? (bf16 ? launch_decode<128, true, 1> : launch_decode<128, false, 1>)
-                                                   : (bf16 ? launch_decode<128, true, 2> : launch_decode<128, false, 2>));
+    auto launch = c->head_dim == 64 ? decode_launch<64>(bf16, d.tile == 16, d.mode) : decode_launch<128>(bf16, d.tile == 16, d.mode);
     return launch(*c, p, d, stream);
 }
 

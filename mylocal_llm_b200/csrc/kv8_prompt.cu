@@ -679,8 +679,6 @@ __global__ void __launch_bounds__(256) kv8_prompt_join_kernel(const b200q_kv8_ca
 }
 
 // ----------------------------------------------------------------------------------------------------------- host side
-int kv8_shared_memory(const void *kernel, int bytes);        // kv8_decode.cu
-
 // Parts of the keys: as many as give every SM two CTAs, of four units at least.
 static int prompt_splits(const b200q_kv8_cache *c, int heads, int batch, int max_new, int max_keys) {
     const long long rows = static_cast<long long>(max_new) * (heads / c->kv_heads), units = (max_keys + KP_KEYS - 1) / KP_KEYS;
@@ -716,7 +714,7 @@ int kv8_prompt(const b200q_kv8_cache *c, const Kv8Attention &a, int max_new, int
                                     : (bf16 ? kv8_prompt_kernel<128, true, false> : kv8_prompt_kernel<128, false, true>);
     const int smem = 1024 + (c->head_dim == 64 ? (bf16 ? PromptShape<64, false>::BYTES : PromptShape<64, true>::BYTES)
                                                : (bf16 ? PromptShape<128, false>::BYTES : PromptShape<128, true>::BYTES));
-    if (int rc = kv8_shared_memory(reinterpret_cast<const void *>(kernel), smem)) return rc;
+    if (int rc = allow_large_shared_memory(reinterpret_cast<const void *>(kernel))) return rc;
     launch_chained(kernel, dim3(static_cast<unsigned>(across), static_cast<unsigned>(blocks)), dim3(KP_THREADS), smem, stream, *c, p);
     if (int rc = check_launch("kv8_attention")) return rc;
     if (p.splits == 1) return B200Q_OK;

@@ -1,9 +1,12 @@
 // Host-side plumbing shared by all entry points: error text, device status word, SM count.
+#include <algorithm>
 #include <cstdarg>
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
 #include <mutex>
+#include <utility>
+#include <vector>
 
 #include "common.cuh"
 
@@ -75,6 +78,25 @@ int sm_count() {
         counts[dev] = n;
     }
     return counts[dev];
+}
+
+int allow_large_shared_memory(const void *kernel) {
+    static std::mutex mu;
+    static std::vector<std::pair<const void *, int>> opted;
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) {
+        cudaGetLastError();
+        return fail(B200Q_ECUDA, "no CUDA device");
+    }
+    std::lock_guard<std::mutex> lock(mu);
+    const std::pair<const void *, int> key(kernel, dev);
+    if (std::find(opted.begin(), opted.end(), key) != opted.end()) return B200Q_OK;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, LARGE_SHARED_MEMORY) != cudaSuccess) {
+        cudaGetLastError();
+        return fail(B200Q_ECUDA, "shared memory opt-in failed");
+    }
+    opted.push_back(key);
+    return B200Q_OK;
 }
 
 }  // namespace b200q

@@ -217,19 +217,30 @@ class PagedKV8Cache:
 
     def compact(self, pages=None):
         """A new cache, independent of this one, with the same sequences and a pool of ``pages`` pages (default: the live ones)
-        that begins with the live pages in their order. Waits for the device to count them."""
+        that begins with the live pages in their order. Waits for the device to count them (not for the copies)."""
         torch = _torch()
-        live = self.read_live_pages()
-        pages = max(1, live) if pages is None else int(pages)
-        if pages < max(1, live):
-            raise ValueError(f"{live} live pages do not fit a pool of {pages}")
+        if pages is None:
+            pages = max(1, self.read_live_pages())
+        pages = int(pages)
+        if pages < 1:
+            raise ValueError("pages must be positive")
         like = lambda t, n=None: torch.empty((n or t.shape[0],) + t.shape[1:], dtype=t.dtype, device=self.device)  # noqa: E731
         new = type(self).__new__(type(self))
         new._bind(like(self.codes, pages), like(self.scales, pages), like(self.tail), like(self.peak), like(self.table),
                   like(self.lengths), like(self.refs, pages), torch.empty(-(-pages // 32), dtype=torch.int32, device=self.device),
                   self.max_length)
-        space = torch.empty(_lib.load().b200q_kv8_compact_workspace(self._c, new._c), dtype=torch.uint8, device=self.device)
-        _launch(self.device, "b200q_kv8_compact", self._c, new._c, space.data_ptr(), space.numel())
+        size = _lib.load().b200q_kv8_compact_workspace(self._c, new._c)
+        space = torch.empty(size // 4, dtype=torch.int32, device=self.device)
+        with torch.cuda.device(self.device):
+            _launch(self.device, "b200q_kv8_compact_plan", self._c, new._c, space.data_ptr(), size)
+            live = torch.empty(1, dtype=torch.int32, pin_memory=True)
+            live.copy_(space[:1], non_blocking=True)
+            counted = torch.cuda.Event()
+            counted.record()
+            _launch(self.device, "b200q_kv8_compact_move", self._c, new._c, space.data_ptr(), size)
+            counted.synchronize()
+        if int(live) > pages:
+            raise ValueError(f"{int(live)} live pages do not fit a pool of {pages}")
         return new
 
     def read_live_pages(self):

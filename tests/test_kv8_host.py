@@ -73,10 +73,11 @@ def test_page_operations_refuse():
     assert rc("b200q_kv8_free", good, ONE, -1, None) == 1
     other = cache(codes=32, tail=32, table=32, pages=5)
     need = rc("b200q_kv8_compact_workspace", good, ctypes.byref(other))
-    assert need == 4 * 15
-    assert rc("b200q_kv8_compact", good, ctypes.byref(other), ONE, need - 1, None) == 1
-    assert rc("b200q_kv8_compact", good, ctypes.byref(cache(codes=32, tail=32, table=32, layers=3)), ONE, 1 << 20, None) == 1
-    assert rc("b200q_kv8_compact", good, ctypes.byref(cache(codes=32, table=32)), ONE, 1 << 20, None) == 1     # shares the tails
+    assert need == 4 * 16
+    for name in ("b200q_kv8_compact_plan", "b200q_kv8_compact_move"):
+        assert rc(name, good, ctypes.byref(other), ONE, need - 1, None) == 1
+        assert rc(name, good, ctypes.byref(cache(codes=32, tail=32, table=32, layers=3)), ONE, 1 << 20, None) == 1
+        assert rc(name, good, ctypes.byref(cache(codes=32, table=32)), ONE, 1 << 20, None) == 1     # shares the tails
     for name, args in (("b200q_kv8_extend", (ONE, ONE, 0, ONE)), ("b200q_kv8_fork", (ONE, ONE, 0, ONE)), ("b200q_kv8_free", (ONE, 0))):
         assert rc(name, good, *args, None) == 0                                  # nothing to do: no launch
 
