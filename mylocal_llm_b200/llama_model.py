@@ -10,6 +10,8 @@ adapter; here they stay packed and resident in HBM, which is the point of the ex
   ``quantized_swiglu`` on ``DevicePackedGGUFWeight`` (tile layouts where they exist);
 * RMSNorm is ``b200q_rmsnorm`` / the fused residual-add variant; the residual stream is FP32;
 * embedding rows are gathered as packed bytes and decoded by ``b200q_dequantize``;
+* the KV cache is dense in the model's type, or, on request (``create_generation_state(..., kv_cache="int8")``), a
+  ``PagedKV8Cache``: 8-bit blocks in pages of a pool, which prompts of any length and decode steps read with its own kernels;
 * the one-token step runs rotate-half RoPE, the KV-cache store and single-query attention over the cache as one
   kernel (``b200q_rope_attention``; ``b200q_rope_kv_store`` + ``b200q_decode_attention`` are the two-launch form), and ``b200q_silu_mul`` on
   the output of the stacked gate|up projection; prefill (and ``fused_decode = False``) does the
@@ -26,6 +28,7 @@ from dataclasses import dataclass
 import numpy as np
 
 from . import _lib
+from .kv8_cache import BLOCK_TOKENS, PagedKV8Cache
 from .moe_layer import RMSNormInference
 from .quantized_linear import (GEMM_MIN_TOKENS, DevicePackedGGUFWeight, dequantize_device, gemm_rule, packed_to_device, quantized_linear,
                                quantized_swiglu, retile_enabled, retile_gate_up, retile_weight)
@@ -70,6 +73,23 @@ class GenerationState:
         self.k = torch.zeros(shape, dtype=dtype, device=device)
         self.v = torch.zeros(shape, dtype=dtype, device=device)
         self.position = torch.zeros(1, dtype=torch.int64, device=device)      # tokens already in the cache
+        self.length = 0                                                        # host copy, for checks only
+        self.batch, self.horizon = batch, horizon
+
+
+class PagedGenerationState:
+    """The same state on an 8-bit paged cache: ``batch`` sequences in the slots 0, 1, ... of ``cache``. More ``sequences`` than that
+    leave slots to fork into, fewer ``pages`` than every sequence's horizon let short ones share the pool."""
+
+    def __init__(self, config, batch, horizon, dtype, device, sequences=None, pages=None):
+        sequences = batch if sequences is None else int(sequences)
+        if sequences < batch:
+            raise ValueError("a state needs at least as many sequences as its batch")
+        pages = max(1, sequences * (horizon // BLOCK_TOKENS)) if pages is None else int(pages)
+        self.cache = PagedKV8Cache(config.num_hidden_layers, config.num_key_value_heads, config.head_dim, pages=pages,
+                                   sequences=sequences, max_length=horizon, dtype=dtype, device=device)
+        self.slots = list(range(batch))
+        self.step = self.cache.batch(self.slots, [1] * batch)                 # a decode step
         self.length = 0                                                        # host copy, for checks only
         self.batch, self.horizon = batch, horizon
 
@@ -215,11 +235,19 @@ class ExternalLlamaModel:
         if not self._loaded:
             raise RuntimeError("External weights have not been loaded")
 
-    def create_generation_state(self, batch_size=1, max_length=None):
+    def create_generation_state(self, batch_size=1, max_length=None, kv_cache=None, *, sequences=None, pages=None):
+        """Dense caches in the model's type, or (``kv_cache="int8"``, head_dim 64 or 128, 16-bit models) an 8-bit paged cache with
+        ``pages`` pages for ``sequences`` sequences (default: room for every sequence of the batch)."""
         self._require_weights()
+        if kv_cache not in (None, "int8"):
+            raise ValueError("kv_cache must be None or 'int8'")
+        if kv_cache is None and (sequences is not None or pages is not None):
+            raise ValueError("sequences and pages belong to the 8-bit cache")
         max_length = self.config.max_position_embeddings if max_length is None else int(max_length)
         if not 1 <= max_length <= self.config.max_position_embeddings:
             raise ValueError("Requested KV horizon exceeds configured positions")
+        if kv_cache == "int8":
+            return PagedGenerationState(self.config, int(batch_size), max_length, self.dtype, self.device, sequences, pages)
         return GenerationState(self.config, int(batch_size), max_length, self.dtype, self.device)
 
     def _embed(self, token_ids):
@@ -316,7 +344,13 @@ class ExternalLlamaModel:
         _lib.call("b200q_decode_attention", ptr(q2), q2.stride(0), ptr(kc), ptr(vc), cache_id, ptr(positions), b, heads,
                   kv_heads, dh, state.horizon, float(dh ** -0.5), ptr(ctx), cache_id, _lib.current_stream())
 
-    def _forward_one_token(self, token_ids, state, positions):
+    def _paged_attention(self, q2, k2, v2, state, step, layer_index, out=None):
+        """RoPE, cache store and attention of a step's tokens on the 8-bit cache."""
+        rope = (self._cos, self._sin)
+        state.cache.append(layer_index, k2, v2, step, rope=rope)
+        return state.cache.attention(layer_index, q2, step, rope=rope, out=out)
+
+    def _forward_one_token(self, token_ids, state, positions, step=None):
         """The one-token step with every residual-add + RMSNorm deferred into the projection that follows it
         (stacked qkv, stacked gate|up, LM head). Returns FP32 logits [B, vocab]."""
         torch = _torch()
@@ -335,7 +369,10 @@ class ExternalLlamaModel:
                 residual, qkv = self._norm_linear(layer["norm1"], residual, pending, layer["qkv"], torch.float32)
             q2, k2, v2 = qkv[:, :qd], qkv[:, qd:qd + kd], qkv[:, qd + kd:]
             ctx = torch.empty((b, heads * dh), dtype=self.dtype, device=residual.device)
-            self._rope_attention(q2, k2, v2, positions, state, i, ctx)
+            if step is not None:
+                self._paged_attention(q2, k2, v2, state, step, i, ctx)
+            else:
+                self._rope_attention(q2, k2, v2, positions, state, i, ctx)
             attn = quantized_linear(ctx, layer["o"])
             residual, gu = self._norm_linear(layer["norm2"], residual, attn, layer["gate_up"], torch.float32)
             pending = self._silu_linear(gu, layer["down"])
@@ -380,9 +417,9 @@ class ExternalLlamaModel:
                   _lib.current_stream())
         return ctx
 
-    def _forward(self, token_ids, state, positions, mask):
+    def _forward(self, token_ids, state, positions, mask, step=None):
         """token_ids [B, T]; positions [T] device int64; mask [T, horizon] additive FP32, or None for a prompt that
-        starts at position 0 and runs on the prompt-attention kernel. Returns the final normalised hidden states
+        starts at position 0 and runs on the prompt-attention kernel; ``step``: the tokens' batch of an 8-bit cache. Returns the final normalised hidden states
         [B*T, d] in the model dtype."""
         torch = _torch()
         cfg = self.config
@@ -399,6 +436,11 @@ class ExternalLlamaModel:
                 q2 = self._linear(hidden, layer["q"], torch.float32)
                 k2 = self._linear(hidden, layer["k"], torch.float32)
                 v2 = self._linear(hidden, layer["v"], torch.float32)
+            if step is not None:
+                attn = self._linear(self._paged_attention(q2, k2, v2, state, step, i), layer["o"])
+                residual, hidden = layer["norm2"].forward_residual_add(residual, attn)
+                hidden, residual = self._ffn(i, layer, hidden, residual)
+                continue
             if t == 1 and dh in (64, 128) and self.fused_decode:
                 # one-token step: RoPE + cache store, then single-query attention, one kernel each
                 ptr = lambda x: ctypes.c_void_p(x.data_ptr())
@@ -509,6 +551,13 @@ class ExternalLlamaModel:
         b, t = token_ids.shape
         if b != state.batch or t > state.horizon:
             raise ValueError("prompt does not fit the generation state")
+        if isinstance(state, PagedGenerationState):
+            step = state.cache.batch(state.slots, [t] * b, max_keys=max(t, 1))
+            state.cache.free(state.slots)                                     # (the prompt starts at position 0)
+            state.cache.extend(step)
+            hidden = self._forward(token_ids, state, None, None, step).reshape(b, t, -1)
+            state.length = t
+            return quantized_linear(hidden[:, -1].contiguous(), self.lm_head, out_dtype=torch.float32)
         positions = mask = None
         if self._prefill_kernel_fits(b, t, state):
             native = self._native(token_ids, state)
@@ -535,6 +584,8 @@ class ExternalLlamaModel:
         torch = _torch()
         if state.length >= state.horizon:
             raise ValueError("generation state is full")
+        if isinstance(state, PagedGenerationState):
+            return self._decode_paged(token_ids, state)
         if (self.fused_norm_linear and os.environ.get("B200Q_SILU_GEMV", "0") != "1"
                 and os.environ.get("B200Q_ROPE_ATTENTION", "1") != "0" and token_ids.numel() == state.batch):
             native = self._native(token_ids, state)
@@ -557,6 +608,19 @@ class ExternalLlamaModel:
         state.position.add_(1)
         state.length += 1
         return quantized_linear(hidden, self.lm_head, out_dtype=torch.float32)
+
+    def _decode_paged(self, token_ids, state):
+        if token_ids.numel() != state.batch:
+            raise ValueError("token_ids do not fit the generation state")
+        token_ids, step = token_ids.reshape(-1, 1), state.step
+        state.cache.extend(step)
+        if (self.fused_decode and self.fused_norm_linear
+                and all(layer["qkv"] is not None and layer["gate_up"] is not None for layer in self.layers)):
+            logits = self._forward_one_token(token_ids, state, None, step)
+        else:
+            logits = quantized_linear(self._forward(token_ids, state, None, None, step), self.lm_head, out_dtype=_torch().float32)
+        state.length += 1
+        return logits
 
     @classmethod
     def synthetic(cls, config, *, fmt="Q8_0", dtype="bfloat16", seed=0, device="cuda"):
