@@ -178,17 +178,15 @@ __device__ __forceinline__ float2 unpack16(uint32_t w) {
 // program computes in. FP32 first: with the error's bound added and taken off, both ends round to the same 16-bit number
 // unless a border lies between them, which about one in 2^11 (BF16) values meets; then the quad goes through 64 bits.
 template <bool BF16>
-static __device__ __noinline__ void rotate_exact(const float (&x0)[4], const float (&x1)[4], const float (&c)[4], const float (&s)[4], uint32_t (&out)[4]) {
-    float lo[4], hi[4];
-    for (int e = 0; e < 4; ++e) {
-        const double a = x0[e], b = x1[e], cc = c[e], ss = s[e];
-        lo[e] = __double2float_rn(__fma_rn(a, cc, -__dmul_rn(b, ss)));
-        hi[e] = __double2float_rn(__fma_rn(a, ss, __dmul_rn(b, cc)));
-    }
-    for (int e = 0; e < 2; ++e) {
-        out[e] = pack16<BF16>(lo[2 * e], lo[2 * e + 1]);
-        out[2 + e] = pack16<BF16>(hi[2 * e], hi[2 * e + 1]);
-    }
+static __device__ __noinline__ uint4 rotate_exact(float4 x0, float4 x1, float4 c, float4 s) {
+    auto lo = [](float a, float b, float cc, float ss) {
+        return __double2float_rn(__fma_rn(static_cast<double>(a), static_cast<double>(cc), -__dmul_rn(static_cast<double>(b), static_cast<double>(ss))));
+    };
+    auto hi = [](float a, float b, float cc, float ss) {
+        return __double2float_rn(__fma_rn(static_cast<double>(a), static_cast<double>(ss), __dmul_rn(static_cast<double>(b), static_cast<double>(cc))));
+    };
+    return make_uint4(pack16<BF16>(lo(x0.x, x1.x, c.x, s.x), lo(x0.y, x1.y, c.y, s.y)), pack16<BF16>(lo(x0.z, x1.z, c.z, s.z), lo(x0.w, x1.w, c.w, s.w)),
+                      pack16<BF16>(hi(x0.x, x1.x, c.x, s.x), hi(x0.y, x1.y, c.y, s.y)), pack16<BF16>(hi(x0.z, x1.z, c.z, s.z), hi(x0.w, x1.w, c.w, s.w)));
 }
 // out: the quad at i as two words, then its partner's.
 template <bool BF16>
@@ -210,11 +208,19 @@ __device__ __forceinline__ void rotate_quad(const float (&x0)[4], const float (&
             out[2 * h + p] = pack16<BF16>(v[0] + w[0], v[1] + w[1]);
             differ |= out[2 * h + p] ^ pack16<BF16>(v[0] - w[0], v[1] - w[1]);
         }
-    if (differ) rotate_exact<BF16>(x0, x1, c, s, out);
+    if (differ) {                                        // (by value: arrays that a call gets by address live in memory)
+        const uint4 r = rotate_exact<BF16>(make_float4(x0[0], x0[1], x0[2], x0[3]), make_float4(x1[0], x1[1], x1[2], x1[3]),
+                                           make_float4(c[0], c[1], c[2], c[3]), make_float4(s[0], s[1], s[2], s[3]));
+        out[0] = r.x;
+        out[1] = r.y;
+        out[2] = r.z;
+        out[3] = r.w;
+    }
 }
 
-// One CTA of 2 DH threads = the keys or the values of one block of 64 tokens of one sequence and head. A thread holds four consecutive tokens x (a quad of dimensions at i and its partner at i + DH / 2, which
-// the rotation needs), as 16-bit pairs. A block that becomes full takes its older tokens from the tail and finds the largest
+// One CTA of 2 DH threads = the keys or the values of one block of 64 tokens of one sequence and head; the CTAs of a row's heads
+// follow one another, so that rows are read whole. A thread holds four consecutive tokens x (a quad of dimensions at i and its
+// partner at i + DH / 2, which the rotation needs), as 16-bit pairs. A block that becomes full takes its older tokens from the tail and finds the largest
 // magnitude (16-bit integers order 16-bit floats, NaN and infinities on top); keys go out as words of four codes, values as words
 // of four tokens of a dimension (a transposition of bytes in registers) that pass through shared memory. One that does not become
 // full goes to the tail. Bound by memory - every new token is read once, as projection output, and written once - and, next to
@@ -228,11 +234,11 @@ __global__ void __launch_bounds__(2 * DH, 1024 / (2 * DH)) kv8_append_kernel(con
     __shared__ uint32_t peaks[WARPS];
     chain_trigger();
     chain_wait();
-    const int at = threadIdx.x, part = blockIdx.y & 1, b = blockIdx.z, head = blockIdx.y >> 1;
+    const int at = threadIdx.x, part = blockIdx.x & 1, b = blockIdx.z, head = blockIdx.x >> 1;
     const int start = a.starts[b], row0 = a.offsets[b], n = a.offsets[b + 1] - row0;
     if (start < 0 || n <= 0) return;
     const int total = start + n, first = start / KV8_BLOCK, last = (total - 1) / KV8_BLOCK;
-    int block = first + blockIdx.x;
+    int block = first + blockIdx.y;
     if (block > last) return;
     const bool opened = start % KV8_BLOCK != 0;          // the first block holds older tokens
     // The tail is read for the first block and written for the last: where these are two blocks, one CTA does both, in that
@@ -630,7 +636,8 @@ extern "C" int b200q_kv8_append(const b200q_kv8_cache *cache, int layer, const v
     a.cos_t = cos_table; a.sin_t = sin_table; a.rope_rows = rope_rows;
     const size_t quad = 4 * dtype_size(in_dtype);
     const bool vec = (reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) % quad == 0 && k_row % 4 == 0 && v_row % 4 == 0;
-    const dim3 grid((max_new + 2 * KV8_BLOCK - 2) / KV8_BLOCK, 2 * cache->kv_heads, batch);
+    const dim3 grid(2 * cache->kv_heads, (max_new + 2 * KV8_BLOCK - 2) / KV8_BLOCK, batch);
+    if (grid.y > 65535) return fail(B200Q_EUNSUPPORTED, "kv8_append: too many new tokens");
     auto kernel = cache->head_dim == 64 ? append_kernel<64>(cache->dtype, in_dtype, vec) : append_kernel<128>(cache->dtype, in_dtype, vec);
     launch_chained(kernel, grid, dim3(2 * cache->head_dim), 0, static_cast<cudaStream_t>(stream), *cache, a);
     return check_launch("kv8_append");
