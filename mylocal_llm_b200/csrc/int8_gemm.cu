@@ -240,7 +240,6 @@ __global__ void __launch_bounds__(I8_THREADS, 1) int8_tile_kernel(const __grid_c
     __shared__ uint32_t tmem_base_slot;
     __shared__ volatile int abort_flag;
     __shared__ float w_scale[NT];
-    chain_trigger();
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int rank = SPLIT > 1 ? static_cast<int>(cluster_cta_rank()) : 0;
@@ -263,6 +262,7 @@ __global__ void __launch_bounds__(I8_THREADS, 1) int8_tile_kernel(const __grid_c
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    chain_trigger();                     // (with the tensor memory in hand: the next kernel may allocate some before it waits)
     const uint32_t tmem_d = tmem_base_slot;
 
     if (warp == 0) {
@@ -418,7 +418,6 @@ __global__ void __launch_bounds__(I8_THREADS, 1) int8_pair_kernel(const __grid_c
     __shared__ uint32_t tmem_base_slot;
     __shared__ volatile int abort_flag;
     __shared__ float w_scale[4][32];
-    chain_trigger();
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, S = a.stages;
     const uint32_t rank = cluster_cta_rank();
@@ -442,6 +441,7 @@ __global__ void __launch_bounds__(I8_THREADS, 1) int8_pair_kernel(const __grid_c
     tc_fence_before();
     cluster_sync_all();
     tc_fence_after();
+    chain_trigger();
     const uint32_t tmem_d = tmem_base_slot;
 
     if (warp == 0) {

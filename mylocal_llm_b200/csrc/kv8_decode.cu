@@ -151,7 +151,7 @@ __global__ void __launch_bounds__(DecodeShape<DH, RT, MODE>::WARPS * 32, DecodeS
         pu += STEP;
         return unit < pfull ? Unit{PAGE, prow[unit], plist, pseq} : Unit{TAIL, 0, plist, pseq};
     };
-    // (a table that lacks the page reads another one, not beyond the pool)
+    // (a table that lacks the page: another one is read, not beyond the pool, and its scale is NaN)
     auto page_of = [&](const Unit &x) { return x.page >= 0 && x.page < c.pages ? x.page : 0; };
     auto tail_of = [&](const Unit &x, int part) {
         return static_cast<const uint16_t *>(c.tail) +
@@ -192,7 +192,10 @@ __global__ void __launch_bounds__(DecodeShape<DH, RT, MODE>::WARPS * 32, DecodeS
     // the unit's scales: lane 0 the keys', lane 1 the values' (of a tail: the largest magnitudes)
     auto scale_of = [&](const Unit &x) -> float {
         if (lane >= 2 || x.kind == NONE) return 0.f;
-        if (x.kind == PAGE) return c.scales[kv8_unit(page_of(x), c.layers, a.layer, lane, c.kv_heads, x.list / p.tiles)];
+        if (x.kind == PAGE) {
+            const float scale = c.scales[kv8_unit(page_of(x), c.layers, a.layer, lane, c.kv_heads, x.list / p.tiles)];
+            return page_of(x) == x.page ? scale : kv8_nan();
+        }
         return c.peak[kv8_unit(a.slots[x.seq], c.layers, a.layer, lane, c.kv_heads, x.list / p.tiles)];
     };
     int kind_at[ST], st = 0;                                 // units in the stages, oldest first

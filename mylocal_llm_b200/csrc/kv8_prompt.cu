@@ -160,7 +160,6 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prompt_kernel(const b200q_k
     __shared__ float factor_s[KP_CTA_ROWS];
     const Kv8Attention &a = p.a;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    chain_trigger();
     chain_wait();
     // blocks of rows are numbered from the last (which sees most keys) to the first
     const int kvh = blockIdx.x % c.kv_heads, part = (blockIdx.x / c.kv_heads) % p.splits, b = blockIdx.x / (c.kv_heads * p.splits);
@@ -211,6 +210,9 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prompt_kernel(const b200q_k
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    // Only now may the next kernel come: one that allocates tensor memory before it waits for this one must not find it free while
+    // a CTA here still needs it.
+    chain_trigger();
     const uint32_t tmem = tmem_base_slot;                    // (all 512 columns: 0)
     const uint32_t S_COL = 0, P_COL = 64, O_COL = 256;       // per tile: S 128 columns, P the second 64 of them, O DH columns
     // the whole warp: false once anybody has given up
@@ -463,9 +465,10 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prompt_kernel(const b200q_k
         auto page_at = [&](int block) { return block < full_pages ? c.table[static_cast<size_t>(slot) * c.blocks + block] : 0; };
         auto scales_at = [&](int block, int page, float &ks, float &vs) {
             if (block < full_pages) {
-                const float *from = layer_scales + static_cast<size_t>(page >= 0 && page < c.pages ? page : 0) * page_scales;
-                ks = from[0];
-                vs = from[c.kv_heads];
+                const bool held = page >= 0 && page < c.pages;
+                const float *from = layer_scales + static_cast<size_t>(held ? page : 0) * page_scales;
+                ks = held ? from[0] : kv8_nan();
+                vs = held ? from[c.kv_heads] : kv8_nan();
             } else if (block * KV8_BLOCK < total) {
                 const size_t u = kv8_unit(slot, c.layers, a.layer, 0, c.kv_heads, kvh);
                 ks = power_of(abs_bits(c.peak[u]));
@@ -683,7 +686,7 @@ __global__ void __launch_bounds__(256) kv8_prompt_join_kernel(const b200q_kv8_ca
 static int prompt_splits(const b200q_kv8_cache *c, int heads, int batch, int max_new, int max_keys) {
     const long long rows = static_cast<long long>(max_new) * (heads / c->kv_heads), units = (max_keys + KP_KEYS - 1) / KP_KEYS;
     const long long ctas = (rows + KP_CTA_ROWS - 1) / KP_CTA_ROWS * c->kv_heads * batch;
-    return static_cast<int>(std::max(1ll, std::min({(2ll * sm_count() + ctas - 1) / ctas, units / 4, 16ll})));
+    return static_cast<int>(std::max(1ll, std::min({(2ll * sm_count() + ctas - 1) / ctas, units / 4, 64ll})));
 }
 
 long long kv8_prompt_workspace(const b200q_kv8_cache *c, int heads, int batch, int rows, int max_new, int max_keys) {

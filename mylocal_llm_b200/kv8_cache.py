@@ -20,7 +20,7 @@ and the ``read_*`` helpers waits for it, and a step whose ``batch`` is kept can 
 ``max_length``, a fork onto a slot that is not empty - changes nothing and sets the device status word (``_lib.device_status``:
 501, 502, 503); the rows of a refused step are NaN. Calls on one cache have to be ordered by their streams.
 
-A key or value that is not finite makes its block (its 64 tokens, of its head and layer) NaN, and with it every row that sees
+A key or value that is not finite (in the cache's type) makes its block (its 64 tokens, of its head and layer) NaN, and with it every row that sees
 the block. Scores, softmax statistics and sums are FP32; queries and softmax weights are rounded to FP16 before the tensor
 cores (relative 2^-12, each row of queries scaled by a power of two), the codes enter the products exactly.
 """

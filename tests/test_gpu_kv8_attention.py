@@ -251,6 +251,39 @@ def test_a_block_that_is_not_finite_leaves_the_rows_before_it_alone(cuda, part, 
     assert torch.equal(out[:count // 2], clean[:count // 2]) and torch.isnan(out[count // 2:]).all()
 
 
+@pytest.mark.parametrize("counts", [[1], [90]])
+@pytest.mark.parametrize("entry", [-1, 10 ** 6])
+def test_a_page_that_the_table_lacks_shows(cuda, counts, entry):
+    """A table entry outside the pool: nothing is read beyond it, and the rows that would see the block are NaN."""
+    torch = cuda
+    cache = random_cache(torch, [200], 1, 2, 64, "bfloat16", 14)
+    q = query(torch, counts[0], 4 * 64, "float32", 14)
+    clean = cache.attention(0, q, step(cache, [200], counts)).clone()
+    cache.table[0, 2] = entry                                         # tokens 128..191
+    out = cache.attention(0, q, step(cache, [200], counts))
+    sees = torch.arange(200 - counts[0], 200, device="cuda") >= 128
+    assert torch.isnan(out[sees]).all() and torch.equal(out[~sees], clean[~sees])
+
+
+def test_a_few_tokens_over_a_very_long_context(cuda):
+    """Few rows and many keys: the keys are divided among many CTAs."""
+    torch = cuda
+    sizes, counts = [60000, 40], [20, 3]
+    cache = random_cache(torch, sizes, 1, 1, 128, "float16", 15)
+    q = query(torch, 23, 4 * 128, "float16", 15)
+    check(torch, cache, 0, q, cache.attention(0, q, step(cache, sizes, counts)), sizes, counts)
+
+
+def test_more_sequences_than_one_launch_takes(cuda):
+    torch = cuda
+    sizes = [1 + (i * 53) % 200 + (4000 if i % 700 == 5 else 0) for i in range(1500)]
+    cache = random_cache(torch, sizes, 1, 1, 64, "bfloat16", 16)
+    q = query(torch, 1500, 2 * 64, "bfloat16", 16)
+    counts = [0 if i % 11 == 3 else 1 for i in range(1500)]
+    q = q[:sum(counts)]
+    check(torch, cache, 0, q, cache.attention(0, q, step(cache, sizes, counts)), sizes, counts)
+
+
 def test_offsets_beyond_32_bits(cuda):
     """A pool of more than 2^32 bytes whose last pages are the ones in use."""
     torch = cuda
