@@ -161,10 +161,37 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prompt_kernel(const b200q_k
     const Kv8Attention &a = p.a;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     chain_wait();
-    // blocks of rows are numbered from the last (which sees most keys) to the first
-    const int kvh = blockIdx.x % c.kv_heads, part = (blockIdx.x / c.kv_heads) % p.splits, b = blockIdx.x / (c.kv_heads * p.splits);
-    const int start = a.starts[b], first = a.offsets[b], n = a.offsets[b + 1] - first, slot = a.slots[b], total = start + n;
-    const int rows = n * p.group, row0 = (gridDim.y - 1 - blockIdx.y) * KP_CTA_ROWS;
+    // CTAs start in the order of their numbers, so the last to start should be short. Blocks of rows go from the last (which sees
+    // most keys) to the first: over all sequences where these are alike, else (up to 32) one sequence after the other, the longest
+    // first (chunks of 512 behind 16000 and 3800 tokens: 381 us in the first order, 336 us in the second; four prompts of 2048
+    // tokens: 198 and 208 us).
+    const int blocks = gridDim.z;
+    int kvh = blockIdx.x, part = 0, b = blockIdx.y, row_block = blockIdx.z;
+    if (p.splits > 1) {
+        part = blockIdx.x / c.kv_heads;
+        kvh = blockIdx.x - part * c.kv_heads;
+    }
+    int start = a.starts[b], first = a.offsets[b], next = a.offsets[b + 1], slot = a.slots[b];
+    if (a.batch > 1 && a.batch <= 32) {
+        const int size = lane < a.batch ? a.starts[lane] + a.offsets[lane + 1] - a.offsets[lane] : 0;
+        const int first_size = __shfl_sync(0xffffffffu, size, 0);
+        if (__any_sync(0xffffffffu, lane < a.batch && size != first_size)) {
+            const int number = b + a.batch * row_block;
+            int rank = 0;
+            for (int q = 0; q < a.batch; ++q) {
+                const int other = __shfl_sync(0xffffffffu, size, q);
+                rank += other > size || (other == size && q < lane);
+            }
+            row_block = number % blocks;
+            b = __ffs(__ballot_sync(0xffffffffu, lane < a.batch && rank == number / blocks)) - 1;
+            start = a.starts[b];
+            first = a.offsets[b];
+            next = a.offsets[b + 1];
+            slot = a.slots[b];
+        }
+    }
+    const int n = next - first, total = start + n;
+    const int rows = n * p.group, row0 = (blocks - 1 - row_block) * KP_CTA_ROWS;
     if (n <= 0 || row0 >= rows) return;
     if (start < 0) {                             // a refused step
         if (part == 0)
@@ -708,9 +735,9 @@ int kv8_prompt(const b200q_kv8_cache *c, const Kv8Attention &a, int max_new, int
     p.status = device_status_word();
     if (!p.status) return fail(B200Q_ECUDA, "kv8_attention: no CUDA device");
     const long long blocks = (static_cast<long long>(max_new) * p.group + KP_CTA_ROWS - 1) / KP_CTA_ROWS;
-    const long long across = static_cast<long long>(c->kv_heads) * p.splits * a.batch;
+    const long long across = static_cast<long long>(c->kv_heads) * p.splits;
     const long long joins = (static_cast<long long>(a.rows) * a.heads + 7) / 8;
-    if (blocks > 65535 || across > 0x7fffffffll || joins > 0x7fffffffll || static_cast<long long>(max_new) * p.group > 0x40000000ll)
+    if (a.batch > 65535 || blocks > 65535 || across > 0x7fffffffll || joins > 0x7fffffffll || static_cast<long long>(max_new) * p.group > 0x40000000ll)
         return fail(B200Q_EUNSUPPORTED, "kv8_attention: too many rows");
     const bool bf16 = c->dtype == B200Q_BF16;
     auto kernel = c->head_dim == 64 ? (bf16 ? kv8_prompt_kernel<64, true, false> : kv8_prompt_kernel<64, false, true>)
@@ -718,7 +745,7 @@ int kv8_prompt(const b200q_kv8_cache *c, const Kv8Attention &a, int max_new, int
     const int smem = 1024 + (c->head_dim == 64 ? (bf16 ? PromptShape<64, false>::BYTES : PromptShape<64, true>::BYTES)
                                                : (bf16 ? PromptShape<128, false>::BYTES : PromptShape<128, true>::BYTES));
     if (int rc = allow_large_shared_memory(reinterpret_cast<const void *>(kernel))) return rc;
-    launch_chained(kernel, dim3(static_cast<unsigned>(across), static_cast<unsigned>(blocks)), dim3(KP_THREADS), smem, stream, *c, p);
+    launch_chained(kernel, dim3(static_cast<unsigned>(across), a.batch, static_cast<unsigned>(blocks)), dim3(KP_THREADS), smem, stream, *c, p);
     if (int rc = check_launch("kv8_attention")) return rc;
     if (p.splits == 1) return B200Q_OK;
     launch_chained(c->head_dim == 64 ? kv8_prompt_join_kernel<64> : kv8_prompt_join_kernel<128>, dim3(static_cast<unsigned>(joins)), dim3(256), 0,
