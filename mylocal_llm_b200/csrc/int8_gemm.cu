@@ -1,5 +1,6 @@
 // Matrix product in 8-bit integers with one scale per token and per output channel, and the quantiser of its operands.
 #include <algorithm>
+#include <type_traits>
 
 #include "kv8_cache.cuh"
 #include "umma.cuh"
@@ -79,46 +80,113 @@ __device__ __forceinline__ uint32_t peak_bits(uint32_t peak) {
     return abs_bits(__half2float(__ushort_as_half(static_cast<unsigned short>(peak))));
 }
 
-// A CTA takes a row at a time: the largest magnitude, then the codes. The row's pieces of eight values stay in registers, as they
-// were loaded, between the two up to 256 * 8 * KEEP columns (longer rows are read again), and the next row's are on their way
-// meanwhile. Bound by memory (4096 x 8192 BF16: one row per CTA and held as floats 34 us; 15 us at the measured bandwidth).
+// Eight values on their way: VEC rows as they are, other rows (whose beginning is no multiple of 16 bytes) as the aligned 16-byte
+// words around them, `off` bytes in front of the first. The words may hold bytes of the rows before and behind, which do not
+// count; where they would begin before the first row or end behind the last one, the values are fetched one by one (`get`).
+template <int IN, bool VEC> struct Piece {
+    Raw8<IN> r;
+    __device__ __forceinline__ void load(const void *x, size_t base, int c, int k, const char *, const char *, bool wanted) {
+        r = Raw8<IN>{};
+        if (wanted) r = load8<IN, VEC>(x, base, c, k);
+    }
+    __device__ __forceinline__ Raw8<IN> get(const void *, size_t, int, int) const { return r; }
+};
+template <int IN> struct Piece<IN, false> {
+    static constexpr int E = IN == B200Q_F32 ? 4 : 2, WORDS = 2 * E + 4;
+    uint32_t w[WORDS];
+    int off;                                             // -1: nothing was requested
+    __device__ __forceinline__ void load(const void *x, size_t base, int c, int, const char *first, const char *end, bool wanted) {
+        const char *q = static_cast<const char *>(x) + (base + c) * E;
+        off = static_cast<int>(reinterpret_cast<uintptr_t>(q) & 15);
+        const char *from = q - off;
+        if (!wanted || from < first || from + 4 * WORDS > end) {
+            off = -1;
+            return;
+        }
+#pragma unroll
+        for (int i = 0; i < WORDS / 4; ++i) {
+            const uint4 v = reinterpret_cast<const uint4 *>(from)[i];
+            w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
+        }
+    }
+    __device__ __forceinline__ Raw8<IN> get(const void *x, size_t base, int c, int k) const {
+        if (off < 0) return load8<IN, false>(x, base, c, k);
+        uint32_t a[WORDS - 2], b[WORDS - 3], v[2 * E];
+#pragma unroll
+        for (int i = 0; i < WORDS - 2; ++i) a[i] = off & 8 ? w[i + 2] : w[i];
+#pragma unroll
+        for (int i = 0; i < WORDS - 3; ++i) b[i] = off & 4 ? a[i + 1] : a[i];
+#pragma unroll
+        for (int i = 0; i < 2 * E; ++i) v[i] = E == 4 ? b[i] : __funnelshift_r(b[i], b[i + 1 < WORDS - 3 ? i + 1 : i], 8 * (off & 2));
+        if (c + 8 > k)
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (c + e >= k) v[e * E / 4] &= E == 4 || e % 2 == 0 ? 0u : 0xffffu;
+        Raw8<IN> r;
+        if constexpr (IN == B200Q_F32) {
+            r.w[0] = make_float4(__uint_as_float(v[0]), __uint_as_float(v[1]), __uint_as_float(v[2]), __uint_as_float(v[3]));
+            r.w[1] = make_float4(__uint_as_float(v[4]), __uint_as_float(v[5]), __uint_as_float(v[6]), __uint_as_float(v[7]));
+        } else {
+            r.w = make_uint4(v[0], v[1], v[2], v[3]);
+        }
+        return r;
+    }
+};
+
+// A team of `team` warps takes a row at a time: the largest magnitude, then the codes. The row's pieces of eight values stay in
+// registers, as they were loaded, between the two up to 256 * team * KEEP columns (longer rows are read again), and the next row's
+// are on their way meanwhile. Teams are as small as the row allows: warps that need not meet (6992 x 706 FP32 by whole CTAs 37 us,
+// by single warps 10). Bound by memory (4096 x 8192 BF16: held as floats 34 us, as loaded 27; 15 at the measured bandwidth).
+constexpr int I8_QUANTIZE_KEEP = 4;                  // pieces of 16-bit values (of FP32: half as many)
 template <int IN, bool VEC>
-__global__ void __launch_bounds__(256, 4) int8_quantize_kernel(const void *x, int rows, int k, long long x_row, int8_t *codes,
-                                                               long long codes_row, float *scales, int early) {
-    constexpr int KEEP = IN == B200Q_F32 ? 2 : 4;
+__global__ void __launch_bounds__(256, VEC ? 4 : 2) int8_quantize_kernel(const void *x, int rows, int k, long long x_row, int8_t *codes,
+                                                                         long long codes_row, float *scales, int team, int early) {
+    constexpr int KEEP = IN == B200Q_F32 ? I8_QUANTIZE_KEEP / 2 : I8_QUANTIZE_KEEP;
     __shared__ uint32_t peaks[8];
     if (early) chain_trigger();
     chain_wait();
-    const int tid = threadIdx.x, padded = (k + 15) & ~15;
-    Raw8<IN> next[KEEP];
+    const int warp = threadIdx.x >> 5, mine = warp & (team - 1), first_warp = warp - mine;
+    const int c0 = (32 * mine + (threadIdx.x & 31)) * 8, width = 256 * team, padded = (k + 15) & ~15;
+    const int row0 = (blockIdx.x * 8 + warp) / team, step = gridDim.x * 8 / team;
+    auto meet = [&] {                                    // (barrier 0 is the CTA's)
+        if (team > 1) asm volatile("bar.sync %0, %1;" ::"r"(1 + first_warp / team), "r"(32 * team) : "memory");
+    };
+    const char *first = static_cast<const char *>(x);
+    const char *end = first + ((rows - 1) * static_cast<size_t>(x_row) + k) * (IN == B200Q_F32 ? 4 : 2);
+    Piece<IN, VEC> next[KEEP];
     auto load_row = [&](int row) {
 #pragma unroll
         for (int j = 0; j < KEEP; ++j) {
-            const int c = (tid + 256 * j) * 8;
-            next[j] = Raw8<IN>{};
-            if (row < rows && c < k) next[j] = load8<IN, VEC>(x, row * static_cast<size_t>(x_row), c, k);
+            const int c = c0 + width * j;
+            next[j].load(x, row * static_cast<size_t>(x_row), c, k, first, end, row < rows && c < k);
         }
     };
-    load_row(blockIdx.x);
-    for (int row = blockIdx.x; row < rows; row += gridDim.x) {
+    load_row(row0);
+    for (int row = row0; row < rows; row += step) {
         const size_t base = row * static_cast<size_t>(x_row);
         Raw8<IN> kept[KEEP];
         uint32_t peak = 0u;
 #pragma unroll
         for (int j = 0; j < KEEP; ++j) {
-            kept[j] = next[j];
+            kept[j] = next[j].get(x, base, c0 + width * j, k);
             peak = max(peak, peak8<IN>(kept[j]));
         }
-        load_row(row + gridDim.x);
-        for (int c = (tid + 256 * KEEP) * 8; c < k; c += 256 * 8) peak = max(peak, peak8<IN>(load8<IN, VEC>(x, base, c, k)));
+        load_row(row + step);
+        auto again = [&](int c) {
+            Piece<IN, VEC> piece;
+            piece.load(x, base, c, k, first, end, true);
+            return piece.get(x, base, c, k);
+        };
+        for (int c = c0 + width * KEEP; c < k; c += width) peak = max(peak, peak8<IN>(again(c)));
         peak = __reduce_max_sync(0xffffffffu, peak);
-        __syncthreads();                                 // (the previous row's peaks have been read)
-        if ((tid & 31) == 0) peaks[tid >> 5] = peak;
-        __syncthreads();
-#pragma unroll
-        for (int w = 0; w < 8; ++w) peak = max(peak, peaks[w]);
+        if (team > 1) {
+            meet();                                      // (the previous row's peaks have been read)
+            if ((threadIdx.x & 31) == 0) peaks[warp] = peak;
+            meet();
+            for (int w = 0; w < team; ++w) peak = max(peak, peaks[first_warp + w]);
+        }
         const float s = int8_scale(peak_bits<IN>(peak)), inv = __fdiv_rn(1.f, s);
-        if (tid == 0) scales[row] = s;
+        if (c0 == 0) scales[row] = s;
         auto put = [&](int c, const Raw8<IN> &r) {
             float f[8];
             r.values(f);
@@ -127,20 +195,17 @@ __global__ void __launch_bounds__(256, 4) int8_quantize_kernel(const void *x, in
         };
 #pragma unroll
         for (int j = 0; j < KEEP; ++j) {
-            const int c = (tid + 256 * j) * 8;
+            const int c = c0 + width * j;
             if (c < padded) put(c, kept[j]);
         }
-        for (int c = (tid + 256 * KEEP) * 8; c < padded; c += 256 * 8) {
-            if (c < k) put(c, load8<IN, VEC>(x, base, c, k));
-            else put(c, Raw8<IN>{});
-        }
+        for (int c = c0 + width * KEEP; c < padded; c += width) put(c, c < k ? again(c) : Raw8<IN>{});
     }
 }
 
 // ---------------------------------------------------------------------------------------------
 // The product. Tokens are the M dimension of tcgen05.mma (kind::i8, signed by signed into 32-bit integers), output channels the
 // N dimension; both operands are K-major slabs of 128 codes a row, brought by TMA with the 128-byte swizzle (rows and codes past
-// the end arrive as zeros). One warp issues the loads, one the MMAs, four read the sums back from tensor memory, scale and
+// the end arrive as zeros). One warp issues the loads, one the MMAs, four or eight read the sums back from tensor memory, scale and
 // store them. There are two kernels:
 //   int8_tile_kernel  one tile of 128 tokens x NT channels per CTA. Few tiles (few tokens, few channels): the K range is
 //                     divided among the 2, 4 or 8 CTAs of a cluster, whose integer sums meet in shared memory - exact, so the
@@ -157,6 +222,7 @@ __global__ void __launch_bounds__(256, 4) int8_quantize_kernel(const void *x, in
 constexpr int I8_BM = 128, I8_BK = 128;              // tokens per CTA; codes per slab (one 128-byte swizzle row)
 constexpr int I8_A_BYTES = I8_BM * I8_BK;
 constexpr int I8_THREADS = 6 * 32;                   // TMA, MMA, four epilogue warps
+constexpr int I8_PAIR_THREADS = 10 * 32;             // TMA, MMA, eight epilogue warps
 constexpr int I8_MAX_STAGES = 8;
 constexpr int STATUS_INT8_WAIT_TMA = 121, STATUS_INT8_WAIT_MMA = 122, STATUS_INT8_WAIT_EPILOGUE = 123;
 
@@ -193,35 +259,36 @@ __device__ __forceinline__ void umma_i8(uint32_t d_tmem, uint64_t a_desc, uint64
             : "memory");
 }
 
-// Thirty-two scaled outputs of one token, channels col .. col + 31 of n.
-__device__ __forceinline__ void store_outputs(void *y, int y_dtype, size_t row_base, int col, int n, const float (&v)[32]) {
-    const size_t at = row_base + col;
-    const int esize = y_dtype == B200Q_F32 ? 4 : 2;
-    uint8_t *p = static_cast<uint8_t *>(y) + at * esize;
-    if (col + 32 <= n && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
-        if (y_dtype == B200Q_F32) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) reinterpret_cast<float4 *>(p)[e] = make_float4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
-        } else {
-            uint32_t w[16];
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                if (y_dtype == B200Q_BF16) {
-                    const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * e], v[2 * e + 1]);
-                    w[e] = *reinterpret_cast<const uint32_t *>(&h);
-                } else {
-                    const __half2 h = __floats2half2_rn(v[2 * e], v[2 * e + 1]);
-                    w[e] = *reinterpret_cast<const uint32_t *>(&h);
-                }
-            }
-#pragma unroll
-            for (int e = 0; e < 4; ++e) reinterpret_cast<uint4 *>(p)[e] = make_uint4(w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3]);
-        }
+// A warp's 32 tokens x 32 channels: each lane's sums of one token, times that token's scale, pass through 4 KB of shared memory so
+// that a lane has one channel of all tokens, whose scale is `w`, and the warp stores a token's 32 outputs together, whatever n and
+// the alignment of rows (lanes that stored their own token's 64 bytes, one by one where rows are not 16-byte aligned, took
+// 113 us for 1262 x 8231 x 2000, these 29 us). `at`: element of the first token, this lane's channel; `rows`: tokens that exist.
+template <typename T>
+__device__ __forceinline__ void store_channel(T *y, size_t n, int rows, const float *stage, int lane, float w) {
+    auto put = [&](int r) {
+        const float v = stage[r * 32 + (lane ^ r)] * w;
+        if constexpr (sizeof(T) == 4) *y = v;
+        else if constexpr (std::is_same_v<T, __half>) *y = __float2half_rn(v);
+        else *y = __float2bfloat16_rn(v);
+        y += n;
+    };
+    if (rows == 32) {
+#pragma unroll 8
+        for (int r = 0; r < 32; ++r) put(r);
     } else {
-#pragma unroll
-        for (int e = 0; e < 32; ++e)
-            if (col + e < n) store_from_float(y, y_dtype, at + e, v[e]);
+        for (int r = 0; r < rows; ++r) put(r);
     }
+}
+__device__ __forceinline__ void store_outputs(void *y, int y_dtype, size_t at, int n, bool exists, int rows, const uint32_t (&sums)[32], float xs,
+                                              float w, float *stage, int lane) {
+    __syncwarp();                                        // (the previous outputs have been read)
+#pragma unroll
+    for (int e = 0; e < 32; ++e) stage[lane * 32 + (e ^ lane)] = static_cast<float>(static_cast<int>(sums[e])) * xs;
+    __syncwarp();
+    if (!exists) return;
+    if (y_dtype == B200Q_F32) store_channel(static_cast<float *>(y) + at, n, rows, stage, lane, w);
+    else if (y_dtype == B200Q_F16) store_channel(static_cast<__half *>(y) + at, n, rows, stage, lane, w);
+    else store_channel(static_cast<__nv_bfloat16 *>(y) + at, n, rows, stage, lane, w);
 }
 
 __device__ __forceinline__ uint32_t ld_cluster_u32(uint32_t addr) {
@@ -347,15 +414,15 @@ __global__ void __launch_bounds__(I8_THREADS, 1) int8_tile_kernel(const __grid_c
             tc_fence_after();
             chain_wait();                // y may still be read by what precedes this kernel; the scales are its result
             const float xs = row < rows ? a.x_scales[m0 + row] : 0.f;
+            float *stage = reinterpret_cast<float *>(smem) + warp % 4 * 1024;        // (the operands have been read)
 #pragma unroll 1
             for (int c = 0; c < NT / 32; ++c) {
+                const int col = n0 + 32 * c + lane;
                 uint32_t r[32];
                 tmem_ld32(tmem_d + (static_cast<uint32_t>(32 * quarter) << 16) + 32 * c, r);
                 tmem_ld_wait();
-                float v[32];
-#pragma unroll
-                for (int e = 0; e < 32; ++e) v[e] = static_cast<float>(static_cast<int>(r[e])) * xs * w_scale[32 * c + e];
-                if (row < rows) store_outputs(a.y, a.y_dtype, static_cast<size_t>(m0 + row) * a.n, n0 + 32 * c, a.n, v);
+                store_outputs(a.y, a.y_dtype, static_cast<size_t>(m0 + 32 * quarter) * a.n + col, a.n, col < a.n, min(32, rows - 32 * quarter),
+                              r, xs, w_scale[32 * c + lane], stage, lane);
             }
         }
         tc_fence_before();
@@ -411,13 +478,12 @@ __device__ __forceinline__ void pair_tile(const Int8Gemm &a, int tile, int &m0, 
     n0 = tn * 256;
 }
 
-__global__ void __launch_bounds__(I8_THREADS, 1) int8_pair_kernel(const __grid_constant__ CUtensorMap xmap,
+__global__ void __launch_bounds__(I8_PAIR_THREADS, 1) int8_pair_kernel(const __grid_constant__ CUtensorMap xmap,
                                                                   const __grid_constant__ CUtensorMap wmap, const Int8Gemm a) {
     extern __shared__ uint8_t smem_raw[];
     __shared__ __align__(8) uint64_t full_bar[I8_MAX_STAGES], free_bar[I8_MAX_STAGES], acc_full[2], acc_free[2];
     __shared__ uint32_t tmem_base_slot;
     __shared__ volatile int abort_flag;
-    __shared__ float w_scale[4][32];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, S = a.stages;
     const uint32_t rank = cluster_cta_rank();
@@ -429,7 +495,7 @@ __global__ void __launch_bounds__(I8_THREADS, 1) int8_pair_kernel(const __grid_c
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&acc_full[i], 1);
-            mbar_init(&acc_free[i], 8);              // four epilogue warps of both CTAs
+            mbar_init(&acc_free[i], 16);             // eight epilogue warps of both CTAs
         }
         abort_flag = 0;
         fence_barrier_init();
@@ -523,15 +589,20 @@ __global__ void __launch_bounds__(I8_THREADS, 1) int8_pair_kernel(const __grid_c
             __syncwarp();
         }
     } else if (warp >= 2) {
-        const int quarter = warp & 3;
+        // two warps per quarter of the rows, 128 channels each
+        const int quarter = warp & 3, half = (warp - 2) >> 2;
+        float *stage = reinterpret_cast<float *>(smem + S * I8_PAIR_STAGE) + (warp - 2) * 1024;
         const uint32_t acc_free0 = cluster_map(smem_u32(&acc_free[0]), 0);
         chain_wait();
         int turn = 0;
         for (int tile = pair; tile < tiles; tile += pairs, ++turn) {
             int m0, n0;
             pair_tile(a, tile, m0, n0);
-            const int acc = turn & 1, row = m0 + 128 * static_cast<int>(rank) + 32 * quarter + lane;
-            const float xs = row < a.m ? a.x_scales[row] : 0.f;
+            const int acc = turn & 1, row0 = m0 + 128 * static_cast<int>(rank) + 32 * quarter, col0 = n0 + 128 * half + lane;
+            const float xs = row0 + lane < a.m ? a.x_scales[row0 + lane] : 0.f;
+            float w[4];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) w[c] = col0 + 32 * c < a.n ? a.w_scales[col0 + 32 * c] : 0.f;
             bool fine = !__any_sync(0xffffffffu, abort_flag != 0);
             if (fine) fine = __all_sync(0xffffffffu, mbar_wait_bounded(&acc_full[acc], (turn >> 1) & 1, a.status, STATUS_INT8_WAIT_MMA));
             if (!fine) {
@@ -539,24 +610,19 @@ __global__ void __launch_bounds__(I8_THREADS, 1) int8_pair_kernel(const __grid_c
                 break;
             }
             tc_fence_after();
-#pragma unroll 1
-            for (int c = 0; c < 8; ++c) {
-                const int col = n0 + 32 * c;
-                __syncwarp();
-                w_scale[quarter][lane] = col + lane < a.n ? a.w_scales[col + lane] : 0.f;
-                __syncwarp();
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const int col = col0 + 32 * c;
                 uint32_t r[32];
-                tmem_ld32(tmem_d + (static_cast<uint32_t>(32 * quarter) << 16) + 256 * acc + 32 * c, r);
+                tmem_ld32(tmem_d + (static_cast<uint32_t>(32 * quarter) << 16) + 256 * acc + 128 * half + 32 * c, r);
                 tmem_ld_wait();
-                if (c == 7) {                        // the accumulator is read: the next tile but one may have it
+                if (c == 3) {                        // the accumulator is read: the next tile but one may have it
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive_cluster(acc_free0 + 8u * acc);
                 }
-                float v[32];
-#pragma unroll
-                for (int e = 0; e < 32; ++e) v[e] = static_cast<float>(static_cast<int>(r[e])) * xs * w_scale[quarter][e];
-                if (row < a.m && col < a.n) store_outputs(a.y, a.y_dtype, static_cast<size_t>(row) * a.n, col, a.n, v);
+                if (row0 < a.m)
+                    store_outputs(a.y, a.y_dtype, static_cast<size_t>(row0) * a.n + col, a.n, col < a.n, min(32, a.m - row0), r, xs, w[c], stage, lane);
             }
         }
     }
@@ -599,9 +665,9 @@ static int int8_gemm(const int8_t *w, long long w_row, const int8_t *x, long lon
         if (int rc = int8_map(&xmap, encode, x, columns, x_row, a.m, 128)) return rc;
         if (int rc = int8_map(&wmap, encode, w, columns, w_row, a.n, 128)) return rc;
         a.stages = 6;
-        const int smem = a.stages * I8_PAIR_STAGE + 1024, pairs = static_cast<int>(std::min<long long>(big, sms / 2));
+        const int smem = a.stages * I8_PAIR_STAGE + 8 * 4096 + 1024, pairs = static_cast<int>(std::min<long long>(big, sms / 2));
         if (int rc = allow_large_shared_memory(reinterpret_cast<const void *>(int8_pair_kernel))) return rc;
-        launch_chained_cluster(int8_pair_kernel, dim3(2 * pairs), dim3(I8_THREADS), smem, stream, 2, xmap, wmap, a);
+        launch_chained_cluster(int8_pair_kernel, dim3(2 * pairs), dim3(I8_PAIR_THREADS), smem, stream, 2, xmap, wmap, a);
         return check_launch("int8_gemm");
     }
     const int token_tiles = (a.m + I8_BM - 1) / I8_BM;
@@ -643,8 +709,11 @@ extern "C" int b200q_int8_quantize(const void *x, int x_dtype, int rows, int k, 
     auto kernel = x_dtype == B200Q_F32   ? (vec ? int8_quantize_kernel<B200Q_F32, true> : int8_quantize_kernel<B200Q_F32, false>)
                   : x_dtype == B200Q_F16 ? (vec ? int8_quantize_kernel<B200Q_F16, true> : int8_quantize_kernel<B200Q_F16, false>)
                                          : (vec ? int8_quantize_kernel<B200Q_BF16, true> : int8_quantize_kernel<B200Q_BF16, false>);
-    launch_chained(kernel, dim3(std::min(rows, 4 * sm_count())), dim3(256), 0, static_cast<cudaStream_t>(stream), x, rows, k, static_cast<long long>(x_row), codes,
-                   static_cast<long long>(codes_row), scales, early);
+    int team = 1;
+    while (team < 8 && 256 * team * (x_dtype == B200Q_F32 ? I8_QUANTIZE_KEEP / 2 : I8_QUANTIZE_KEEP) < k) team *= 2;
+    const int teams = 8 / team, ctas = std::min((rows + teams - 1) / teams, (vec ? 4 : 2) * sm_count());
+    launch_chained(kernel, dim3(ctas), dim3(256), 0, static_cast<cudaStream_t>(stream), x, rows, k, static_cast<long long>(x_row), codes,
+                   static_cast<long long>(codes_row), scales, team, early);
     return check_launch("int8_quantize");
 }
 
