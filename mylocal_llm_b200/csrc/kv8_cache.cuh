@@ -34,36 +34,73 @@ __device__ __forceinline__ float int8_scale(uint32_t peak) {
     return fmaxf(__fdiv_rn(__uint_as_float(peak), 127.0f), KV8_MIN_SCALE);
 }
 
-// The integer nearest to x / s, ties to even, of the exact quotient: the product with the reciprocal is off by less than
-// 2^-15 (|x / s| < 128), so only the neighbours can be nearer, and the sign of x - (q +- 1/2) s as one FMA tells (an FMA
-// rounds once, so its sign is that of the exact difference). Scales near the smallest normal number, where that difference
-// can underflow, divide in 64 bits instead.
-static __device__ __noinline__ int int8_code_exact(float x, float s, float inv) {
-    if (s < 7.8886e-31f) return __double2int_rn(static_cast<double>(x) / static_cast<double>(s));
-    const float q = rintf(__fmul_rn(x, inv));
-    const float up = __fmaf_rn(-(q + 0.5f), s, x), down = __fmaf_rn(-(q - 0.5f), s, x);
-    int code = __float2int_rn(q);                        // (NaN: 0, and the scale is NaN)
-    if (up > 0.f || (up == 0.f && (code & 1))) ++code;
-    else if (down < 0.f || (down == 0.f && (code & 1))) --code;
-    return code;
+// Two FP32 values in one 64-bit register, and the instructions that work on both at once.
+struct Pair {
+    uint64_t v;
+    __device__ __forceinline__ float lo() const { return __uint_as_float(static_cast<uint32_t>(v)); }
+    __device__ __forceinline__ float hi() const { return __uint_as_float(static_cast<uint32_t>(v >> 32)); }
+};
+__device__ __forceinline__ Pair pair(float lo, float hi) {
+    Pair p;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(p.v) : "f"(lo), "f"(hi));
+    return p;
+}
+__device__ __forceinline__ Pair pair_fma(Pair a, Pair b, Pair c) {
+    Pair d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+    return d;
+}
+__device__ __forceinline__ Pair pair_mul(Pair a, Pair b) {
+    Pair d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
+    return d;
+}
+__device__ __forceinline__ Pair pair_add(Pair a, Pair b) {
+    Pair d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
+    return d;
 }
 
-// The codes of four values as bytes of a word. x * inv + 1.5 * 2^23 has the nearest integer of x * inv in its low bits, and that
-// is the code unless x * inv lies within 2^-16 of a border (x / s does not differ from it by more than 2^-17 there): then, in
-// one of 2^13 groups or so, each of the four is looked at exactly.
+// The integer nearest to x / s, ties to even, of the exact quotient, for scales near the smallest normal number.
+static __device__ __noinline__ uint32_t int8_code_tiny(float x, float s) {
+    return static_cast<uint32_t>(__double2int_rn(static_cast<double>(x) / static_cast<double>(s)));
+}
+
+// The codes of four values as bytes of a word: the integers nearest to x / s, ties to even, of the exact quotients.
+// x * inv + 1.5 * 2^23 has the nearest integer of x * inv in its low bits, and that is the code unless x * inv lies within 2^-16 of
+// a border (x / s does not differ from it by more than 2^-17 there). Then only the neighbours can be nearer, and the sign of
+// x - (q +- 1/2) s as one FMA tells (an FMA rounds once, so its sign is that of the exact difference, which does not underflow
+// from 7.9e-31 on). Values of few bits and scales of few bits meet borders often: one group of 128 BF16 values in seven.
 __device__ __forceinline__ uint32_t int8_codes(const float (&x)[4], float s, float inv) {
-    constexpr float MAGIC = 12582912.f;
+    constexpr float MAGIC = 12582912.f, TINY = 7.8886e-31f;
     uint32_t t[4];
-    float far = s < 7.8886e-31f ? 1.f : 0.f;
+    Pair q[2];
+    float far = s < TINY ? 1.f : 0.f;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        const float y = __fmaf_rn(x[e], inv, MAGIC);
-        far = fmaxf(far, fabsf(__fmaf_rn(x[e], inv, -__fadd_rn(y, -MAGIC))));
-        t[e] = __float_as_uint(y);
+    for (int e = 0; e < 2; ++e) {
+        const Pair v = pair(x[2 * e], x[2 * e + 1]), k = pair(inv, inv);
+        const Pair y = pair_fma(v, k, pair(MAGIC, MAGIC));
+        q[e] = pair_add(y, pair(-MAGIC, -MAGIC));
+        const Pair negative{q[e].v ^ 0x8000000080000000ull};
+        const Pair r = pair_fma(v, k, negative);
+        far = fmaxf(far, fmaxf(fabsf(r.lo()), fabsf(r.hi())));
+        t[2 * e] = static_cast<uint32_t>(y.v);
+        t[2 * e + 1] = static_cast<uint32_t>(y.v >> 32);
     }
     if (far > 0.49998f) {
+        if (s < TINY) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) t[e] = static_cast<uint32_t>(int8_code_exact(x[e], s, inv));
+            for (int e = 0; e < 4; ++e) t[e] = int8_code_tiny(x[e], s);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float whole = e & 1 ? q[e >> 1].hi() : q[e >> 1].lo();
+                const float up = __fmaf_rn(-(whole + 0.5f), s, x[e]), down = __fmaf_rn(-(whole - 0.5f), s, x[e]);
+                const bool odd = t[e] & 1u;
+                if (up > 0.f || (up == 0.f && odd)) ++t[e];
+                else if (down < 0.f || (down == 0.f && odd)) --t[e];
+            }
+        }
     }
     return __byte_perm(__byte_perm(t[0], t[1], 0x0040), __byte_perm(t[2], t[3], 0x0040), 0x5410);
 }
