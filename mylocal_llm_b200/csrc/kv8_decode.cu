@@ -29,7 +29,7 @@ template <int DH, int RT, int MODE> struct DecodeShape {
 struct Kv8Decode {
     Kv8Attention a;
     int group, tiles;             // query heads per key/value head; lists of 8 RT rows (tokens x heads of the group) per head
-    float *partial;               // [CTA][2][8 RT][DH + 2]
+    float *partial;               // [CTA][2][8 RT][DH + 4]: values, maximum, sum
     int4 *cuts;                   // [CTA], for the joining kernel: slot of the sequence that begins in the part and goes on behind
                                   // it (-1: none), its list, its number; list * batch + number of the one that goes on from
                                   // the part before (-1: none)
@@ -440,7 +440,7 @@ __global__ void __launch_bounds__(DecodeShape<DH, RT, MODE>::WARPS * 32, DecodeS
                     store_from_float(a.out, c.dtype, (static_cast<size_t>(row_of + token) * a.heads + head * p.group + rr - token * p.group) * DH + d,
                                      value / weight);
                 } else {
-                    float *to = p.partial + ((static_cast<size_t>(blockIdx.x) * 2 + (at == 0 ? 0 : 1)) * 8 * RT + 4 * r4 + row) * (DH + 2);
+                    float *to = p.partial + ((static_cast<size_t>(blockIdx.x) * 2 + (at == 0 ? 0 : 1)) * 8 * RT + 4 * r4 + row) * (DH + 4);
                     to[d] = value;
                     if (d == 0) {
                         to[DH] = top;
@@ -474,53 +474,99 @@ __global__ void __launch_bounds__(DecodeShape<DH, RT, MODE>::WARPS * 32, DecodeS
     }
 }
 
-// Joins the partial results of the sequences that were cut: CTA i joins the one that begins in part i and goes on behind it.
+// Joins the partial results of a sequence that was cut, one row of it per CTA (grid: sequences x rows). Which sequence: that of
+// number blockIdx.x, or, where there are fewer parts than sequences, the one that begins in part blockIdx.x and goes on behind it.
+// A part's results are a row of DH values away from the next one's, so the parts are read by 8 or 16 groups of threads at once
+// (one thread after the other's 72 parts took 110 us for five sequences of up to 11771 keys).
 template <int DH>
-__global__ void __launch_bounds__(256) kv8_decode_join_kernel(const b200q_kv8_cache c, const Kv8Decode p, int ctas, int tile) {
-    __shared__ uint8_t holds[KV8_MAX_PARTS];                 // parts that hold some of the sequence (some parts are empty)
-    __shared__ int last_s;
+__global__ void __launch_bounds__(256) kv8_decode_join_kernel(const b200q_kv8_cache c, const Kv8Decode p, int ctas, int tile, int by_part) {
+    constexpr int LANES = DH / 4, GROUPS = 256 / LANES;
+    __shared__ float factors[KV8_MAX_PARTS];                 // of the parts' results; -1: the part holds none of the sequence
+    __shared__ float4 sums[GROUPS][LANES];
+    __shared__ float warp_top[8], warp_weight[8];
+    __shared__ int first_s, last_s, slot_s;
     chain_trigger();
     chain_wait();
     const Kv8Attention &a = p.a;
-    const int i = blockIdx.x;
-    const int4 cut = p.cuts[i];
-    if (cut.x < 0) return;
-    const int list = cut.y, s = cut.z, slot0 = cut.x;
-    if (threadIdx.x == 0) last_s = i;
-    __syncthreads();
-    for (int q = i + threadIdx.x; q < ctas; q += 256) {
-        const bool mine = q == i || p.cuts[q].w == list * a.batch + s;
-        holds[q] = mine;
-        if (mine && q > i) atomicMax(&last_s, q);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    int segment = blockIdx.x;
+    if (by_part) {
+        const int4 cut = p.cuts[blockIdx.x];
+        if (cut.x < 0) return;
+        segment = cut.y * a.batch + cut.z;
     }
+    const int list = segment / a.batch, s = segment - list * a.batch, head = list / p.tiles, row0 = (list - head * p.tiles) * tile;
+    const int row = blockIdx.y, row_of = a.offsets[s];
+    if (row >= min((a.offsets[s + 1] - row_of) * p.group - row0, tile)) return;
+    if (tid == 0) first_s = last_s = -1;
     __syncthreads();
-    const int last = last_s;
-    const int head = list / p.tiles, row0 = (list - head * p.tiles) * tile;
-    const int rows = min((a.offsets[s + 1] - a.offsets[s]) * p.group - row0, tile);
-    for (int j = threadIdx.x; j < rows * DH; j += 256) {
-        const int row = j / DH, d = j - row * DH;
-        auto part = [&](int q) { return p.partial + ((static_cast<size_t>(q) * 2 + (q == i ? slot0 : 0)) * tile + row) * (DH + 2); };
-        float top = -INFINITY;
-        for (int q = i; q <= last; ++q)
-            if (holds[q]) top = fmaxf(top, part(q)[DH]);
-        const float shift = top == -INFINITY ? 0.f : top;
-        float value = 0.f, weight = 0.f;
-        for (int q = i; q <= last; ++q) {
-            if (!holds[q]) continue;
-            const float *from = part(q), f = exp2_approx(from[DH] - shift);
-            value += f * from[d];
-            weight += f * from[DH + 1];
+    for (int q = tid; q < ctas; q += 256) {
+        const int4 cut = p.cuts[q];
+        const bool begins = cut.x >= 0 && cut.y * a.batch + cut.z == segment;
+        if (begins) {
+            first_s = q;
+            slot_s = cut.x;
         }
-        const int rr = row0 + row, token = rr / p.group;
-        store_from_float(a.out, c.dtype, (static_cast<size_t>(a.offsets[s] + token) * a.heads + head * p.group + rr - token * p.group) * DH + d,
-                         value / weight);
+        factors[q] = begins || cut.w == segment ? 0.f : -1.f;
+        if (cut.w == segment) atomicMax(&last_s, q);
     }
+    __syncthreads();
+    const int first = first_s, last = last_s, slot0 = slot_s;
+    if (first < 0) return;                                   // not cut
+    auto part = [&](int q) { return p.partial + ((static_cast<size_t>(q) * 2 + (q == first ? slot0 : 0)) * tile + row) * (DH + 4); };
+    constexpr int MINE = KV8_MAX_PARTS / 256;
+    float2 stat[MINE];                                       // maximum and sum of weights
+    float top = -INFINITY, weight = 0.f;
+#pragma unroll
+    for (int j = 0; j < MINE; ++j) {
+        const int q = first + tid + 256 * j;
+        stat[j] = make_float2(-INFINITY, 0.f);
+        if (q <= last && factors[q] >= 0.f) stat[j] = *reinterpret_cast<const float2 *>(part(q) + DH);
+        top = fmaxf(top, stat[j].x);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if (lane == 0) warp_top[warp] = top;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < 8; ++w) top = fmaxf(top, warp_top[w]);
+    const float shift = top == -INFINITY ? 0.f : top;
+#pragma unroll
+    for (int j = 0; j < MINE; ++j) {
+        const int q = first + tid + 256 * j;
+        const float f = exp2_approx(stat[j].x - shift);
+        weight += f * stat[j].y;
+        if (q <= last && factors[q] >= 0.f) factors[q] = f;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) weight += __shfl_xor_sync(0xffffffffu, weight, o);
+    if (lane == 0) warp_weight[warp] = weight;
+    __syncthreads();
+    const int group = tid / LANES, at = tid - group * LANES;
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int q = first + group; q <= last; q += GROUPS) {
+        const float f = factors[q];
+        if (!(f < 0.f)) {                                    // (NaN belongs to the result)
+            const float4 v = reinterpret_cast<const float4 *>(part(q))[at];
+            sum.x += f * v.x; sum.y += f * v.y; sum.z += f * v.z; sum.w += f * v.w;
+        }
+    }
+    sums[group][at] = sum;
+    __syncthreads();
+    if (tid >= DH) return;
+    float value = 0.f;
+    weight = 0.f;
+    for (int g = 0; g < GROUPS; ++g) value += reinterpret_cast<const float *>(sums[g])[tid];
+    for (int w = 0; w < 8; ++w) weight += warp_weight[w];
+    const int rr = row0 + row, token = rr / p.group;
+    store_from_float(a.out, c.dtype, (static_cast<size_t>(row_of + token) * a.heads + head * p.group + rr - token * p.group) * DH + tid, value / weight);
 }
 
 // ----------------------------------------------------------------------------------------------------------- host side
 // How a call is divided: CTAs, and whether parts are cut at the borders of sequences.
 struct DecodePlan {
-    int tile, tiles, ctas, mode;        // rows per list (8 or 16), lists per head
+    int tile, tiles, rows, ctas, mode;  // rows per list (8 or 16), lists per head, rows that a list has at most
     long long bytes;
 };
 
@@ -530,6 +576,7 @@ static DecodePlan decode_plan(const b200q_kv8_cache *c, int heads, int batch, in
     const int b = std::min(batch, KV8_MAX_BATCH);
     d.tile = max_new * group <= 8 ? 8 : 16;
     d.tiles = (max_new * group + d.tile - 1) / d.tile;
+    d.rows = std::min(max_new * group, d.tile);
     const int warps = d.tile == 8 ? DecodeShape<64, 1, WHOLE>::WARPS : DecodeShape<64, 2, WHOLE>::WARPS;
     const long long units = (max_keys + KV8_BLOCK - 1) / KV8_BLOCK, segments = static_cast<long long>(c->kv_heads) * d.tiles * b;
     const int sms = sm_count();
@@ -539,7 +586,7 @@ static DecodePlan decode_plan(const b200q_kv8_cache *c, int heads, int batch, in
     d.mode = units > 4 * warps ? CUT : units <= 4 || segments >= 4ll * sms * warps ? SOLO : WHOLE;
     const long long work = d.mode == SOLO ? (segments + warps - 1) / warps : d.mode == WHOLE ? segments : std::max<long long>(1, segments * units / (warps / 2));
     d.ctas = static_cast<int>(std::min<long long>({d.mode == CUT ? 2 * sms : sms, work, KV8_MAX_PARTS}));
-    d.bytes = d.mode != CUT ? 0 : static_cast<long long>(d.ctas) * (16 + 2 * d.tile * (c->head_dim + 2) * 4);
+    d.bytes = d.mode != CUT ? 0 : static_cast<long long>(d.ctas) * (16 + 2 * d.tile * (c->head_dim + 4) * 4);
     return d;
 }
 
@@ -563,7 +610,11 @@ static int launch_decode(const b200q_kv8_cache &c, Kv8Decode p, const DecodePlan
         launch_chained(kv8_decode_kernel<DH, BF16, RT, MODE>, dim3(d.ctas), dim3(W * 32), smem, stream, c, p);
         if (int rc = check_launch("kv8_attention")) return rc;
         if (MODE != CUT) continue;
-        if (d.ctas > 1) launch_chained(kv8_decode_join_kernel<DH>, dim3(d.ctas - 1), dim3(256), 0, stream, c, p, d.ctas, d.tile);
+        const long long segments = static_cast<long long>(c.kv_heads) * p.tiles * p.a.batch;
+        const int by_part = segments >= d.ctas;
+        if (d.ctas > 1)
+            launch_chained(kv8_decode_join_kernel<DH>, dim3(by_part ? d.ctas - 1 : static_cast<int>(segments), d.rows), dim3(256), 0, stream, c, p,
+                           d.ctas, d.tile, by_part);
         if (int rc = check_launch("kv8_attention (join)")) return rc;
     }
     return B200Q_OK;
