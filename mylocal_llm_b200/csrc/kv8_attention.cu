@@ -8,16 +8,21 @@ int kv8_check(const char *what, const b200q_kv8_cache *c);       // kv8_cache.cu
 
 // kv8_decode.cu
 long long kv8_decode_workspace(const b200q_kv8_cache *c, int heads, int batch, int max_new, int max_keys);
+double kv8_decode_time(const b200q_kv8_cache *c, int heads, int batch, int max_new, int max_keys);
 int kv8_decode(const b200q_kv8_cache *c, const Kv8Attention &a, int max_new, int max_keys, void *workspace,
                long long workspace_bytes, cudaStream_t stream);
 // kv8_prompt.cu
 long long kv8_prompt_workspace(const b200q_kv8_cache *c, int heads, int batch, int rows, int max_new, int max_keys);
+double kv8_prompt_time(const b200q_kv8_cache *c, int heads, int batch, int rows, int max_new, int max_keys);
 int kv8_prompt(const b200q_kv8_cache *c, const Kv8Attention &a, int max_new, int max_keys, void *workspace, long long workspace_bytes,
                cudaStream_t stream);
 
-// Whether a step goes to the kernel for few tokens per sequence: all rows of a key/value head are one tile of 16, or single
-// tokens.
-static bool few_rows(const b200q_kv8_cache *c, int heads, int max_new) { return max_new == 1 || max_new * (heads / c->kv_heads) <= 16; }
+// Whether a step goes to the kernel for few tokens per sequence: single tokens, and where it is estimated to take less time, as for
+// chunks that are short next to their context: tiles of 16 rows against tiles of 128 (16 sequences of 8000 keys, 8 heads shared by
+// 4: 8 new tokens each 160 us against 203, 16 new tokens 294 against 214).
+static bool few_rows(const b200q_kv8_cache *c, int heads, int batch, int rows, int max_new, int max_keys) {
+    return max_new == 1 || kv8_decode_time(c, heads, batch, max_new, max_keys) < kv8_prompt_time(c, heads, batch, rows, max_new, max_keys);
+}
 
 }  // namespace b200q
 
@@ -26,7 +31,7 @@ using namespace b200q;
 extern "C" long long b200q_kv8_attention_workspace(const b200q_kv8_cache *cache, int heads, int batch, int rows, int max_new,
                                                    int max_keys) {
     if (!cache || heads < 1 || cache->kv_heads < 1 || heads % cache->kv_heads || max_new < 1) return 0;
-    return few_rows(cache, heads, max_new) ? kv8_decode_workspace(cache, heads, batch, max_new, max_keys)
+    return few_rows(cache, heads, batch, rows, max_new, max_keys) ? kv8_decode_workspace(cache, heads, batch, max_new, max_keys)
                                                : kv8_prompt_workspace(cache, heads, batch, rows, max_new, max_keys);
 }
 
@@ -56,7 +61,7 @@ extern "C" int b200q_kv8_attention(const b200q_kv8_cache *cache, int layer, cons
     a.slots = slots; a.offsets = offsets; a.starts = starts; a.batch = batch; a.rows = rows;
     a.cos_t = cos_table; a.sin_t = sin_table; a.scale = scale; a.out = out;
     a.vec = (reinterpret_cast<uintptr_t>(q) & 15) == 0 && q_row * dtype_size(q_dtype) % 16 == 0;
-    if (few_rows(cache, heads, max_new))
+    if (few_rows(cache, heads, batch, rows, max_new, max_keys))
         return kv8_decode(cache, a, max_new, max_keys, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
     return kv8_prompt(cache, a, max_new, max_keys, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
 }

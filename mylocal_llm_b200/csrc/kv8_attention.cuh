@@ -228,9 +228,9 @@ __device__ __forceinline__ void score_codes(const uint8_t *k, const uint32_t (&q
     }
 }
 
-// The same for the tail (16-bit values in global memory): keys from `rest` on are not read.
+// The same for the tail (16-bit values in shared memory): keys from `rest` on count as zeros.
 template <int DH, bool BF16, int RT>
-__device__ __forceinline__ void score_tail(const uint16_t *k, float inv, int rest, const uint32_t (&qf)[RT][DH / 16][4], int g, int t,
+__device__ __forceinline__ void score_tail(const uint8_t *k, float inv, int rest, const uint32_t (&qf)[RT][DH / 16][4], int g, int t,
                                            float (&acc)[RT][8][4]) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
@@ -239,7 +239,7 @@ __device__ __forceinline__ void score_tail(const uint16_t *k, float inv, int res
         for (int h = 0; h < DH / 64; ++h) {
             uint4 w[2] = {make_uint4(0u, 0u, 0u, 0u), make_uint4(0u, 0u, 0u, 0u)};
             if (key < rest) {
-                const uint4 *p = reinterpret_cast<const uint4 *>(k + key * DH + 64 * h + 16 * t);
+                const uint4 *p = reinterpret_cast<const uint4 *>(k + (key * DH + 64 * h + 16 * t) * 2);
                 w[0] = p[0];
                 w[1] = p[1];
             }

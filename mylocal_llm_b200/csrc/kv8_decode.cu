@@ -158,8 +158,8 @@ __global__ void __launch_bounds__(DecodeShape<DH, RT, MODE>::WARPS * 32, DecodeS
                kv8_unit(a.slots[x.seq], c.layers, a.layer, part, c.kv_heads, x.list / p.tiles) * HALF_PAGE;
     };
     // part 0: the keys, 1: the values. A stage's keys are replaced as soon as the scores are formed, its values after the value
-    // product: each half has the time of the other's work to arrive. A tail's values (16 bits, so they fill both halves)
-    // arrive as values; its keys are read directly.
+    // product: each half has the time of the other's work to arrive. A tail's values are 16 bits, so its keys take both halves
+    // and its values follow them when the scores are formed (asked into L2 with the keys).
     bool gave_up = false;                                    // the whole warp: a copy did not arrive, nothing more is requested
     auto arrived = [&](int part, int st, uint32_t &phases) {
         if (!gave_up)
@@ -178,14 +178,13 @@ __global__ void __launch_bounds__(DecodeShape<DH, RT, MODE>::WARPS * 32, DecodeS
             }
         } else {
             const int bytes = (a.starts[x.seq] + a.offsets[x.seq + 1] - a.offsets[x.seq]) % KV8_BLOCK * DH * 2;
-            if (part == 1) {
-                if (lane == 0) {
-                    mbar_arrive_expect_tx(bar, bytes);
-                    bulk_copy_g2s(to, tail_of(x, 1), bytes, bar);
-                }
-            } else {                                         // ask L2 for the keys
-                const char *k = reinterpret_cast<const char *>(tail_of(x, 0));
-                for (int o = lane * 128; o < bytes; o += 32 * 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(k + o));
+            if (lane == 0) {
+                mbar_arrive_expect_tx(bar, bytes);
+                bulk_copy_g2s(to, tail_of(x, part), bytes, bar);
+            }
+            if (part == 0) {
+                const char *v = reinterpret_cast<const char *>(tail_of(x, 1));
+                for (int o = lane * 128; o < bytes; o += 32 * 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(v + o));
             }
         }
     };
@@ -206,7 +205,7 @@ __global__ void __launch_bounds__(DecodeShape<DH, RT, MODE>::WARPS * 32, DecodeS
         const Unit x = look_up();
         kind_at[i] = x.kind;
         request(0, x, i);
-        request(1, x, i);
+        if (x.kind == PAGE) request(1, x, i);
         scale_at[i] = scale_of(x);
     }
     Unit next = look_up();
@@ -257,16 +256,18 @@ __global__ void __launch_bounds__(DecodeShape<DH, RT, MODE>::WARPS * 32, DecodeS
                 float acc[RT][8][4];
                 float kscale = __shfl_sync(0xffffffffu, scale_at[0], 0), vscale = __shfl_sync(0xffffffffu, scale_at[0], 1), vinv = 0.f;
                 const int rest = total - unit * KV8_BLOCK;   // keys of the block (64 or more: all)
+                arrived(0, st, k_phases);
                 if (!tail) {
-                    arrived(0, st, k_phases);
                     score_codes<DH, RT>(stage, qf, g, t, acc);
                     __syncwarp();
-                    request(0, next, st);
+                    if (next.kind == PAGE) request(0, next, st);
                 } else {
                     kscale = power_of(abs_bits(kscale));
                     vscale = power_of(abs_bits(vscale));
                     vinv = power_inverse(vscale);
-                    score_tail<DH, BF16, RT>(tail_of({TAIL, 0, list, s}, 0), power_inverse(kscale), rest, qf, g, t, acc);
+                    score_tail<DH, BF16, RT>(stage, power_inverse(kscale), rest, qf, g, t, acc);
+                    __syncwarp();
+                    request(1, {TAIL, 0, list, s}, st);
                 }
                 // ---- softmax weights; a row sees the keys up to its own position
                 uint32_t pf[RT][4][4];
@@ -374,16 +375,16 @@ __global__ void __launch_bounds__(DecodeShape<DH, RT, MODE>::WARPS * 32, DecodeS
                     }
                 }
                 __syncwarp();
-                if (tail) request(0, next, st);
-                request(1, next, st);
+                if (tail || next.kind == TAIL) request(0, next, st);
+                if (next.kind == PAGE) request(1, next, st);
                 advance();
             }
         } else {
             for (; u < end; u += STEP) {                     // rows that do not exist: the units pass by
-                if (kind_at[0] == PAGE) arrived(0, st, k_phases);
-                arrived(1, st, v_phases);
+                arrived(0, st, k_phases);
+                if (kind_at[0] == PAGE) arrived(1, st, v_phases);
                 request(0, next, st);
-                request(1, next, st);
+                if (next.kind == PAGE) request(1, next, st);
                 advance();
             }
         }
@@ -564,30 +565,51 @@ __global__ void __launch_bounds__(256) kv8_decode_join_kernel(const b200q_kv8_ca
 }
 
 // ----------------------------------------------------------------------------------------------------------- host side
-// How a call is divided: CTAs, and whether parts are cut at the borders of sequences.
+// How a call is divided: CTAs, and what their parts consist of.
 struct DecodePlan {
     int tile, tiles, rows, ctas, mode;  // rows per list (8 or 16), lists per head, rows that a list has at most
     long long bytes;
+    double time;                        // estimate, us
+};
+
+// What a mode costs, in us, as measured with 8 to 4096 sequences x heads of 1 to 94 units (caches in L2): a CTA per sequence (its
+// queries and the warps' meeting) and round of its warps; a warp by itself per sequence and unit; parts per sequence and unit of
+// the whole device. Estimates are within a third of the measured times; what they decide (head dimension 128, four rows): 8
+// sequences x heads of 1500 keys 13.7 cut, 16.1 whole, 87 by single warps; 256 of 777 keys 30 / 30 / 66; 4096 of 60 keys
+// 133 / 253 / 58.
+struct DecodeTimes {
+    double whole, whole_round, solo, solo_unit, cut, cut_unit;
+};
+static constexpr DecodeTimes DECODE_TIMES[2][2] = {          // [head dimension 128][16 rows]
+    {{3.0, 2.9, 8.0, 2.7, 0.02, 0.0018}, {5.5, 3.3, 9.5, 3.2, 0.04, 0.0031}},
+    {{4.0, 4.2, 11.0, 3.6, 0.03, 0.0029}, {9.0, 4.9, 15.0, 5.2, 0.06, 0.0046}},
 };
 
 static DecodePlan decode_plan(const b200q_kv8_cache *c, int heads, int batch, int max_new, int max_keys) {
     DecodePlan d{};
     const int group = heads / c->kv_heads;
     const int b = std::min(batch, KV8_MAX_BATCH);
-    d.tile = max_new * group <= 8 ? 8 : 16;
-    d.tiles = (max_new * group + d.tile - 1) / d.tile;
-    d.rows = std::min(max_new * group, d.tile);
+    d.tile = max_new * static_cast<long long>(group) <= 8 ? 8 : 16;
+    d.tiles = static_cast<int>((max_new * static_cast<long long>(group) + d.tile - 1) / d.tile);
+    d.rows = static_cast<int>(std::min<long long>(max_new * static_cast<long long>(group), d.tile));
     const int warps = d.tile == 8 ? DecodeShape<64, 1, WHOLE>::WARPS : DecodeShape<64, 2, WHOLE>::WARPS;
     const long long units = (max_keys + KV8_BLOCK - 1) / KV8_BLOCK, segments = static_cast<long long>(c->kv_heads) * d.tiles * b;
     const int sms = sm_count();
-    // Up to four rounds of a CTA's warps per sequence are not worth a second kernel. A CTA takes about 5 us per sequence whatever
-    // its length (queries, the warps' meeting), a warp by itself one unit in 2 us: 112 sequences of one token and 32 heads took
-    // 117 us by CTAs and take 26 us by warps.
-    d.mode = units > 4 * warps ? CUT : units <= 4 || segments >= 4ll * sms * warps ? SOLO : WHOLE;
+    const DecodeTimes &t = DECODE_TIMES[c->head_dim == 128][d.tile == 16];
+    const double whole = 2.5 + (segments + sms - 1) / sms * (t.whole + t.whole_round * ((units + warps - 1) / warps));
+    const double solo = 3. + (segments + sms * warps - 1) / (sms * warps) * (t.solo + t.solo_unit * units);
+    const double cut = 13. + segments * (t.cut + t.cut_unit * units) * (148. / sms);
+    // Long sequences are always cut, which also evens out lengths that differ (the estimates know the longest only).
+    d.time = units > 4 * warps ? cut : std::min(std::min(whole, solo), cut);
+    d.mode = d.time == cut ? CUT : d.time == whole ? WHOLE : SOLO;
     const long long work = d.mode == SOLO ? (segments + warps - 1) / warps : d.mode == WHOLE ? segments : std::max<long long>(1, segments * units / (warps / 2));
     d.ctas = static_cast<int>(std::min<long long>({d.mode == CUT ? 2 * sms : sms, work, KV8_MAX_PARTS}));
     d.bytes = d.mode != CUT ? 0 : static_cast<long long>(d.ctas) * (16 + 2 * d.tile * (c->head_dim + 4) * 4);
     return d;
+}
+
+double kv8_decode_time(const b200q_kv8_cache *c, int heads, int batch, int max_new, int max_keys) {
+    return decode_plan(c, heads, batch, max_new, max_keys).time;
 }
 
 long long kv8_decode_workspace(const b200q_kv8_cache *c, int heads, int batch, int max_new, int max_keys) {

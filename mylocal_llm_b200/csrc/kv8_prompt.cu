@@ -413,20 +413,30 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prompt_kernel(const b200q_k
             }
             const int have = block == full_pages ? rest : 0;
             const float inv = have ? tail_inverse(!keys) : 0.f;
-            if (keys) {
-                for (int id = ct; id < KV8_BLOCK * DH / 8; id += 128) {
-                    const int key = id / (DH / 8), chunk = id % (DH / 8);
-                    uint4 x = make_uint4(0u, 0u, 0u, 0u);
-                    if (key < have) x = *reinterpret_cast<const uint4 *>(tail_k + key * DH + 8 * chunk);
-                    *reinterpret_cast<uint4 *>(to + (chunk >> 3) * K_SLAB + swizzled(key, chunk & 7)) =
-                        make_uint4(half_of(x.x, inv), half_of(x.y, inv), half_of(x.z, inv), half_of(x.w, inv));
+            // eight dimensions of a key at a time, four loads on their way
+            constexpr int CHUNKS = DH / 8;
+            const uint16_t *from = keys ? tail_k : tail_v;
+#pragma unroll 1
+            for (int id0 = ct; id0 < KV8_BLOCK * CHUNKS; id0 += 4 * 128) {
+                uint4 x[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int id = id0 + 128 * j, key = keys ? id / CHUNKS : id % KV8_BLOCK, chunk = keys ? id % CHUNKS : id / KV8_BLOCK;
+                    x[j] = make_uint4(0u, 0u, 0u, 0u);
+                    if (key < have) x[j] = *reinterpret_cast<const uint4 *>(from + key * DH + 8 * chunk);
                 }
-            } else {
-                for (int id = ct; id < KV8_BLOCK * DH / 2; id += 128) {
-                    const int key = id / (DH / 2), d = id % (DH / 2) * 2;
-                    const uint32_t x = key < have ? half_of(*reinterpret_cast<const uint32_t *>(tail_v + key * DH + d), inv) : 0u;
-                    *reinterpret_cast<uint16_t *>(to + swizzled(d, key >> 3) + (key & 7) * 2) = static_cast<uint16_t>(x);
-                    *reinterpret_cast<uint16_t *>(to + swizzled(d + 1, key >> 3) + (key & 7) * 2) = static_cast<uint16_t>(x >> 16);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int id = id0 + 128 * j, key = keys ? id / CHUNKS : id % KV8_BLOCK, chunk = keys ? id % CHUNKS : id / KV8_BLOCK;
+                    const uint32_t w[4] = {half_of(x[j].x, inv), half_of(x[j].y, inv), half_of(x[j].z, inv), half_of(x[j].w, inv)};
+                    if (keys) {
+                        *reinterpret_cast<uint4 *>(to + (chunk >> 3) * K_SLAB + swizzled(key, chunk & 7)) = make_uint4(w[0], w[1], w[2], w[3]);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            *reinterpret_cast<uint16_t *>(to + swizzled(8 * chunk + e, key >> 3) + (key & 7) * 2) =
+                                static_cast<uint16_t>(e & 1 ? w[e / 2] >> 16 : w[e / 2]);
+                    }
                 }
             }
         };
@@ -444,6 +454,12 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prompt_kernel(const b200q_k
                 asm volatile("prefetch.global.L2 [%0];" ::"l"(from + (ct < LINES ? ct : ct - LINES) * 128 + (ct < LINES ? 0 : static_cast<size_t>(c.kv_heads) * HALF_PAGE)));
         };
         static_assert(2 * HALF_PAGE / 128 <= KP_CONVERT_WARPS * 32, "one line per thread");
+        // the tail is read late, by loads that are waited for: asked into L2 now
+        if (rest && (u1 - 1) * 2 + 1 >= full_pages)
+            for (int o = ct * 64; o < rest * DH; o += 128 * 64) {
+                asm volatile("prefetch.global.L2 [%0];" ::"l"(tail_k + o));
+                asm volatile("prefetch.global.L2 [%0];" ::"l"(tail_v + o));
+            }
         Half even, odd;                          // the unit's first and second page: keys, then values
         int far0 = page_at(2 * (u0 + KP_AHEAD)), far1 = page_at(2 * (u0 + KP_AHEAD) + 1);
         int page0 = page_at(2 * u0), page1 = page_at(2 * u0 + 1);
@@ -709,15 +725,39 @@ __global__ void __launch_bounds__(256) kv8_prompt_join_kernel(const b200q_kv8_ca
 }
 
 // ----------------------------------------------------------------------------------------------------------- host side
-// Parts of the keys: as many as give every SM two CTAs, of four units at least.
-static int prompt_splits(const b200q_kv8_cache *c, int heads, int batch, int max_new, int max_keys) {
-    const long long rows = static_cast<long long>(max_new) * (heads / c->kv_heads), units = (max_keys + KP_KEYS - 1) / KP_KEYS;
-    const long long ctas = (rows + KP_CTA_ROWS - 1) / KP_CTA_ROWS * c->kv_heads * batch;
-    return static_cast<int>(std::max(1ll, std::min({(2ll * sm_count() + ctas - 1) / ctas, units / 4, 64ll})));
+// Parts of the keys, and the time that is estimated for them, in us: CTAs (one per SM; where they do not all start at once, half a
+// CTA's time is lost at the end), each with its beginning and end and its units, and, for more than one part, the results on their way
+// through memory and the joining kernel. Measured for a head dimension of 128: 18 us for one CTA with one tile of rows and four
+// units, 27 with two tiles. 128 CTAs of 63 units (16 sequences of 8000 keys) took 218 us in three parts, so in three rounds, and
+// take 196 in one; 32 of 32 units 87 in eight parts, 59 in four. A further part has to gain a twentieth: three instead of two for
+// the 192 CTAs of three chunks of 512 tokens behind up to 16000 took 369 us instead of 336.
+struct PromptPlan {
+    int splits;
+    double time;
+};
+static PromptPlan prompt_plan(const b200q_kv8_cache *c, int heads, int batch, int rows, int max_new, int max_keys) {
+    const long long list = static_cast<long long>(max_new) * (heads / c->kv_heads), units = (max_keys + KP_KEYS - 1) / KP_KEYS;
+    const double ctas = static_cast<double>((list + KP_CTA_ROWS - 1) / KP_CTA_ROWS) * c->kv_heads * batch / sm_count();      // per SM
+    const bool two = list > KP_ROWS, wide = c->head_dim == 128;
+    const double once = two ? (wide ? 10. : 7.7) : (wide ? 5.5 : 4.6), unit = two ? (wide ? 4.2 : 3.) : (wide ? 3.1 : 2.2);
+    const double part_bytes = 2. * rows * heads * (c->head_dim + 2) * 4.;
+    PromptPlan best{1, 0.};
+    for (int s = 1; s <= std::min(64ll, std::max(1ll, units / 2)); ++s) {
+        const double rounds = ctas * s <= 1. ? 1. : ctas * s + 0.5;
+        const double time = 3. + rounds * (once + unit * ((units + s - 1) / s)) + (s > 1 ? 4. + s * part_bytes * 2e-7 : 0.);
+        if (s == 1 || time < 0.95 * best.time) best = {s, time};
+    }
+    return best;
+}
+static int prompt_splits(const b200q_kv8_cache *c, int heads, int batch, int rows, int max_new, int max_keys) {
+    return prompt_plan(c, heads, batch, rows, max_new, max_keys).splits;
+}
+double kv8_prompt_time(const b200q_kv8_cache *c, int heads, int batch, int rows, int max_new, int max_keys) {
+    return prompt_plan(c, heads, batch, rows, max_new, max_keys).time;
 }
 
 long long kv8_prompt_workspace(const b200q_kv8_cache *c, int heads, int batch, int rows, int max_new, int max_keys) {
-    const int splits = prompt_splits(c, heads, batch, max_new, max_keys);
+    const int splits = prompt_splits(c, heads, batch, rows, max_new, max_keys);
     return splits == 1 ? 0 : static_cast<long long>(splits) * rows * heads * (c->head_dim + 2) * 4;
 }
 
@@ -726,7 +766,7 @@ int kv8_prompt(const b200q_kv8_cache *c, const Kv8Attention &a, int max_new, int
     Kv8Prompt p{};
     p.a = a;
     p.group = a.heads / c->kv_heads;
-    p.splits = prompt_splits(c, a.heads, a.batch, max_new, max_keys);
+    p.splits = prompt_splits(c, a.heads, a.batch, a.rows, max_new, max_keys);
     const long long bytes = kv8_prompt_workspace(c, a.heads, a.batch, a.rows, max_new, max_keys);
     if (bytes > workspace_bytes || (bytes && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15))))
         return fail(B200Q_EINVAL, "kv8_attention: workspace of %lld bytes, 16-byte aligned, needed", bytes);
