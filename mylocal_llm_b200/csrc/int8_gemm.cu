@@ -183,7 +183,7 @@ __global__ void __launch_bounds__(256, VEC ? 4 : 2) int8_quantize_kernel(const v
             meet();                                      // (the previous row's peaks have been read)
             if ((threadIdx.x & 31) == 0) peaks[warp] = peak;
             meet();
-            for (int w = 0; w < team; ++w) peak = max(peak, peaks[first_warp + w]);
+            peak = __reduce_max_sync(0xffffffffu, peaks[first_warp + (threadIdx.x & (team - 1))]);
         }
         const float s = int8_scale(peak_bits<IN>(peak)), inv = __fdiv_rn(1.f, s);
         if (c0 == 0) scales[row] = s;
@@ -710,7 +710,9 @@ extern "C" int b200q_int8_quantize(const void *x, int x_dtype, int rows, int k, 
                   : x_dtype == B200Q_F16 ? (vec ? int8_quantize_kernel<B200Q_F16, true> : int8_quantize_kernel<B200Q_F16, false>)
                                          : (vec ? int8_quantize_kernel<B200Q_BF16, true> : int8_quantize_kernel<B200Q_BF16, false>);
     int team = 1;
-    while (team < 8 && 256 * team * (x_dtype == B200Q_F32 ? I8_QUANTIZE_KEEP / 2 : I8_QUANTIZE_KEEP) < k) team *= 2;
+    const int keep = x_dtype == B200Q_F32 ? I8_QUANTIZE_KEEP / 2 : I8_QUANTIZE_KEEP;
+    // (few rows: as many warps as there are, one row of 2048 took 1 us longer by two)
+    while (team < 8 && (256 * team * keep < k || static_cast<long long>(rows) * team <= 2 * sm_count())) team *= 2;
     const int teams = 8 / team, ctas = std::min((rows + teams - 1) / teams, (vec ? 4 : 2) * sm_count());
     launch_chained(kernel, dim3(ctas), dim3(256), 0, static_cast<cudaStream_t>(stream), x, rows, k, static_cast<long long>(x_row), codes,
                    static_cast<long long>(codes_row), scales, team, early);
