@@ -21,8 +21,10 @@ and the ``read_*`` helpers waits for it, and a step whose ``batch`` is kept can 
 501, 502, 503); the rows of a refused step are NaN. Calls on one cache have to be ordered by their streams.
 
 A key or value that is not finite (in the cache's type) makes its block (its 64 tokens, of its head and layer) NaN, and with it every row that sees
-the block. Scores, softmax statistics and sums are FP32; queries and softmax weights are rounded to FP16 before the tensor
-cores (relative 2^-12, each row of queries scaled by a power of two), the codes enter the products exactly.
+the block. Scores, softmax statistics and sums are FP32, and
+the codes enter the products exactly. Steps of few tokens keep 22 bits of queries and softmax weights (an FP16 number and its
+remainder); prompts and chunks round weights, and for BF16 caches queries, to FP16 (relative 2^-12, each row of queries scaled
+by a power of two). Which of the two kernels a step takes follows from an estimate of their times.
 """
 
 import ctypes
