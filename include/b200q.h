@@ -512,7 +512,7 @@ int b200q_kv8_append(const b200q_kv8_cache *cache, int layer, const void *k, con
 /* Causal attention of the new tokens of one layer over the cache they are in: row r of q (heads * head_dim wide, heads a
  * multiple of kv_heads, q_row elements from row to row, not rotated yet where tables are given) is the query at position
  * starts[b] + r - offsets[b] of slots[b] and sees the keys up to its own position. out [rows][heads * head_dim] has the
- * cache's `dtype`. `rows` = offsets[batch]; max_new: most new tokens of a sequence; max_keys: most tokens a sequence holds
+ * cache's `dtype` and is 16-byte aligned. `rows` = offsets[batch]; max_new: most new tokens of a sequence; max_keys: most tokens a sequence holds
  * after the step (a bound that the division of the work goes by; max_length is always right). The rows of a sequence with
  * starts[b] < 0 are NaN. Scores and softmax statistics are FP32. workspace: b200q_kv8_attention_workspace(...) bytes,
  * 16-byte aligned, used by one call at a time. */

@@ -55,6 +55,7 @@ extern "C" int b200q_kv8_attention(const b200q_kv8_cache *cache, int layer, cons
         return fail(B200Q_EINVAL, "kv8_attention: RoPE tables of %d rows for sequences of up to %d tokens", rope_rows, cache->max_length);
     if ((reinterpret_cast<uintptr_t>(cos_table) | reinterpret_cast<uintptr_t>(sin_table)) & 15)
         return fail(B200Q_EINVAL, "kv8_attention: RoPE tables must be 16-byte aligned");
+    if (reinterpret_cast<uintptr_t>(out) & 15) return fail(B200Q_EINVAL, "kv8_attention: out must be 16-byte aligned");
     if (heads > 65535) return fail(B200Q_EUNSUPPORTED, "kv8_attention: too many heads");
     Kv8Attention a{};
     a.q = q; a.q_row = q_row; a.q_dtype = q_dtype; a.layer = layer; a.heads = heads;

@@ -608,8 +608,15 @@ static DecodePlan decode_plan(const b200q_kv8_cache *c, int heads, int batch, in
     return d;
 }
 
+// Sizes whose units a CTA can number.
+static bool decode_supported(const b200q_kv8_cache *c, const DecodePlan &d) {
+    return static_cast<long long>(c->kv_heads) * d.tiles <= 65535 &&
+           static_cast<long long>(KV8_MAX_BATCH) * ((c->max_length + KV8_BLOCK - 1) / KV8_BLOCK) <= 0x7fffffffll / std::max(1, c->kv_heads * d.tiles / d.ctas + 1);
+}
+
 double kv8_decode_time(const b200q_kv8_cache *c, int heads, int batch, int max_new, int max_keys) {
-    return decode_plan(c, heads, batch, max_new, max_keys).time;
+    const DecodePlan d = decode_plan(c, heads, batch, max_new, max_keys);
+    return decode_supported(c, d) ? d.time : 1e30;
 }
 
 long long kv8_decode_workspace(const b200q_kv8_cache *c, int heads, int batch, int max_new, int max_keys) {
@@ -658,8 +665,7 @@ int kv8_decode(const b200q_kv8_cache *c, const Kv8Attention &a, int max_new, int
     const DecodePlan d = decode_plan(c, a.heads, a.batch, max_new, max_keys);
     if (d.bytes > workspace_bytes || (d.bytes && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15))))
         return fail(B200Q_EINVAL, "kv8_attention: workspace of %lld bytes, 16-byte aligned, needed", d.bytes);
-    if (static_cast<long long>(c->kv_heads) * d.tiles > 65535 ||
-        static_cast<long long>(KV8_MAX_BATCH) * ((c->max_length + KV8_BLOCK - 1) / KV8_BLOCK) > 0x7fffffffll / std::max(1, c->kv_heads * d.tiles / d.ctas + 1))
+    if (!decode_supported(c, d))
         return fail(B200Q_EUNSUPPORTED, "kv8_attention: too many heads or keys");
     Kv8Decode p{};
     p.a = a;

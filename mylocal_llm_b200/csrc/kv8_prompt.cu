@@ -770,7 +770,6 @@ int kv8_prompt(const b200q_kv8_cache *c, const Kv8Attention &a, int max_new, int
     const long long bytes = kv8_prompt_workspace(c, a.heads, a.batch, a.rows, max_new, max_keys);
     if (bytes > workspace_bytes || (bytes && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15))))
         return fail(B200Q_EINVAL, "kv8_attention: workspace of %lld bytes, 16-byte aligned, needed", bytes);
-    if (reinterpret_cast<uintptr_t>(a.out) & 15) return fail(B200Q_EINVAL, "kv8_attention: out must be 16-byte aligned");
     p.partial = static_cast<float *>(workspace);
     p.status = device_status_word();
     if (!p.status) return fail(B200Q_ECUDA, "kv8_attention: no CUDA device");

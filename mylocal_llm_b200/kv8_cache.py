@@ -66,7 +66,8 @@ class KV8Batch:
     (tokens before the step, written by ``PagedKV8Cache.extend``), int32 on the device; on the host the number of rows, the most
     new tokens of a sequence and a bound on the tokens a sequence holds after the step."""
 
-    def __init__(self, slots, offsets, starts, rows, max_new, max_keys):
+    def __init__(self, slots, offsets, starts, rows, max_new, max_keys, limits):
+        self.limits = limits                             # sequences and max_length of the cache that it was made for
         self.slots, self.offsets, self.starts = slots, offsets, starts
         self.rows, self.max_new, self.max_keys = rows, max_new, max_keys
         self.size = slots.shape[0]
@@ -159,11 +160,14 @@ class PagedKV8Cache:
             raise ValueError("too many tokens in one step")
         ints = torch.tensor(slots + offsets + [-1] * len(slots), dtype=torch.int32).to(self.device)
         b = len(slots)
-        return KV8Batch(ints[:b], ints[b:2 * b + 1], ints[2 * b + 1:], offsets[-1], max(counts), max_keys)
+        return KV8Batch(ints[:b], ints[b:2 * b + 1], ints[2 * b + 1:], offsets[-1], max(counts), max_keys,
+                        (self.sequences, self.max_length))
 
     def _check_batch(self, batch):
         if not isinstance(batch, KV8Batch) or batch.slots.device != self.device:
             raise TypeError("batch must come from this cache's batch()")
+        if batch.limits != (self.sequences, self.max_length):
+            raise ValueError("batch was made for a cache of other sizes")
         return batch
 
     def extend(self, batch):

@@ -6,7 +6,7 @@ import math
 
 import pytest
 
-from mylocal_llm_b200 import Int8Weight, int8_linear, int8_matmul, packed_to_device, quantize_int8_rows
+from mylocal_llm_b200 import _lib, Int8Weight, int8_linear, int8_matmul, packed_to_device, quantize_int8_rows
 from mylocal_llm_b200.quantize import quantize
 
 pytestmark = pytest.mark.gpu
@@ -158,3 +158,36 @@ def test_refusals(cuda):
         Int8Weight(torch.ones(4, 40, device="cuda"), torch.ones(4, device="cuda"))
     with pytest.raises(TypeError):
         Int8Weight.from_packed(x)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("rows,k,stride", [(9, 1, 1), (9, 7, 9), (5, 1023, 1023), (40, 300, 307), (3, 4100, 4101), (700, 33, 41), (4, 8200, 8203), (2, 20001, 20002)])
+def test_rows_at_every_offset_among_what_does_not_count(cuda, rows, k, stride, dtype):
+    """Rows that begin at every element of 16 bytes; NaN and infinities before, between and behind them."""
+    torch = cuda
+    gen = torch.Generator(device="cuda").manual_seed(rows + k)
+    for first in range(9):
+        flat = torch.full((first + rows * stride + 9,), math.nan, dtype=getattr(torch, dtype), device="cuda")
+        flat[::2] = math.inf
+        x = flat[first:first + rows * stride].view(rows, stride)[:, :k]
+        x.copy_(torch.randn(rows, k, device="cuda", generator=gen))
+        codes, scales = quantize_int8_rows(x)
+        want, scale = quantised(torch, x)
+        assert torch.equal(codes[:, :k], want) and torch.equal(scales, scale) and not codes[:, k:].any()
+
+
+@pytest.mark.parametrize("m,n,k", [(130, 8231, 300), (1262, 4099, 200), (300, 9000, 17), (257, 16383, 129), (32, 77, 64), (31, 4001, 128)])
+def test_rows_of_outputs_at_any_alignment(cuda, m, n, k):
+    """Outputs whose rows are not 16-byte aligned, and nothing written behind the last row."""
+    torch = cuda
+    gen = torch.Generator(device="cuda").manual_seed(m + n)
+    weight = random_weight(torch, n, k, gen)
+    codes, scales = quantize_int8_rows(torch.randn(m, k, device="cuda", generator=gen))
+    for dtype, ident in ((torch.float32, 0), (torch.float16, 1), (torch.bfloat16, 2)):
+        for first in (0, 1, 3):
+            flat = torch.full((first + m * n + 64,), 77.0, dtype=dtype, device="cuda")
+            y = flat[first:first + m * n].view(m, n)
+            _lib.call("b200q_int8_gemm", weight.codes.data_ptr(), weight.codes.shape[1], weight.scales.data_ptr(), n, k, codes.data_ptr(),
+                      codes.shape[1], scales.data_ptr(), m, y.data_ptr(), ident, torch.cuda.current_stream().cuda_stream)
+            check(torch, y, codes, scales, weight, k)
+            assert (flat[:first] == 77).all() and (flat[first + m * n:] == 77).all()

@@ -375,3 +375,47 @@ def test_two_steps_at_once_on_two_caches(cuda):
                 got.append(c.attention(0, q, b))
     torch.cuda.synchronize()
     assert all(torch.equal(g, want[i % 2]) for i, g in enumerate(got))
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("heads,kv_heads,dh", [(8, 2, 128), (8, 2, 64), (3, 3, 128), (15, 1, 64)])
+@pytest.mark.parametrize("sizes,counts", [
+    ([8000, 8000, 5003, 7999], [8, 8, 3, 1]),                            # a few tokens each behind long contexts
+    ([4001], [64]), ([4001], [300]), ([700], [17]),                      # chunks of one sequence, tails of 33 and 60 tokens
+    ([11771, 127, 64, 5000, 63], [5, 5, 5, 0, 5]),                       # cut into many parts, some of them empty
+    ([215], [3]), ([60] * 40, [7] * 40), ([1500] * 3, [33] * 3)])
+def test_chunks_between_single_tokens_and_prompts(cuda, dtype, heads, kv_heads, dh, sizes, counts):
+    """Sizes at which the kernels for few and for many rows meet, each with its ways to divide the work."""
+    torch = cuda
+    cache = random_cache(torch, sizes, 1, kv_heads, dh, dtype, heads + sum(counts))
+    q = query(torch, sum(counts), heads * dh, dtype, 3)
+    rope = rope_tables(torch, cache.max_length, dh)
+    for max_keys in (None, max(sizes)):
+        out = cache.attention(0, q, step(cache, sizes, counts, max_keys=max_keys), rope=rope)
+        check(torch, cache, 0, q, out, sizes, counts, rope)
+        assert torch.equal(out, cache.attention(0, q, step(cache, sizes, counts, max_keys=max_keys), rope=rope))
+
+
+@pytest.mark.parametrize("rest", [1, 2, 15, 16, 17, 33, 63])
+@pytest.mark.parametrize("heads,kv_heads,dh", [(2, 2, 64), (4, 1, 128), (16, 1, 64), (12, 1, 128)])
+def test_tails_of_every_kind(cuda, rest, heads, kv_heads, dh):
+    """Single tokens and a few, whose own keys are in the tail, over contexts of a tail alone and of pages and a tail."""
+    torch = cuda
+    sizes = [rest, 64 + rest, 640 + rest, 6400 + rest]
+    for n in (1, min(rest, 6)):
+        cache = random_cache(torch, sizes, 1, kv_heads, dh, "float16", rest)
+        q = query(torch, n * len(sizes), heads * dh, "float32", rest)
+        out = cache.attention(0, q, step(cache, sizes, [n] * len(sizes)))
+        check(torch, cache, 0, q, out, sizes, [n] * len(sizes))
+
+
+def test_a_batch_belongs_to_its_cache(cuda):
+    torch = cuda
+    cache = random_cache(torch, [100, 70], 1, 1, 64, "bfloat16", 0)
+    other = random_cache(torch, [100], 1, 1, 64, "bfloat16", 0)
+    q = query(torch, 1, 64, "bfloat16", 0)
+    with pytest.raises(ValueError):
+        other.attention(0, q, step(cache, [100, 70], [1], slots=[1]))
+    out = torch.empty(65, dtype=torch.bfloat16, device="cuda")[1:].view(1, 64)
+    with pytest.raises(ValueError):
+        cache.attention(0, q, step(cache, [100, 70], [1], slots=[0]), out=out)              # not 16-byte aligned

@@ -112,3 +112,9 @@ def test_python_layers_refuse_host_tensors():
         PagedKV8Cache(1, 1, 64, pages=1, sequences=1, max_length=64, device="cpu")
     with pytest.raises(ValueError):
         PagedKV8Cache(1, 1, 64, pages=0, sequences=1, max_length=64)
+
+
+@pytest.mark.parametrize("max_new,rows", [(1, 2), (4, 5), (200, 300)])
+def test_attention_refuses_outputs_that_are_not_aligned(max_new, rows):
+    assert rc("b200q_kv8_attention", ctypes.byref(cache()), 0, ONE, 0, 512, 8, ONE, ONE, ONE, 2, rows, max_new, 100, None, None, 0, 0.1, ONE + 8,
+              ONE, 1 << 20, None) == 1
