@@ -98,8 +98,12 @@ __global__ void __launch_bounds__(DecodeShape<DH, RT, MODE>::WARPS * 32, DecodeS
         lo = s0 / a.batch * total_units + prefix[s0 % a.batch];
         hi = s1 / a.batch * total_units + prefix[s1 % a.batch];
     } else {
-        lo = all * blockIdx.x / gridDim.x;
-        hi = all * (blockIdx.x + 1) / gridDim.x;
+        // (contexts may be far shorter than the bound that the grid was made for: with a round of units per sequence on average, a
+        // part each, 256 of four units 15 us instead of 21 by cutting)
+        const long long segments = static_cast<long long>(lists) * a.batch;
+        const long long parts = segments < gridDim.x && all <= segments * W ? segments : gridDim.x;
+        lo = all * min(static_cast<long long>(blockIdx.x), parts) / parts;
+        hi = all * min(blockIdx.x + 1ll, parts) / parts;
     }
     if (lo >= hi) {                                          // (SOLO: the warp; nothing below is for the whole CTA then)
         if (MODE == CUT && tid == 0) p.cuts[blockIdx.x] = make_int4(-1, 0, 0, -1);
