@@ -265,26 +265,32 @@ __device__ __forceinline__ void umma_i8(uint32_t d_tmem, uint64_t a_desc, uint64
 // the alignment of rows (lanes that stored their own token's 64 bytes, one by one where rows are not 16-byte aligned: 1262 x 8231 x
 // 2000 with its quantiser 140 us, so 40 us; 1993 x 12581 x 317 257 and 43 us). `at`: element of the first token, this lane's channel; `rows`: tokens that exist.
 template <typename T>
-__device__ __forceinline__ void store_channel(T *y, size_t n, int rows, const float *stage, int lane, float w) {
-    auto put = [&](int r) {
-        const float v = stage[r * 32 + (lane ^ r)] * w;
-        if constexpr (sizeof(T) == 4) *y = v;
-        else if constexpr (std::is_same_v<T, __half>) *y = __float2half_rn(v);
-        else *y = __float2bfloat16_rn(v);
-        y += n;
+__device__ __forceinline__ void store_channel(T *y, size_t n, int rows, uint32_t stage, int lane, float w) {
+    auto put = [&](int r) {                              // (r * 128 + 4 * (lane ^ r): one exclusive or where r is a constant)
+        float v;
+        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"((stage ^ (4u * (lane ^ r))) + r * 128u));
+        v *= w;
+        T *to = y + r * n;
+        if constexpr (sizeof(T) == 4) *to = v;
+        else if constexpr (std::is_same_v<T, __half>) *to = __float2half_rn(v);
+        else *to = __float2bfloat16_rn(v);
     };
     if (rows == 32) {
-#pragma unroll 8
+#pragma unroll
         for (int r = 0; r < 32; ++r) put(r);
     } else {
+#pragma unroll 1
         for (int r = 0; r < rows; ++r) put(r);
     }
 }
+// `stage`: 4 KB, on a multiple of 128 bytes.
 __device__ __forceinline__ void store_outputs(void *y, int y_dtype, size_t at, int n, bool exists, int rows, const uint32_t (&sums)[32], float xs,
-                                              float w, float *stage, int lane) {
+                                              float w, uint32_t stage, int lane) {
     __syncwarp();                                        // (the previous outputs have been read)
+    const uint32_t mine = stage + lane * 132u;           // lane * 128 + 4 * (e ^ lane)
 #pragma unroll
-    for (int e = 0; e < 32; ++e) stage[lane * 32 + (e ^ lane)] = static_cast<float>(static_cast<int>(sums[e])) * xs;
+    for (int e = 0; e < 32; ++e)
+        asm volatile("st.shared.f32 [%0], %1;" ::"r"(mine ^ (4u * e)), "f"(static_cast<float>(static_cast<int>(sums[e])) * xs) : "memory");
     __syncwarp();
     if (!exists) return;
     if (y_dtype == B200Q_F32) store_channel(static_cast<float *>(y) + at, n, rows, stage, lane, w);
@@ -415,7 +421,7 @@ __global__ void __launch_bounds__(I8_THREADS, 1) int8_tile_kernel(const __grid_c
             tc_fence_after();
             chain_wait();                // y may still be read by what precedes this kernel; the scales are its result
             const float xs = row < rows ? a.x_scales[m0 + row] : 0.f;
-            float *stage = reinterpret_cast<float *>(smem) + warp % 4 * 1024;        // (the operands have been read)
+            const uint32_t stage = smem_u32(smem) + warp % 4 * 4096u;            // (the operands have been read)
 #pragma unroll 1
             for (int c = 0; c < NT / 32; ++c) {
                 const int col = n0 + 32 * c + lane;
@@ -592,7 +598,7 @@ __global__ void __launch_bounds__(I8_PAIR_THREADS, 1) int8_pair_kernel(const __g
     } else if (warp >= 2) {
         // two warps per quarter of the rows, 128 channels each
         const int quarter = warp & 3, half = (warp - 2) >> 2;
-        float *stage = reinterpret_cast<float *>(smem + S * I8_PAIR_STAGE) + (warp - 2) * 1024;
+        const uint32_t stage = smem_u32(smem + S * I8_PAIR_STAGE) + (warp - 2) * 4096u;
         const uint32_t acc_free0 = cluster_map(smem_u32(&acc_free[0]), 0);
         chain_wait();
         int turn = 0;
@@ -601,9 +607,7 @@ __global__ void __launch_bounds__(I8_PAIR_THREADS, 1) int8_pair_kernel(const __g
             pair_tile(a, tile, m0, n0);
             const int acc = turn & 1, row0 = m0 + 128 * static_cast<int>(rank) + 32 * quarter, col0 = n0 + 128 * half + lane;
             const float xs = row0 + lane < a.m ? a.x_scales[row0 + lane] : 0.f;
-            float w[4];
-#pragma unroll
-            for (int c = 0; c < 4; ++c) w[c] = col0 + 32 * c < a.n ? a.w_scales[col0 + 32 * c] : 0.f;
+            float w_next = col0 < a.n ? a.w_scales[col0] : 0.f;
             bool fine = !__any_sync(0xffffffffu, abort_flag != 0);
             if (fine) fine = __all_sync(0xffffffffu, mbar_wait_bounded(&acc_full[acc], (turn >> 1) & 1, a.status, STATUS_INT8_WAIT_MMA));
             if (!fine) {
@@ -611,9 +615,11 @@ __global__ void __launch_bounds__(I8_PAIR_THREADS, 1) int8_pair_kernel(const __g
                 break;
             }
             tc_fence_after();
-#pragma unroll
+#pragma unroll 1
             for (int c = 0; c < 4; ++c) {
                 const int col = col0 + 32 * c;
+                const float w = w_next;
+                if (c < 3) w_next = col + 32 < a.n ? a.w_scales[col + 32] : 0.f;
                 uint32_t r[32];
                 tmem_ld32(tmem_d + (static_cast<uint32_t>(32 * quarter) << 16) + 256 * acc + 128 * half + 32 * c, r);
                 tmem_ld_wait();
@@ -623,7 +629,7 @@ __global__ void __launch_bounds__(I8_PAIR_THREADS, 1) int8_pair_kernel(const __g
                     if (lane == 0) mbar_arrive_cluster(acc_free0 + 8u * acc);
                 }
                 if (row0 < a.m)
-                    store_outputs(a.y, a.y_dtype, static_cast<size_t>(row0) * a.n + col, a.n, col < a.n, min(32, a.m - row0), r, xs, w[c], stage, lane);
+                    store_outputs(a.y, a.y_dtype, static_cast<size_t>(row0) * a.n + col, a.n, col < a.n, min(32, a.m - row0), r, xs, w, stage, lane);
             }
         }
     }
