@@ -154,8 +154,17 @@ __global__ void __launch_bounds__(256, VEC ? 4 : 2) int8_quantize_kernel(const v
     };
     const char *first = static_cast<const char *>(x);
     const char *end = first + ((rows - 1) * static_cast<size_t>(x_row) + k) * (IN == B200Q_F32 ? 4 : 2);
+    // (a row of which the thread has KEEP whole pieces needs no looking at their ends)
+    const bool whole = VEC && c0 + width * (KEEP - 1) + 8 <= k;
     Piece<IN, VEC> next[KEEP];
     auto load_row = [&](int row) {
+        if constexpr (VEC)
+            if (whole && row < rows) {
+                const char *from = first + (row * static_cast<size_t>(x_row) + c0) * (IN == B200Q_F32 ? 4 : 2);
+#pragma unroll
+                for (int j = 0; j < KEEP; ++j) next[j].r = *reinterpret_cast<const Raw8<IN> *>(from + static_cast<size_t>(width * j) * (IN == B200Q_F32 ? 4 : 2));
+                return;
+            }
 #pragma unroll
         for (int j = 0; j < KEEP; ++j) {
             const int c = c0 + width * j;
@@ -188,16 +197,17 @@ __global__ void __launch_bounds__(256, VEC ? 4 : 2) int8_quantize_kernel(const v
         }
         const float s = int8_scale(peak_bits<IN>(peak)), inv = __fdiv_rn(1.f, s);
         if (c0 == 0) scales[row] = s;
+        int8_t *to = codes + row * static_cast<size_t>(codes_row);
         auto put = [&](int c, const Raw8<IN> &r) {
             float f[8];
             r.values(f);
             const float lo[4] = {f[0], f[1], f[2], f[3]}, hi[4] = {f[4], f[5], f[6], f[7]};
-            *reinterpret_cast<uint2 *>(codes + row * static_cast<size_t>(codes_row) + c) = make_uint2(int8_codes(lo, s, inv), int8_codes(hi, s, inv));
+            *reinterpret_cast<uint2 *>(to + c) = make_uint2(int8_codes(lo, s, inv), int8_codes(hi, s, inv));
         };
 #pragma unroll
         for (int j = 0; j < KEEP; ++j) {
             const int c = c0 + width * j;
-            if (c < padded) put(c, kept[j]);
+            if (whole || c < padded) put(c, kept[j]);
         }
         for (int c = c0 + width * KEEP; c < padded; c += width) put(c, c < k ? again(c) : Raw8<IN>{});
     }
