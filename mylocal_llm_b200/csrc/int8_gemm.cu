@@ -136,8 +136,8 @@ template <int IN> struct Piece<IN, false> {
 // A team of `team` warps takes a row at a time: the largest magnitude, then the codes. The row's pieces of eight values stay in
 // registers, as they were loaded, between the two up to 256 * team * KEEP columns (longer rows are read again), and the next row's
 // are on their way meanwhile. Teams are as small as the row allows: warps that need not meet (6992 x 706 FP32, cold: by whole CTAs
-// 37 us, by small teams 17). 4096 x 8192 BF16 take 28 us (held as floats instead of as loaded 34 us), 15 at the measured bandwidth:
-// bound by issue slots (0.70 of them, some 22 instructions per value).
+// 37 us, by small teams 17). 4096 x 8192 BF16 take 26 us (held as floats instead of as loaded 34 us), 15 at the measured bandwidth:
+// bound by issue slots (0.69 of them, some 19 instructions per value).
 constexpr int I8_QUANTIZE_KEEP = 4;                  // pieces of 16-bit values (of FP32: half as many)
 template <int IN, bool VEC>
 __global__ void __launch_bounds__(256, VEC ? 4 : 2) int8_quantize_kernel(const void *x, int rows, int k, long long x_row, int8_t *codes,
@@ -273,7 +273,7 @@ __device__ __forceinline__ void umma_i8(uint32_t d_tmem, uint64_t a_desc, uint64
 // A warp's 32 tokens x 32 channels: each lane's sums of one token, times that token's scale, pass through 4 KB of shared memory so
 // that a lane has one channel of all tokens, whose scale is `w`, and the warp stores a token's 32 outputs together, whatever n and
 // the alignment of rows (lanes that stored their own token's 64 bytes, one by one where rows are not 16-byte aligned: 1262 x 8231 x
-// 2000 with its quantiser 140 us, so 40 us; 1993 x 12581 x 317 257 and 43 us). `at`: element of the first token, this lane's channel; `rows`: tokens that exist.
+// 2000 with its quantiser 140 us, so 39 us; 1993 x 12581 x 317 257 and 37 us). `at`: element of the first token, this lane's channel; `rows`: tokens that exist.
 template <typename T>
 __device__ __forceinline__ void store_channel(T *y, size_t n, int rows, uint32_t stage, int lane, float w) {
     auto put = [&](int r) {                              // (r * 128 + 4 * (lane ^ r): one exclusive or where r is a constant)
