@@ -43,39 +43,52 @@ __global__ void __launch_bounds__(EXTEND_THREADS) kv8_extend_kernel(const b200q_
                                                                     int *status) {
     chain_trigger();
     chain_wait();
-    __shared__ int first_s[EXTEND_THREADS];              // of a batch that fits: searched for every page taken
-    const int tid = threadIdx.x;
+    // A batch that fits is held by the threads, entry by entry; shared memory has what every page taken looks up: its entry's
+    // first request, slot and length.
+    __shared__ int first_s[EXTEND_THREADS], slot_s[EXTEND_THREADS], have_s[EXTEND_THREADS];
+    const int tid = threadIdx.x, words = (c.pages + 31) / 32;
     const bool small = batch <= EXTEND_THREADS;
-    int carry = 0, bad = 0;
+    const uint32_t early = tid < words ? c.free_bits[tid] : 0u;          // the first words are on their way meanwhile
+    int carry = 0, bad = 0, my_slot = 0, my_have = 0, my_add = 0;
     for (int b0 = 0; b0 < batch; b0 += EXTEND_THREADS) {
         const int b = b0 + tid;
         int need = 0;
         if (b < batch) {
-            const int slot = slots[b], add = offsets[b + 1] - offsets[b];
-            if (slot < 0 || slot >= c.sequences || add < 0) {
+            my_slot = slots[b];
+            my_add = offsets[b + 1] - offsets[b];
+            if (my_slot < 0 || my_slot >= c.sequences || my_add < 0) {
                 bad = 1;
             } else {
-                const int have = c.lengths[slot];
-                if (add > c.max_length - have) bad = 1;
-                else need = (have + add) / KV8_BLOCK - have / KV8_BLOCK;
+                my_have = c.lengths[my_slot];
+                if (my_add > c.max_length - my_have) bad = 1;
+                else need = (my_have + my_add) / KV8_BLOCK - my_have / KV8_BLOCK;
             }
         }
         int sum;
         const int before = block_prefix(need, &sum);
         if (b < batch) {                                 // first page request of the entry, until the pages are assigned
-            if (small) first_s[b] = before;
-            else starts[b] = carry + before;
+            if (small) {
+                first_s[b] = before;
+                slot_s[b] = my_slot;
+                have_s[b] = my_have;
+            } else {
+                starts[b] = carry + before;
+            }
         }
         carry += sum;
     }
     bad = __syncthreads_or(bad);
     const int *request = small ? first_s : starts;
-    const int total = carry, words = (c.pages + 31) / 32;
+    const int total = carry;
     if (total > 0 && !bad) {
-        int have = 0;
-        for (int w = tid; w < words; w += EXTEND_THREADS) have += __popc(c.free_bits[w]);
-        int all;
-        block_prefix(have, &all);
+        int all, first_rank = 0;
+        if (words <= EXTEND_THREADS) {                   // one pass over the words
+            first_rank = block_prefix(__popc(early), &all);
+        } else {
+            int have = 0;
+            for (int w = tid; w < words; w += EXTEND_THREADS) have += __popc(c.free_bits[w]);
+            block_prefix(have, &all);
+        }
         if (all < total) {
             if (tid == 0) atomicExch(status, STATUS_KV8_POOL);
             for (int b = tid; b < batch; b += EXTEND_THREADS) starts[b] = -1;
@@ -84,9 +97,9 @@ __global__ void __launch_bounds__(EXTEND_THREADS) kv8_extend_kernel(const b200q_
         int rank = 0;
         for (int w0 = 0; w0 < words && rank < total; w0 += EXTEND_THREADS) {
             const int w = w0 + tid;
-            uint32_t bits = w < words ? c.free_bits[w] : 0u;
-            int sum;
-            int r = rank + block_prefix(__popc(bits), &sum);
+            const uint32_t bits = w0 == 0 ? early : w < words ? c.free_bits[w] : 0u;
+            int sum = all, r = first_rank;
+            if (words > EXTEND_THREADS) r = rank + block_prefix(__popc(bits), &sum);
             rank += sum;
             if (bits == 0u || r >= total) continue;
             uint32_t left = bits;
@@ -99,8 +112,8 @@ __global__ void __launch_bounds__(EXTEND_THREADS) kv8_extend_kernel(const b200q_
                 const int bit = __ffs(left) - 1;
                 left &= left - 1;
                 while (e + 1 < batch && request[e + 1] <= r) ++e;
-                const int page = w * 32 + bit, slot = slots[e];
-                c.table[static_cast<size_t>(slot) * c.blocks + c.lengths[slot] / KV8_BLOCK + (r - request[e])] = page;
+                const int page = w * 32 + bit, slot = small ? slot_s[e] : slots[e], have = small ? have_s[e] : c.lengths[slot];
+                c.table[static_cast<size_t>(slot) * c.blocks + have / KV8_BLOCK + (r - request[e])] = page;
                 c.refs[page] = 1;
                 ++r;
             }
@@ -113,9 +126,13 @@ __global__ void __launch_bounds__(EXTEND_THREADS) kv8_extend_kernel(const b200q_
         if (bad) {
             starts[b] = -1;
         } else {
-            const int slot = slots[b], have = c.lengths[slot];
-            starts[b] = have;
-            c.lengths[slot] = have + (offsets[b + 1] - offsets[b]);
+            if (!small) {
+                my_slot = slots[b];
+                my_have = c.lengths[my_slot];
+                my_add = offsets[b + 1] - offsets[b];
+            }
+            starts[b] = my_have;
+            c.lengths[my_slot] = my_have + my_add;
         }
     }
 }
