@@ -342,3 +342,25 @@ def test_refusals_of_the_python_layer(cuda):
     with pytest.raises(ValueError):
         PagedKV8Cache.from_tensors(cache.codes, cache.scales, cache.tail, cache.peak, cache.table, cache.lengths, cache.refs, max_length=200)
     assert _lib.device_status() == 0
+
+
+@pytest.mark.parametrize("pages", [30000, 40000])
+def test_steps_of_more_sequences_than_a_cta_has_threads(cuda, pages):
+    torch = cuda
+    sequences = 2300
+    cache = PagedKV8Cache(1, 1, 64, pages=pages, sequences=sequences, max_length=64 * 40)
+    free, rows, lengths = list(range(pages)), [[] for _ in range(sequences)], [0] * sequences
+    for counts in ([(i * 89) % 800 for i in range(sequences)], [64] * sequences, [i % 2 for i in range(sequences)]):
+        slots = [(7 * i + 3) % sequences for i in range(sequences)]
+        batch = cache.extend(cache.batch(slots, counts))
+        assert batch.starts.tolist() == [lengths[s] for s in slots]
+        for s, n in zip(slots, counts):
+            need = (lengths[s] + n) // 64 - lengths[s] // 64
+            rows[s] += free[:need]
+            free, lengths[s] = free[need:], lengths[s] + n
+        assert cache.read_lengths() == lengths
+        assert all(t[:len(r)] == r for t, r in zip(cache.table.tolist(), rows))
+    bookkeeping(torch, cache)
+    assert _lib.device_status() == 0
+    refused = cache.extend(cache.batch(range(sequences), [1500] * sequences))           # more pages than there are
+    assert set(refused.starts.tolist()) == {-1} and cache.read_lengths() == lengths and _lib.device_status() in (501, 502)
