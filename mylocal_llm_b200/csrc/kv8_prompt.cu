@@ -13,15 +13,17 @@
 //               products run while the other's softmax does. (One warp for both tiles needed more time to issue the
 //               instructions, among three other busy warps of its scheduler, than the tensor cores to execute them.)
 //   softmax     (2 x 4 warps) a thread per row: maximum, weights, sum; the weights go back to tensor memory as FP16, times the
-//               block's value scale relative to a power of two U that follows the largest scale seen (as an addend of the
-//               exponent, which costs nothing; the sum is divided by it). A row's reference maximum
-//               moves only when it is passed by 2^8, so O is rescaled rarely (FP16 has the room for weights up to 2^8).
+//               block's value scale (its logarithm is an addend of the exponent, which costs nothing; the sum is divided by it).
+//               A row's reference M is the largest such product that it has seen, as a power of two, so a block counts by what
+//               it adds to the row and not by its scale: a large scale under a small weight does not push the others out of
+//               FP16's range. M moves only when it is passed by 2^8, so O is rescaled rarely; products are held as 2^7 times
+//               what they are next to M, FP16's whole range. What lies 2^-40 below M only enters the sum.
 // 128 keys per step because an MMA of 128 rows x 64 keys reads 6 KB of operands for 32 clocks of work, more than shared memory
 // gives: with units of 64 keys the MMAs took 3200 of 3900 clocks per 64 keys (head dimension 128, SPLIT). With a head dimension
 // of 128 the tensor cores and the 16 exponentials per clock of an SM take about the same time, with 64 the exponentials take
 // twice as long. Queries are rounded to FP16 (a power of two per row keeps them in range); where the result is FP16 too the
 // rounding would show next to the result's own, and a second product with the remainders (SPLIT) removes it. Weights are rounded
-// to FP16. Block scales below 2^-14 of the largest lose bits of their share accordingly.
+// to FP16 (relative 2^-12, or 2^-32 of the row's M).
 //
 // Every wait is bounded: on expiry the status word tells, all roles leave, and the CTA ends.
 #include <algorithm>
@@ -47,6 +49,10 @@ template <int DH, bool SPLIT> struct PromptShape {
     static constexpr int BYTES = (SPLIT ? 2 : 1) * Q + (KS + VS) * K;
 };
 constexpr int KP_AHEAD = 4;                  // units between a page's request to L2 and its use
+// Exponents of two: products of weight and value scale are held times 2^KP_RANGE / M (they pass M by 2^8 at most, so 2^15 fits FP16),
+// sums of weights times 2^KP_SUM / M (between 2^-81 and 2^100 with value scales up to 2^121 and 2^20 keys); products below 2^-KP_NOTHING
+// M count as nothing. An output is the quotient of the two times KP_GAIN = 2^(KP_SUM - KP_RANGE).
+constexpr float KP_RANGE = 7.f, KP_SUM = 40.f, KP_NOTHING = 40.f, KP_GAIN = 8589934592.f;
 
 struct Kv8Prompt {
     Kv8Attention a;
@@ -499,7 +505,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prompt_kernel(const b200q_k
         const int token = valid ? row / p.group : 0, pos = start + token;
         const size_t out_row = static_cast<size_t>(first + token) * a.heads + kvh * p.group + (valid ? row - token * p.group : 0);
         const uint32_t lanes = static_cast<uint32_t>(32 * (warp & 3)) << 16;
-        float m = -INFINITY, l = 0.f, reference = 0.f, per_reference = power_inverse(0.f);      // U and its reciprocal
+        float m = -INFINITY, l = 0.f;            // log2 M; the sum of the weights, times 2^KP_SUM / M
         bool fine = wait(&q_full, 0);
         const float factor = factor_s[t * KP_ROWS + local];
         const float *layer_scales = c.scales + kv8_unit(0, c.layers, a.layer, 0, c.kv_heads, kvh);
@@ -529,36 +535,19 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prompt_kernel(const b200q_k
         }
         for (int i = 0; fine && i < mine; ++i) {
             const int block = 2 * (u0 + i), key0 = block * KV8_BLOCK;
-            float f[2], relative[2], alpha = 1.f;
+            float f[2], vs[2], log_scale[2], alpha = 1.f;
+            bool sees[2];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const float ks = ks_next[h], vs = vs_next[h];
+                const float ks = ks_next[h];
+                vs[h] = vs_next[h];
+                log_scale[h] = log2_approx(vs[h]);
                 if (i + 1 < mine) scales_at(block + 2 + h, page_next[h], ks_next[h], vs_next[h]);
                 if (i + 2 < mine) page_next[h] = page_at(block + 4 + h);
-                const bool sees = pos >= key0 + h * KV8_BLOCK;
+                sees[h] = pos >= key0 + h * KV8_BLOCK;
                 // (not below the smallest normal number, where a hidden key's -inf would meet a zero)
                 f[h] = factor * ks;
-                if (f[h] < KV8_MIN_SCALE || !sees) f[h] = KV8_MIN_SCALE;
-                // U follows the largest scale: the same in every thread
-                const float power = power_of(abs_bits(vs));
-                if (power > 8.f * reference) {
-                    alpha *= reference * power_inverse(power);
-                    reference = power;
-                    per_reference = power_inverse(power);
-                }
-                relative[h] = vs;
-            }
-            // a weight's factor `relative` as an addend of its exponent; one too small to matter next to U counts as zero, and
-            // its weights only enter the sum
-            float addend[2], divide[2];
-            bool nothing[2];
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const float r = relative[h] * per_reference;
-                nothing[h] = r < 8.6736174e-19f;             // 2^-60
-                const bool plain = nothing[h] || pos < key0 + h * KV8_BLOCK;
-                addend[h] = plain ? 0.f : log2_approx(r);
-                divide[h] = plain ? 1.f : __fdividef(1.f, r);
+                if (f[h] < KV8_MIN_SCALE || !sees[h]) f[h] = KV8_MIN_SCALE;
             }
             fine = wait(&s_full[t], i & 1);
             if (!fine) break;
@@ -583,11 +572,14 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prompt_kernel(const b200q_k
 #pragma unroll
                 for (int e = 2; e < 32; e += 2) tops[q] = max3(tops[q], __uint_as_float(s[q][e]), __uint_as_float(s[q][e + 1]));
             }
-            const float top = fmaxf(fmaxf(tops[0], tops[1]) * f[0], fmaxf(tops[2], tops[3]) * f[1]);
+            // (where the scales are tiny M stays within 2^-40 of the largest weight, so that the sum has the range; of a block that is
+            // hidden or not finite nothing comes through fmaxf)
+            const float peak[2] = {fmaxf(tops[0], tops[1]) * f[0], fmaxf(tops[2], tops[3]) * f[1]};
+            const float product[2] = {sees[0] ? peak[0] + log_scale[0] : -INFINITY, sees[1] ? peak[1] + log_scale[1] : -INFINITY};
+            const float top = fmaxf(fmaxf(product[0], product[1]), fmaxf(peak[0], peak[1]) - KP_NOTHING);
             if (top > m + 8.f) {
-                const float keep = exp2_approx(m - top);
-                alpha *= keep;
-                l *= keep;
+                alpha = exp2_approx(m - top);
+                l *= alpha;
                 m = top;
             }
             if (i > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {            // (S of this unit follows the last value product)
@@ -601,10 +593,11 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prompt_kernel(const b200q_k
                     tmem_st16(tmem + lanes + O_COL + DH * t + d, o);
                 }
             }
-            const float shift = m == -INFINITY ? 0.f : m;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const float move = addend[h] - shift;
+                const bool nothing = product[h] < m - KP_NOTHING;
+                const float move = !sees[h] ? 0.f : nothing ? -peak[h] : log_scale[h] - m + KP_RANGE;
+                const float weigh = !sees[h] ? 0.f : nothing ? exp2_approx(peak[h] - m + KP_SUM) : __fdividef(KP_GAIN, vs[h]);
                 const uint64_t f2 = pack2(f[h], f[h]), move2 = pack2(move, move);        // pairs: two per instruction
                 uint64_t sums[2] = {0ull, 0ull};
                 uint32_t w[32];
@@ -619,14 +612,14 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prompt_kernel(const b200q_k
                         sums[q] = add2(sums[q], pack2(lo, hi));
                         w[16 * q + e / 2] = pack_half(lo, hi);
                     }
-                if (nothing[h]) {
+                if (nothing) {
 #pragma unroll
                     for (int e = 0; e < 32; ++e) w[e] = 0u;
                 }
                 tmem_st32(at + P_COL + 32 * h, w);
                 float lo, hi;
                 unpack2(add2(sums[0], sums[1]), lo, hi);
-                l = fmaf(lo + hi, divide[h], l);
+                l = fmaf(lo + hi, weigh, l);
             }
             tmem_st_wait();
             tc_fence_before();
@@ -636,7 +629,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prompt_kernel(const b200q_k
         // ---- results
         if (mine && fine && wait(&o_done[t], 0)) {
             tc_fence_after();
-            const float gain = p.splits == 1 ? __fdiv_rn(reference, l) : reference;
+            const float gain = p.splits == 1 ? __fdiv_rn(KP_GAIN, l) : 1.f;
             float *to = p.splits == 1 ? nullptr : p.partial + ((static_cast<size_t>(part) * a.rows) * a.heads + out_row) * (DH + 2);
 #pragma unroll 1
             for (int d = 0; d < DH; d += 32) {
@@ -721,7 +714,7 @@ __global__ void __launch_bounds__(256) kv8_prompt_join_kernel(const b200q_kv8_ca
         for (int e = 0; e < DH / 32; ++e) value[e] += f * from[lane + 32 * e];
     }
 #pragma unroll
-    for (int e = 0; e < DH / 32; ++e) store_from_float(a.out, c.dtype, at * DH + lane + 32 * e, value[e] / weight);
+    for (int e = 0; e < DH / 32; ++e) store_from_float(a.out, c.dtype, at * DH + lane + 32 * e, value[e] / weight * KP_GAIN);
 }
 
 // ----------------------------------------------------------------------------------------------------------- host side

@@ -1,0 +1,123 @@
+"""What the attention over the paged 8-bit cache keeps of small contributions, against 64-bit arithmetic on the cache's content.
+
+The bounds count what the kernels round. With S = scale * sum |q_i k_i|, p the exact softmax weights, A = sum of p |v| and V the
+largest p times the block's value scale: a score (products of exact codes and of queries, FP32 sums, the rotation) is off by at
+most d = 2^-19 (1 + S) and 2^-11 S more where queries are rounded to FP16, so a weight by a factor within exp(+-2 d); the rounding of a weight
+is relative to it, and 2^-31 * 127 V at most below FP16's normal numbers; the result is rounded to the cache's type (half a step)."""
+
+import math
+
+import pytest
+
+from mylocal_llm_b200 import _lib
+from test_gpu_kv8_attention import query, random_cache, step
+
+pytestmark = pytest.mark.gpu
+
+BLOCK = 64
+
+
+@pytest.fixture(autouse=True)
+def healthy(cuda):
+    _lib.clear_device_status()
+    yield
+    cuda.cuda.synchronize()
+    assert _lib.device_status() == 0
+
+
+def exact(torch, cache, layer, q, sizes, counts, scale):
+    """(result, A, largest S, V, keys) of every row and head in 64 bits, [rows, heads, dh] or [rows, heads, 1]."""
+    dh, kv_heads = cache.head_dim, cache.kv_heads
+    heads, row, out = q.shape[1] // dh, 0, []
+    for s, (total, n) in enumerate(zip(sizes, counts)):
+        if not n:
+            continue
+        pages, rest = cache.table[s, :total // BLOCK].long(), total % BLOCK
+        codes, sc = cache.codes[pages, layer].double(), cache.scales[pages, layer].double()
+        tail = cache.tail[s, layer, :, :, :rest].double()
+        k = torch.cat([(codes[:, 0].reshape(-1, kv_heads, BLOCK, dh) * sc[:, 0, :, None, None]).transpose(0, 1).reshape(kv_heads, -1, dh), tail[0]], 1)
+        v = torch.cat([(codes[:, 1].reshape(-1, kv_heads, dh, BLOCK) * sc[:, 1, :, None, None]).permute(1, 0, 3, 2).reshape(kv_heads, -1, dh), tail[1]], 1)
+        step_of = torch.cat([sc[:, 1].T.repeat_interleave(BLOCK, 1), cache.peak[s, layer, 1].double()[:, None].expand(-1, rest)], 1)
+        x = q[row:row + n].double().reshape(n, kv_heads, heads // kv_heads, dh).permute(1, 2, 0, 3)
+        hidden = torch.arange(total, device="cuda") > (torch.arange(n, device="cuda") + total - n)[:, None]
+        k, v = k[:, None], v[:, None]
+        p = torch.softmax((x @ k.transpose(-1, -2) * scale).masked_fill(hidden, -math.inf), -1)
+        big = (x.abs() @ k.abs().transpose(-1, -2) * abs(scale)).masked_fill(hidden, 0).amax(-1, keepdim=True)
+        parts = p @ v, p @ v.abs(), big, (p * step_of[:, None, None]).amax(-1, keepdim=True), torch.full_like(big, total)
+        out.append([t.permute(2, 0, 1, 3).reshape(n, heads, -1) for t in parts])
+        row += n
+    return [torch.cat(t) for t in zip(*out)]
+
+
+def check(torch, cache, layer, q, out, sizes, counts, scale, relative, query_rounding=0.0):
+    want, a, big, v, total = exact(torch, cache, layer, q, sizes, counts, scale)
+    kind = torch.finfo(out.dtype)
+    d = 2.0 ** -19 * (1 + big) + query_rounding * big
+    bound = (torch.exp(2 * d) - 1 + relative) * a + total * 2.0 ** -31 * 127 * v + kind.eps / 2 * 1.01 * want.abs() + kind.tiny * kind.eps
+    got = out.double().reshape(want.shape)
+    assert torch.isfinite(got).all()
+    off = ((got - want).abs() / bound).max()
+    assert off <= 1, f"{float(off)} of the bound"
+
+
+def levelled_cache(torch, sizes, kv_heads, dh, dtype, levels, value_scales, seed):
+    """Every block's keys score about ``levels[b % len]`` (in natural units, for queries of ones and scale 1 / dh) and its values
+    have the scale ``value_scales[b % len]``."""
+    cache = random_cache(torch, sizes, 1, kv_heads, dh, dtype, seed)
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    for s, n in enumerate(sizes):
+        for b in range(n // BLOCK):
+            page, level = int(cache.table[s, b]), levels[b % len(levels)]
+            keys = torch.randint(60, 69, (kv_heads, BLOCK * dh), device="cuda", generator=gen)
+            cache.codes[page, 0, 0] = (keys if level > 0 else -keys).to(torch.int8)
+            cache.scales[page, 0, 0] = abs(level) / 64
+            cache.scales[page, 0, 1] = value_scales[b % len(value_scales)]
+        rest = n % BLOCK
+        if rest:
+            cache.tail[s, 0, 0, :, :rest] = levels[n // BLOCK % len(levels)]
+            cache.peak[s, 0, 0] = cache.tail[s, 0, 0, :, :rest].float().abs().amax((-1, -2))
+            values = torch.randn(kv_heads, rest, dh, device="cuda", generator=gen) * 60 * value_scales[n // BLOCK % len(value_scales)]
+            cache.tail[s, 0, 1, :, :rest] = values.to(cache.dtype)
+            cache.peak[s, 0, 1] = cache.tail[s, 0, 1, :, :rest].float().abs().amax((-1, -2))
+    return cache
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("heads,kv_heads,dh", [(4, 4, 64), (8, 2, 128)])
+@pytest.mark.parametrize("levels,value_scales", [
+    ([-20, 5], [0.25, 2.0 ** -30]),              # large values under weights of e^-25: what counts is 2^-28 of them in scale
+    ([5, -20], [2.0 ** -30, 0.25]),
+    ([-30, -10, 10], [0.25, 2.0 ** -20, 2.0 ** -42]),
+    ([10, -10, -30], [2.0 ** -42, 2.0 ** -20, 0.25]),
+    ([3, 3, 3, 3, 3, 3, -40], [2.0 ** -40] * 6 + [0.25])])
+@pytest.mark.parametrize("sizes,counts", [([700, 260], [700, 260]), ([3000, 900], [400, 300]), ([3000, 900], [1, 1])])
+def test_large_value_scales_under_small_weights(cuda, dtype, heads, kv_heads, dh, levels, value_scales, sizes, counts):
+    """Blocks count by weight times value, whatever the scales of blocks that hardly count or that a row does not see."""
+    torch = cuda
+    if dtype == "float16":                       # results in its range
+        value_scales = [v * 2.0 ** 12 if v < 0.2 else v for v in value_scales]
+    cache = levelled_cache(torch, sizes, kv_heads, dh, dtype, levels, value_scales, 1)
+    q = torch.ones(sum(counts), heads * dh, device="cuda", dtype=getattr(torch, dtype))
+    out = cache.attention(0, q, step(cache, sizes, counts), scale=1 / dh)
+    check(torch, cache, 0, q, out, sizes, counts, 1 / dh, 2.0 ** -11)
+
+
+@pytest.mark.parametrize("scale", [0.0, 2.0 ** -126, 2.0 ** -60, 2.0 ** -30, 2.0 ** 60, 2.0 ** 100])
+@pytest.mark.parametrize("counts", [[200], [500], [1]])
+def test_value_scales_of_any_size(cuda, scale, counts):
+    """All values zero, tiny or huge, and blocks of ordinary ones among them."""
+    torch = cuda
+    for mixed in (False, True):
+        cache = random_cache(torch, [500], 1, 2, 64, "bfloat16", 3)
+        pages = cache.table[0, :7].long()
+        cache.scales[pages[::2] if mixed else pages, 0, 1] = max(scale, 2.0 ** -126)
+        if scale == 0:
+            cache.codes[pages[::2] if mixed else pages, 0, 1] = 0
+        if not mixed:
+            cache.tail[0, 0, 1, :, :52] *= 0.0 if scale == 0 else scale
+            cache.peak[0, 0, 1] = cache.tail[0, 0, 1, :, :52].float().abs().amax((-1, -2))
+        q = query(torch, counts[0], 4 * 64, "bfloat16", 3)
+        out = cache.attention(0, q, step(cache, [500], counts))
+        if scale == 0 and not mixed:
+            assert not out.any()
+        check(torch, cache, 0, q, out, [500], counts, 0.125, 2.0 ** -11, 2.0 ** -11)
