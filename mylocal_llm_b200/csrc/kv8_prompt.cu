@@ -9,7 +9,7 @@
 //               sequence goes the same way. (A ring of codes in shared memory took 64 KB of its traffic per unit, which the
 //               operands of the MMAs need: at head dimension 128 they read 256 to 320 KB per unit at 128 bytes a clock.)
 //   MMA         (a warp per tile) scores S = Q K^T (FP32, tensor memory), then, when the tile's softmax is done, O += P V with
-//               the softmax weights P read from tensor memory, where they replace the second half of their scores; one tile's
+//               the softmax weights P read from tensor memory, where they and their remainders replace their scores; one tile's
 //               products run while the other's softmax does. (One warp for both tiles needed more time to issue the
 //               instructions, among three other busy warps of its scheduler, than the tensor cores to execute them.)
 //   softmax     (2 x 4 warps) a thread per row: maximum, weights, sum; the weights go back to tensor memory as FP16, times the
@@ -17,13 +17,16 @@
 //               A row's reference M is the largest such product that it has seen, as a power of two, so a block counts by what
 //               it adds to the row and not by its scale: a large scale under a small weight does not push the others out of
 //               FP16's range. M moves only when it is passed by 2^8, so O is rescaled rarely; products are held as 2^7 times
-//               what they are next to M, FP16's whole range. What lies 2^-40 below M only enters the sum.
+//               what they are next to M, FP16's whole range. What lies 2^-40 below M only enters the sum. A unit's first page is
+//               handed over before the second's weights are worked out (chunks of head dimension 128 397 -> 363 us). The sum and the largest
+//               weight have a reference of their own, since M may lie 2^126 above or below it.
 // 128 keys per step because an MMA of 128 rows x 64 keys reads 6 KB of operands for 32 clocks of work, more than shared memory
-// gives: with units of 64 keys the MMAs took 3200 of 3900 clocks per 64 keys (head dimension 128, SPLIT). With a head dimension
-// of 128 the tensor cores and the 16 exponentials per clock of an SM take about the same time, with 64 the exponentials take
-// twice as long. Queries are rounded to FP16 (a power of two per row keeps them in range); where the result is FP16 too the
-// rounding would show next to the result's own, and a second product with the remainders (SPLIT) removes it. Weights are rounded
-// to FP16 (relative 2^-12, or 2^-32 of the row's M).
+// gives: with units of 64 keys the MMAs took 3200 of 3900 clocks per 64 keys (head dimension 128). Queries (a power of two per row
+// keeps them in range) and products of weight and scale are an FP16 number and what is left of it as another, each with an MMA of
+// its own, so both keep 22 bits as in kv8_decode.cu, whichever kernel a step gets. As FP16 numbers alone
+// the weights cost 1.4 times the result's own rounding in FP16 results (2.9e-4 for 2.1e-4 against 64 bits); prompts of head dimension 64
+// took 207 us instead of 235, chunks of dimension 128 and FP16 (queries in two parts) 321 instead of 358. Below FP16's normal numbers
+// 2^-32 of the row's M is kept.
 //
 // Every wait is bounded: on expiry the status word tells, all roles leave, and the CTA ends.
 #include <algorithm>
@@ -37,22 +40,24 @@ constexpr int STATUS_KV8_PROMPT = 512;       // gave up waiting at a barrier of 
 constexpr int KP_ROWS = 128, KP_CTA_ROWS = 256;
 constexpr int KP_SOFTMAX_WARPS = 8, KP_CONVERT_WARPS = 4;
 constexpr int KP_THREADS = 512;              // and two MMA warps and two that only help with the queries
-// Registers per thread: a softmax thread holds its row's 128 scores. 256 x 176 + 256 x 80 = 512 x 128, what the launch has.
-constexpr int KP_SOFTMAX_REGS = 176, KP_OTHER_REGS = 80;
+// Registers per thread: a softmax thread holds its row's 128 scores, a converter DH / 8 words of codes (4 x 2048 tokens of head
+// dimension 64: 253 us with 176 and 80, 241 so; three chunks of dimension 128 with 184 and 72 the same time, with 192 and 64 16 us more).
+// Together 512 x 128, what the launch has.
+template <int DH> constexpr int KP_SOFTMAX_REGS = DH == 64 ? 192 : 176;
+template <int DH> constexpr int KP_OTHER_REGS = 256 - KP_SOFTMAX_REGS<DH>;
 
 constexpr int KP_KEYS = 2 * KV8_BLOCK;       // keys of a unit
 
-// Operand stages of keys and values (of a unit each), by what shared memory holds.
-template <int DH, bool SPLIT> struct PromptShape {
-    static constexpr int KS = 2, VS = DH == 128 && SPLIT ? 1 : 2;
+// Operand stages of keys and values (of a unit each), by what shared memory holds next to the queries and their remainders.
+template <int DH> struct PromptShape {
+    static constexpr int KS = 2, VS = DH == 128 ? 1 : 2;
     static constexpr int Q = 2 * KP_ROWS * DH * 2, K = KP_KEYS * DH * 2;
-    static constexpr int BYTES = (SPLIT ? 2 : 1) * Q + (KS + VS) * K;
+    static constexpr int BYTES = 2 * Q + (KS + VS) * K;
 };
 constexpr int KP_AHEAD = 4;                  // units between a page's request to L2 and its use
-// Exponents of two: products of weight and value scale are held times 2^KP_RANGE / M (they pass M by 2^8 at most, so 2^15 fits FP16),
-// sums of weights times 2^KP_SUM / M (between 2^-81 and 2^100 with value scales up to 2^121 and 2^20 keys); products below 2^-KP_NOTHING
-// M count as nothing. An output is the quotient of the two times KP_GAIN = 2^(KP_SUM - KP_RANGE).
-constexpr float KP_RANGE = 7.f, KP_SUM = 40.f, KP_NOTHING = 40.f, KP_GAIN = 8589934592.f;
+// Exponents of two: products of weight and value scale are held times 2^KP_RANGE / M (they pass M by 2^8 at most, so 2^15 fits FP16);
+// those below 2^-KP_NOTHING M count as nothing.
+constexpr float KP_RANGE = 7.f, KP_NOTHING = 40.f;
 
 struct Kv8Prompt {
     Kv8Attention a;
@@ -134,6 +139,12 @@ __device__ __forceinline__ float max3(float x, float y, float z) {
     asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
     return r;
 }
+// A pair as FP16 numbers, cut off.
+__device__ __forceinline__ uint32_t cut_half(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
 __device__ __forceinline__ float log2_approx(float x) {
     float y;
     asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -154,13 +165,13 @@ __device__ __forceinline__ void convert16(const uint4 &w, uint8_t *operand, int 
     *reinterpret_cast<uint4 *>(operand + swizzled(row, 2 * q + 1)) = b;
 }
 
-template <int DH, bool BF16, bool SPLIT>
+template <int DH, bool BF16>
 __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prompt_kernel(const b200q_kv8_cache c, const Kv8Prompt p) {
-    using Shape = PromptShape<DH, SPLIT>;
+    using Shape = PromptShape<DH>;
     constexpr int KS = Shape::KS, VS = Shape::VS, SLABS = DH / 64, HALF_PAGE = KV8_BLOCK * DH;
     constexpr int K_SLAB = KP_KEYS * 128, V_PAGE = DH * 128;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ __align__(8) uint64_t k_full[KS], k_free[KS], v_full[VS], v_free[VS], s_full[2], p_full[2], o_done[2], q_full;
+    __shared__ __align__(8) uint64_t k_full[KS], k_free[KS], v_full[VS], v_free[VS], s_full[2], p_full[2][2], o_done[2], q_full;
     __shared__ uint32_t tmem_base_slot;
     __shared__ volatile int abort_flag;
     __shared__ float factor_s[KP_CTA_ROWS];
@@ -217,7 +228,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prompt_kernel(const b200q_k
     const int full_pages = total / KV8_BLOCK;    // the block after them is the tail, what follows does not exist
 
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint8_t *q_s = smem, *k_s = smem + (SPLIT ? 2 : 1) * Shape::Q, *v_s = k_s + KS * Shape::K;
+    uint8_t *q_s = smem, *k_s = smem + 2 * Shape::Q, *v_s = k_s + KS * Shape::K;
     if (tid == 0) {
         for (int s = 0; s < KS; ++s) {
             mbar_init(&k_full[s], KP_CONVERT_WARPS);
@@ -229,7 +240,8 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prompt_kernel(const b200q_k
         }
         for (int t = 0; t < 2; ++t) {
             mbar_init(&s_full[t], 1);
-            mbar_init(&p_full[t], 4);
+            mbar_init(&p_full[t][0], 4);
+            mbar_init(&p_full[t][1], 4);
             mbar_init(&o_done[t], 1);
         }
         mbar_init(&q_full, KP_THREADS / 32);
@@ -247,7 +259,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prompt_kernel(const b200q_k
     // a CTA here still needs it.
     chain_trigger();
     const uint32_t tmem = tmem_base_slot;                    // (all 512 columns: 0)
-    const uint32_t S_COL = 0, P_COL = 64, O_COL = 256;       // per tile: S 128 columns, P the second 64 of them, O DH columns
+    const uint32_t S_COL = 0, P_COL = 64, O_COL = 256;       // per tile: S 128 columns (then the remainders of P, and P from column 64), O DH columns
     // the whole warp: false once anybody has given up
     auto wait = [&](uint64_t *bar, uint32_t parity) -> bool {
         bool ok = mbar_try_wait(bar, parity);
@@ -265,7 +277,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prompt_kernel(const b200q_k
     constexpr int MMA = KP_SOFTMAX_WARPS + KP_CONVERT_WARPS;
     {
         // ---- queries, by all warps: DH / 8 lanes hold four dimensions of a row and their partners; the largest
-        // magnitude, then FP16 (and remainders) relative to its power of two
+        // magnitude, then FP16 numbers and remainders relative to its power of two
         constexpr int HALF = DH / 2, LANES = DH / 8, AT_ONCE = 32 / LANES, WARPS = KP_THREADS / 32, STEPS = (KP_CTA_ROWS / AT_ONCE + WARPS - 1) / WARPS;
         const int i = lane % LANES * 4;
 #pragma unroll 3
@@ -309,7 +321,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prompt_kernel(const b200q_k
                     split_half(x[h][2] * inv, x[h][3] * inv, hi[1], lo[1]);
                     uint8_t *to = q_to + (d / 64) * (KP_ROWS * 128) + swizzled(local % KP_ROWS, d % 64 / 8) + d % 8 * 2;
                     *reinterpret_cast<uint2 *>(to) = make_uint2(hi[0], hi[1]);
-                    if (SPLIT) *reinterpret_cast<uint2 *>(to + Shape::Q) = make_uint2(lo[0], lo[1]);
+                    *reinterpret_cast<uint2 *>(to + Shape::Q) = make_uint2(lo[0], lo[1]);
                 }
             }
         }
@@ -319,7 +331,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prompt_kernel(const b200q_k
     }
 
     if (warp >= MMA) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(KP_OTHER_REGS));
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(KP_OTHER_REGS<DH>));
         if (warp < MMA + 2) {
         // ---- MMAs of tile t (the whole warp walks the loop, one elected lane issues). Units that the tile does not need are
         // released as they come.
@@ -327,7 +339,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prompt_kernel(const b200q_k
         const int t = warp - MMA, mine = t ? count1 : count0;
         const uint64_t any_desc = smem_desc_sw128(smem);
         const uint32_t hi = static_cast<uint32_t>(any_desc >> 32), lo = static_cast<uint32_t>(any_desc);
-        const uint32_t q_lo = lo + t * (Shape::Q / 2 >> 4), k_lo = lo + ((SPLIT ? 2 : 1) * Shape::Q >> 4), v_lo = k_lo + (KS * Shape::K >> 4);
+        const uint32_t q_lo = lo + t * (Shape::Q / 2 >> 4), k_lo = lo + (2 * Shape::Q >> 4), v_lo = k_lo + (KS * Shape::K >> 4);
         const uint32_t s_at = tmem + S_COL + 128 * t, o_at = tmem + O_COL + DH * t;
         auto scores = [&](int i) {
             const int s = i % KS;
@@ -335,7 +347,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prompt_kernel(const b200q_k
             if (elect_one()) {
                 if (i < mine) {
 #pragma unroll
-                    for (int part_q = 0; part_q < (SPLIT ? 2 : 1); ++part_q)
+                    for (int part_q = 0; part_q < 2; ++part_q)
 #pragma unroll
                         for (int k = 0; k < DH / 16; ++k)
                             umma_f16_ss(s_at, q_lo + ((part_q * Shape::Q + (k / 4) * (KP_ROWS * 128)) >> 4) + 2 * (k % 4),
@@ -348,17 +360,20 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prompt_kernel(const b200q_k
             }
             __syncwarp();
         };
-        auto values = [&](int i) {
+        // (the products of the first page's keys run while the second page's weights are worked out)
+        auto values = [&](int i, int page) {
             const int s = i % VS;
-            const uint32_t vd = v_lo + s * (Shape::K >> 4);
+            const uint32_t vd = v_lo + s * (Shape::K >> 4) + page * (V_PAGE >> 4);
             if (elect_one()) {
                 if (i < mine) {
 #pragma unroll
-                    for (int k = 0; k < 8; ++k)
-                        umma_f16_ts(o_at, s_at + P_COL + 8 * k, vd + (((k / 4) * V_PAGE) >> 4) + 2 * (k % 4), hi, o_idesc, k > 0 ? 1u : i > 0);
-                    if (i + 1 == mine) umma_commit<false>(smem_u32(&o_done[t]));
-                    umma_commit<false>(smem_u32(&v_free[s]));
-                } else {
+                    for (int k = 0; k < 4; ++k) {
+                        umma_f16_ts(o_at, s_at + P_COL + 32 * page + 8 * k, vd + 2 * k, hi, o_idesc, i + page + k > 0);
+                        umma_f16_ts(o_at, s_at + 32 * page + 8 * k, vd + 2 * k, hi, o_idesc, 1u);
+                    }
+                    if (page && i + 1 == mine) umma_commit<false>(smem_u32(&o_done[t]));
+                    if (page) umma_commit<false>(smem_u32(&v_free[s]));
+                } else if (page) {
                     mbar_arrive(&v_free[s]);
                 }
             }
@@ -369,10 +384,14 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prompt_kernel(const b200q_k
         if (fine) scores(0);
         for (int i = 0; fine && i < count; ++i) {
             const int next = i + 1;
-            fine = wait(&v_full[i % VS], (i / VS) & 1) && (i >= mine || wait(&p_full[t], i & 1));
+            fine = wait(&v_full[i % VS], (i / VS) & 1);
+            for (int page = 0; fine && page < 2; ++page) {
+                fine = i >= mine || wait(&p_full[t][page], i & 1);
+                if (!fine) break;
+                tc_fence_after();
+                values(i, page);
+            }
             if (!fine) break;
-            tc_fence_after();
-            values(i);
             if (next == count) break;
             fine = wait(&k_full[next % KS], (next / KS) & 1);
             if (!fine) break;
@@ -382,7 +401,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prompt_kernel(const b200q_k
         }
     } else if (warp >= KP_SOFTMAX_WARPS) {
         // ---- converters
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(KP_OTHER_REGS));
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(KP_OTHER_REGS<DH>));
         const int ct = tid - KP_SOFTMAX_WARPS * 32;
         const size_t tail = kv8_unit(slot, c.layers, a.layer, 0, c.kv_heads, kvh);
         const uint16_t *tail_k = static_cast<const uint16_t *>(c.tail) + tail * HALF_PAGE, *tail_v = tail_k + static_cast<size_t>(c.kv_heads) * HALF_PAGE;
@@ -499,13 +518,13 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prompt_kernel(const b200q_k
         }
     } else {
         // ---- softmax: a thread per row
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(KP_SOFTMAX_REGS));
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(KP_SOFTMAX_REGS<DH>));
         const int t = warp >> 2, local = 32 * (warp & 3) + lane, row = row0 + t * KP_ROWS + local, mine = t ? count1 : count0;
         const bool valid = row < rows;
         const int token = valid ? row / p.group : 0, pos = start + token;
         const size_t out_row = static_cast<size_t>(first + token) * a.heads + kvh * p.group + (valid ? row - token * p.group : 0);
         const uint32_t lanes = static_cast<uint32_t>(32 * (warp & 3)) << 16;
-        float m = -INFINITY, l = 0.f;            // log2 M; the sum of the weights, times 2^KP_SUM / M
+        float m = -INFINITY, l = 0.f, product_m = -INFINITY;     // largest score and sum of the weights relative to it; log2 M
         bool fine = wait(&q_full, 0);
         const float factor = factor_s[t * KP_ROWS + local];
         const float *layer_scales = c.scales + kv8_unit(0, c.layers, a.layer, 0, c.kv_heads, kvh);
@@ -535,13 +554,12 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prompt_kernel(const b200q_k
         }
         for (int i = 0; fine && i < mine; ++i) {
             const int block = 2 * (u0 + i), key0 = block * KV8_BLOCK;
-            float f[2], vs[2], log_scale[2], alpha = 1.f;
+            float f[2], log_scale[2], alpha = 1.f;
             bool sees[2];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const float ks = ks_next[h];
-                vs[h] = vs_next[h];
-                log_scale[h] = log2_approx(vs[h]);
+                log_scale[h] = log2_approx(vs_next[h]);
                 if (i + 1 < mine) scales_at(block + 2 + h, page_next[h], ks_next[h], vs_next[h]);
                 if (i + 2 < mine) page_next[h] = page_at(block + 4 + h);
                 sees[h] = pos >= key0 + h * KV8_BLOCK;
@@ -572,15 +590,17 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prompt_kernel(const b200q_k
 #pragma unroll
                 for (int e = 2; e < 32; e += 2) tops[q] = max3(tops[q], __uint_as_float(s[q][e]), __uint_as_float(s[q][e + 1]));
             }
-            // (where the scales are tiny M stays within 2^-40 of the largest weight, so that the sum has the range; of a block that is
-            // hidden or not finite nothing comes through fmaxf)
+            // (of a block that is hidden or not finite nothing comes through fmaxf)
             const float peak[2] = {fmaxf(tops[0], tops[1]) * f[0], fmaxf(tops[2], tops[3]) * f[1]};
             const float product[2] = {sees[0] ? peak[0] + log_scale[0] : -INFINITY, sees[1] ? peak[1] + log_scale[1] : -INFINITY};
-            const float top = fmaxf(fmaxf(product[0], product[1]), fmaxf(peak[0], peak[1]) - KP_NOTHING);
+            const float top = fmaxf(peak[0], peak[1]), top_product = fmaxf(product[0], product[1]);
             if (top > m + 8.f) {
-                alpha = exp2_approx(m - top);
-                l *= alpha;
+                l *= exp2_approx(m - top);
                 m = top;
+            }
+            if (top_product > product_m + 8.f) {
+                alpha = exp2_approx(product_m - top_product);
+                product_m = top_product;
             }
             if (i > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {            // (S of this unit follows the last value product)
 #pragma unroll 1
@@ -595,41 +615,50 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prompt_kernel(const b200q_k
             }
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const bool nothing = product[h] < m - KP_NOTHING;
-                const float move = !sees[h] ? 0.f : nothing ? -peak[h] : log_scale[h] - m + KP_RANGE;
-                const float weigh = !sees[h] ? 0.f : nothing ? exp2_approx(peak[h] - m + KP_SUM) : __fdividef(KP_GAIN, vs[h]);
+                const bool nothing = product[h] < product_m - KP_NOTHING || log_scale[h] == -INFINITY;
+                const float move = !sees[h] ? 0.f : nothing ? -peak[h] : log_scale[h] - product_m + KP_RANGE;
+                const float weigh = !sees[h] ? 0.f : exp2_approx(-move - m);
                 const uint64_t f2 = pack2(f[h], f[h]), move2 = pack2(move, move);        // pairs: two per instruction
                 uint64_t sums[2] = {0ull, 0ull};
-                uint32_t w[32];
 #pragma unroll
-                for (int e = 0; e < 32; e += 2)
+                for (int q = 0; q < 2; ++q) {
+                    uint32_t w[16], left[16];
 #pragma unroll
-                    for (int q = 0; q < 2; ++q) {
-                        float lo, hi;
+                    for (int e = 0; e < 32; e += 2) {
+                        float lo, hi, lo_left, hi_left;
                         unpack2(fma2(pack2(__uint_as_float(s[2 * h + q][e]), __uint_as_float(s[2 * h + q][e + 1])), f2, move2), lo, hi);
                         lo = exp2_approx(lo);
                         hi = exp2_approx(hi);
-                        sums[q] = add2(sums[q], pack2(lo, hi));
-                        w[16 * q + e / 2] = pack_half(lo, hi);
+                        sums[e / 2 & 1] = add2(sums[e / 2 & 1], pack2(lo, hi));
+                        // (cut off at eleven bits, so that what is left is one exact subtraction)
+                        const float lo_top = __uint_as_float((__float_as_uint(lo) & 0xffffe000u) | 0x80000000u), hi_top = __uint_as_float((__float_as_uint(hi) & 0xffffe000u) | 0x80000000u);
+                        unpack2(add2(pack2(lo, hi), pack2(lo_top, hi_top)), lo_left, hi_left);
+                        w[e / 2] = cut_half(lo, hi);
+                        left[e / 2] = pack_half(lo_left, hi_left);
                     }
-                if (nothing) {
+                    if (__any_sync(0xffffffffu, nothing)) {
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) w[e] = 0u;
+                        for (int e = 0; e < 16; ++e) {
+                            if (nothing) w[e] = left[e] = 0u;
+                        }
+                    }
+                    tmem_st16(at + P_COL + 32 * h + 16 * q, w);
+                    tmem_st16(at + 32 * h + 16 * q, left);
                 }
-                tmem_st32(at + P_COL + 32 * h, w);
                 float lo, hi;
                 unpack2(add2(sums[0], sums[1]), lo, hi);
                 l = fmaf(lo + hi, weigh, l);
+                tmem_st_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&p_full[t][h]);
             }
-            tmem_st_wait();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&p_full[t]);
         }
         // ---- results
         if (mine && fine && wait(&o_done[t], 0)) {
             tc_fence_after();
-            const float gain = p.splits == 1 ? __fdiv_rn(KP_GAIN, l) : 1.f;
+            // (in two factors: M and the largest weight may lie 2^126 apart; a part of which the row sees no key adds nothing)
+            const float half_gain = m == -INFINITY ? 0.f : exp2_approx(0.5f * (product_m - KP_RANGE - m)), gain = p.splits == 1 ? __fdiv_rn(half_gain, l) : half_gain;
             float *to = p.splits == 1 ? nullptr : p.partial + ((static_cast<size_t>(part) * a.rows) * a.heads + out_row) * (DH + 2);
 #pragma unroll 1
             for (int d = 0; d < DH; d += 32) {
@@ -639,7 +668,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prompt_kernel(const b200q_k
                 if (!valid) continue;
                 float v[32];
 #pragma unroll
-                for (int e = 0; e < 32; ++e) v[e] = __uint_as_float(o[e]) * gain;
+                for (int e = 0; e < 32; ++e) v[e] = __uint_as_float(o[e]) * half_gain * gain;
                 if (p.splits == 1) {
                     uint4 *out = reinterpret_cast<uint4 *>(static_cast<uint16_t *>(a.out) + out_row * DH + d);
 #pragma unroll
@@ -714,15 +743,15 @@ __global__ void __launch_bounds__(256) kv8_prompt_join_kernel(const b200q_kv8_ca
         for (int e = 0; e < DH / 32; ++e) value[e] += f * from[lane + 32 * e];
     }
 #pragma unroll
-    for (int e = 0; e < DH / 32; ++e) store_from_float(a.out, c.dtype, at * DH + lane + 32 * e, value[e] / weight * KP_GAIN);
+    for (int e = 0; e < DH / 32; ++e) store_from_float(a.out, c.dtype, at * DH + lane + 32 * e, value[e] / weight);
 }
 
 // ----------------------------------------------------------------------------------------------------------- host side
 // Parts of the keys, and the time that is estimated for them, in us: CTAs (one per SM; where they do not all start at once, half a
 // CTA's time is lost at the end), each with its beginning and end and its units, and, for more than one part, the results on their way
-// through memory and the joining kernel. Measured for a head dimension of 128: 18 us for one CTA with one tile of rows and four
-// units, 27 with two tiles. 128 CTAs of 63 units (16 sequences of 8000 keys) took 218 us in three parts, so in three rounds, and
-// take 196 in one; 32 of 32 units 87 in eight parts, 59 in four. A further part has to gain a twentieth: three instead of two for
+// through memory and the joining kernel. Measured with one CTA per SM for a head dimension of 128: 25 us for one tile of rows and four
+// units, 31 with two tiles, 37 and 48 for eight units. 128 CTAs of 63 units (16 sequences of 8000 keys) took 218 us in three parts, so in three rounds, when they
+// took 196 in one (215 since the weights have remainders); 32 of 32 units 87 in eight parts, 59 in four. A further part has to gain a twentieth: three instead of two for
 // the 192 CTAs of three chunks of 512 tokens behind up to 16000 took 369 us instead of 336.
 struct PromptPlan {
     int splits;
@@ -732,7 +761,7 @@ static PromptPlan prompt_plan(const b200q_kv8_cache *c, int heads, int batch, in
     const long long list = static_cast<long long>(max_new) * (heads / c->kv_heads), units = (max_keys + KP_KEYS - 1) / KP_KEYS;
     const double ctas = static_cast<double>((list + KP_CTA_ROWS - 1) / KP_CTA_ROWS) * c->kv_heads * batch / sm_count();      // per SM
     const bool two = list > KP_ROWS, wide = c->head_dim == 128;
-    const double once = two ? (wide ? 10. : 7.7) : (wide ? 5.5 : 4.6), unit = two ? (wide ? 4.2 : 3.) : (wide ? 3.1 : 2.2);
+    const double once = two ? (wide ? 10.5 : 8.1) : (wide ? 5.7 : 4.8), unit = two ? (wide ? 5.2 : 3.7) : (wide ? 3.7 : 3.);
     const double part_bytes = 2. * rows * heads * (c->head_dim + 2) * 4.;
     PromptPlan best{1, 0.};
     for (int s = 1; s <= std::min(64ll, std::max(1ll, units / 2)); ++s) {
@@ -772,10 +801,9 @@ int kv8_prompt(const b200q_kv8_cache *c, const Kv8Attention &a, int max_new, int
     if (a.batch > 65535 || blocks > 65535 || across > 0x7fffffffll || joins > 0x7fffffffll || static_cast<long long>(max_new) * p.group > 0x40000000ll)
         return fail(B200Q_EUNSUPPORTED, "kv8_attention: too many rows");
     const bool bf16 = c->dtype == B200Q_BF16;
-    auto kernel = c->head_dim == 64 ? (bf16 ? kv8_prompt_kernel<64, true, false> : kv8_prompt_kernel<64, false, true>)
-                                    : (bf16 ? kv8_prompt_kernel<128, true, false> : kv8_prompt_kernel<128, false, true>);
-    const int smem = 1024 + (c->head_dim == 64 ? (bf16 ? PromptShape<64, false>::BYTES : PromptShape<64, true>::BYTES)
-                                               : (bf16 ? PromptShape<128, false>::BYTES : PromptShape<128, true>::BYTES));
+    auto kernel = c->head_dim == 64 ? (bf16 ? kv8_prompt_kernel<64, true> : kv8_prompt_kernel<64, false>)
+                                    : (bf16 ? kv8_prompt_kernel<128, true> : kv8_prompt_kernel<128, false>);
+    const int smem = 1024 + (c->head_dim == 64 ? PromptShape<64>::BYTES : PromptShape<128>::BYTES);
     if (int rc = allow_large_shared_memory(reinterpret_cast<const void *>(kernel))) return rc;
     launch_chained(kernel, dim3(static_cast<unsigned>(across), a.batch, static_cast<unsigned>(blocks)), dim3(KP_THREADS), smem, stream, *c, p);
     if (int rc = check_launch("kv8_attention")) return rc;

@@ -20,11 +20,11 @@ and the ``read_*`` helpers waits for it, and a step whose ``batch`` is kept can 
 ``max_length``, a fork onto a slot that is not empty - changes nothing and sets the device status word (``_lib.device_status``:
 501, 502, 503); the rows of a refused step are NaN. Calls on one cache have to be ordered by their streams.
 
-A key or value that is not finite (in the cache's type) makes its block (its 64 tokens, of its head and layer) NaN, and with it every row that sees
-the block. Scores, softmax statistics and sums are FP32, and
-the codes enter the products exactly. Steps of few tokens keep 22 bits of queries and softmax weights (an FP16 number and its
-remainder); prompts and chunks round weights, and for BF16 caches queries, to FP16 (relative 2^-12, each row of queries scaled
-by a power of two). Which of the two kernels a step takes follows from an estimate of their times.
+A key or value that is not finite (in the cache's type) makes its block (its 64 tokens, of its head and layer) NaN, and with it
+every row that sees the block. Scores, softmax statistics and sums are FP32, and the codes enter the products exactly. Queries and
+softmax weights enter them with 22 bits (an FP16 number and its remainder), whichever of two kernels a step takes, which follows
+from an estimate of their times. Below that a weight is lost where weight times value lies 2^-32 below the row's largest (single tokens: weights
+2^-24 below the largest); values of the tail are held to 2^-24 of the largest magnitude among them.
 """
 
 import ctypes

@@ -1,9 +1,9 @@
 """What the attention over the paged 8-bit cache keeps of small contributions, against 64-bit arithmetic on the cache's content.
 
 The bounds count what the kernels round. With S = scale * sum |q_i k_i|, p the exact softmax weights, A = sum of p |v| and V the
-largest p times the block's value scale: a score (products of exact codes and of queries, FP32 sums, the rotation) is off by at
-most d = 2^-19 (1 + S) and 2^-11 S more where queries are rounded to FP16, so a weight by a factor within exp(+-2 d); the rounding of a weight
-is relative to it, and 2^-31 * 127 V at most below FP16's normal numbers; the result is rounded to the cache's type (half a step)."""
+largest p times the block's value scale: a score (products of exact codes and of queries of 22 bits, FP32 sums, the rotation)
+is off by at most d = 2^-19 (1 + S), so a weight by a factor within exp(+-2 d); weights keep 22 bits (2^-20 with their factor and
+their sum), and 2^-31 * 127 V below FP16's normal numbers; the result is rounded to the cache's type (half a step)."""
 
 import math
 
@@ -49,11 +49,11 @@ def exact(torch, cache, layer, q, sizes, counts, scale):
     return [torch.cat(t) for t in zip(*out)]
 
 
-def check(torch, cache, layer, q, out, sizes, counts, scale, relative, query_rounding=0.0):
+def check(torch, cache, layer, q, out, sizes, counts, scale):
     want, a, big, v, total = exact(torch, cache, layer, q, sizes, counts, scale)
     kind = torch.finfo(out.dtype)
-    d = 2.0 ** -19 * (1 + big) + query_rounding * big
-    bound = (torch.exp(2 * d) - 1 + relative) * a + total * 2.0 ** -31 * 127 * v + kind.eps / 2 * 1.01 * want.abs() + kind.tiny * kind.eps
+    d = 2.0 ** -19 * (1 + big)
+    bound = (torch.exp(2 * d) - 1 + 2.0 ** -20) * a + total * 2.0 ** -31 * 127 * v + kind.eps / 2 * 1.01 * want.abs() + kind.tiny * kind.eps
     got = out.double().reshape(want.shape)
     assert torch.isfinite(got).all()
     off = ((got - want).abs() / bound).max()
@@ -99,7 +99,7 @@ def test_large_value_scales_under_small_weights(cuda, dtype, heads, kv_heads, dh
     cache = levelled_cache(torch, sizes, kv_heads, dh, dtype, levels, value_scales, 1)
     q = torch.ones(sum(counts), heads * dh, device="cuda", dtype=getattr(torch, dtype))
     out = cache.attention(0, q, step(cache, sizes, counts), scale=1 / dh)
-    check(torch, cache, 0, q, out, sizes, counts, 1 / dh, 2.0 ** -11)
+    check(torch, cache, 0, q, out, sizes, counts, 1 / dh)
 
 
 @pytest.mark.parametrize("scale", [0.0, 2.0 ** -126, 2.0 ** -60, 2.0 ** -30, 2.0 ** 60, 2.0 ** 100])
@@ -116,8 +116,40 @@ def test_value_scales_of_any_size(cuda, scale, counts):
         if not mixed:
             cache.tail[0, 0, 1, :, :52] *= 0.0 if scale == 0 else scale
             cache.peak[0, 0, 1] = cache.tail[0, 0, 1, :, :52].float().abs().amax((-1, -2))
-        q = query(torch, counts[0], 4 * 64, "bfloat16", 3)
+        q = query(torch, counts[0], 32 * 64, "bfloat16", 3)
         out = cache.attention(0, q, step(cache, [500], counts))
         if scale == 0 and not mixed:
             assert not out.any()
-        check(torch, cache, 0, q, out, [500], counts, 0.125, 2.0 ** -11, 2.0 ** -11)
+        check(torch, cache, 0, q, out, [500], counts, 0.125)
+
+
+@pytest.mark.parametrize("dtype,q_dtype", [("bfloat16", "float32"), ("float16", "float32"), ("float16", "float16")])
+@pytest.mark.parametrize("heads,kv_heads,dh", [(96, 6, 64), (96, 6, 128)])
+@pytest.mark.parametrize("pairs,count", [(1, 1), (20, 1), (200, 1), (1, 9), (1, 63), (4, 50), (10, 33), (16, 63), (40, 60)])
+def test_weights_and_queries_keep_22_bits(cuda, dtype, q_dtype, heads, kv_heads, dh, pairs, count):
+    """Pairs of blocks whose contributions cancel, so that neither the result's rounding nor an average hides what is lost: the
+    queries lie between two FP16 numbers, the weights anywhere. (The tokens behind them have values of zero.)"""
+    torch = cuda
+    size = 128 * pairs + count
+    cache = random_cache(torch, [size], 1, kv_heads, dh, dtype, pairs + count)
+    gen = torch.Generator().manual_seed(pairs)
+    cache.codes[:, :, 0] = 64
+    cache.codes[:, :, 1] = 100
+    cache.tail[0, 0, 1, :, :count] = 0
+    cache.peak[0, 0, 1] = 0
+    cache.tail[0, 0, 0, :, :count] = 0.125
+    cache.peak[0, 0, 0] = 0.125
+    level = 1.0 + 2.0 ** -12 if q_dtype == "float32" else 1.0
+    q = torch.full((count, heads * dh), level, device="cuda", dtype=getattr(torch, q_dtype))
+    keys = torch.rand(2 * pairs, kv_heads, generator=gen).float() * 0.5 / 64              # a block's keys score 64 times that
+    values = torch.rand(2 * pairs, kv_heads, generator=gen).float() * 0.5 + 0.5
+    scores = keys.double() * 64 * level
+    values[1::2] = (values[::2].double() * torch.exp(scores[::2] - scores[1::2]) * 100 / 64).float()
+    pages = cache.table[0, :2 * pairs].long()
+    cache.scales[pages, 0, 0] = keys.cuda()
+    cache.scales[pages, 0, 1] = values.cuda()
+    cache.codes[pages[1::2], 0, 1] = -64                                        # (as large a product as 100, by another weight)
+    out = cache.attention(0, q, step(cache, [size], [count]), scale=1 / dh)
+    want = exact(torch, cache, 0, q, [size], [count], 1 / dh)
+    assert (want[0].abs() <= 2.0 ** -20 * want[1]).all()                        # they do cancel
+    check(torch, cache, 0, q, out, [size], [count], 1 / dh)
