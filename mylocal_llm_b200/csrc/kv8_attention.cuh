@@ -12,7 +12,8 @@
 //
 // The instruction has sixteen rows. Where memory bounds the kernel a tile is eight rows of queries: rows 0..7 hold the FP16
 // parts of queries and softmax weights, rows 8..15 what is left of them, again as FP16, and the two results are added. That
-// keeps 22 bits of both for no additional instruction.
+// keeps 22 bits of both for no additional instruction, down to FP16's smallest normal number (rows of queries and weights are scaled
+// to the top of its range).
 #pragma once
 
 #include "kv8_cache.cuh"

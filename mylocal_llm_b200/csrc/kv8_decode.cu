@@ -26,6 +26,11 @@ template <int DH, int RT, int MODE> struct DecodeShape {
     static constexpr int CTAS = MODE == CUT ? 2 : 1, WARPS = (RT == 1 ? 12 : 8) / CTAS, STAGES = DH == 64 ? 2 : 1;
 };
 
+// Weights pass the tensor cores times 2^15, so that the largest one is at the top of FP16's range: a number and its remainder then
+// keep 22 bits down to 2^-29 of it and 2^-40 of it below. (At 1 the many small weights behind a dominant key lost theirs, up to all:
+// 131071 keys at 2^-25 of it are 0.4 % of the result.) The factor is taken off with the block's value scale and in the sum.
+constexpr float KV8_WEIGHT_RANGE = 15.f, KV8_WEIGHT_UNIT = 1.f / 32768.f;
+
 struct Kv8Decode {
     Kv8Attention a;
     int group, tiles;             // query heads per key/value head; lists of 8 RT rows (tokens x heads of the group) per head
@@ -300,17 +305,18 @@ __global__ void __launch_bounds__(DecodeShape<DH, RT, MODE>::WARPS * 32, DecodeS
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
                     top = fmaxf(m[r], top * f);              // (f >= 0)
                     const float shift = top == -INFINITY ? 0.f : top;        // (no key seen yet: weights are 0)
+                    const float move = KV8_WEIGHT_RANGE - shift;
                     alpha[r] = exp2_approx(m[r] - shift);
                     moved |= alpha[r] != 1.f;
                     m[r] = top;
                     float sum = 0.f;
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
-                        const float p0 = exp2_approx(fmaf(x[j][0], f, -shift)), p1 = exp2_approx(fmaf(x[j][1], f, -shift));
+                        const float p0 = exp2_approx(fmaf(x[j][0], f, move)), p1 = exp2_approx(fmaf(x[j][1], f, move));
                         sum += p0 + p1;
                         split_half(p0, p1, pf[r][j >> 1][2 * (j & 1)], pf[r][j >> 1][2 * (j & 1) + 1]);
                     }
-                    l[r] = l[r] * alpha[r] + sum;
+                    l[r] = fmaf(sum, KV8_WEIGHT_UNIT, l[r] * alpha[r]);
                 }
                 if (__any_sync(0xffffffffu, moved)) {        // a maximum moved: rarely, after the first pages
 #pragma unroll
@@ -323,7 +329,7 @@ __global__ void __launch_bounds__(DecodeShape<DH, RT, MODE>::WARPS * 32, DecodeS
                 // ---- values, four tiles at a time (a block that a row does not see leaves it alone, even where its values are
                 // not finite)
                 arrived(1, st, v_phases);
-                if (gave_up) vscale = kv8_nan();
+                vscale = gave_up ? kv8_nan() : vscale * KV8_WEIGHT_UNIT;
                 auto add = [&](int i, const float (&v)[RT][4][4]) {
 #pragma unroll
                     for (int r = 0; r < RT; ++r)

@@ -16,7 +16,7 @@
 //               block's value scale (its logarithm is an addend of the exponent, which costs nothing; the sum is divided by it).
 //               A row's reference M is the largest such product that it has seen, as a power of two, so a block counts by what
 //               it adds to the row and not by its scale: a large scale under a small weight does not push the others out of
-//               FP16's range. M moves only when it is passed by 2^8, so O is rescaled rarely; products are held as 2^7 times
+//               FP16's range. M moves only when it is passed by 2^4, so O is rescaled rarely; products are held as 2^11 times
 //               what they are next to M, FP16's whole range. What lies 2^-40 below M only enters the sum. A unit's first page is
 //               handed over before the second's weights are worked out (chunks of head dimension 128 397 -> 363 us). The sum and the largest
 //               weight have a reference of their own, since M may lie 2^126 above or below it.
@@ -25,8 +25,8 @@
 // keeps them in range) and products of weight and scale are an FP16 number and what is left of it as another, each with an MMA of
 // its own, so both keep 22 bits as in kv8_decode.cu, whichever kernel a step gets. As FP16 numbers alone
 // the weights cost 1.4 times the result's own rounding in FP16 results (2.9e-4 for 2.1e-4 against 64 bits); prompts of head dimension 64
-// took 207 us instead of 235, chunks of dimension 128 and FP16 (queries in two parts) 321 instead of 358. Below FP16's normal numbers
-// 2^-32 of the row's M is kept.
+// took 207 us instead of 235, chunks of dimension 128 and FP16 (queries in two parts) 321 instead of 363. Below FP16's normal numbers
+// 2^-36 of the row's M is kept.
 //
 // Every wait is bounded: on expiry the status word tells, all roles leave, and the CTA ends.
 #include <algorithm>
@@ -55,9 +55,10 @@ template <int DH> struct PromptShape {
     static constexpr int BYTES = 2 * Q + (KS + VS) * K;
 };
 constexpr int KP_AHEAD = 4;                  // units between a page's request to L2 and its use
-// Exponents of two: products of weight and value scale are held times 2^KP_RANGE / M (they pass M by 2^8 at most, so 2^15 fits FP16);
-// those below 2^-KP_NOTHING M count as nothing.
-constexpr float KP_RANGE = 7.f, KP_NOTHING = 40.f;
+// Exponents of two: products of weight and value scale are held times 2^KP_RANGE / M and pass M by 2^KP_SLACK at most, which uses
+// FP16's range up to 2^15; those below 2^-KP_NOTHING M count as nothing. (Ranges of 7, 11 and 13: 235, 235 and 240 us for 4 x 2048 tokens of
+// head dimension 64, 358, 363 and 370 for three chunks of dimension 128: more room below, O rescaled more often.)
+constexpr float KP_RANGE = 11.f, KP_SLACK = 15.f - KP_RANGE, KP_NOTHING = 40.f;
 
 struct Kv8Prompt {
     Kv8Attention a;
@@ -598,7 +599,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prompt_kernel(const b200q_k
                 l *= exp2_approx(m - top);
                 m = top;
             }
-            if (top_product > product_m + 8.f) {
+            if (top_product > product_m + KP_SLACK) {
                 alpha = exp2_approx(product_m - top_product);
                 product_m = top_product;
             }

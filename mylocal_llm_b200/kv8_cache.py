@@ -23,8 +23,9 @@ and the ``read_*`` helpers waits for it, and a step whose ``batch`` is kept can 
 A key or value that is not finite (in the cache's type) makes its block (its 64 tokens, of its head and layer) NaN, and with it
 every row that sees the block. Scores, softmax statistics and sums are FP32, and the codes enter the products exactly. Queries and
 softmax weights enter them with 22 bits (an FP16 number and its remainder), whichever of two kernels a step takes, which follows
-from an estimate of their times. Below that a weight is lost where weight times value lies 2^-32 below the row's largest (single tokens: weights
-2^-24 below the largest); values of the tail are held to 2^-24 of the largest magnitude among them.
+from an estimate of their times. Below FP16's normal numbers
+2^-36 of a row's largest product of weight and value scale is kept in steps of many tokens, 2^-40 of its largest weight in steps
+of few; values of the tail are held to 2^-24 of the largest magnitude among them.
 """
 
 import ctypes

@@ -1,9 +1,10 @@
 """What the attention over the paged 8-bit cache keeps of small contributions, against 64-bit arithmetic on the cache's content.
 
-The bounds count what the kernels round. With S = scale * sum |q_i k_i|, p the exact softmax weights, A = sum of p |v| and V the
-largest p times the block's value scale: a score (products of exact codes and of queries of 22 bits, FP32 sums, the rotation)
-is off by at most d = 2^-19 (1 + S), so a weight by a factor within exp(+-2 d); weights keep 22 bits (2^-20 with their factor and
-their sum), and 2^-31 * 127 V below FP16's normal numbers; the result is rounded to the cache's type (half a step)."""
+The bounds count what the kernels round. With S = scale * sum |q_i k_i|, p the exact softmax weights and A = sum of p |v|: a score
+(products of exact codes and of queries of 22 bits, FP32 sums, the rotation) is off by at most d = 2^-19 (1 + S), so a weight by a
+factor within exp(+-2 d); weights keep 22 bits (2^-20 with their factor and their sum), and below FP16's normal numbers (a step is
+rounded by half of it) 2^-40 of the row's largest weight in steps of single tokens, else 2^-36 of its largest product of weight
+and value scale, per unit of a code; the result is rounded to the cache's type (half a step)."""
 
 import math
 
@@ -26,7 +27,7 @@ def healthy(cuda):
 
 
 def exact(torch, cache, layer, q, sizes, counts, scale):
-    """(result, A, largest S, V, keys) of every row and head in 64 bits, [rows, heads, dh] or [rows, heads, 1]."""
+    """(result, A, largest S, what may be lost below FP16's normal numbers) of every row and head in 64 bits, [rows, heads, dh or 1]."""
     dh, kv_heads = cache.head_dim, cache.kv_heads
     heads, row, out = q.shape[1] // dh, 0, []
     for s, (total, n) in enumerate(zip(sizes, counts)):
@@ -43,17 +44,22 @@ def exact(torch, cache, layer, q, sizes, counts, scale):
         k, v = k[:, None], v[:, None]
         p = torch.softmax((x @ k.transpose(-1, -2) * scale).masked_fill(hidden, -math.inf), -1)
         big = (x.abs() @ k.abs().transpose(-1, -2) * abs(scale)).masked_fill(hidden, 0).amax(-1, keepdim=True)
-        parts = p @ v, p @ v.abs(), big, (p * step_of[:, None, None]).amax(-1, keepdim=True), torch.full_like(big, total)
+        seen, step_of = (~hidden).double(), step_of[:, None, :]
+        if max(counts) == 1:
+            lost = 2.0 ** -39 * p.amax(-1, keepdim=True) * (seen @ v.abs())
+        else:
+            lost = 2.0 ** -35 * (p * step_of[:, :, None]).amax(-1, keepdim=True) * (seen @ (v.abs() / step_of[..., None].clamp_min(1e-300)))
+        parts = p @ v, p @ v.abs(), big, lost
         out.append([t.permute(2, 0, 1, 3).reshape(n, heads, -1) for t in parts])
         row += n
     return [torch.cat(t) for t in zip(*out)]
 
 
 def check(torch, cache, layer, q, out, sizes, counts, scale):
-    want, a, big, v, total = exact(torch, cache, layer, q, sizes, counts, scale)
+    want, a, big, lost = exact(torch, cache, layer, q, sizes, counts, scale)
     kind = torch.finfo(out.dtype)
     d = 2.0 ** -19 * (1 + big)
-    bound = (torch.exp(2 * d) - 1 + 2.0 ** -20) * a + total * 2.0 ** -31 * 127 * v + kind.eps / 2 * 1.01 * want.abs() + kind.tiny * kind.eps
+    bound = (torch.exp(2 * d) - 1 + 2.0 ** -20) * a + lost + kind.eps / 2 * 1.01 * want.abs() + kind.tiny * kind.eps
     got = out.double().reshape(want.shape)
     assert torch.isfinite(got).all()
     off = ((got - want).abs() / bound).max()
@@ -152,4 +158,31 @@ def test_weights_and_queries_keep_22_bits(cuda, dtype, q_dtype, heads, kv_heads,
     out = cache.attention(0, q, step(cache, [size], [count]), scale=1 / dh)
     want = exact(torch, cache, 0, q, [size], [count], 1 / dh)
     assert (want[0].abs() <= 2.0 ** -20 * want[1]).all()                        # they do cancel
+    check(torch, cache, 0, q, out, [size], [count], 1 / dh)
+
+
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("heads,kv_heads,dh,count", [(2, 2, 64, 1), (4, 1, 128, 1), (16, 1, 64, 1), (4, 1, 64, 3), (32, 1, 64, 40)])
+@pytest.mark.parametrize("bits", [18.3, 23.7, 24.4, 25.1])
+def test_many_small_weights_behind_a_dominant_one(cuda, dtype, heads, kv_heads, dh, count, bits):
+    """One key of weight 1 with values of zero, then tens of thousands of keys of nearly equal weights 2^-bits whose values do not
+    average out: they are the result."""
+    torch = cuda
+    size = 64 * 1100 + count
+    cache = random_cache(torch, [size], 1, kv_heads, dh, dtype, 2)
+    pages = cache.table[0, :1100].long()
+    gap = bits * math.log(2)
+    keys = torch.zeros(kv_heads, BLOCK, dh, device="cuda", dtype=torch.int8)
+    keys[:, 0] = 127
+    cache.codes[:, 0, 0] = 0
+    cache.codes[pages[0], 0, 0] = keys.reshape(kv_heads, -1)
+    cache.scales[:, :, 0] = gap / 127
+    values = torch.randint(40, 128, (1100, kv_heads, dh, BLOCK), device="cuda", dtype=torch.int8, generator=torch.Generator("cuda").manual_seed(3))
+    values[0] = 0
+    cache.codes[pages, 0, 1] = values.reshape(1100, kv_heads, -1)
+    cache.scales[:, :, 1] = 2.0 ** 7
+    cache.tail[0, :, :, :, :count] = 0
+    cache.peak[0] = 0
+    q = torch.ones(count, heads * dh, device="cuda", dtype=getattr(torch, dtype))
+    out = cache.attention(0, q, step(cache, [size], [count]), scale=1 / dh)
     check(torch, cache, 0, q, out, [size], [count], 1 / dh)
