@@ -484,7 +484,8 @@ int b200q_expert_ffn_static(const void *gate, int gate_fmt, const void *up, int 
  * arrived per call. head_dim 64 or 128; at most 65536 sequences and 2^20 pages. All of it lives on the device, every call
  * but the sizes of b200q_kv8_compact's new pool is decided there, and calls on one cache have to be ordered by their stream.
  * Device status words of refusals: 501 too few free pages, 502 a sequence would pass max_length (or a slot is out of range),
- * 503 fork / free of slots out of range, of a target named twice, not empty or also a source; of waits that gave up: 511, 512. */
+ * 503 fork / free of slots out of range, of a target named twice, not empty or also a source, 504 a step behind a refused one;
+ * of waits that gave up: 511, 512. */
 typedef struct b200q_kv8_cache {
     int8_t *codes;
     float *scales;
@@ -502,6 +503,11 @@ typedef struct b200q_kv8_cache {
  * impossible nothing changes, every start is -1 and the status word is 501 or 502. */
 int b200q_kv8_extend(const b200q_kv8_cache *cache, const int32_t *slots, const int32_t *offsets, int batch,
                      int32_t *starts, void *stream);
+/* The same for a batch that goes on: `starts` holds those of its step before, and where one of them is -1 - that step was refused -
+ * this one is refused too (status 504, unless the word says why already), so that no sequence goes on without what it was refused. Other negative numbers
+ * stand for a batch that has had no step. */
+int b200q_kv8_extend_after(const b200q_kv8_cache *cache, const int32_t *slots, const int32_t *offsets, int batch,
+                           int32_t *starts, void *stream);
 /* Keys and values of the new tokens of one layer, after b200q_kv8_extend: rows offsets[b] .. offsets[b + 1] - 1 of k and v
  * (FP32, FP16 or BF16, kv_heads * head_dim wide, k_row / v_row elements from row to row) are positions starts[b] .. of
  * slots[b]; at most max_new per sequence. Keys are rotated (rotate-half RoPE, tables [rope_rows][head_dim / 2] FP32 with at

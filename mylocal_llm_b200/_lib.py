@@ -111,6 +111,7 @@ SIGNATURES = {
 
 SIGNATURES.update({
     "b200q_kv8_extend": [_ptr, _ptr, _ptr, _c_int, _ptr, _ptr],
+    "b200q_kv8_extend_after": [_ptr, _ptr, _ptr, _c_int, _ptr, _ptr],
     "b200q_kv8_append": [_ptr, _c_int, _ptr, _ptr, _c_int, _c_i64, _c_i64, _ptr, _ptr, _ptr, _c_int, _c_int, _ptr, _ptr, _c_int,
                          _ptr],
     "b200q_kv8_attention_workspace": [_ptr, _c_int, _c_int, _c_int, _c_int, _c_int],

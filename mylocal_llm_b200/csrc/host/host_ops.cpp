@@ -35,7 +35,7 @@ struct Api {
     FN(residual_rmsnorm); FN(gemv_norm); FN(gemv_norm_supported); FN(router_logits_t); FN(router_topk_ex);
     FN(router_topk_plan_row); FN(shared_gate); FN(moe_plan_ex); FN(moe_token_image_bytes); FN(moe_token_images);
     FN(moe_gate_up); FN(moe_gate_up_images); FN(moe_down); FN(moe_hidden_image_bytes); FN(moe_gate_up_streams); FN(moe_down_streams); FN(moe_hidden_images); FN(moe_down_images); FN(moe_combine); FN(silu_mul); FN(rope_attention);
-    FN(prefill_attention); FN(embed_tokens); FN(int8_quantize); FN(int8_gemm); FN(kv8_extend); FN(kv8_append); FN(kv8_attention);
+    FN(prefill_attention); FN(embed_tokens); FN(int8_quantize); FN(int8_gemm); FN(kv8_extend); FN(kv8_extend_after); FN(kv8_append); FN(kv8_attention);
     FN(kv8_attention_workspace); FN(kv8_fork); FN(kv8_free);
 #undef FN
 } api;
@@ -47,7 +47,7 @@ void bind(const py::dict &addresses, py::object error_type) {
     FN(residual_rmsnorm); FN(gemv_norm); FN(gemv_norm_supported); FN(router_logits_t); FN(router_topk_ex);
     FN(router_topk_plan_row); FN(shared_gate); FN(moe_plan_ex); FN(moe_token_image_bytes); FN(moe_token_images);
     FN(moe_gate_up); FN(moe_gate_up_images); FN(moe_down); FN(moe_hidden_image_bytes); FN(moe_gate_up_streams); FN(moe_down_streams); FN(moe_hidden_images); FN(moe_down_images); FN(moe_combine); FN(silu_mul); FN(rope_attention);
-    FN(prefill_attention); FN(embed_tokens); FN(int8_quantize); FN(int8_gemm); FN(kv8_extend); FN(kv8_append); FN(kv8_attention);
+    FN(prefill_attention); FN(embed_tokens); FN(int8_quantize); FN(int8_gemm); FN(kv8_extend); FN(kv8_extend_after); FN(kv8_append); FN(kv8_attention);
     FN(kv8_attention_workspace); FN(kv8_fork); FN(kv8_free);
 #undef FN
     b200q_error = error_type.release().ptr();
@@ -299,7 +299,7 @@ PyObject *kv8_attention_fast(PyObject *, PyObject *const *args, Py_ssize_t nargs
 }
 FAST_METHOD(kv8_attention);
 
-// kv8_extend(cache, device, slots, offsets, batch, starts); kv8_fork(cache, device, src, dst, count); kv8_free(cache, device, slots,
+// kv8_extend(cache, device, slots, offsets, batch, starts, after); kv8_fork(cache, device, src, dst, count); kv8_free(cache, device, slots,
 // count), arrays as addresses -> True
 template <typename F>
 PyObject *on_cache(PyObject *const *args, F launch) {
@@ -318,13 +318,15 @@ PyObject *on_cache(PyObject *const *args, F launch) {
     END_HANDLE_TH_ERRORS
 }
 PyObject *kv8_extend_fast(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
-    if (nargs != 6) Py_RETURN_NONE;
+    if (nargs != 7) Py_RETURN_NONE;
     return on_cache(args, [&](const b200q_kv8_cache *c, int) {
         const int32_t *slots = pointer<int32_t>(args[2]), *offsets = pointer<int32_t>(args[3]);
         int32_t *starts = pointer<int32_t>(args[5]);
         const int batch = as_int(args[4]);
+        const bool after = args[6] == Py_True;
         py::gil_scoped_release unlocked;
-        CALL(kv8_extend, c, slots, offsets, batch, starts, stream());
+        if (after) CALL(kv8_extend_after, c, slots, offsets, batch, starts, stream());
+        else CALL(kv8_extend, c, slots, offsets, batch, starts, stream());
     });
 }
 FAST_METHOD(kv8_extend);

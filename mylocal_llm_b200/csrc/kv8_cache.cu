@@ -36,10 +36,12 @@ __device__ __forceinline__ int block_prefix(int v, int *total) {
 // Every sequence slots[b] grows by offsets[b + 1] - offsets[b] tokens: it gets a page for each block that becomes full
 // (the lowest free pages, in the order of the requests), starts[b] its length before. All or nothing: without enough pages,
 // or where a sequence would pass max_length, nothing changes, every start is -1 (which the other kernels skip) and the
-// status word tells. One CTA: the work is a prefix sum over the batch and, only when a block becomes full, a pass over the
-// free bits (32 pages per word), so a decode step costs little more than its launch.
+// status word tells. `after`: the batch's starts are those of the step before, and where that was refused this one is too: a
+// program that has not looked must not go on with a sequence that lacks those tokens. One CTA: the work is a prefix sum over the
+// batch and, only when a block becomes full, a pass over the free bits (32 pages per word), so a decode step costs little more
+// than its launch.
 __global__ void __launch_bounds__(EXTEND_THREADS) kv8_extend_kernel(const b200q_kv8_cache c, const int32_t *slots,
-                                                                    const int32_t *offsets, int batch, int32_t *starts,
+                                                                    const int32_t *offsets, int batch, int32_t *starts, int after,
                                                                     int *status) {
     chain_trigger();
     chain_wait();
@@ -49,18 +51,20 @@ __global__ void __launch_bounds__(EXTEND_THREADS) kv8_extend_kernel(const b200q_
     const int tid = threadIdx.x, words = (c.pages + 31) / 32;
     const bool small = batch <= EXTEND_THREADS;
     const uint32_t early = tid < words ? c.free_bits[tid] : 0u;          // the first words are on their way meanwhile
-    int carry = 0, bad = 0, my_slot = 0, my_have = 0, my_add = 0;
+    int carry = 0, bad = 0, my_slot = 0, my_have = 0, my_add = 0;        // bad: the status word
     for (int b0 = 0; b0 < batch; b0 += EXTEND_THREADS) {
         const int b = b0 + tid;
         int need = 0;
         if (b < batch) {
             my_slot = slots[b];
             my_add = offsets[b + 1] - offsets[b];
-            if (my_slot < 0 || my_slot >= c.sequences || my_add < 0) {
-                bad = 1;
+            if (after && starts[b] == KV8_REFUSED) {
+                bad = STATUS_KV8_FOLLOWS;
+            } else if (my_slot < 0 || my_slot >= c.sequences || my_add < 0) {
+                bad = STATUS_KV8_LENGTH;
             } else {
                 my_have = c.lengths[my_slot];
-                if (my_add > c.max_length - my_have) bad = 1;
+                if (my_add > c.max_length - my_have) bad = STATUS_KV8_LENGTH;
                 else need = (my_have + my_add) / KV8_BLOCK - my_have / KV8_BLOCK;
             }
         }
@@ -77,6 +81,8 @@ __global__ void __launch_bounds__(EXTEND_THREADS) kv8_extend_kernel(const b200q_
         }
         carry += sum;
     }
+    if (bad == STATUS_KV8_FOLLOWS) atomicCAS(status, 0, bad);            // (the first refusal's word says why)
+    else if (bad) atomicExch(status, bad);
     bad = __syncthreads_or(bad);
     const int *request = small ? first_s : starts;
     const int total = carry;
@@ -91,7 +97,7 @@ __global__ void __launch_bounds__(EXTEND_THREADS) kv8_extend_kernel(const b200q_
         }
         if (all < total) {
             if (tid == 0) atomicExch(status, STATUS_KV8_POOL);
-            for (int b = tid; b < batch; b += EXTEND_THREADS) starts[b] = -1;
+            for (int b = tid; b < batch; b += EXTEND_THREADS) starts[b] = KV8_REFUSED;
             return;
         }
         int rank = 0;
@@ -121,10 +127,9 @@ __global__ void __launch_bounds__(EXTEND_THREADS) kv8_extend_kernel(const b200q_
         }
         __syncthreads();
     }
-    if (bad && tid == 0) atomicExch(status, STATUS_KV8_LENGTH);
     for (int b = tid; b < batch; b += EXTEND_THREADS) {
         if (bad) {
-            starts[b] = -1;
+            starts[b] = KV8_REFUSED;
         } else {
             if (!small) {
                 my_slot = slots[b];
@@ -615,8 +620,8 @@ int kv8_check(const char *what, const b200q_kv8_cache *c) {
 
 using namespace b200q;
 
-extern "C" int b200q_kv8_extend(const b200q_kv8_cache *cache, const int32_t *slots, const int32_t *offsets, int batch,
-                                int32_t *starts, void *stream) {
+static int extend(const b200q_kv8_cache *cache, const int32_t *slots, const int32_t *offsets, int batch, int32_t *starts, int after,
+                  void *stream) {
     if (int rc = kv8_check("kv8_extend", cache)) return rc;
     if (batch == 0) return B200Q_OK;
     if (!slots || !offsets || !starts) return fail(B200Q_EINVAL, "kv8_extend: NULL pointer");
@@ -624,8 +629,18 @@ extern "C" int b200q_kv8_extend(const b200q_kv8_cache *cache, const int32_t *slo
     int *status = device_status_word();
     if (!status) return fail(B200Q_ECUDA, "kv8_extend: no CUDA device");
     launch_chained(kv8_extend_kernel, dim3(1), dim3(EXTEND_THREADS), 0, static_cast<cudaStream_t>(stream), *cache, slots,
-                   offsets, batch, starts, status);
+                   offsets, batch, starts, after, status);
     return check_launch("kv8_extend");
+}
+
+extern "C" int b200q_kv8_extend(const b200q_kv8_cache *cache, const int32_t *slots, const int32_t *offsets, int batch,
+                                int32_t *starts, void *stream) {
+    return extend(cache, slots, offsets, batch, starts, 0, stream);
+}
+
+extern "C" int b200q_kv8_extend_after(const b200q_kv8_cache *cache, const int32_t *slots, const int32_t *offsets, int batch,
+                                      int32_t *starts, void *stream) {
+    return extend(cache, slots, offsets, batch, starts, 1, stream);
 }
 
 extern "C" int b200q_kv8_append(const b200q_kv8_cache *cache, int layer, const void *k, const void *v, int in_dtype,

@@ -20,6 +20,8 @@ constexpr int KV8_MAX_PAGES = 1 << 20;
 constexpr int STATUS_KV8_POOL = 501;       // extend: the pool has too few free pages (nothing was taken)
 constexpr int STATUS_KV8_LENGTH = 502;     // extend: a sequence would pass max_length, or a slot is out of range
 constexpr int STATUS_KV8_SLOTS = 503;      // fork / free: a slot out of range, named twice, or a target that is not empty
+constexpr int STATUS_KV8_FOLLOWS = 504;    // extend_after: the step before was refused
+constexpr int KV8_REFUSED = -1;            // starts of a refused step
 
 // Smallest scale: the smallest normal number, so that no quotient by it overflows and no scale is zero.
 constexpr float KV8_MIN_SCALE = 1.17549435e-38f;

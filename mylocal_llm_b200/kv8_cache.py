@@ -18,7 +18,8 @@ All bookkeeping (lengths, page table, reference counts, the pool's free pages) l
 and the ``read_*`` helpers waits for it, and a step whose ``batch`` is kept can be captured into a CUDA graph and replayed:
 ``extend`` reads the lengths anew each time. What the device refuses - too few free pages, a sequence that would pass
 ``max_length``, a fork onto a slot that is not empty - changes nothing and sets the device status word (``_lib.device_status``:
-501, 502, 503); the rows of a refused step are NaN. Calls on one cache have to be ordered by their streams.
+501, 502, 503); the rows of a refused step are NaN, and so are those of the steps behind it where a batch is extended with
+``after=True``. Calls on one cache have to be ordered by their streams.
 
 A key or value that is not finite (in the cache's type) makes its block (its 64 tokens, of its head and layer) NaN, and with it
 every row that sees the block. Scores, softmax statistics and sums are FP32, and the codes enter the products exactly. Queries and
@@ -64,7 +65,7 @@ def _dtype_id(t, what):
 
 class KV8Batch:
     """One step's sequences: ``slots`` [B], ``offsets`` [B + 1] (row of each sequence's first new token) and ``starts`` [B]
-    (tokens before the step, written by ``PagedKV8Cache.extend``), int32 on the device; on the host the number of rows, the most
+    (tokens before the step, written by ``PagedKV8Cache.extend``; -1: it was refused, -2: there was none yet), int32 on the device; on the host the number of rows, the most
     new tokens of a sequence and a bound on the tokens a sequence holds after the step."""
 
     def __init__(self, slots, offsets, starts, rows, max_new, max_keys, limits):
@@ -159,7 +160,7 @@ class PagedKV8Cache:
             offsets.append(offsets[-1] + n)
         if offsets[-1] >= 2 ** 31:
             raise ValueError("too many tokens in one step")
-        ints = torch.tensor(slots + offsets + [-1] * len(slots), dtype=torch.int32).to(self.device)
+        ints = torch.tensor(slots + offsets + [-2] * len(slots), dtype=torch.int32).to(self.device)
         b = len(slots)
         return KV8Batch(ints[:b], ints[b:2 * b + 1], ints[2 * b + 1:], offsets[-1], max(counts), max_keys,
                         (self.sequences, self.max_length))
@@ -171,14 +172,15 @@ class PagedKV8Cache:
             raise ValueError("batch was made for a cache of other sizes")
         return batch
 
-    def extend(self, batch):
+    def extend(self, batch, *, after=False):
         """The sequences of ``batch`` grow by their new tokens: ``batch.starts`` gets their lengths before, pages are taken for the
-        blocks that become full. All sequences or none (status 501 / 502, ``starts`` -1)."""
+        blocks that become full. All sequences or none (status 501 / 502, ``starts`` -1). ``after``: a batch whose step before was
+        refused (its ``starts`` are -1) is refused again (status 504), for programs that do not look at every step."""
         self._check_batch(batch)
         slots, offsets, starts = batch._pointers
         host = _lib.host()
-        if host is None or not host.kv8_extend(self._c, self._index, slots, offsets, batch.size, starts):
-            _launch(self.device, "b200q_kv8_extend", self._c, slots, offsets, batch.size, starts)
+        if host is None or not host.kv8_extend(self._c, self._index, slots, offsets, batch.size, starts, bool(after)):
+            _launch(self.device, "b200q_kv8_extend_after" if after else "b200q_kv8_extend", self._c, slots, offsets, batch.size, starts)
         return batch
 
     def _slots(self, slots):

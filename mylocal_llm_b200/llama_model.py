@@ -79,7 +79,8 @@ class GenerationState:
 
 class PagedGenerationState:
     """The same state on an 8-bit paged cache: ``batch`` sequences in the slots 0, 1, ... of ``cache``. More ``sequences`` than that
-    leave slots to fork into, fewer ``pages`` than every sequence's horizon let short ones share the pool."""
+    leave slots to fork into, fewer ``pages`` than every sequence's horizon let short ones share the pool. Where the pool has too few
+    for a step, the logits of that step and of all that follow are NaN until the next ``prefill``."""
 
     def __init__(self, config, batch, horizon, dtype, device, sequences=None, pages=None):
         sequences = batch if sequences is None else int(sequences)
@@ -555,6 +556,7 @@ class ExternalLlamaModel:
             step = state.cache.batch(state.slots, [t] * b, max_keys=max(t, 1))
             state.cache.free(state.slots)                                     # (the prompt starts at position 0)
             state.cache.extend(step)
+            state.step.starts.copy_(step.starts)                              # (what is refused stays refused, see _decode_paged)
             hidden = self._forward(token_ids, state, None, None, step).reshape(b, t, -1)
             state.length = t
             return quantized_linear(hidden[:, -1].contiguous(), self.lm_head, out_dtype=torch.float32)
@@ -613,7 +615,7 @@ class ExternalLlamaModel:
         if token_ids.numel() != state.batch:
             raise ValueError("token_ids do not fit the generation state")
         token_ids, step = token_ids.reshape(-1, 1), state.step
-        state.cache.extend(step)
+        state.cache.extend(step, after=True)
         if (self.fused_decode and self.fused_norm_linear
                 and all(layer["qkv"] is not None and layer["gate_up"] is not None for layer in self.layers)):
             logits = self._forward_one_token(token_ids, state, None, step)
