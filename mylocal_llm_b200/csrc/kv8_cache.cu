@@ -64,7 +64,7 @@ __global__ void __launch_bounds__(EXTEND_THREADS) kv8_extend_kernel(const b200q_
                 bad = STATUS_KV8_LENGTH;
             } else {
                 my_have = c.lengths[my_slot];
-                if (my_add > c.max_length - my_have) bad = STATUS_KV8_LENGTH;
+                if (my_have < 0 || my_add > c.max_length - my_have) bad = STATUS_KV8_LENGTH;
                 else need = (my_have + my_add) / KV8_BLOCK - my_have / KV8_BLOCK;
             }
         }

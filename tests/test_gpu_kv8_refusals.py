@@ -100,3 +100,18 @@ def test_extending_after_a_refusal(cuda, sequences):
     assert cache.read_lengths() == [0] * sequences
     assert (cache.extend(batch).starts == 0).all() and _lib.device_status() == 0                    # the caller knows
     bookkeeping(torch, cache)
+
+
+@pytest.mark.parametrize("length", [-1, -64, -200, -2 ** 31, 257, 2 ** 31 - 1])
+@pytest.mark.parametrize("sequences", [3, 1100])
+def test_lengths_that_no_sequence_has(cuda, length, sequences):
+    """A cache over existing tensors with a length outside 0 .. max_length: the step is refused, nothing is written."""
+    torch = cuda
+    first = PagedKV8Cache(1, 1, 64, pages=40, sequences=sequences, max_length=256)
+    first.lengths[1] = length
+    parts = [getattr(first, n) for n in ("codes", "scales", "tail", "peak", "table", "lengths", "refs")]
+    before = [t.clone() for t in parts]
+    cache = PagedKV8Cache.from_tensors(*parts, max_length=256)
+    batch = cache.extend(cache.batch(list(range(sequences)), [70, 200] + [1] * (sequences - 2)))
+    assert _lib.device_status() == 502 and (batch.starts == -1).all()
+    assert all(torch.equal(a, b) for a, b in zip(before, parts))
