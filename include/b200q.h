@@ -554,12 +554,17 @@ int b200q_kv8_compact_move(const b200q_kv8_cache *from, const b200q_kv8_cache *t
  * b200q_int8_quantize: x[rows, k] (FP32, FP16, BF16; x_row elements from row to row) -> codes [rows][codes_row], scales
  * [rows]: scale = max |x| / 127 of the row (at least 2^-126), codes = x / scale rounded to nearest, ties to even; a row with
  * a NaN or an infinity has scale NaN. It serves activations (a row is a token) and weights (a row is an output channel).
- * early != 0 lets the next kernel on the stream be set up before this one has ended: for activations only, since
- * b200q_int8_gemm requests its weights while what precedes it still runs. */
+ * early != 0 lets the next kernel on the stream start when this one has begun, which is when everything in front of it is
+ * complete. Any kernel may follow; b200q_int8_gemm_behind_quantize makes use of it.
+ * b200q_int8_gemm_behind_quantize: b200q_int8_gemm as the next call on the stream behind a b200q_int8_quantize of activations (early
+ * or not): its weights, which that call must not have written, are requested before the quantiser has ended. */
 int b200q_int8_quantize(const void *x, int x_dtype, int rows, int k, int64_t x_row, int8_t *codes, int64_t codes_row,
                         float *scales, int early, void *stream);
 int b200q_int8_gemm(const int8_t *w_codes, int64_t w_row, const float *w_scales, int n, int k, const int8_t *x_codes,
                     int64_t x_row, const float *x_scales, int m, void *y, int y_dtype, void *stream);
+int b200q_int8_gemm_behind_quantize(const int8_t *w_codes, int64_t w_row, const float *w_scales, int n, int k,
+                                    const int8_t *x_codes, int64_t x_row, const float *x_scales, int m, void *y, int y_dtype,
+                                    void *stream);
 
 #ifdef __cplusplus
 }

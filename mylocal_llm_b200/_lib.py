@@ -124,6 +124,7 @@ SIGNATURES.update({
     "b200q_kv8_compact_move": [_ptr, _ptr, _ptr, _c_i64, _ptr],
     "b200q_int8_quantize": [_ptr, _c_int, _c_int, _c_int, _c_i64, _ptr, _c_i64, _ptr, _c_int, _ptr],
     "b200q_int8_gemm": [_ptr, _c_i64, _ptr, _c_int, _c_int, _ptr, _c_i64, _ptr, _c_int, _ptr, _c_int, _ptr],
+    "b200q_int8_gemm_behind_quantize": [_ptr, _c_i64, _ptr, _c_int, _c_int, _ptr, _c_i64, _ptr, _c_int, _ptr, _c_int, _ptr],
 })
 _RETURNS_BYTES = ("b200q_moe_decode_stack_workspace", "b200q_gemm_workspace_bytes", "b200q_kv8_attention_workspace",
                   "b200q_kv8_compact_workspace")

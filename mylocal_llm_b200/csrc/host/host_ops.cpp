@@ -35,7 +35,7 @@ struct Api {
     FN(residual_rmsnorm); FN(gemv_norm); FN(gemv_norm_supported); FN(router_logits_t); FN(router_topk_ex);
     FN(router_topk_plan_row); FN(shared_gate); FN(moe_plan_ex); FN(moe_token_image_bytes); FN(moe_token_images);
     FN(moe_gate_up); FN(moe_gate_up_images); FN(moe_down); FN(moe_hidden_image_bytes); FN(moe_gate_up_streams); FN(moe_down_streams); FN(moe_hidden_images); FN(moe_down_images); FN(moe_combine); FN(silu_mul); FN(rope_attention);
-    FN(prefill_attention); FN(embed_tokens); FN(int8_quantize); FN(int8_gemm); FN(kv8_extend); FN(kv8_extend_after); FN(kv8_append); FN(kv8_attention);
+    FN(prefill_attention); FN(embed_tokens); FN(int8_quantize); FN(int8_gemm_behind_quantize); FN(kv8_extend); FN(kv8_extend_after); FN(kv8_append); FN(kv8_attention);
     FN(kv8_attention_workspace); FN(kv8_fork); FN(kv8_free);
 #undef FN
 } api;
@@ -47,7 +47,7 @@ void bind(const py::dict &addresses, py::object error_type) {
     FN(residual_rmsnorm); FN(gemv_norm); FN(gemv_norm_supported); FN(router_logits_t); FN(router_topk_ex);
     FN(router_topk_plan_row); FN(shared_gate); FN(moe_plan_ex); FN(moe_token_image_bytes); FN(moe_token_images);
     FN(moe_gate_up); FN(moe_gate_up_images); FN(moe_down); FN(moe_hidden_image_bytes); FN(moe_gate_up_streams); FN(moe_down_streams); FN(moe_hidden_images); FN(moe_down_images); FN(moe_combine); FN(silu_mul); FN(rope_attention);
-    FN(prefill_attention); FN(embed_tokens); FN(int8_quantize); FN(int8_gemm); FN(kv8_extend); FN(kv8_extend_after); FN(kv8_append); FN(kv8_attention);
+    FN(prefill_attention); FN(embed_tokens); FN(int8_quantize); FN(int8_gemm_behind_quantize); FN(kv8_extend); FN(kv8_extend_after); FN(kv8_append); FN(kv8_attention);
     FN(kv8_attention_workspace); FN(kv8_fork); FN(kv8_free);
 #undef FN
     b200q_error = error_type.release().ptr();
@@ -191,7 +191,7 @@ PyObject *int8_linear_fast(PyObject *, PyObject *const *args, Py_ssize_t nargs) 
             int8_t *codes = static_cast<int8_t *>(scratch.data_ptr());
             float *scales = reinterpret_cast<float *>(codes + m * padded);
             CALL(int8_quantize, x.data_ptr(), dt, static_cast<int>(m), k, x_row, codes, padded, scales, 1, stream());
-            CALL(int8_gemm, static_cast<const int8_t *>(w.data_ptr()), padded, ws.data_ptr<float>(), n, k, codes, padded, scales,
+            CALL(int8_gemm_behind_quantize, static_cast<const int8_t *>(w.data_ptr()), padded, ws.data_ptr<float>(), n, k, codes, padded, scales,
                  static_cast<int>(m), y.data_ptr(), ydt, stream());
         } catch (const CallError &e) {
             e.raise();

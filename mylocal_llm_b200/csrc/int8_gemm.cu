@@ -144,8 +144,8 @@ __global__ void __launch_bounds__(256, VEC ? 4 : 2) int8_quantize_kernel(const v
                                                                          long long codes_row, float *scales, int team, int early) {
     constexpr int KEEP = IN == B200Q_F32 ? I8_QUANTIZE_KEEP / 2 : I8_QUANTIZE_KEEP;
     __shared__ uint32_t peaks[8];
-    if (early) chain_trigger();
     chain_wait();
+    if (early) chain_trigger();                          // (only now: what the next kernel reads early was written before this one)
     const int warp = threadIdx.x >> 5, mine = warp & (team - 1), first_warp = warp - mine;
     const int c0 = (32 * mine + (threadIdx.x & 31)) * 8, width = 256 * team, padded = (k + 15) & ~15;
     const int row0 = (blockIdx.x * 8 + warp) / team, step = gridDim.x * 8 / team;
@@ -220,8 +220,8 @@ __global__ void __launch_bounds__(256, VEC ? 4 : 2) int8_quantize_kernel(const v
 // store them. There are two kernels:
 //   int8_tile_kernel  one tile of 128 tokens x NT channels per CTA. Few tiles (few tokens, few channels): the K range is
 //                     divided among the 2, 4 or 8 CTAs of a cluster, whose integer sums meet in shared memory - exact, so the
-//                     division does not show in the result. Weights that do not depend on the preceding kernel are requested
-//                     before it has ended.
+//                     division does not show in the result. Behind the quantiser of the activations (`early`), which lets this
+//                     kernel start when everything in front of it is complete, weights are requested before it has ended.
 //   int8_pair_kernel  many tokens: CTAs 2p and 2p + 1 are one tensor-core unit (cta_group::2) and own 256 x 256 tiles, each
 //                     with half of both operands in its shared memory; the pairs walk the tiles in turn, and the sums of a tile
 //                     are stored while the next one is computed (two accumulators fill the tensor memory).
@@ -245,6 +245,7 @@ struct Int8Gemm {
     int x_rows;               // rows of the activation box (a multiple of 8)
     int stages, slabs;        // slabs of K
     int tiles_m, tiles_n;     // int8_pair_kernel
+    bool early;               // int8_tile_kernel: the preceding kernel does not write the weights, and what did is complete
     int *status;
 };
 
@@ -342,6 +343,7 @@ __global__ void __launch_bounds__(I8_THREADS, 1) int8_tile_kernel(const __grid_c
         tmem_alloc<false>(&tmem_base_slot, NT);
         tmem_relinquish<false>();
     }
+    if (!a.early) chain_wait();
     for (int i = tid; i < NT; i += I8_THREADS) w_scale[i] = n0 + i < a.n ? a.w_scales[n0 + i] : 0.f;
     tc_fence_before();
     __syncthreads();
@@ -350,7 +352,7 @@ __global__ void __launch_bounds__(I8_THREADS, 1) int8_tile_kernel(const __grid_c
     const uint32_t tmem_d = tmem_base_slot;
 
     if (warp == 0) {
-        // ---- loads: the first stages' weights do not wait for the preceding kernel, whose result the activations are
+        // ---- loads: `early`, the first stages' weights do not wait for the preceding kernel, whose result the activations are
         const uint32_t bytes = static_cast<uint32_t>(a.x_rows * I8_BK + NT * I8_BK);
         const int early = min(S, nslab);
         if (elect_one())
@@ -736,9 +738,8 @@ extern "C" int b200q_int8_quantize(const void *x, int x_dtype, int rows, int k, 
     return check_launch("int8_quantize");
 }
 
-extern "C" int b200q_int8_gemm(const int8_t *w_codes, int64_t w_row, const float *w_scales, int n, int k,
-                               const int8_t *x_codes, int64_t x_row, const float *x_scales, int m, void *y, int y_dtype,
-                               void *stream) {
+static int checked_gemm(const int8_t *w_codes, int64_t w_row, const float *w_scales, int n, int k, const int8_t *x_codes, int64_t x_row,
+                        const float *x_scales, int m, void *y, int y_dtype, bool early, void *stream) {
     if (m == 0) return B200Q_OK;
     if (!w_codes || !w_scales || !x_codes || !x_scales || !y) return fail(B200Q_EINVAL, "int8_gemm: NULL pointer");
     if (!dtype_valid(y_dtype)) return fail(B200Q_EINVAL, "int8_gemm: bad dtype");
@@ -748,6 +749,18 @@ extern "C" int b200q_int8_gemm(const int8_t *w_codes, int64_t w_row, const float
         ((reinterpret_cast<uintptr_t>(w_codes) | reinterpret_cast<uintptr_t>(x_codes)) & 15))
         return fail(B200Q_EINVAL, "int8_gemm: code rows must be 16-byte aligned and at least k long");
     Int8Gemm a{};
-    a.w_scales = w_scales; a.x_scales = x_scales; a.n = n; a.k = k; a.m = m; a.y = y; a.y_dtype = y_dtype;
+    a.w_scales = w_scales; a.x_scales = x_scales; a.n = n; a.k = k; a.m = m; a.y = y; a.y_dtype = y_dtype; a.early = early;
     return int8_gemm(w_codes, w_row, x_codes, x_row, a, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int b200q_int8_gemm(const int8_t *w_codes, int64_t w_row, const float *w_scales, int n, int k,
+                               const int8_t *x_codes, int64_t x_row, const float *x_scales, int m, void *y, int y_dtype,
+                               void *stream) {
+    return checked_gemm(w_codes, w_row, w_scales, n, k, x_codes, x_row, x_scales, m, y, y_dtype, false, stream);
+}
+
+extern "C" int b200q_int8_gemm_behind_quantize(const int8_t *w_codes, int64_t w_row, const float *w_scales, int n, int k,
+                                               const int8_t *x_codes, int64_t x_row, const float *x_scales, int m, void *y,
+                                               int y_dtype, void *stream) {
+    return checked_gemm(w_codes, w_row, w_scales, n, k, x_codes, x_row, x_scales, m, y, y_dtype, true, stream);
 }

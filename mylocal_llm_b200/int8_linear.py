@@ -101,6 +101,10 @@ class Int8Weight:
 def int8_matmul(codes, scales, weight, *, out_dtype=None):
     """``(codes * scales) @ weight.T`` -> ``[rows, N]`` (FP32 unless ``out_dtype`` says otherwise) for rows from
     ``quantize_int8_rows``: one quantisation can serve several projections."""
+    return _matmul("b200q_int8_gemm", codes, scales, weight, out_dtype)
+
+
+def _matmul(entry, codes, scales, weight, out_dtype):
     torch = _torch()
     if not isinstance(weight, Int8Weight):
         raise TypeError("Expected an Int8Weight")
@@ -116,7 +120,7 @@ def int8_matmul(codes, scales, weight, *, out_dtype=None):
     if codes.data_ptr() % 16:
         raise ValueError("codes must be 16-byte aligned")
     if codes.shape[0]:
-        _launch(codes.device, "b200q_int8_gemm", weight.codes.data_ptr(), padded, weight.scales.data_ptr(), n, k, codes.data_ptr(),
+        _launch(codes.device, entry, weight.codes.data_ptr(), padded, weight.scales.data_ptr(), n, k, codes.data_ptr(),
                 padded, scales.data_ptr(), codes.shape[0], out.data_ptr(), ident)
     return out
 
@@ -135,5 +139,5 @@ def int8_linear(x, weight, *, out_dtype=None):
     if x.shape[-1] != weight.shape[1]:
         raise ValueError(f"Input K={x.shape[-1]} does not match weight K={weight.shape[1]}")
     codes, scales = _quantize(x, 1)
-    y = int8_matmul(codes, scales, weight, out_dtype=out_dtype or x.dtype)
+    y = _matmul("b200q_int8_gemm_behind_quantize", codes, scales, weight, out_dtype or x.dtype)
     return y.reshape(x.shape[:-1] + (weight.shape[0],))
