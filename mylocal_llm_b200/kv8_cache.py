@@ -63,6 +63,13 @@ def _dtype_id(t, what):
     return ident
 
 
+def _ints(values, device):
+    """Python integers as an int32 tensor on ``device``, on its current stream: from pinned memory, so that nothing waits for what
+    the stream still has to do."""
+    torch = _torch()
+    return torch.tensor(values, dtype=torch.int32, pin_memory=True).to(device, non_blocking=True)
+
+
 class KV8Batch:
     """One step's sequences: ``slots`` [B], ``offsets`` [B + 1] (row of each sequence's first new token) and ``starts`` [B]
     (tokens before the step, written by ``PagedKV8Cache.extend``; -1: it was refused, -2: there was none yet), int32 on the device; on the host the number of rows, the most
@@ -144,7 +151,6 @@ class PagedKV8Cache:
         """The sequences of a step (distinct slots, Python integers) and how many new tokens each brings (0: it takes part
         without any). ``max_keys`` bounds the tokens a sequence holds after the step; the default ``max_length`` is always right,
         a smaller one lets ``attention`` divide short contexts better."""
-        torch = _torch()
         slots, counts = [int(s) for s in slots], [int(n) for n in counts]
         if not slots or len(slots) != len(counts):
             raise ValueError("slots and counts must be of the same length, at least one")
@@ -160,7 +166,7 @@ class PagedKV8Cache:
             offsets.append(offsets[-1] + n)
         if offsets[-1] >= 2 ** 31:
             raise ValueError("too many tokens in one step")
-        ints = torch.tensor(slots + offsets + [-2] * len(slots), dtype=torch.int32).to(self.device)
+        ints = _ints(slots + offsets + [-2] * len(slots), self.device)
         b = len(slots)
         return KV8Batch(ints[:b], ints[b:2 * b + 1], ints[2 * b + 1:], offsets[-1], max(counts), max_keys,
                         (self.sequences, self.max_length))
@@ -194,7 +200,7 @@ class PagedKV8Cache:
         slots = [int(s) for s in slots]
         if len(set(slots)) != len(slots) or (slots and (min(slots) < 0 or max(slots) >= self.sequences)):
             raise ValueError(f"slots must be distinct and within 0..{self.sequences - 1}")
-        return torch.tensor(slots, dtype=torch.int32).to(self.device)
+        return _ints(slots, self.device)
 
     def fork(self, src, dst):
         """Every empty sequence ``dst[i]`` becomes a copy of ``src[i]`` (sources may repeat): full pages are shared, the tail is
@@ -206,7 +212,7 @@ class PagedKV8Cache:
                 raise ValueError(f"slots must be within 0..{self.sequences - 1}")
             if not isinstance(dst, torch.Tensor) and set(src) & {int(d) for d in dst}:
                 raise ValueError("a target of a fork cannot be a source too")
-            src = torch.tensor(src, dtype=torch.int32).to(self.device)
+            src = _ints(src, self.device)
         src, dst = self._slots(src), self._slots(dst)
         if src.shape != dst.shape:
             raise ValueError("src and dst must be of the same length")
