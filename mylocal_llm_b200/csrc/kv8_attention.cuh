@@ -78,6 +78,12 @@ __device__ __forceinline__ float power_inverse(float p) {
     return __uint_as_float(e < 254 ? (254 - e) << 23 : e == 254 ? 0x00400000u : 0x7fc00000u);
 }
 
+// Scale of a tail whose largest magnitude has the bits `peak`: a power of two, by which its values are below 128 like codes. What a
+// value loses as FP16 number is then 2^-31 of the largest at most, so nothing of an FP16 tail of magnitudes below 128; NaN for what is not finite.
+__device__ __forceinline__ float tail_scale(uint32_t peak) {
+    return power_of(peak >= 0x7f800000u ? peak : max(peak, 0x08800000u)) * (1.f / 64.f);         // (2^-110: the inverse is finite)
+}
+
 // Two 16-bit values of the tail (as stored) times a power of two, as FP16.
 template <bool BF16>
 __device__ __forceinline__ uint32_t tail_to_half(uint32_t w, float inv) {

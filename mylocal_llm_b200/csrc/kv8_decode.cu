@@ -271,8 +271,8 @@ __global__ void __launch_bounds__(DecodeShape<DH, RT, MODE>::WARPS * 32, DecodeS
                     __syncwarp();
                     if (next.kind == PAGE) request(0, next, st);
                 } else {
-                    kscale = power_of(abs_bits(kscale));
-                    vscale = power_of(abs_bits(vscale));
+                    kscale = tail_scale(abs_bits(kscale));
+                    vscale = tail_scale(abs_bits(vscale));
                     vinv = power_inverse(vscale);
                     score_tail<DH, BF16, RT>(stage, power_inverse(kscale), rest, qf, g, t, acc);
                     __syncwarp();

@@ -411,7 +411,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prompt_kernel(const b200q_k
         // NaN here would reach rows that do not see the block).
         auto tail_inverse = [&](int values_part) {
             const uint32_t top = abs_bits(c.peak[tail + (values_part ? c.kv_heads : 0)]);
-            return top < 0x7f800000u ? power_inverse(power_of(top)) : 0.f;
+            return top < 0x7f800000u ? power_inverse(tail_scale(top)) : 0.f;
         };
         auto half_of = [&](uint32_t w, float inv) { return inv == 0.f ? 0u : tail_to_half<BF16>(w, inv); };
         auto page_at = [&](int block) {
@@ -540,8 +540,8 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prompt_kernel(const b200q_k
                 vs = held ? from[c.kv_heads] : kv8_nan();
             } else if (block * KV8_BLOCK < total) {
                 const size_t u = kv8_unit(slot, c.layers, a.layer, 0, c.kv_heads, kvh);
-                ks = power_of(abs_bits(c.peak[u]));
-                vs = power_of(abs_bits(c.peak[u + c.kv_heads]));
+                ks = tail_scale(abs_bits(c.peak[u]));
+                vs = tail_scale(abs_bits(c.peak[u + c.kv_heads]));
             } else {
                 ks = vs = 0.f;
             }

@@ -26,7 +26,7 @@ every row that sees the block. Scores, softmax statistics and sums are FP32, and
 softmax weights enter them with 22 bits (an FP16 number and its remainder), whichever of two kernels a step takes, which follows
 from an estimate of their times. Below FP16's normal numbers
 2^-36 of a row's largest product of weight and value scale is kept in steps of many tokens, 2^-40 of its largest weight in steps
-of few; values of the tail are held to 2^-24 of the largest magnitude among them.
+of few; values of the tail are held to 2^-31 of the largest magnitude among them.
 """
 
 import ctypes

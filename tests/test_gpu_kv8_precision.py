@@ -186,3 +186,23 @@ def test_many_small_weights_behind_a_dominant_one(cuda, dtype, heads, kv_heads, 
     q = torch.ones(count, heads * dh, device="cuda", dtype=getattr(torch, dtype))
     out = cache.attention(0, q, step(cache, [size], [count]), scale=1 / dh)
     check(torch, cache, 0, q, out, [size], [count], 1 / dh)
+
+
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("heads,kv_heads,dh", [(4, 2, 64), (32, 2, 128)])
+@pytest.mark.parametrize("count", [1, 4, 50])
+def test_small_values_next_to_large_ones_in_the_tail(cuda, dtype, heads, kv_heads, dh, count):
+    """Every dimension has its own order of magnitude: values of one token, seen alone, come back as they are, and keys that only
+    score by their small dimensions decide the weights."""
+    torch = cuda
+    cache = random_cache(torch, [count], 1, kv_heads, dh, dtype, count)
+    size = 2.0 ** torch.linspace(0, -16, dh, device="cuda")                     # (FP16: normal numbers of eleven bits)
+    cache.tail[0, 0, :, :, :count] = ((1 + torch.rand(2, kv_heads, count, dh, device="cuda", generator=torch.Generator("cuda").manual_seed(5))) * size * 8).to(cache.dtype)
+    cache.peak[0, 0] = cache.tail[0, 0, :, :, :count].float().abs().amax((-1, -2))
+    q = torch.zeros(count, heads, dh, device="cuda")
+    q[..., dh // 2:] = 1 / (8 * size[dh // 2:])
+    q = q.reshape(count, -1)
+    out = cache.attention(0, q, step(cache, [count], [count]))
+    first = cache.tail[0, 0, 1, :, 0].repeat_interleave(heads // kv_heads, 0).reshape(-1)
+    assert torch.equal(out[0], first)
+    check(torch, cache, 0, q, out, [count], [count], dh ** -0.5)
