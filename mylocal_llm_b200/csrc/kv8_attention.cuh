@@ -78,6 +78,12 @@ __device__ __forceinline__ float power_inverse(float p) {
     return __uint_as_float(e < 254 ? (254 - e) << 23 : e == 254 ? 0x00400000u : 0x7fc00000u);
 }
 
+// Scale of a row of queries: a power of two, by which its values are below 2^15, the top of FP16's range, so that a number and its
+// remainder keep 22 bits of values down to 2^-28 of the largest; NaN for what is not finite.
+__device__ __forceinline__ float query_scale(uint32_t top) {
+    return power_of(top >= 0x7f800000u ? top : max(top, 0x07800000u)) * (1.f / 16384.f);          // (2^-112: the scale is a normal number)
+}
+
 // Scale of a tail whose largest magnitude has the bits `peak`: a power of two, by which its values are below 128 like codes. What a
 // value loses as FP16 number is then 2^-31 of the largest at most, so nothing of an FP16 tail of magnitudes below 128; NaN for what is not finite.
 __device__ __forceinline__ float tail_scale(uint32_t peak) {
@@ -181,9 +187,9 @@ __device__ __forceinline__ void split_half(float x0, float x1, uint32_t &hi, uin
     lo = pack_half(x0 - f.x, x1 - f.y);
 }
 
-// The lane's part of the query operand of an eight-row tile, for row g of it: the row is scaled by a power of two into FP16's
-// range; the result is that power times |scale| times log2(e), which turns sums of products into base-2 exponents (a negative scale's
-// sign is in the query: larger sums are larger scores). base < 0: a row that does not exist (zeros).
+// The lane's part of the query operand of an eight-row tile, for row g of it, relative to the row's scale; the result is that scale
+// times |scale| times log2(e), which turns sums of products into base-2 exponents (a negative scale's sign is in the query: larger
+// sums are larger scores). base < 0: a row that does not exist (zeros).
 template <int DH>
 __device__ __forceinline__ float query_split(const Kv8Attention &a, long long base, int pos, int t, uint32_t (&qf)[DH / 16][4]) {
     float x[DH / 4];
@@ -195,7 +201,7 @@ __device__ __forceinline__ float query_split(const Kv8Attention &a, long long ba
     for (int e = 0; e < DH / 4; ++e) top = max(top, abs_bits(x[e]));
     top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
     top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    const float p = power_of(top), inv = a.scale < 0.f ? -power_inverse(p) : power_inverse(p);
+    const float p = query_scale(top), inv = a.scale < 0.f ? -power_inverse(p) : power_inverse(p);
 #pragma unroll
     for (int s = 0; s < DH / 16; ++s) {
         split_half(x[4 * s] * inv, x[4 * s + 1] * inv, qf[s][0], qf[s][1]);

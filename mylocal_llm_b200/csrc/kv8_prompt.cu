@@ -310,7 +310,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prompt_kernel(const b200q_k
             for (int e = 0; e < 4; ++e) top = max(top, max(abs_bits(x[0][e]), abs_bits(x[1][e])));
 #pragma unroll
             for (int o = 1; o < LANES; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-            const float power = power_of(top), inv = a.scale < 0.f ? -power_inverse(power) : power_inverse(power);
+            const float power = query_scale(top), inv = a.scale < 0.f ? -power_inverse(power) : power_inverse(power);
             if (local < KP_CTA_ROWS) {
                 if (i == 0) factor_s[local] = power * (fabsf(a.scale) * 1.4426950408889634f);
                 uint8_t *q_to = q_s + (local / KP_ROWS) * (Shape::Q / 2);

@@ -206,3 +206,33 @@ def test_small_values_next_to_large_ones_in_the_tail(cuda, dtype, heads, kv_head
     first = cache.tail[0, 0, 1, :, 0].repeat_interleave(heads // kv_heads, 0).reshape(-1)
     assert torch.equal(out[0], first)
     check(torch, cache, 0, q, out, [count], [count], dh ** -0.5)
+
+
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("heads,kv_heads,dh", [(4, 2, 64), (32, 2, 128)])
+@pytest.mark.parametrize("count,few", [(5, 1), (60, 1), (4, 4), (50, 50), (300, 300)])
+def test_small_values_next_to_large_ones_in_a_row_of_queries(cuda, dtype, heads, kv_heads, dh, count, few):
+    """One dimension of the queries is 2^15 times the others that score; those decide the weights."""
+    torch = cuda
+    gen = torch.Generator("cuda").manual_seed(count)
+    rest = count % BLOCK
+    cache = random_cache(torch, [count], 1, kv_heads, dh, dtype, count)
+    signs = lambda *shape: torch.randint(0, 2, shape, device="cuda", generator=gen) * 2 - 1  # noqa: E731
+    cache.codes[:, 0] = 0
+    for b in range(count // BLOCK):
+        page = int(cache.table[0, b])
+        keys = torch.zeros(kv_heads, BLOCK, dh, device="cuda")
+        keys[..., -8:] = signs(kv_heads, BLOCK, 8) * 64
+        cache.codes[page, 0, 0] = keys.reshape(kv_heads, -1).to(torch.int8)
+        cache.codes[page, 0, 1] = (signs(kv_heads, dh, BLOCK) * 64).reshape(kv_heads, -1).to(torch.int8)
+        cache.scales[page, 0, 0], cache.scales[page, 0, 1] = 1 / 16, 1 / 64
+    cache.tail[0, 0, :, :, :rest] = 0
+    cache.tail[0, 0, 0, :, :rest, -8:] = signs(kv_heads, rest, 8).to(cache.dtype) * 4
+    cache.tail[0, 0, 1, :, :rest] = signs(kv_heads, rest, dh).to(cache.dtype)
+    cache.peak[0, 0, 0], cache.peak[0, 0, 1] = 4, 1
+    q = torch.zeros(few, heads, dh, device="cuda")
+    q[..., 0] = 2.0 ** 10
+    q[..., -8:] = (1 + torch.rand(few, heads, 8, device="cuda", generator=gen)) * 2.0 ** -5
+    q = q.reshape(few, -1)
+    out = cache.attention(0, q, step(cache, [count], [few]), scale=1.0)
+    check(torch, cache, 0, q, out, [count], [few], 1.0)
