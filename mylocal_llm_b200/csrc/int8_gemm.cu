@@ -438,6 +438,7 @@ __global__ void __launch_bounds__(I8_THREADS, 1) int8_tile_kernel(const __grid_c
             for (int c = 0; c < NT / 32; ++c) {
                 const int col = n0 + 32 * c + lane;
                 uint32_t r[32];
+                __syncwarp();                            // (lanes whose outputs do not exist)
                 tmem_ld32(tmem_d + (static_cast<uint32_t>(32 * quarter) << 16) + 32 * c, r);
                 tmem_ld_wait();
                 store_outputs(a.y, a.y_dtype, static_cast<size_t>(m0 + 32 * quarter) * a.n + col, a.n, col < a.n, min(32, rows - 32 * quarter),
@@ -455,6 +456,7 @@ __global__ void __launch_bounds__(I8_THREADS, 1) int8_tile_kernel(const __grid_c
 #pragma unroll 1
             for (int c = 0; c < NT / 32; ++c) {
                 uint32_t r[32];
+                __syncwarp();                            // (lanes whose outputs do not exist)
                 tmem_ld32(tmem_d + (static_cast<uint32_t>(32 * quarter) << 16) + 32 * c, r);
                 tmem_ld_wait();
                 if (row < rows)
@@ -633,6 +635,7 @@ __global__ void __launch_bounds__(I8_PAIR_THREADS, 1) int8_pair_kernel(const __g
                 const float w = w_next;
                 if (c < 3) w_next = col + 32 < a.n ? a.w_scales[col + 32] : 0.f;
                 uint32_t r[32];
+                __syncwarp();                        // (lanes whose outputs do not exist)
                 tmem_ld32(tmem_d + (static_cast<uint32_t>(32 * quarter) << 16) + 256 * acc + 128 * half + 32 * c, r);
                 tmem_ld_wait();
                 if (c == 3) {                        // the accumulator is read: the next tile but one may have it

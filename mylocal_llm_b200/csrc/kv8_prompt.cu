@@ -17,16 +17,16 @@
 //               A row's reference M is the largest such product that it has seen, as a power of two, so a block counts by what
 //               it adds to the row and not by its scale: a large scale under a small weight does not push the others out of
 //               FP16's range. M moves only when it is passed by 2^4, so O is rescaled rarely; products are held as 2^11 times
-//               what they are next to M, FP16's whole range. What lies 2^-40 below M only enters the sum. A unit's first page is
-//               handed over before the second's weights are worked out (chunks of head dimension 128 397 -> 363 us). The sum and the largest
-//               weight have a reference of their own, since M may lie 2^126 above or below it.
+//               what they are next to M, FP16's whole range. The sum and the largest weight have a reference of their own,
+//               since M may lie 2^126 above or below it. A unit's first page is handed over before the second's weights are
+//               worked out (chunks of head dimension 128 397 -> 363 us).
 // 128 keys per step because an MMA of 128 rows x 64 keys reads 6 KB of operands for 32 clocks of work, more than shared memory
 // gives: with units of 64 keys the MMAs took 3200 of 3900 clocks per 64 keys (head dimension 128). Queries (a power of two per row
 // keeps them in range) and products of weight and scale are an FP16 number and what is left of it as another, each with an MMA of
-// its own, so both keep 22 bits as in kv8_decode.cu, whichever kernel a step gets. As FP16 numbers alone
-// the weights cost 1.4 times the result's own rounding in FP16 results (2.9e-4 for 2.1e-4 against 64 bits); prompts of head dimension 64
-// took 207 us instead of 235, chunks of dimension 128 and FP16 (queries in two parts) 321 instead of 363. Below FP16's normal numbers
-// 2^-36 of the row's M is kept.
+// its own, so both keep 22 bits as in kv8_decode.cu, whichever kernel a step gets. As FP16 numbers alone the weights cost 1.4 times
+// the result's own rounding in FP16 results (2.9e-4 for 2.1e-4 against 64 bits); prompts of head dimension 64 took 207 us instead of
+// 243, chunks of dimension 128 and FP16 (queries in two parts) 321 instead of 358. Below FP16's normal numbers 2^-36 of the row's M
+// is kept.
 //
 // Every wait is bounded: on expiry the status word tells, all roles leave, and the CTA ends.
 #include <algorithm>
@@ -56,9 +56,9 @@ template <int DH> struct PromptShape {
 };
 constexpr int KP_AHEAD = 4;                  // units between a page's request to L2 and its use
 // Exponents of two: products of weight and value scale are held times 2^KP_RANGE / M and pass M by 2^KP_SLACK at most, which uses
-// FP16's range up to 2^15; those below 2^-KP_NOTHING M count as nothing. (Ranges of 7, 11 and 13: 235, 235 and 240 us for 4 x 2048 tokens of
+// FP16's range up to 2^15; those below 2^-KP_NOTHING M only enter the sum. (Ranges of 7, 11 and 13: 235, 235 and 240 us for 4 x 2048 tokens of
 // head dimension 64, 358, 363 and 370 for three chunks of dimension 128: more room below, O rescaled more often.)
-constexpr float KP_RANGE = 11.f, KP_SLACK = 15.f - KP_RANGE, KP_NOTHING = 40.f;
+constexpr float KP_RANGE = 11.f, KP_SLACK = 15.f - KP_RANGE, KP_NOTHING = 100.f;
 
 struct Kv8Prompt {
     Kv8Attention a;
@@ -329,6 +329,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prompt_kernel(const b200q_k
         fence_proxy_async();
         __syncwarp();
         if (lane == 0) mbar_arrive(&q_full);
+        __syncwarp();                            // (the roles begin with an instruction of the whole warp)
     }
 
     if (warp >= MMA) {
@@ -617,8 +618,16 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prompt_kernel(const b200q_k
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const bool nothing = product[h] < product_m - KP_NOTHING || log_scale[h] == -INFINITY;
-                const float move = !sees[h] ? 0.f : nothing ? -peak[h] : log_scale[h] - product_m + KP_RANGE;
-                const float weigh = !sees[h] ? 0.f : exp2_approx(-move - m);
+                const float move = !sees[h] ? 0.f : nothing ? -INFINITY : log_scale[h] - product_m + KP_RANGE;
+                const float weigh = !sees[h] || nothing ? 0.f : exp2_approx(-move - m);
+                if (__any_sync(0xffffffffu, nothing && sees[h])) {               // (rare; selected, so that the lanes stay together)
+                    float only = 0.f;
+#pragma unroll
+                    for (int q = 0; q < 2; ++q)
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) only += exp2_approx(fmaf(__uint_as_float(s[2 * h + q][e]), f[h], -peak[h]));
+                    l += nothing && sees[h] ? only * exp2_approx(peak[h] - m) : 0.f;
+                }
                 const uint64_t f2 = pack2(f[h], f[h]), move2 = pack2(move, move);        // pairs: two per instruction
                 uint64_t sums[2] = {0ull, 0ull};
 #pragma unroll
@@ -636,12 +645,6 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prompt_kernel(const b200q_k
                         unpack2(add2(pack2(lo, hi), pack2(lo_top, hi_top)), lo_left, hi_left);
                         w[e / 2] = cut_half(lo, hi);
                         left[e / 2] = pack_half(lo_left, hi_left);
-                    }
-                    if (__any_sync(0xffffffffu, nothing)) {
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) {
-                            if (nothing) w[e] = left[e] = 0u;
-                        }
                     }
                     tmem_st16(at + P_COL + 32 * h + 16 * q, w);
                     tmem_st16(at + 32 * h + 16 * q, left);
@@ -664,6 +667,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prompt_kernel(const b200q_k
 #pragma unroll 1
             for (int d = 0; d < DH; d += 32) {
                 uint32_t o[32];
+                __syncwarp();                    // (lanes whose rows do not exist)
                 tmem_ld32(tmem + lanes + O_COL + DH * t + d, o);
                 tmem_ld_wait();
                 if (!valid) continue;

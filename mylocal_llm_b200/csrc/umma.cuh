@@ -13,9 +13,12 @@ namespace b200q {
 // tcgen05 / TMA wrappers (sm_100a)
 // ---------------------------------------------------------------------------------------------
 // PAIR: the two CTAs of a cluster work as one tensor-core unit (cta_group::2). Tensor memory is then allocated
-// and freed by the same warp of both CTAs, with the same shared-memory slot for the address.
+// and freed by the same warp of both CTAs, with the same shared-memory slot for the address. These instructions, and the loads and
+// stores of tensor memory below, want the whole warp at them at once: lanes that a branch has parted meet first, here in the
+// function, for loads and stores at the call.
 template <bool PAIR>
 __device__ __forceinline__ void tmem_alloc(uint32_t *dst_smem, uint32_t cols) {
+    __syncwarp();
     if (PAIR)
         asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(dst_smem)),
                      "r"(cols)
@@ -32,6 +35,7 @@ __device__ __forceinline__ void tmem_relinquish() {
 }
 template <bool PAIR>
 __device__ __forceinline__ void tmem_dealloc(uint32_t taddr, uint32_t cols) {
+    __syncwarp();
     if (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(cols) : "memory");
     else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(cols) : "memory");
 }

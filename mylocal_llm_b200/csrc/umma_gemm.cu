@@ -600,6 +600,7 @@ __global__ void __launch_bounds__(UG_THREADS, 1) umma_gemm_kernel(const __grid_c
             if (tile_t0 >= a.m) break;                           // whole token tile beyond m (uniform in the CTA)
             for (int c = group; c < nchunks; c += UG_DECODE_THREADS / 128) {
                 uint32_t r[32];
+                __syncwarp();                                    // (lanes whose rows do not exist)
                 tmem_ld32(tmem_d + (static_cast<uint32_t>(32 * quarter) << 16) + mt * acc_stride + 32 * c, r);
                 tmem_ld_wait();
                 if (staged) {

@@ -236,3 +236,16 @@ def test_small_values_next_to_large_ones_in_a_row_of_queries(cuda, dtype, heads,
     q = q.reshape(few, -1)
     out = cache.attention(0, q, step(cache, [count], [few]), scale=1.0)
     check(torch, cache, 0, q, out, [count], [few], 1.0)
+
+
+@pytest.mark.parametrize("count", [11, 31, 43, 54, 85, 86, 97, 171])
+@pytest.mark.parametrize("context", [0, 6000])
+def test_rows_that_fill_no_warp(cuda, count, context):
+    """Three rows per token: lanes without a row next to lanes with one, in one part of the keys and in many."""
+    torch = cuda
+    sizes, counts = [context + count, context // 2 + 200], [count, 190]
+    for dh in (64, 128):
+        cache = random_cache(torch, sizes, 1, 2, dh, "float16", count)
+        q = query(torch, sum(counts), 6 * dh, "float16", count)
+        out = cache.attention(0, q, step(cache, sizes, counts))
+        check(torch, cache, 0, q, out, sizes, counts, dh ** -0.5)
