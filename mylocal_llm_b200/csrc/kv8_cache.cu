@@ -149,7 +149,6 @@ struct Kv8Append {
     int layer;
     const int32_t *slots, *offsets, *starts;
     const float *cos_t, *sin_t;           // [rope_rows][head_dim / 2], or NULL: keys are stored as they come
-    int rope_rows;
 };
 
 // Four consecutive values of type IN as they are loaded (held in few registers until they are used). VEC: base and strides are
@@ -666,7 +665,7 @@ extern "C" int b200q_kv8_append(const b200q_kv8_cache *cache, int layer, const v
     Kv8Append a{};
     a.k = k; a.v = v; a.k_row = k_row; a.v_row = v_row; a.layer = layer;
     a.slots = slots; a.offsets = offsets; a.starts = starts;
-    a.cos_t = cos_table; a.sin_t = sin_table; a.rope_rows = rope_rows;
+    a.cos_t = cos_table; a.sin_t = sin_table;
     const size_t quad = 4 * dtype_size(in_dtype);
     const bool vec = (reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) % quad == 0 && k_row % 4 == 0 && v_row % 4 == 0;
     const dim3 grid(2 * cache->kv_heads, (max_new + 2 * KV8_BLOCK - 2) / KV8_BLOCK, batch);

@@ -52,11 +52,6 @@ __device__ __forceinline__ Pair pair_fma(Pair a, Pair b, Pair c) {
     asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d.v) : "l"(a.v), "l"(b.v), "l"(c.v));
     return d;
 }
-__device__ __forceinline__ Pair pair_mul(Pair a, Pair b) {
-    Pair d;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
-    return d;
-}
 __device__ __forceinline__ Pair pair_add(Pair a, Pair b) {
     Pair d;
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));

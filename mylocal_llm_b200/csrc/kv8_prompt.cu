@@ -118,23 +118,6 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// Pairs of FP32 numbers in one 64-bit register.
-__device__ __forceinline__ uint64_t pack2(float lo, float hi) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
-    return r;
-}
-__device__ __forceinline__ void unpack2(uint64_t x, float &lo, float &hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(x)); }
-__device__ __forceinline__ uint64_t fma2(uint64_t x, uint64_t y, uint64_t z) {
-    uint64_t r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(x), "l"(y), "l"(z));
-    return r;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t x, uint64_t y) {
-    uint64_t r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
-    return r;
-}
 __device__ __forceinline__ float max3(float x, float y, float z) {
     float r;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
@@ -628,30 +611,27 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prompt_kernel(const b200q_k
                         for (int e = 0; e < 32; ++e) only += exp2_approx(fmaf(__uint_as_float(s[2 * h + q][e]), f[h], -peak[h]));
                     l += nothing && sees[h] ? only * exp2_approx(peak[h] - m) : 0.f;
                 }
-                const uint64_t f2 = pack2(f[h], f[h]), move2 = pack2(move, move);        // pairs: two per instruction
-                uint64_t sums[2] = {0ull, 0ull};
+                const Pair f2 = pair(f[h], f[h]), move2 = pair(move, move);        // pairs: two per instruction
+                Pair sums[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
 #pragma unroll
                 for (int q = 0; q < 2; ++q) {
                     uint32_t w[16], left[16];
 #pragma unroll
                     for (int e = 0; e < 32; e += 2) {
-                        float lo, hi, lo_left, hi_left;
-                        unpack2(fma2(pack2(__uint_as_float(s[2 * h + q][e]), __uint_as_float(s[2 * h + q][e + 1])), f2, move2), lo, hi);
-                        lo = exp2_approx(lo);
-                        hi = exp2_approx(hi);
-                        sums[e / 2 & 1] = add2(sums[e / 2 & 1], pack2(lo, hi));
+                        const Pair exponents = pair_fma(pair(__uint_as_float(s[2 * h + q][e]), __uint_as_float(s[2 * h + q][e + 1])), f2, move2);
+                        const float lo = exp2_approx(exponents.lo()), hi = exp2_approx(exponents.hi());
+                        sums[e / 2 & 1] = pair_add(sums[e / 2 & 1], pair(lo, hi));
                         // (cut off at eleven bits, so that what is left is one exact subtraction)
                         const float lo_top = __uint_as_float((__float_as_uint(lo) & 0xffffe000u) | 0x80000000u), hi_top = __uint_as_float((__float_as_uint(hi) & 0xffffe000u) | 0x80000000u);
-                        unpack2(add2(pack2(lo, hi), pack2(lo_top, hi_top)), lo_left, hi_left);
+                        const Pair rest = pair_add(pair(lo, hi), pair(lo_top, hi_top));
                         w[e / 2] = cut_half(lo, hi);
-                        left[e / 2] = pack_half(lo_left, hi_left);
+                        left[e / 2] = pack_half(rest.lo(), rest.hi());
                     }
                     tmem_st16(at + P_COL + 32 * h + 16 * q, w);
                     tmem_st16(at + 32 * h + 16 * q, left);
                 }
-                float lo, hi;
-                unpack2(add2(sums[0], sums[1]), lo, hi);
-                l = fmaf(lo + hi, weigh, l);
+                const Pair sum = pair_add(sums[0], sums[1]);
+                l = fmaf(sum.lo() + sum.hi(), weigh, l);
                 tmem_st_wait();
                 tc_fence_before();
                 __syncwarp();
