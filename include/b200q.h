@@ -481,7 +481,7 @@ int b200q_expert_ffn_static(const void *gate, int gate_fmt, const void *up, int 
  *   lengths[sequences] int32: tokens held;  refs [pages] int32: sequences that refer to a page
  *   free_bits[(pages + 31) / 32]: bit p % 32 of word p / 32 is set while refs[p] == 0
  * Keys and values are rounded to `dtype` before anything else, so the content of a cache does not depend on how many tokens
- * arrived per call. head_dim 64 or 128; at most 65536 sequences and 2^20 pages. All of it lives on the device, every call
+ * arrived per call. head_dim 64 or 128; at most 65536 sequences (65535 of them in a step) and 2^20 pages. All of it lives on the device, every call
  * but the sizes of b200q_kv8_compact's new pool is decided there, and calls on one cache have to be ordered by their stream.
  * Device status words of refusals: 501 too few free pages, 502 a sequence would pass max_length (or a slot or a length is out of range),
  * 503 fork / free of slots out of range, of a target named twice, not empty or also a source, 504 a step behind a refused one;

@@ -625,6 +625,7 @@ static int extend(const b200q_kv8_cache *cache, const int32_t *slots, const int3
     if (batch == 0) return B200Q_OK;
     if (!slots || !offsets || !starts) return fail(B200Q_EINVAL, "kv8_extend: NULL pointer");
     if (batch < 0 || batch > cache->sequences) return fail(B200Q_EINVAL, "kv8_extend: batch %d out of range", batch);
+    if (batch > KV8_MAX_STEP) return fail(B200Q_EUNSUPPORTED, "kv8_extend: at most %d sequences per step", KV8_MAX_STEP);
     int *status = device_status_word();
     if (!status) return fail(B200Q_ECUDA, "kv8_extend: no CUDA device");
     launch_chained(kv8_extend_kernel, dim3(1), dim3(EXTEND_THREADS), 0, static_cast<cudaStream_t>(stream), *cache, slots,
@@ -661,7 +662,7 @@ extern "C" int b200q_kv8_append(const b200q_kv8_cache *cache, int layer, const v
                     cache->max_length);
     if ((reinterpret_cast<uintptr_t>(cos_table) | reinterpret_cast<uintptr_t>(sin_table)) & 15)
         return fail(B200Q_EINVAL, "kv8_append: RoPE tables must be 16-byte aligned");
-    if (batch > 65535) return fail(B200Q_EUNSUPPORTED, "kv8_append: at most 65535 sequences per call");
+    if (batch > KV8_MAX_STEP) return fail(B200Q_EUNSUPPORTED, "kv8_append: at most %d sequences per step", KV8_MAX_STEP);
     Kv8Append a{};
     a.k = k; a.v = v; a.k_row = k_row; a.v_row = v_row; a.layer = layer;
     a.slots = slots; a.offsets = offsets; a.starts = starts;

@@ -17,6 +17,7 @@ namespace b200q {
 constexpr int KV8_BLOCK = 64;
 constexpr int KV8_MAX_SEQUENCES = 65536;
 constexpr int KV8_MAX_PAGES = 1 << 20;
+constexpr int KV8_MAX_STEP = 65535;        // sequences of a step: what a grid holds along z
 constexpr int STATUS_KV8_POOL = 501;       // extend: the pool has too few free pages (nothing was taken)
 constexpr int STATUS_KV8_LENGTH = 502;     // extend: a sequence would pass max_length, or a slot is out of range
 constexpr int STATUS_KV8_SLOTS = 503;      // fork / free: a slot out of range, named twice, or a target that is not empty

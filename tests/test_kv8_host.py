@@ -118,3 +118,11 @@ def test_python_layers_refuse_host_tensors():
 def test_attention_refuses_outputs_that_are_not_aligned(max_new, rows):
     assert rc("b200q_kv8_attention", ctypes.byref(cache()), 0, ONE, 0, 512, 8, ONE, ONE, ONE, 2, rows, max_new, 100, None, None, 0, 0.1, ONE + 8,
               ONE, 1 << 20, None) == 1
+
+
+def test_a_step_that_append_could_not_take_is_not_begun():
+    """The lengths would have grown by tokens that no call can store."""
+    whole = ctypes.byref(cache(sequences=65536))
+    for name in ("b200q_kv8_extend", "b200q_kv8_extend_after"):
+        assert rc(name, whole, ONE, ONE, 65536, ONE, None) == 3
+    assert rc("b200q_kv8_append", whole, 0, ONE, ONE, 0, 256, 256, ONE, ONE, ONE, 65536, 1, None, None, 0, None) == 3
