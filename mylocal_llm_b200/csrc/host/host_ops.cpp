@@ -17,6 +17,7 @@
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 
+#include <climits>
 #include <cmath>
 #include <cstdlib>
 #include <cstring>
@@ -155,7 +156,11 @@ PyMethodDef linear_def = {"linear", reinterpret_cast<PyCFunction>(reinterpret_ca
 // ------------------------------------------------------------------------------------------------ int8 product, 8-bit cache
 // Like linear: positional arguments, None when the call needs the Python layer (other devices, what it has to refuse).
 #define FAST_METHOD(name) PyMethodDef name##_def = {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name##_fast)), METH_FASTCALL, nullptr}
-int as_int(PyObject *o) { return static_cast<int>(PyLong_AsLong(o)); }
+// (-1, which every entry point refuses where the number counts, for what 32 bits do not hold)
+int as_int(PyObject *o) {
+    const long v = PyLong_AsLong(o);
+    return v < INT_MIN || v > INT_MAX ? -1 : static_cast<int>(v);
+}
 // Rows of consecutive elements that do not overlap: elements from row to row, or -1.
 int64_t row_stride(const at::Tensor &x) {
     const int64_t rows = x.size(0), width = x.size(1);

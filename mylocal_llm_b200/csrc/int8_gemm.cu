@@ -133,6 +133,8 @@ template <int IN> struct Piece<IN, false> {
     }
 };
 
+constexpr int I8_MAX_SIZE = 1 << 30;                 // rows and columns: sums of an index and a step fit 32 bits
+
 // A team of `team` warps takes a row at a time: the largest magnitude, then the codes. The row's pieces of eight values stay in
 // registers, as they were loaded, between the two up to 256 * team * KEEP columns (longer rows are read again), and the next row's
 // are on their way meanwhile. Teams are as small as the row allows: warps that need not meet (6992 x 706 FP32, cold: by whole CTAs
@@ -724,7 +726,7 @@ extern "C" int b200q_int8_quantize(const void *x, int x_dtype, int rows, int k, 
     if (!dtype_valid(x_dtype)) return fail(B200Q_EINVAL, "int8_quantize: bad dtype");
     if (rows < 0 || k < 1 || x_row < k || codes_row % 16 || codes_row < k)
         return fail(B200Q_EINVAL, "int8_quantize: bad shape rows=%d k=%d (code rows are multiples of 16 bytes)", rows, k);
-    if (rows > 0x7fff0000) return fail(B200Q_EUNSUPPORTED, "int8_quantize: too many rows");
+    if (rows > I8_MAX_SIZE || k > I8_MAX_SIZE) return fail(B200Q_EUNSUPPORTED, "int8_quantize: at most %d rows and columns", I8_MAX_SIZE);
     if (reinterpret_cast<uintptr_t>(codes) & 15) return fail(B200Q_EINVAL, "int8_quantize: codes must be 16-byte aligned");
     const size_t e = dtype_size(x_dtype);
     const bool vec = (reinterpret_cast<uintptr_t>(x) & 15) == 0 && x_row * e % 16 == 0;
@@ -747,6 +749,7 @@ static int checked_gemm(const int8_t *w_codes, int64_t w_row, const float *w_sca
     if (!w_codes || !w_scales || !x_codes || !x_scales || !y) return fail(B200Q_EINVAL, "int8_gemm: NULL pointer");
     if (!dtype_valid(y_dtype)) return fail(B200Q_EINVAL, "int8_gemm: bad dtype");
     if (m < 0 || n < 1 || k < 1) return fail(B200Q_EINVAL, "int8_gemm: bad shape m=%d n=%d k=%d", m, n, k);
+    if (m > I8_MAX_SIZE || n > I8_MAX_SIZE) return fail(B200Q_EUNSUPPORTED, "int8_gemm: at most %d rows and channels", I8_MAX_SIZE);
     if (k > 131071) return fail(B200Q_EUNSUPPORTED, "int8_gemm: sums of more than 131071 products do not fit 32 bits");
     if (w_row % 16 || x_row % 16 || w_row < k || x_row < k ||
         ((reinterpret_cast<uintptr_t>(w_codes) | reinterpret_cast<uintptr_t>(x_codes)) & 15))

@@ -14,6 +14,7 @@ from .kv8_cache import _dtype_id, _launch
 from .quantized_linear import DevicePackedGGUFWeight, dequantize_device
 
 INT8_MAX_K = 131071         # so many products of two codes fit a 32-bit sum
+INT8_MAX_SIZE = 2 ** 30     # rows or columns of a matrix
 
 
 def _torch():
@@ -42,6 +43,8 @@ def _quantize(x, early):
         rows, x_row = x.numel() // k, k
     else:
         raise ValueError("x must be contiguous, or two-dimensional with rows of consecutive elements")
+    if max(rows, k) > INT8_MAX_SIZE:
+        raise NotImplementedError(f"at most {INT8_MAX_SIZE} rows and columns")
     padded = -(-k // 16) * 16
     codes = torch.empty((rows, padded), dtype=torch.int8, device=x.device)
     scales = torch.empty(rows, dtype=torch.float32, device=x.device)
@@ -69,6 +72,8 @@ class Int8Weight:
             raise ValueError(f"scales must be FP32 [{n}] on {codes.device}")
         if k > INT8_MAX_K:
             raise NotImplementedError(f"sums of more than {INT8_MAX_K} products do not fit 32 bits")
+        if n > INT8_MAX_SIZE:
+            raise NotImplementedError(f"at most {INT8_MAX_SIZE} channels")
         padded = -(-k // 16) * 16
         if padded != columns:
             wide = torch.zeros((n, padded), dtype=torch.int8, device=codes.device)
@@ -119,6 +124,8 @@ def _matmul(entry, codes, scales, weight, out_dtype):
     ident = _dtype_id(out, "out_dtype")
     if codes.data_ptr() % 16:
         raise ValueError("codes must be 16-byte aligned")
+    if codes.shape[0] > INT8_MAX_SIZE:
+        raise NotImplementedError(f"at most {INT8_MAX_SIZE} rows")
     if codes.shape[0]:
         _launch(codes.device, entry, weight.codes.data_ptr(), padded, weight.scales.data_ptr(), n, k, codes.data_ptr(),
                 padded, scales.data_ptr(), codes.shape[0], out.data_ptr(), ident)

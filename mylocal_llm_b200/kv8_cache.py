@@ -280,6 +280,11 @@ class PagedKV8Cache:
             raise ValueError(f"RoPE tables of {cos.shape[0]} positions for sequences of up to {self.max_length} tokens")
         return cos.data_ptr(), sin.data_ptr(), cos.shape[0]
 
+    def _layer(self, layer):
+        if not 0 <= layer < self.layers:
+            raise ValueError(f"layer {layer} out of range 0..{self.layers - 1}")
+        return layer
+
     def _rows(self, x, batch, width, what):
         if x.ndim != 2 or x.shape[0] != batch.rows or x.shape[1] != width or x.device != self.device:
             raise ValueError(f"{what} must be [{batch.rows}, {width}] on {self.device}, got {tuple(x.shape)} on {x.device}")
@@ -303,7 +308,7 @@ class PagedKV8Cache:
             raise TypeError("k and v must have the same type")
         cos, sin, positions = self._rope(rope)
         if batch.rows:
-            _launch(self.device, "b200q_kv8_append", self._c, layer, k.data_ptr(), v.data_ptr(), _dtype_id(k, "k"), k_row, v_row,
+            _launch(self.device, "b200q_kv8_append", self._c, self._layer(layer), k.data_ptr(), v.data_ptr(), _dtype_id(k, "k"), k_row, v_row,
                     *batch._pointers, batch.size, batch.max_new, cos, sin, positions)
 
     def attention(self, layer, q, batch, *, rope=None, scale=None, out=None):
@@ -331,7 +336,7 @@ class PagedKV8Cache:
         if batch.rows:
             size = _lib.load().b200q_kv8_attention_workspace(self._c, heads, batch.size, batch.rows, batch.max_new, batch.max_keys)
             space = torch.empty(size, dtype=torch.uint8, device=self.device) if size else None
-            _launch(self.device, "b200q_kv8_attention", self._c, layer, q.data_ptr(), _dtype_id(q, "q"), q_row, heads,
+            _launch(self.device, "b200q_kv8_attention", self._c, self._layer(layer), q.data_ptr(), _dtype_id(q, "q"), q_row, heads,
                     *batch._pointers, batch.size, batch.rows, batch.max_new, batch.max_keys, cos, sin, positions,
                     float(self.head_dim ** -0.5 if scale is None else scale), out.data_ptr(), _ptr(space), size)
         return out

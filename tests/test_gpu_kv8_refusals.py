@@ -3,7 +3,7 @@
 import numpy as np
 import pytest
 
-from mylocal_llm_b200 import PagedKV8Cache, _lib
+from mylocal_llm_b200 import Int8Weight, PagedKV8Cache, _lib, int8_linear, quantize_int8_rows
 from mylocal_llm_b200.llama_model import ExternalLlamaConfig, ExternalLlamaModel
 from test_gpu_kv8_cache import bookkeeping
 from test_gpu_llama_model import CFG, make_weights
@@ -115,3 +115,30 @@ def test_lengths_that_no_sequence_has(cuda, length, sequences):
     batch = cache.extend(cache.batch(list(range(sequences)), [70, 200] + [1] * (sequences - 2)))
     assert _lib.device_status() == 502 and (batch.starts == -1).all()
     assert all(torch.equal(a, b) for a, b in zip(before, parts))
+
+
+@pytest.mark.parametrize("layer", [2 ** 32, 2 ** 32 + 1, -2 ** 32, 2 ** 31, 2, -1])
+@pytest.mark.parametrize("native", ["0", "1"])
+def test_layers_that_the_cache_lacks(cuda, monkeypatch, layer, native):
+    """Also those whose low 32 bits name one."""
+    torch = cuda
+    monkeypatch.setenv("B200Q_HOST", native)
+    cache = PagedKV8Cache(2, 1, 64, pages=2, sequences=1, max_length=64)
+    batch = cache.extend(cache.batch([0], [3]))
+    x = torch.ones(3, 64, device="cuda")
+    with pytest.raises(ValueError):
+        cache.append(layer, x, x, batch)
+    with pytest.raises(ValueError):
+        cache.attention(layer, x, batch)
+    assert not cache.tail.any()
+
+
+def test_more_rows_than_32_bits_count(cuda):
+    """Not the rows that the low 32 bits count."""
+    torch = cuda
+    weight = Int8Weight(torch.ones(4, 1, dtype=torch.int8, device="cuda"), torch.ones(4, device="cuda"))
+    x = torch.empty(2 ** 32 + 1, 1, dtype=torch.float16, device="cuda")
+    for call in (lambda: quantize_int8_rows(x), lambda: int8_linear(x, weight), lambda: int8_linear(x[None], weight),
+                 lambda: quantize_int8_rows(x.reshape(1, -1))):
+        with pytest.raises(NotImplementedError):
+            call()

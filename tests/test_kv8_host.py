@@ -126,3 +126,13 @@ def test_a_step_that_append_could_not_take_is_not_begun():
     for name in ("b200q_kv8_extend", "b200q_kv8_extend_after"):
         assert rc(name, whole, ONE, ONE, 65536, ONE, None) == 3
     assert rc("b200q_kv8_append", whole, 0, ONE, ONE, 0, 256, 256, ONE, ONE, ONE, 65536, 1, None, None, 0, None) == 3
+
+
+@pytest.mark.parametrize("size", [2 ** 30 + 1, 2 ** 31 - 1])
+def test_int8_sizes_whose_indexes_do_not_fit_32_bits(size):
+    wide = -(-size // 16) * 16
+    assert rc("b200q_int8_quantize", ONE, 0, size, 100, 100, ONE, 112, ONE, 0, None) == 3
+    assert rc("b200q_int8_quantize", ONE, 0, 3, size, wide, ONE, wide, ONE, 0, None) == 3
+    for name in ("b200q_int8_gemm", "b200q_int8_gemm_behind_quantize"):
+        assert rc(name, ONE, 112, ONE, size, 100, ONE, 112, ONE, 3, ONE, 0, None) == 3
+        assert rc(name, ONE, 112, ONE, 5, 100, ONE, 112, ONE, size, ONE, 0, None) == 3
