@@ -684,7 +684,11 @@ static int int8_gemm(const int8_t *w, long long w_row, const int8_t *x, long lon
     a.tiles_m = (a.m + 255) / 256;
     a.tiles_n = (a.n + 255) / 256;
     const long long big = static_cast<long long>(a.tiles_m) * a.tiles_n;
-    if (2 * big >= sms) {
+    const int token_tiles = (a.m + I8_BM - 1) / I8_BM;
+    // The tile kernel's CTAs have one tile each: it is the faster one while all of them run at once (K 4096: 512 tokens x 4096 channels,
+    // 128 tiles, 18 us against 20 by pairs; 256 x 8192 20 against 22), the pairs with more tiles (512 x 6144 22 against 33, 1024 x 8192
+    // 33 against 61, 64 x 24576 37 against 39).
+    if (static_cast<long long>((a.n + 127) / 128) * token_tiles > sms) {
         if (big > 0x3fffffff) return fail(B200Q_EUNSUPPORTED, "int8_gemm: too many tiles");
         if (int rc = int8_map(&xmap, encode, x, columns, x_row, a.m, 128)) return rc;
         if (int rc = int8_map(&wmap, encode, w, columns, w_row, a.n, 128)) return rc;
@@ -694,13 +698,17 @@ static int int8_gemm(const int8_t *w, long long w_row, const int8_t *x, long lon
         launch_chained_cluster(int8_pair_kernel, dim3(2 * pairs), dim3(I8_PAIR_THREADS), smem, stream, 2, xmap, wmap, a);
         return check_launch("int8_gemm");
     }
-    const int token_tiles = (a.m + I8_BM - 1) / I8_BM;
+    // Tiles of 64 channels where those of 128 would leave half of the SMs idle (K 4096: one token x 4096 channels 16 us by both, 128 x
+    // 8192 18 against 20, but one token x 12288 29 against 20).
     int nt = 128;
     if (static_cast<long long>((a.n + 127) / 128) * token_tiles * 2 <= sms) nt = 64;
     const int tiles_n = (a.n + nt - 1) / nt;
     const long long tiles = static_cast<long long>(tiles_n) * token_tiles;
+    // K in parts of at least four slabs, as long as all CTAs run at once; eight only for a handful of tiles (one token, tiles of 64, in 1,
+    // 2, 4 and 8 parts: 512 x 2048 12, 10, 10 and 8 us; 1024 x 4096 16, 12, 10 and 14; 2048 x 8192 25, 18, 14 and 25; 4096 x 8192 25,
+    // 18, 22 and 37).
     int split = 1;
-    while (split < 8 && tiles * split * 2 <= sms && a.slabs >= split * 4) split *= 2;
+    while (split < (tiles <= 8 ? 8 : 4) && tiles * split * 2 <= sms && a.slabs >= split * 4) split *= 2;
     a.x_rows = a.m < I8_BM ? (a.m + 7) / 8 * 8 : I8_BM;
     const int stage = I8_A_BYTES + nt * I8_BK;
     a.stages = std::min(I8_MAX_STAGES, 200 * 1024 / stage);
