@@ -582,11 +582,12 @@ struct DecodePlan {
     double time;                        // estimate, us
 };
 
-// What a mode costs, in us, as measured with 8 to 4096 sequences x heads of 1 to 94 units (caches in L2): a CTA per sequence (its
-// queries and the warps' meeting) and round of its warps; a warp by itself per sequence and unit; parts per sequence and unit of
-// the whole device. The best mode's estimate is within a third of its measured time. Measured (head dimension 128, four rows): 8
-// sequences x heads of 1500 keys 13.7 cut, 16.1 whole, 87 by single warps; 256 of 777 keys 30 / 30 / 66; 4096 of 60 keys
-// 133 / 253 / 58.
+// What a mode costs, in us, as measured with 8 to 4096 sequences x heads of 1 to 94 units, all of the same length (caches in L2): a
+// CTA per sequence (its queries and the warps' meeting) and round of its warps; a warp by itself per sequence and unit; parts per
+// sequence and unit of the whole device. For such batches the best mode's estimate is within a third of its measured time; of ragged
+// ones the longest sequence alone is known, so they are overestimated (48 of up to 8192 keys: 167 for 93). Measured (head
+// dimension 128, four rows): 8 sequences x heads of 1500 keys 13.7 cut, 16.1 whole, 87 by single warps; 256 of 777 keys 30 / 30 /
+// 66; 4096 of 60 keys 133 / 253 / 58.
 struct DecodeTimes {
     double whole, whole_round, solo, solo_unit, cut, cut_unit;
 };
