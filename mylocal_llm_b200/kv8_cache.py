@@ -16,10 +16,10 @@ page is written once, so sequences share pages by reference: a fork copies only 
 
 All bookkeeping (lengths, page table, reference counts, the pool's free pages) lives on the device, nothing but ``compact``
 and the ``read_*`` helpers waits for it, and a step whose ``batch`` is kept can be captured into a CUDA graph and replayed:
-``extend`` reads the lengths anew each time. What the device refuses - too few free pages, a sequence that would pass
-``max_length``, a fork onto a slot that is not empty - changes nothing and sets the device status word (``_lib.device_status``:
-501, 502, 503); the rows of a refused step are NaN, and so are those of the steps behind it where a batch is extended with
-``after=True``. Calls on one cache have to be ordered by their streams.
+``extend`` reads the lengths anew each time (``fork`` and ``free`` are captured with slots in device tensors). What the device
+refuses - too few free pages, a sequence that would pass ``max_length``, a fork onto a slot that is not empty - changes nothing
+and sets the device status word (``_lib.device_status``: 501, 502, 503); the rows of a refused step are NaN, and so are those of
+the steps behind it where a batch is extended with ``after=True``. Calls on one cache have to be ordered by their streams.
 
 A key or value that is not finite (in the cache's type) makes its block (its 64 tokens, of its head and layer) NaN, and with it
 every row that sees the block. Scores, softmax statistics and sums are FP32, and the codes enter the products exactly. Queries and
@@ -65,8 +65,11 @@ def _dtype_id(t, what):
 
 def _ints(values, device):
     """Python integers as an int32 tensor on ``device``, on its current stream: from pinned memory, so that nothing waits for what
-    the stream still has to do."""
+    the stream still has to do. Not while the stream is captured: a replay would read host memory that others have by then."""
     torch = _torch()
+    with torch.cuda.device(device):
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("make batches before the capture, and give fork and free tensors on the device")
     return torch.tensor(values, dtype=torch.int32, pin_memory=True).to(device, non_blocking=True)
 
 

@@ -67,3 +67,29 @@ def test_a_prompt_of_the_model_does_not_wait(cuda):
     got = [model.prefill(tokens, state), model.decode_one(tokens[:, 0].contiguous(), state)]
     assert not event.query()
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_python_integers_are_not_captured(cuda):
+    """A graph would copy them from host memory that is used for something else by then; tensors on the device it may hold."""
+    torch = cuda
+    cache = PagedKV8Cache(1, 1, 64, pages=8, sequences=6, max_length=200)
+    batch = cache.extend(cache.batch([0], [70]))
+    src, dst = (torch.tensor([i], dtype=torch.int32, device="cuda") for i in (0, 1))
+    cache.fork(src, dst)
+    cache.free(dst)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for call in (lambda: cache.batch([1], [1]), lambda: cache.fork([0], [1]), lambda: cache.fork(src, [1]), lambda: cache.free([0])):
+            with pytest.raises(RuntimeError):
+                call()
+        cache.fork(src, dst)
+        cache.extend(batch)
+        cache.free(dst)
+    for _ in range(3):
+        graph.replay()
+    torch.cuda.synchronize()
+    assert _lib.device_status() == 502                       # 70 + 70 + 70 > 200
+    _lib.clear_device_status()
+    assert cache.read_lengths() == [140, 0, 0, 0, 0, 0]
+    bookkeeping(torch, cache)
