@@ -238,7 +238,9 @@ class ExternalLlamaModel:
 
     def create_generation_state(self, batch_size=1, max_length=None, kv_cache=None, *, sequences=None, pages=None):
         """Dense caches in the model's type, or (``kv_cache="int8"``, head_dim 64 or 128, 16-bit models) an 8-bit paged cache with
-        ``pages`` pages for ``sequences`` sequences (default: room for every sequence of the batch)."""
+        ``pages`` pages for ``sequences`` sequences (default: room for every sequence of the batch): half the memory, and the
+        faster step for many or long sequences (16 of 4000 tokens 3.8 ms for 5.5), the slower one for few short ones (one of
+        512 tokens 1.4 ms for 1.1; 24 layers, 32 heads of 64)."""
         self._require_weights()
         if kv_cache not in (None, "int8"):
             raise ValueError("kv_cache must be None or 'int8'")
