@@ -14,12 +14,12 @@
 //               instructions, among three other busy warps of its scheduler, than the tensor cores to execute them.)
 //   softmax     (2 x 4 warps) a thread per row: maximum, weights, sum; the weights go back to tensor memory as FP16, times the
 //               block's value scale (its logarithm is an addend of the exponent, which costs nothing; the sum is divided by it).
-//               A row's reference M is the largest such product that it has seen, as a power of two, so a block counts by what
-//               it adds to the row and not by its scale: a large scale under a small weight does not push the others out of
-//               FP16's range. M moves only when it is passed by 2^4, so O is rescaled rarely; products are held as 2^11 times
-//               what they are next to M, FP16's whole range. The sum and the largest weight have a reference of their own,
-//               since M may lie 2^126 above or below it. A unit's first page is handed over before the second's weights are
-//               worked out (chunks of head dimension 128 397 -> 363 us).
+//               A row's reference M is the largest such product that it has seen, so a block counts by what it adds to the
+//               row and not by its scale: a large scale under a small weight does not push the others out of FP16's range.
+//               M moves only when it is passed by 2^4, so O is rescaled rarely; products are held as 2^11 times what they are
+//               next to M, FP16's whole range. The sum and the largest weight have a reference of their own, since M may lie
+//               2^126 above or below it. A unit's first page is handed over before the second's weights are worked out (chunks
+//               of head dimension 128 397 -> 363 us).
 // 128 keys per step because an MMA of 128 rows x 64 keys reads 6 KB of operands for 32 clocks of work, more than shared memory
 // gives: with units of 64 keys the MMAs took 3200 of 3900 clocks per 64 keys (head dimension 128). Queries (a power of two per row
 // keeps them in range) and products of weight and scale are an FP16 number and what is left of it as another, each with an MMA of
@@ -622,8 +622,8 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prompt_kernel(const b200q_k
                         const float lo = exp2_approx(exponents.lo()), hi = exp2_approx(exponents.hi());
                         sums[e / 2 & 1] = pair_add(sums[e / 2 & 1], pair(lo, hi));
                         // (cut off at eleven bits, so that what is left is one exact subtraction)
-                        const float lo_top = __uint_as_float((__float_as_uint(lo) & 0xffffe000u) | 0x80000000u), hi_top = __uint_as_float((__float_as_uint(hi) & 0xffffe000u) | 0x80000000u);
-                        const Pair rest = pair_add(pair(lo, hi), pair(lo_top, hi_top));
+                        auto minus_top = [](float x) { return __uint_as_float((__float_as_uint(x) & 0xffffe000u) | 0x80000000u); };
+                        const Pair rest = pair_add(pair(lo, hi), pair(minus_top(lo), minus_top(hi)));
                         w[e / 2] = cut_half(lo, hi);
                         left[e / 2] = pack_half(rest.lo(), rest.hi());
                     }
@@ -642,7 +642,8 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prompt_kernel(const b200q_k
         if (mine && fine && wait(&o_done[t], 0)) {
             tc_fence_after();
             // (in two factors: M and the largest weight may lie 2^126 apart; a part of which the row sees no key adds nothing)
-            const float half_gain = m == -INFINITY ? 0.f : exp2_approx(0.5f * (product_m - KP_RANGE - m)), gain = p.splits == 1 ? __fdiv_rn(half_gain, l) : half_gain;
+            const float half_gain = m == -INFINITY ? 0.f : exp2_approx(0.5f * (product_m - KP_RANGE - m));
+            const float gain = p.splits == 1 ? __fdiv_rn(half_gain, l) : half_gain;
             float *to = p.splits == 1 ? nullptr : p.partial + ((static_cast<size_t>(part) * a.rows) * a.heads + out_row) * (DH + 2);
 #pragma unroll 1
             for (int d = 0; d < DH; d += 32) {
